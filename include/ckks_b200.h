@@ -74,7 +74,8 @@ double ckks_ctx_scale(const ckks_ctx* ctx, int level);
 /* Synchronize() (T123.cpp:1626, 1662, 1671).  Also reports, as CKKS_ECUDA,
  * a bounded device wait that gave up since the last call (a bulk copy into
  * shared memory that did not complete within one second); the outputs of
- * the calls since then are not valid, and the context stays usable. */
+ * the calls since then are not valid, and the context stays usable.  Reports
+ * as CKKS_ECAPACITY the sequences that a ckks_draft_commit left unchanged. */
 int ckks_sync(ckks_ctx* ctx);
 /* the cudaStream_t the context enqueues on (for event timing by callers) */
 void* ckks_ctx_stream(ckks_ctx* ctx);
@@ -331,6 +332,13 @@ int ckks_block_mlp_chunks(const ckks_block* b);
 int ckks_block_state_get(ckks_block* b, int kind, int group, ckks_ct* out);
 int ckks_block_state_set(ckks_block* b, int kind, int group, const ckks_ct* in);
 
+/* The last n tokens (0 <= n <= 64, n <= the block's tokens) of the following
+ * forwards are a tree of drafted tokens: parents[i] (host) is -1 or an
+ * earlier node.  The owner's softmax then lets node i see the tokens before
+ * the drafts, itself and its ancestors; all other tokens stay causal.  n = 0
+ * makes every token causal again. */
+int ckks_block_set_drafts(ckks_block* b, const int* parents, int n);
+
 /* drop the block's encoded BSGS diagonals and masks (about 26 GB per block
  * at N = 2^16); the next forward encodes them again on the device */
 int ckks_block_release_cache(ckks_block* b, size_t* released_bytes);
@@ -402,6 +410,155 @@ int ckks_schedule_diagonal(const double* W, int out_dim, int in_dim, int ld, int
  * first call on a device looks up the array's address (make it before any
  * stream capture); calls that overlap on the GPU race on the shared array. */
 int ckks_rotate_noalloc(ckks_ctx* ctx, const uint64_t* in_dev, int limbs, int k, uint64_t* out_dev);
+
+/* ---- drafted decoding: the data owner's plain operators -------------------
+ * An encrypted forward costs about the same for one token as for the tokens
+ * that share its ciphertexts, so the data owner drafts several tokens with a
+ * small plain model, evaluates all of them in one encrypted forward
+ * (ckks_block_set_drafts) and keeps those that the target's probabilities
+ * confirm.  These are the owner's steps between two forwards.  No
+ * counterpart in the reference, whose client only refreshes.
+ *
+ * All tensors are on the context's device, at addresses aligned to their
+ * elements; no key is needed.  Calls are asynchronous on `stream` (a
+ * cudaStream_t of that device; NULL is the default stream), allocate nothing
+ * and can be captured into a CUDA graph.  Calls that overlap on the GPU must
+ * not share a workspace.  The context's device is made current for the call
+ * and the caller's device restored.
+ *
+ * A tree has `nodes` (1..64) nodes in each sequence: parents[b][i] is -1 (the
+ * node follows the cached keys directly) or an earlier node of the same
+ * sequence.  A node with any other parent is padding, and so is what hangs
+ * below it: it sees nothing and nothing sees it. */
+#define CKKS_BF16 0
+#define CKKS_FP16 1
+#define CKKS_FP32 2
+#define CKKS_FP64 3
+
+/* a device tensor of rows: element (b, h, t, d) at data + b * batch +
+ * h * head + t * row + d, strides in elements and not negative; the d are
+ * contiguous */
+typedef struct {
+  void* data;
+  int64_t batch, head, row;
+} ckks_rows;
+
+typedef struct {
+  int32_t dtype; /* CKKS_BF16, CKKS_FP16 or CKKS_FP32: q, caches, new rows, out */
+  int32_t batch, q_heads, kv_heads, head_dim; /* q_heads a multiple of kv_heads; head_dim 1..256 */
+  int32_t nodes;                              /* 1..64 */
+  int32_t capacity;                           /* rows of each cache */
+  int32_t reserved;                           /* 0 */
+  double scale;                               /* of the scores, usually 1 / sqrt(head_dim) */
+  ckks_rows q;       /* row = node: [batch][nodes][q_heads][head_dim] in any strides */
+  ckks_rows k_cache; /* row = cached key: [batch][kv_heads][capacity][head_dim] */
+  ckks_rows v_cache;
+  ckks_rows k_new; /* row = node: [batch][nodes][kv_heads][head_dim] */
+  ckks_rows v_new;
+  ckks_rows out;          /* as q */
+  const int32_t* lens;    /* [batch] keys in the cache; taken as 0..capacity */
+  const int32_t* parents; /* [batch][nodes] */
+  float* lse;             /* [batch][nodes][q_heads] out */
+  void* workspace;        /* ckks_draft_attention_workspace bytes, 16-byte aligned */
+  size_t workspace_bytes;
+} ckks_draft_attention_args;
+
+/* Attention of every node over the cached keys [0, lens[b]) and the new keys
+ * of itself and its ancestors: out = sum_s softmax(scale q.k)_s v_s, and the
+ * natural log of the softmax's sum in lse.  nodes = 1 is the single-token
+ * decode step.  The row of a node that is padding is 0 and its lse -inf.
+ * Rows of the cache behind lens[b] are not used, whatever they hold.
+ * q_heads / kv_heads query heads share each key/value head. */
+int ckks_draft_attention(ckks_ctx* ctx, const ckks_draft_attention_args* args, void* stream);
+/* workspace bytes for these sizes (the pointers are not looked at), or -1 */
+long long ckks_draft_attention_workspace(ckks_ctx* ctx, const ckks_draft_attention_args* args);
+
+typedef struct {
+  int32_t target_dtype, draft_dtype; /* CKKS_FP32 or CKKS_FP64 */
+  int32_t batch, nodes, vocab, reserved;
+  /* probabilities, row 0 behind the cached tokens and row i + 1 behind node
+   * i; element (b, r, x) at data + b * batch + r * row + x (head unused) */
+  ckks_rows target, draft;
+  const int32_t* tokens;  /* [batch][nodes] the drafts */
+  const int32_t* parents; /* [batch][nodes] */
+  const double* uniforms; /* [batch][nodes + 1] in [0, 1) */
+  int32_t* path;          /* [batch][nodes] out: accepted nodes from the root on, then -1 */
+  int32_t* count;         /* [batch] out: accepted nodes */
+  int32_t* token;         /* [batch] out: the token that follows them */
+} ckks_draft_verify_args;
+
+/* Walks each tree from the root: the children of the node reached are tried
+ * in their order, child c with token x being accepted when
+ * uniforms[b][c] * q(x) < p(x), with q = the draft's row of the node reached
+ * and p the target's; each child refused replaces p by
+ * max(p - q, 0) / sum max(p - q, 0) (p stays where that sum is 0).  When no
+ * child is left, the next token is the first x at which the running sum of p
+ * passes uniforms[b][nodes] times the whole sum.  With children drawn from q,
+ * the tokens are distributed as the target's.  A draft outside the
+ * vocabulary is refused; a probability that is not above 0 counts as 0.
+ * Computed in float64. */
+int ckks_draft_verify(ckks_ctx* ctx, const ckks_draft_verify_args* args, void* stream);
+
+typedef struct {
+  int32_t dtype; /* CKKS_BF16, CKKS_FP16, CKKS_FP32 */
+  int32_t batch, kv_heads, head_dim, nodes, capacity;
+  ckks_rows k_cache, v_cache, k_new, v_new; /* as for ckks_draft_attention */
+  const int32_t* lens;                      /* [batch] */
+  const int32_t* path;                      /* [batch][nodes] */
+  const int32_t* count;                     /* [batch] */
+  int32_t* lens_out;                        /* [batch] out, not overlapping lens */
+} ckks_draft_commit_args;
+
+/* Appends the new keys and values of nodes path[b][0..count[b]) behind
+ * lens[b] and writes the new lengths.  A sequence whose count, path or length
+ * does not fit (count outside 0..nodes, a node outside 0..nodes-1, more rows
+ * than the capacity) is left as it is, with its length unchanged, and is
+ * reported as CKKS_ECAPACITY by a ckks_sync that runs after the stream
+ * reached it. */
+int ckks_draft_commit(ckks_ctx* ctx, const ckks_draft_commit_args* args, void* stream);
+
+typedef struct {
+  int32_t dtype;
+  int32_t batch, q_heads, kv_heads, head_dim, nodes, capacity, reserved;
+  double scale;
+  ckks_rows q, k_cache;
+  ckks_rows acc;        /* float32: element (b, h, s) at data + b * batch + h * head + s; row unused */
+  const float* lse;     /* [batch][nodes][q_heads] of ckks_draft_attention */
+  const int32_t* lens;  /* [batch] before the commit */
+  const int32_t* path;  /* [batch][nodes] */
+  const int32_t* count; /* [batch] */
+} ckks_draft_accumulate_args;
+
+/* Adds to acc[b][h][s] the attention weights exp(scale q.k_s - lse) that the
+ * accepted nodes' rows of every query head on h give key s of the cache
+ * after the commit: node path[b][j] sees keys s <= lens[b] + j.  The keys
+ * behind lens[b] start from 0.  A sequence whose count, path or length does
+ * not fit (as for ckks_draft_commit) is left as it is. */
+int ckks_draft_accumulate(ckks_ctx* ctx, const ckks_draft_accumulate_args* args, void* stream);
+
+typedef struct {
+  int32_t dtype;
+  int32_t batch, kv_heads, head_dim, capacity;
+  int32_t out_capacity;        /* rows of the outputs, at least budget */
+  int32_t budget, recent;      /* 0 <= recent <= budget, budget >= 1 */
+  ckks_rows k_cache, v_cache;  /* inputs */
+  ckks_rows acc;               /* float32 weights, as for ckks_draft_accumulate */
+  ckks_rows k_out, v_out;      /* outputs, not overlapping the inputs */
+  ckks_rows acc_out;           /* float32 */
+  const int32_t* lens;         /* [batch]; taken as 0..capacity */
+  int32_t* index;              /* [batch][kv_heads][budget] out: rows kept, then -1 */
+  int32_t* lens_out;           /* [batch] out, not overlapping lens */
+  void* workspace;             /* ckks_draft_evict_workspace bytes, 16-byte aligned */
+  size_t workspace_bytes;
+} ckks_draft_evict_args;
+
+/* Copies at most `budget` rows of each head's cache, in their order: the
+ * last `recent` ones and, of the others, those with the largest weights (the
+ * lower index first among equals; a weight that is not a number counts as
+ * -inf).  A shorter cache is copied whole.  Output rows behind the last one
+ * kept are left as they were. */
+int ckks_draft_evict(ckks_ctx* ctx, const ckks_draft_evict_args* args, void* stream);
+long long ckks_draft_evict_workspace(ckks_ctx* ctx, const ckks_draft_evict_args* args);
 
 /* Diagnostic of the bounded waits: one CTA stages 4 KiB through a bulk copy
  * into shared memory and back.  starve = 0: CKKS_OK when the data came back

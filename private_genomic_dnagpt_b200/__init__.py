@@ -31,6 +31,8 @@ from dataclasses import dataclass
 
 import numpy as np
 
+from . import drafting
+
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libckks_b200.so")
 HEADER = os.path.join(os.path.dirname(HERE), "include", "ckks_b200.h")
@@ -181,6 +183,15 @@ _SIGS = [
                                         ctypes.POINTER(_vp)]),
     ("ckks_lane_shift", ctypes.c_int, [_vp, ctypes.POINTER(_vp), ctypes.c_int, ctypes.POINTER(ctypes.c_int),
                                        ctypes.c_int, ctypes.c_int, ctypes.POINTER(_vp)]),
+    # the argument structs of the drafted-decoding operators are packed by drafting.py
+    ("ckks_draft_attention", ctypes.c_int, [_vp, ctypes.c_char_p, _vp]),
+    ("ckks_draft_attention_workspace", ctypes.c_longlong, [_vp, ctypes.c_char_p]),
+    ("ckks_draft_verify", ctypes.c_int, [_vp, ctypes.c_char_p, _vp]),
+    ("ckks_draft_commit", ctypes.c_int, [_vp, ctypes.c_char_p, _vp]),
+    ("ckks_draft_accumulate", ctypes.c_int, [_vp, ctypes.c_char_p, _vp]),
+    ("ckks_draft_evict", ctypes.c_int, [_vp, ctypes.c_char_p, _vp]),
+    ("ckks_draft_evict_workspace", ctypes.c_longlong, [_vp, ctypes.c_char_p]),
+    ("ckks_block_set_drafts", ctypes.c_int, [_vp, ctypes.POINTER(ctypes.c_int), ctypes.c_int]),
 ]
 
 _lib = None
@@ -327,6 +338,8 @@ class Diagonals:
 class CryptoContext:
     """GenCryptoContext result: parameters, device tables and keys."""
 
+    _draft_device = None  # torch device of the drafted-decoding operators, made on their first use
+
     def __init__(self, params: CCParams):
         p = ckks_params(params.ring_dim_log, params.limbs, params.dnum, params.first_mod_bits,
                         params.scale_mod_bits, params.special_mod_bits, params.seed, params.device)
@@ -344,6 +357,7 @@ class CryptoContext:
         m = np.zeros(self.L + self.K, np.uint64)
         _check(lib().ckks_ctx_moduli(h, _u64(m), m.size))
         self.moduli = m
+        self._draft_sizes = {}
 
     def __del__(self):
         try:
@@ -728,6 +742,33 @@ class CryptoContext:
         _check(lib().ckks_window_sum_batch_radix(self.h, (_vp * max(1, n))(*[c.h for c in cts]), n, window, stride,
                                                  radix, (_vp * max(1, n))(*[o.h for o in outs])))
         return outs
+
+
+    # -- drafted decoding: the data owner's plain operators (drafting.py) ----
+    def draft_attention(self, q, k_cache, v_cache, lens, k_new, v_new, parents, scale=None):
+        """Attention of a tree of drafted nodes over a key/value cache:
+        (out, lse); see ``drafting.attention``."""
+        return drafting.attention(self, q, k_cache, v_cache, lens, k_new, v_new, parents, scale)
+
+    def draft_verify(self, target, draft, tokens, parents, uniforms):
+        """Drafts that the target's probabilities confirm: (path, count,
+        token); see ``drafting.verify``."""
+        return drafting.verify(self, target, draft, tokens, parents, uniforms)
+
+    def draft_commit(self, k_cache, v_cache, lens, k_new, v_new, path, count):
+        """The accepted nodes' rows appended to the cache: the new lengths;
+        see ``drafting.commit``."""
+        return drafting.commit(self, k_cache, v_cache, lens, k_new, v_new, path, count)
+
+    def draft_accumulate(self, q, lse, k_cache, lens, path, count, acc, scale=None):
+        """The accepted nodes' attention weights added to acc; see
+        ``drafting.accumulate``."""
+        return drafting.accumulate(self, q, lse, k_cache, lens, path, count, acc, scale)
+
+    def draft_evict(self, k_cache, v_cache, acc, lens, budget, recent, out=None):
+        """The cache cut to ``budget`` rows: (k, v, acc, index, lens); see
+        ``drafting.evict``."""
+        return drafting.evict(self, k_cache, v_cache, acc, lens, budget, recent, out)
 
 
 def GenCryptoContext(params: CCParams) -> CryptoContext:

@@ -507,6 +507,39 @@ __global__ void score_gather_kernel(const double* __restrict__ vals, const Score
   scores[((size_t)q * H + h) * T + k] = vals[(size_t)tg.v * slots + (size_t)f * B + ql];
 }
 
+// the tree of drafted tokens that the last n tokens form: bit j of mask[i] is
+// set where drafted token i sees drafted token j (n = 0: every token causal)
+struct DraftTree {
+  unsigned long long mask[64];
+  int n;
+};
+
+// whether token q sees token k <= q of T
+__device__ __forceinline__ bool draft_sees(const DraftTree& tree, int T, int q, int k) {
+  const int first = T - tree.n;
+  return q < first || k < first || (tree.mask[q - first] >> (k - first) & 1);
+}
+
+// stable softmax of row (q, h) over the drafted tokens' ancestors and the
+// tokens before the drafts; a missing score poisons the row
+__global__ void softmax_tree_kernel(const double* __restrict__ scores, double* __restrict__ prob, int T, int H,
+                                    DraftTree tree, int* __restrict__ bad) {
+  const int r = blockIdx.x * kThreads + threadIdx.x;
+  if (r >= T * H) return;
+  const int q = r / H;
+  const double* row = scores + (size_t)r * T;
+  double* out = prob + (size_t)r * T;
+  double mx = -INFINITY;
+  for (int k = 0; k <= q; ++k) {
+    if (!isfinite(row[k])) atomicExch(bad, 1);
+    if (draft_sees(tree, T, q, k)) mx = fmax(mx, row[k]);
+  }
+  double den = 0.0;
+  for (int k = 0; k <= q; ++k)
+    if (draft_sees(tree, T, q, k)) den += exp(row[k] - mx);
+  for (int k = 0; k < T; ++k) out[k] = k <= q && draft_sees(tree, T, q, k) ? exp(row[k] - mx) / den : 0.0;
+}
+
 // stable causal softmax of row (q, h) over k <= q; a missing score poisons the row
 __global__ void softmax_kernel(const double* __restrict__ scores, double* __restrict__ prob, int T, int H,
                                int* __restrict__ bad) {
@@ -1172,6 +1205,7 @@ struct ckks_block {
   // evaluation state between the stages of one forward
   std::vector<Ciphertext> st_x, st_q, st_k, st_v, st_ctx, st_r1, st_mlp;
   double* st_prob = nullptr;
+  blk::DraftTree drafts{};  // the drafted tokens of the following forwards (ckks_block_set_drafts)
   cudaEvent_t ev_in = nullptr, ev_out = nullptr;
   double t_start = 0.0, t_stage = 0.0, alloc_s0 = 0.0;
   long alloc_n0 = 0;
@@ -1404,8 +1438,11 @@ void ckks_block::shard_softmax(const double* d_scores) {
   if (!st_prob) st_prob = (double*)C.alloc(sizeof(double) * (size_t)T * H * T);
   int* bad = (int*)C.alloc(sizeof(int));
   CKKS_CUDA(cudaMemsetAsync(bad, 0, sizeof(int), C.stream));
-  blk::softmax_kernel<<<(T * H + blk::kThreads - 1) / blk::kThreads, blk::kThreads, 0, C.stream>>>(d_scores, st_prob,
-                                                                                                     T, H, bad);
+  const int nb = (T * H + blk::kThreads - 1) / blk::kThreads;
+  if (drafts.n)
+    blk::softmax_tree_kernel<<<nb, blk::kThreads, 0, C.stream>>>(d_scores, st_prob, T, H, drafts, bad);
+  else
+    blk::softmax_kernel<<<nb, blk::kThreads, 0, C.stream>>>(d_scores, st_prob, T, H, bad);
   int hbad = 0;
   CKKS_CUDA(cudaMemcpyAsync(&hbad, bad, sizeof(int), cudaMemcpyDeviceToHost, C.stream));
   CKKS_CUDA(cudaStreamSynchronize(C.stream));
@@ -1798,6 +1835,23 @@ int ckks_head_forward(ckks_block* h, const double* x_last, double* margin) {
     if (h->orphaned) throw ckks::Error(CKKS_ESTATE, "the head's context was destroyed");
     if (!h->d_head) throw ckks::Error(CKKS_EARG, "not a head object");
     *margin = h->head_forward(x_last);
+  });
+}
+
+int ckks_block_set_drafts(ckks_block* b, const int* parents, int n) {
+  return bguard([&] {
+    if (!b || (n && !parents)) throw ckks::Error(CKKS_EARG, "null argument");
+    if (b->orphaned) throw ckks::Error(CKKS_ESTATE, "the block's context was destroyed");
+    if (b->d_head) throw ckks::Error(CKKS_EARG, "a head evaluates one token");
+    if (n < 0 || n > 64 || n > b->s.T) throw ckks::Error(CKKS_EARG, "draft count outside 0..64 or above the token count");
+    blk::DraftTree t{};
+    t.n = n;
+    for (int i = 0; i < n; ++i) {
+      if (parents[i] < -1 || parents[i] >= i)
+        throw ckks::Error(CKKS_EARG, "a drafted token's parent is -1 or an earlier drafted token");
+      t.mask[i] = 1ull << i | (parents[i] >= 0 ? t.mask[parents[i]] : 0ull);
+    }
+    b->drafts = t;
   });
 }
 

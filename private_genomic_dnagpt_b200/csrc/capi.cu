@@ -658,11 +658,15 @@ int ckks_sync(ckks_ctx* ctx) {
   return guard([&] {
     Context& c = C(ctx);
     CKKS_CUDA(cudaStreamSynchronize(c.stream));
-    const unsigned int f = ckks::take_device_faults(c);
+    unsigned int r = 0;
+    const unsigned int f = ckks::take_device_faults(c, &r);
     if (f)
       throw Error(CKKS_ECUDA, std::to_string(f) +
                                   " bounded device wait(s) gave up (a bulk copy into shared memory did not complete); "
                                   "the outputs since the last synchronisation are not valid");
+    if (r)
+      throw Error(CKKS_ECAPACITY, std::to_string(r) + " sequence(s) left unchanged by ckks_draft_commit: the count, the "
+                                                      "path or the length does not fit the cache");
   });
 }
 

@@ -197,7 +197,8 @@ class Context {
 
   // device tables
   Mod* d_mods = nullptr;            // [P]
-  unsigned int* d_faults = nullptr;  // bounded device waits that gave up (bulk copies)
+  // [0] bounded device waits that gave up (bulk copies), [1] sequences that a draft commit left unchanged
+  unsigned int* d_faults = nullptr;
   ulonglong2* d_tw = nullptr;       // [P][N] forward (w, w')
   ulonglong2* d_itw = nullptr;      // [P][N] inverse (w, w')
   double2* d_twd = nullptr;         // [P][N] forward (w, fl(w/q)) as doubles (primes below 2^50.3)
@@ -444,7 +445,9 @@ void keyswitch_batch(const Context& c, int limbs, const KsBatch& b, bool shared_
 // Count of bounded device waits that gave up since the last call (each
 // leaves its CTA's outputs unwritten), read after the stream drains and
 // reset to zero.
-unsigned int take_device_faults(const Context& c);
+// (and, where the caller reports them, the sequences that draft commits left
+// unchanged, once there is no fault)
+unsigned int take_device_faults(const Context& c, unsigned int* refused_commits = nullptr);
 // One CTA stages 4 KiB of src through a bulk copy and writes it to dst;
 // with `starve` its barrier expects twice the bytes copied, so its wait
 // runs out and counts one fault (tests of the bounded wait).

@@ -235,8 +235,8 @@ Context::Context(const Params& p) : params(p) {
     pmod[i] = shoup_pair(i < L ? pm : 0, q);
   }
   d_mods = upload(mods);
-  CKKS_CUDA(cudaMalloc(&d_faults, sizeof(unsigned int)));
-  CKKS_CUDA(cudaMemset(d_faults, 0, sizeof(unsigned int)));
+  CKKS_CUDA(cudaMalloc(&d_faults, 2 * sizeof(unsigned int)));
+  CKKS_CUDA(cudaMemset(d_faults, 0, 2 * sizeof(unsigned int)));
   d_tw = upload(tw);
   d_itw = upload(itw);
   d_twd = upload(twd);

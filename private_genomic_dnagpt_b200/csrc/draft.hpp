@@ -1,0 +1,164 @@
+// draft.hpp -- what the translation units of the drafted-decoding operators
+// share: argument checks, the device guard, element conversions and the
+// ancestor masks of a tree of drafted nodes.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <string>
+
+#include "../../include/ckks_b200.h"
+#include "capi_types.hpp"
+#include "ckks_internal.hpp"
+
+namespace ckks {
+namespace draft {
+
+constexpr int kMaxNodes = 64;  // a node's ancestors are the bits of one 64-bit word
+constexpr int kMaxHeadDim = 256;
+
+inline void need(bool ok, const char* msg) {
+  if (!ok) throw Error(CKKS_EARG, msg);
+}
+
+template <typename F>
+int guard(F&& f) {
+  try {
+    f();
+    return CKKS_OK;
+  } catch (const Error& e) {
+    set_last_error(e.what());
+    return e.code;
+  } catch (const std::exception& e) {
+    set_last_error(e.what());
+    return CKKS_EARG;
+  } catch (...) {
+    set_last_error("unknown error");
+    return CKKS_EARG;
+  }
+}
+
+inline Context& context_of(ckks_ctx* x) {
+  need(x && x->c, "null context");
+  return *x->c;
+}
+
+// makes the context's device current for one call
+struct OnDevice {
+  int prev = -1;
+  explicit OnDevice(const Context& c) {
+    int cur = -1;
+    CKKS_CUDA(cudaGetDevice(&cur));
+    if (cur != c.params.device) {
+      CKKS_CUDA(cudaSetDevice(c.params.device));
+      prev = cur;
+    }
+  }
+  ~OnDevice() {
+    if (prev >= 0) cudaSetDevice(prev);
+  }
+};
+
+inline int element_bytes(int dtype) {
+  switch (dtype) {
+    case CKKS_BF16:
+    case CKKS_FP16:
+      return 2;
+    case CKKS_FP32:
+      return 4;
+    case CKKS_FP64:
+      return 8;
+  }
+  throw Error(CKKS_EARG, "element type is none of CKKS_BF16, CKKS_FP16, CKKS_FP32, CKKS_FP64");
+}
+
+inline void check_rows(const ckks_rows& r, int bytes, const char* what) {
+  if (!r.data) throw Error(CKKS_EARG, std::string(what) + ": null device buffer");
+  if (reinterpret_cast<uintptr_t>(r.data) % bytes)
+    throw Error(CKKS_EARG, std::string(what) + ": address not aligned to its elements");
+  if (r.batch < 0 || r.head < 0 || r.row < 0) throw Error(CKKS_EARG, std::string(what) + ": negative stride");
+}
+
+template <typename P>
+void check_ptr(const P* p, const char* what) {
+  if (!p) throw Error(CKKS_EARG, std::string(what) + ": null device buffer");
+  if (reinterpret_cast<uintptr_t>(p) % alignof(P))
+    throw Error(CKKS_EARG, std::string(what) + ": address not aligned to its elements");
+}
+
+// whether every row starts on a 16-byte boundary and holds whole 16-byte
+// pieces (wide loads; TMA asks the same of bases and strides).  A stride
+// along which there is one entry is never used.
+inline bool wide_rows(const ckks_rows& r, int batch, int heads, int rows, int head_dim, int bytes) {
+  auto fits = [&](int64_t s, int n) { return n <= 1 || (s * bytes) % 16 == 0; };
+  return reinterpret_cast<uintptr_t>(r.data) % 16 == 0 && (head_dim * bytes) % 16 == 0 && fits(r.batch, batch) &&
+         fits(r.head, heads) && fits(r.row, rows);
+}
+
+// last byte + 1 of a tensor of rows
+inline const char* end_of(const ckks_rows& r, int batch, int heads, int rows, int row_elems, int bytes) {
+  const int64_t last = (batch - 1) * r.batch + (heads - 1) * r.head + (int64_t)(rows - 1) * r.row + row_elems;
+  return static_cast<const char*>(r.data) + last * bytes;
+}
+
+template <typename T>
+__device__ __forceinline__ float to_f32(T x) {
+  if constexpr (std::is_same_v<T, __nv_bfloat16>)
+    return __bfloat162float(x);
+  else if constexpr (std::is_same_v<T, __half>)
+    return __half2float(x);
+  else
+    return (float)x;
+}
+
+template <typename T>
+__device__ __forceinline__ T from_f32(float x) {
+  if constexpr (std::is_same_v<T, __nv_bfloat16>)
+    return __float2bfloat16_rn(x);
+  else if constexpr (std::is_same_v<T, __half>)
+    return __float2half_rn(x);
+  else
+    return (T)x;
+}
+
+// Ancestor masks of one tree, by one warp: mask[i] gets the bits of node i
+// and of the nodes above it, 0 where i is padding.  Six rounds of pointer
+// doubling cover every depth up to 64.  `jump` is scratch of 64 ints.
+__device__ __forceinline__ void tree_masks(const int32_t* __restrict__ parents, int n, uint64_t* mask, int* jump) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const int i = lane + 32 * k;
+    const int p = i < n ? parents[i] : -2;
+    const bool ok = p >= -1 && p < i;  // a parent comes before its children
+    mask[i] = ok ? 1ull << i : 0ull;
+    jump[i] = ok ? p : -2;
+  }
+  __syncwarp();
+#pragma unroll 1
+  for (int r = 0; r < 6; ++r) {
+    uint64_t m[2];
+    int j[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int i = lane + 32 * k;
+      const int p = jump[i];
+      m[k] = mask[i] | (p >= 0 ? mask[p] : 0ull);
+      j[k] = p >= 0 ? jump[p] : p;
+    }
+    __syncwarp();
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      mask[lane + 32 * k] = m[k];
+      jump[lane + 32 * k] = j[k];
+    }
+    __syncwarp();
+  }
+#pragma unroll
+  for (int k = 0; k < 2; ++k)
+    if (jump[lane + 32 * k] != -1) mask[lane + 32 * k] = 0ull;
+  __syncwarp();
+}
+
+}  // namespace draft
+}  // namespace ckks

@@ -1,0 +1,417 @@
+// draft_cache.cu -- what happens to the draft model's key/value cache once
+// the target has confirmed drafts: the accepted rows are appended
+// (ckks_draft_commit), the attention weight they give each cached key is
+// added up (ckks_draft_accumulate), and a cache that has grown past its
+// budget keeps its latest and its heaviest keys (ckks_draft_evict).
+#include <algorithm>
+#include <cmath>
+
+#include "draft.hpp"
+
+namespace ckks {
+namespace draft {
+namespace {
+
+// Whether a sequence's count, path and length fit; evaluated alike by every
+// thread of a CTA from `count` entries of path
+__device__ __forceinline__ bool fits(const int32_t* path, int count, int len, int nodes, int capacity) {
+  if (count < 0 || count > nodes || len < 0 || len > capacity || count > capacity - len) return false;
+  bool ok = true;
+  for (int j = 0; j < count; ++j) ok = ok && path[j] >= 0 && path[j] < nodes;
+  return ok;
+}
+
+// ---- commit --------------------------------------------------------------------
+struct CommitParams {
+  ckks_rows kc, vc, kn, vn;
+  const int32_t* lens;
+  const int32_t* path;
+  const int32_t* count;
+  int32_t* lens_out;
+  unsigned int* refused;
+  int batch, kv_heads, head_dim, nodes, capacity;
+};
+
+// CTA = (sequence, head): copies its accepted rows in pieces of V elements
+template <typename T, typename V>
+__global__ void __launch_bounds__(128) commit_kernel(CommitParams p) {
+  const int b = blockIdx.x, h = blockIdx.y;
+  const int32_t* path = p.path + (size_t)b * p.nodes;
+  const int len = p.lens[b], count = p.count[b];
+  const bool ok = fits(path, count, len, p.nodes, p.capacity);
+  if (h == 0 && threadIdx.x == 0) {
+    p.lens_out[b] = ok ? len + count : len;
+    if (!ok) atomicAdd(p.refused, 1u);
+  }
+  if (!ok) return;
+  constexpr int W = sizeof(V) / sizeof(T);
+  const int per = p.head_dim / W;
+  T* kc = static_cast<T*>(p.kc.data) + b * p.kc.batch + h * p.kc.head;
+  T* vc = static_cast<T*>(p.vc.data) + b * p.vc.batch + h * p.vc.head;
+  const T* kn = static_cast<const T*>(p.kn.data) + b * p.kn.batch + h * p.kn.head;
+  const T* vn = static_cast<const T*>(p.vn.data) + b * p.vn.batch + h * p.vn.head;
+  for (int i = threadIdx.x; i < count * per; i += blockDim.x) {
+    const int j = i / per, d = i % per * W, node = path[j];
+    *reinterpret_cast<V*>(kc + (len + j) * p.kc.row + d) = *reinterpret_cast<const V*>(kn + node * p.kn.row + d);
+    *reinterpret_cast<V*>(vc + (len + j) * p.vc.row + d) = *reinterpret_cast<const V*>(vn + node * p.vn.row + d);
+  }
+}
+
+// ---- accumulate -----------------------------------------------------------------
+struct AccParams {
+  ckks_rows q, kc, acc;
+  const float* lse;
+  const int32_t* lens;
+  const int32_t* path;
+  const int32_t* count;
+  int batch, kv_heads, group, head_dim, nodes, capacity;
+  float scale;
+};
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kAccKeys = 128, kAccRows = 8;
+
+// CTA = (sequence x head, 128 keys): one key per thread, the accepted rows
+// in shared memory eight at a time; a key's weights are added in the order of
+// the rows, so results do not depend on timing
+template <typename T>
+__global__ void __launch_bounds__(kAccKeys) accumulate_kernel(AccParams p) {
+  __shared__ float sq[kAccRows][kMaxHeadDim], sl[kAccRows];
+  const int b = blockIdx.x / p.kv_heads, h = blockIdx.x % p.kv_heads;
+  const int32_t* path = p.path + (size_t)b * p.nodes;
+  const int len = p.lens[b], count = p.count[b], D = p.head_dim;
+  if (count == 0 || !fits(path, count, len, p.nodes, p.capacity)) return;
+  const int total = len + count, rows = count * p.group;
+  for (int base = blockIdx.y * kAccKeys; base < total; base += gridDim.y * kAccKeys) {
+    const int s = base + threadIdx.x;
+    float sum = 0.0f;
+    for (int r0 = 0; r0 < rows; r0 += kAccRows) {
+      __syncthreads();
+      const int nr = min(kAccRows, rows - r0);
+      for (int i = threadIdx.x; i < nr * D; i += kAccKeys) {
+        const int row = r0 + i / D, node = path[row / p.group], qh = h * p.group + row % p.group;
+        sq[i / D][i % D] = p.scale * kLog2e *
+                           to_f32(static_cast<const T*>(p.q.data)[b * p.q.batch + qh * p.q.head + node * p.q.row + i % D]);
+      }
+      if (threadIdx.x < nr) {
+        const int row = r0 + threadIdx.x, node = path[row / p.group], qh = h * p.group + row % p.group;
+        sl[threadIdx.x] = kLog2e * p.lse[((size_t)b * p.nodes + node) * p.kv_heads * p.group + qh];
+      }
+      __syncthreads();
+      if (s < total) {
+        const T* k = static_cast<const T*>(p.kc.data) + b * p.kc.batch + h * p.kc.head + s * p.kc.row;
+        float x[kAccRows];
+#pragma unroll
+        for (int r = 0; r < kAccRows; ++r) x[r] = 0.0f;
+        for (int d = 0; d < D; ++d) {
+          const float kd = to_f32(k[d]);
+#pragma unroll
+          for (int r = 0; r < kAccRows; ++r)
+            if (r < nr) x[r] = fmaf(kd, sq[r][d], x[r]);
+        }
+#pragma unroll
+        for (int r = 0; r < kAccRows; ++r)
+          if (r < nr && s <= len + (r0 + r) / p.group) sum += exp2f(x[r] - sl[r]);
+      }
+    }
+    if (s < total) {
+      float* a = static_cast<float*>(p.acc.data) + b * p.acc.batch + h * p.acc.head + s;
+      *a = s < len ? *a + sum : sum;
+    }
+  }
+}
+
+// ---- evict ----------------------------------------------------------------------
+struct EvictParams {
+  ckks_rows kc, vc, acc, ko, vo, ao;
+  const int32_t* lens;
+  int32_t* index;
+  int32_t* lens_out;
+  int batch, kv_heads, head_dim, capacity, budget, recent;
+};
+
+// unsigned order of floats: larger weight, larger word; -0 equals 0, NaN is
+// the smallest
+__device__ __forceinline__ uint32_t order_of(float x) {
+  if (isnan(x)) return 0u;
+  const uint32_t u = __float_as_uint(x + 0.0f);
+  return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+
+constexpr int kSelThreads = 1024;
+
+// CTA = (sequence, head): the rows to keep, in order.  Four passes over the
+// weights narrow the smallest weight kept down to its 32 bits (histograms of
+// 8 bits); a last one lists the rows above it and the first of those at it.
+__global__ void __launch_bounds__(kSelThreads) select_kernel(EvictParams p) {
+  __shared__ int s_hist[256];
+  __shared__ uint32_t s_prefix;
+  __shared__ int s_left, s_warp[kSelThreads / 32][2];
+  const int b = blockIdx.x / p.kv_heads, h = blockIdx.x % p.kv_heads, tid = threadIdx.x;
+  const int len = min(max(p.lens[b], 0), p.capacity);
+  const int kept = min(len, p.budget), recent = min(p.recent, kept);
+  const int older = len - recent, pick = kept - recent;
+  const float* acc = static_cast<const float*>(p.acc.data) + b * p.acc.batch + h * p.acc.head;
+  float* ao = static_cast<float*>(p.ao.data) + b * p.ao.batch + h * p.ao.head;
+  int32_t* index = p.index + (size_t)blockIdx.x * p.budget;
+  if (h == 0 && tid == 0) p.lens_out[b] = kept;
+  for (int i = kept + tid; i < p.budget; i += kSelThreads) index[i] = -1;
+  for (int i = tid; i < recent; i += kSelThreads) {
+    index[pick + i] = older + i;
+    ao[pick + i] = acc[older + i];
+  }
+  if (pick == 0) return;
+  if (pick == older) {
+    for (int i = tid; i < pick; i += kSelThreads) {
+      index[i] = i;
+      ao[i] = acc[i];
+    }
+    return;
+  }
+  if (tid == 0) {
+    s_prefix = 0;
+    s_left = pick;
+  }
+  for (int shift = 24; shift >= 0; shift -= 8) {
+    if (tid < 256) s_hist[tid] = 0;
+    __syncthreads();
+    const uint32_t prefix = s_prefix;
+    for (int i = tid; i < older; i += kSelThreads) {
+      const uint32_t u = order_of(acc[i]);
+      if (shift == 24 || u >> (shift + 8) == prefix >> (shift + 8)) atomicAdd(&s_hist[u >> shift & 255], 1);
+    }
+    __syncthreads();
+    if (tid == 0) {
+      int left = s_left, d = 255;
+      while (d > 0 && s_hist[d] < left) left -= s_hist[d--];
+      s_left = left;
+      s_prefix = prefix | (uint32_t)d << shift;
+    }
+    __syncthreads();
+  }
+  const uint32_t edge = s_prefix;
+  const int ties = s_left;  // rows at the edge weight that are kept, the first ones
+  int above = 0, at_edge = 0;  // counts before this round
+  for (int base = 0; base < older; base += kSelThreads) {
+    const int i = base + tid;
+    const uint32_t u = i < older ? order_of(acc[i]) : 0u;
+    const bool gt = i < older && u > edge, eq = i < older && u == edge;
+    const uint32_t mg = __ballot_sync(0xffffffffu, gt), me = __ballot_sync(0xffffffffu, eq);
+    const int lane = tid & 31, warp = tid >> 5;
+    if (lane == 0) {
+      s_warp[warp][0] = __popc(mg);
+      s_warp[warp][1] = __popc(me);
+    }
+    __syncthreads();
+    int bg = above, be = at_edge;
+    for (int w = 0; w < kSelThreads / 32; ++w) {
+      if (w < warp) {
+        bg += s_warp[w][0];
+        be += s_warp[w][1];
+      }
+      above += s_warp[w][0];
+      at_edge += s_warp[w][1];
+    }
+    const uint32_t below = (1u << lane) - 1u;
+    bg += __popc(mg & below);
+    be += __popc(me & below);
+    if (gt || (eq && be < ties)) {
+      const int slot = bg + min(be, ties);
+      index[slot] = i;
+      ao[slot] = acc[i];
+    }
+    __syncthreads();
+  }
+}
+
+// copies the rows listed in index, in pieces of V elements: CTA.x = (sequence
+// x head), CTA.y strides over the budget
+template <typename T, typename V>
+__global__ void __launch_bounds__(256) gather_kernel(EvictParams p) {
+  constexpr int W = sizeof(V) / sizeof(T);
+  const int b = blockIdx.x / p.kv_heads, h = blockIdx.x % p.kv_heads;
+  const int kept = min(min(max(p.lens[b], 0), p.capacity), p.budget);
+  const int per = p.head_dim / W;
+  const int32_t* index = p.index + (size_t)blockIdx.x * p.budget;
+  const T* kc = static_cast<const T*>(p.kc.data) + b * p.kc.batch + h * p.kc.head;
+  const T* vc = static_cast<const T*>(p.vc.data) + b * p.vc.batch + h * p.vc.head;
+  T* ko = static_cast<T*>(p.ko.data) + b * p.ko.batch + h * p.ko.head;
+  T* vo = static_cast<T*>(p.vo.data) + b * p.vo.batch + h * p.vo.head;
+  const long long n = (long long)kept * per;
+  for (long long i = (long long)blockIdx.y * blockDim.x + threadIdx.x; i < n; i += (long long)gridDim.y * blockDim.x) {
+    const int r = (int)(i / per), d = (int)(i % per) * W, s = index[r];
+    const V k = *reinterpret_cast<const V*>(kc + s * p.kc.row + d);
+    const V v = *reinterpret_cast<const V*>(vc + s * p.vc.row + d);
+    *reinterpret_cast<V*>(ko + r * p.ko.row + d) = k;
+    *reinterpret_cast<V*>(vo + r * p.vo.row + d) = v;
+  }
+}
+
+void check_cache(int dtype, int batch, int kv_heads, int head_dim, int capacity) {
+  need(dtype == CKKS_BF16 || dtype == CKKS_FP16 || dtype == CKKS_FP32,
+       "caches are CKKS_BF16, CKKS_FP16 or CKKS_FP32");
+  need(batch >= 0 && capacity >= 0, "negative batch or capacity");
+  need(kv_heads >= 1 && kv_heads <= 65535, "key/value head count out of range");
+  need(head_dim >= 1 && head_dim <= kMaxHeadDim, "head_dim outside 1..256");
+  need((long long)batch * kv_heads < (1ll << 31) - 1 && capacity < (1 << 30), "sizes too large");
+}
+
+bool disjoint(const void* a0, const void* a1, const void* b0, const void* b1) { return a1 <= b0 || b1 <= a0; }
+
+// rows as 16-byte pieces, or as single elements of a type of their size
+template <typename F>
+void by_piece(int bytes, bool wide, F&& f) {
+  if (bytes == 2)
+    wide ? f(uint16_t{}, uint4{}) : f(uint16_t{}, uint16_t{});
+  else
+    wide ? f(uint32_t{}, uint4{}) : f(uint32_t{}, uint32_t{});
+}
+
+}  // namespace
+}  // namespace draft
+}  // namespace ckks
+
+using namespace ckks;
+using namespace ckks::draft;
+
+extern "C" int ckks_draft_commit(ckks_ctx* ctx, const ckks_draft_commit_args* args, void* stream) {
+  return guard([&] {
+    Context& c = context_of(ctx);
+    need(args != nullptr, "null argument");
+    const ckks_draft_commit_args& a = *args;
+    check_cache(a.dtype, a.batch, a.kv_heads, a.head_dim, a.capacity);
+    need(a.nodes >= 1 && a.nodes <= kMaxNodes, "node count outside 1..64");
+    if (a.batch == 0) return;
+    const int e = element_bytes(a.dtype);
+    if (a.capacity) {
+      check_rows(a.k_cache, e, "k_cache");
+      check_rows(a.v_cache, e, "v_cache");
+    }
+    check_rows(a.k_new, e, "k_new");
+    check_rows(a.v_new, e, "v_new");
+    check_ptr(a.lens, "lens");
+    check_ptr(a.path, "path");
+    check_ptr(a.count, "count");
+    check_ptr(a.lens_out, "lens_out");
+    need(disjoint(a.lens, a.lens + a.batch, a.lens_out, a.lens_out + a.batch), "lens_out overlaps lens");
+    CommitParams p{a.k_cache, a.v_cache,  a.k_new,    a.v_new, a.lens,    a.path, a.count, a.lens_out,
+                   c.d_faults + 1, a.batch, a.kv_heads, a.head_dim, a.nodes, a.capacity};
+    const bool wide = a.capacity && wide_rows(a.k_cache, a.batch, a.kv_heads, a.capacity, a.head_dim, e) &&
+                      wide_rows(a.v_cache, a.batch, a.kv_heads, a.capacity, a.head_dim, e) &&
+                      wide_rows(a.k_new, a.batch, a.kv_heads, a.nodes, a.head_dim, e) &&
+                      wide_rows(a.v_new, a.batch, a.kv_heads, a.nodes, a.head_dim, e);
+    OnDevice dev(c);
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    ProfScope ps(c, "draft_commit", 4.0 * e * a.batch * a.kv_heads * a.nodes * a.head_dim, st);
+    by_piece(e, wide, [&](auto t, auto v) {
+      commit_kernel<decltype(t), decltype(v)><<<dim3(a.batch, a.kv_heads), 128, 0, st>>>(p);
+    });
+    CKKS_CUDA(cudaGetLastError());
+  });
+}
+
+extern "C" int ckks_draft_accumulate(ckks_ctx* ctx, const ckks_draft_accumulate_args* args, void* stream) {
+  return guard([&] {
+    Context& c = context_of(ctx);
+    need(args != nullptr, "null argument");
+    const ckks_draft_accumulate_args& a = *args;
+    check_cache(a.dtype, a.batch, a.kv_heads, a.head_dim, a.capacity);
+    need(a.nodes >= 1 && a.nodes <= kMaxNodes, "node count outside 1..64");
+    need(a.q_heads >= 1 && a.q_heads % a.kv_heads == 0, "query heads are not a multiple of the key/value heads");
+    need(std::isfinite(a.scale), "scale is not finite");
+    if (a.batch == 0 || a.capacity == 0) return;
+    const int e = element_bytes(a.dtype);
+    check_rows(a.q, e, "q");
+    check_rows(a.k_cache, e, "k_cache");
+    check_rows(a.acc, 4, "acc");
+    check_ptr(a.lse, "lse");
+    check_ptr(a.lens, "lens");
+    check_ptr(a.path, "path");
+    check_ptr(a.count, "count");
+    AccParams p{a.q,     a.k_cache, a.acc,     a.lse, a.lens, a.path, a.count, a.batch, a.kv_heads, a.q_heads / a.kv_heads,
+                a.head_dim, a.nodes, a.capacity, (float)a.scale};
+    OnDevice dev(c);
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    ProfScope ps(c, "draft_accumulate", (double)e * a.batch * a.kv_heads * a.capacity * a.head_dim, st);
+    const dim3 grid((unsigned)(a.batch * a.kv_heads), (unsigned)std::min(65535, (a.capacity + kAccKeys - 1) / kAccKeys));
+    if (a.dtype == CKKS_BF16)
+      accumulate_kernel<__nv_bfloat16><<<grid, kAccKeys, 0, st>>>(p);
+    else if (a.dtype == CKKS_FP16)
+      accumulate_kernel<__half><<<grid, kAccKeys, 0, st>>>(p);
+    else
+      accumulate_kernel<float><<<grid, kAccKeys, 0, st>>>(p);
+    CKKS_CUDA(cudaGetLastError());
+  });
+}
+
+namespace {
+void check_evict(const ckks_draft_evict_args& a) {
+  check_cache(a.dtype, a.batch, a.kv_heads, a.head_dim, a.capacity);
+  need(a.budget >= 1 && a.recent >= 0 && a.recent <= a.budget, "need budget >= 1 and 0 <= recent <= budget");
+  need(a.out_capacity >= a.budget && a.out_capacity < (1 << 30), "output capacity below the budget");
+}
+}  // namespace
+
+extern "C" long long ckks_draft_evict_workspace(ckks_ctx* ctx, const ckks_draft_evict_args* args) {
+  long long n = -1;
+  guard([&] {
+    context_of(ctx);
+    need(args != nullptr, "null argument");
+    check_evict(*args);
+    n = 0;
+  });
+  return n;
+}
+
+extern "C" int ckks_draft_evict(ckks_ctx* ctx, const ckks_draft_evict_args* args, void* stream) {
+  return guard([&] {
+    Context& c = context_of(ctx);
+    need(args != nullptr, "null argument");
+    const ckks_draft_evict_args& a = *args;
+    check_evict(a);
+    if (a.batch == 0) return;
+    const int e = element_bytes(a.dtype);
+    check_rows(a.k_out, e, "k_out");
+    check_rows(a.v_out, e, "v_out");
+    check_rows(a.acc_out, 4, "acc_out");
+    check_ptr(a.lens, "lens");
+    check_ptr(a.index, "index");
+    check_ptr(a.lens_out, "lens_out");
+    need(disjoint(a.lens, a.lens + a.batch, a.lens_out, a.lens_out + a.batch), "lens_out overlaps lens");
+    if (a.capacity) {
+      check_rows(a.k_cache, e, "k_cache");
+      check_rows(a.v_cache, e, "v_cache");
+      check_rows(a.acc, 4, "acc");
+      const ckks_rows ins[3] = {a.k_cache, a.v_cache, a.acc}, outs[3] = {a.k_out, a.v_out, a.acc_out};
+      for (int i = 0; i < 3; ++i)
+        for (int o = 0; o < 3; ++o) {
+          auto end = [&](const ckks_rows& r, int k, int rows) {
+            ckks_rows x = r;
+            if (k == 2) x.row = 1;
+            return end_of(x, a.batch, a.kv_heads, rows, k == 2 ? 1 : a.head_dim, k == 2 ? 4 : e);
+          };
+          need(disjoint(ins[i].data, end(ins[i], i, a.capacity), outs[o].data, end(outs[o], o, a.budget)),
+               "output overlaps input");
+        }
+    }
+    EvictParams p{a.k_cache, a.v_cache, a.acc,      a.k_out,    a.v_out,    a.acc_out, a.lens, a.index,
+                  a.lens_out, a.batch,  a.kv_heads, a.head_dim, a.capacity, a.budget,  a.recent};
+    const bool wide = wide_rows(a.k_out, a.batch, a.kv_heads, a.budget, a.head_dim, e) &&
+                      wide_rows(a.v_out, a.batch, a.kv_heads, a.budget, a.head_dim, e) &&
+                      (a.capacity == 0 || (wide_rows(a.k_cache, a.batch, a.kv_heads, a.capacity, a.head_dim, e) &&
+                                           wide_rows(a.v_cache, a.batch, a.kv_heads, a.capacity, a.head_dim, e)));
+    OnDevice dev(c);
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    const int heads = a.batch * a.kv_heads;
+    ProfScope ps(c, "draft_evict", heads * (4.0 * a.capacity + a.budget * (4.0 * e * a.head_dim + 8.0)), st);
+    select_kernel<<<heads, kSelThreads, 0, st>>>(p);
+    CKKS_CUDA(cudaGetLastError());
+    by_piece(e, wide, [&](auto t, auto v) {
+      const long long pieces = (long long)a.budget * a.head_dim * e / (long long)sizeof(v);
+      const long long most = std::max(1ll, 16ll * c.sms / heads);
+      const unsigned y = (unsigned)std::min({(pieces + 255) / 256, most, 65535ll});
+      gather_kernel<decltype(t), decltype(v)><<<dim3(heads, y), 256, 0, st>>>(p);
+    });
+    CKKS_CUDA(cudaGetLastError());
+  });
+}

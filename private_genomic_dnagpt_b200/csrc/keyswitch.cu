@@ -1050,15 +1050,23 @@ void launch_ks_inner_bulk(const Context& c, bool multi, dim3 grid, const KsBatch
 
 }  // namespace
 
-unsigned int take_device_faults(const Context& c) {
-  unsigned int v = 0;
-  CKKS_CUDA(cudaMemcpyAsync(&v, c.d_faults, sizeof(v), cudaMemcpyDeviceToHost, c.stream));
+static __global__ void take_kernel(unsigned int* counter, unsigned int n) { atomicSub(counter, n); }
+
+unsigned int take_device_faults(const Context& c, unsigned int* refused_commits) {
+  unsigned int v[2] = {0, 0};
+  const int n = refused_commits ? 2 : 1;
+  CKKS_CUDA(cudaMemcpyAsync(v, c.d_faults, n * sizeof(unsigned int), cudaMemcpyDeviceToHost, c.stream));
   CKKS_CUDA(cudaStreamSynchronize(c.stream));
-  if (v) {
-    CKKS_CUDA(cudaMemsetAsync(c.d_faults, 0, sizeof(unsigned int), c.stream));
+  // what is reported is subtracted, so that a count added meanwhile on
+  // another stream stays for the next report; a fault is reported alone
+  const int k = v[0] ? 0 : 1;
+  if (v[k]) {
+    take_kernel<<<1, 1, 0, c.stream>>>(c.d_faults + k, v[k]);
+    CKKS_CUDA(cudaGetLastError());
     CKKS_CUDA(cudaStreamSynchronize(c.stream));
   }
-  return v;
+  if (refused_commits) *refused_commits = k ? v[1] : 0;
+  return v[0];
 }
 
 void bulk_wait_probe(const Context& c, const uint64_t* src, uint64_t* dst, bool starve, cudaStream_t st) {
