@@ -13,6 +13,7 @@
 #include <cmath>
 
 #include "draft.hpp"
+#include "tcgen.cuh"
 
 namespace ckks {
 namespace draft {
@@ -272,6 +273,491 @@ __global__ void __launch_bounds__(kThreads) join_kernel(AttnParams p) {
     p.lse[((size_t)b * p.nodes + node) * p.kv_heads * p.group + qh] = l != 0.0f ? kLn2 * (m + log2f(l)) : -INFINITY;
 }
 
+// Adds to one finished row the new keys whose values are not finite, which
+// the product left out so that they do not reach the rows that may not see
+// them: what they add is infinite or no number, unless their weight is 0.
+template <typename T>
+__device__ __noinline__ void add_spoiled(const AttnParams& p, int b, int h, int node, int qh, unsigned long long which,
+                                         float m, float inv, T* out) {
+  const T* q = static_cast<const T*>(p.q.data) + b * p.q.batch + qh * p.q.head + node * p.q.row;
+  for (; which; which &= which - 1) {
+    const int j = __ffsll((long long)which) - 1;
+    const T* k = static_cast<const T*>(p.kn.data) + b * p.kn.batch + h * p.kn.head + j * p.kn.row;
+    const T* v = static_cast<const T*>(p.vn.data) + b * p.vn.batch + h * p.vn.head + j * p.vn.row;
+    float s = 0.0f;
+    for (int d = 0; d < p.head_dim; ++d) s = fmaf(to_f32(q[d]), to_f32(k[d]), s);
+    const float w = exp2f(s * (p.scale * kLog2e) - m) * inv;
+    if (w == 0.0f) continue;
+    for (int d = 0; d < p.head_dim; ++d) out[d] = from_f32<T>(fmaf(w, to_f32(v[d]), to_f32(out[d])));
+  }
+}
+
+// ---- 16-bit types: tensor cores -------------------------------------------------
+// The rows of one key/value head (nodes x query heads on it) are the M = 128
+// rows of a tile; a unit of work is (sequence, head, 128 rows), and its keys
+// are tiles of 128: ceil(len / 128) of the cache, then one with the new keys.
+// Scores S = Q K^T go to tensor memory; each row belongs to one thread, which
+// takes its 128 scores into registers, keeps the running maximum and sum, and
+// puts the weights back as the 16-bit A operand of O += P V, O staying in
+// tensor memory.  Both products are issued by one thread; K and V arrive by
+// tiled copies in a ring of slots.  Two CTAs share an SM, so one's products
+// and copies run under the other's exponentials.
+//
+// The lengths are known on the device only, so the CTAs of one wave divide
+// the list of all units' tiles evenly: a CTA may finish one unit, take some
+// whole ones and begin another.  A unit that more than one CTA has part of
+// leaves (m, l, O) in the workspace for the second kernel.
+//
+// A row's reference point m follows the maximum only when that has grown by
+// more than 2^8 (the weights then stay below 2^8, far inside 16-bit range):
+// O is seldom rescaled.
+constexpr int kM = 128, kKeys = 128, kTcThreads = 192, kTmemCols = 256;
+constexpr uint32_t kPanel = 128 * 128;  // 128 rows x 64 elements
+constexpr float kSlack = 8.0f;
+
+struct TileMaps {
+  CUtensorMap kc, vc, kn, vn;
+};
+
+// the place of tile `w` of the list: sequence, unit within it, tile within it
+struct Cursor {
+  int b, unit, tile, tiles;
+};
+
+__device__ __forceinline__ int tiles_of(const AttnParams& p, int b) { return (length_of(p, b) + kKeys - 1) / kKeys + 1; }
+
+// tiles of one unit of every sequence, summed; by a whole warp
+__device__ __forceinline__ long long tile_sum(const AttnParams& p) {
+  long long s = 0;
+  for (int b = threadIdx.x & 31; b < p.batch; b += 32) s += tiles_of(p, b);
+#pragma unroll
+  for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  return s;
+}
+
+// by a whole warp
+__device__ __forceinline__ Cursor find_tile(const AttnParams& p, int units, long long w) {
+  const int lane = threadIdx.x & 31;
+  long long before = 0;
+  for (int b0 = 0;; b0 += 32) {
+    const int t = b0 + lane < p.batch ? tiles_of(p, b0 + lane) : 0;
+    long long sum = (long long)t * units;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long y = __shfl_up_sync(0xffffffffu, sum, o);
+      if (lane >= o) sum += y;
+    }
+    const uint32_t past = __ballot_sync(0xffffffffu, before + sum > w);
+    if (past || b0 + 32 >= p.batch) {
+      const int k = past ? __ffs(past) - 1 : 31;
+      const int tk = __shfl_sync(0xffffffffu, t, k);
+      const long long start = before + __shfl_sync(0xffffffffu, sum, k) - (long long)tk * units;
+      const long long off = w - start;
+      return {b0 + k, tk ? (int)(off / tk) : 0, tk ? (int)(off % tk) : 0, tk};
+    }
+    before += __shfl_sync(0xffffffffu, sum, 31);
+  }
+}
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  } else {
+    const __half2 v = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
+}
+
+// any of eight 16-bit elements infinite or NaN
+template <typename T>
+__device__ __forceinline__ bool not_finite(uint4 v) {
+  constexpr uint32_t e = std::is_same_v<T, __nv_bfloat16> ? 0x7F80u : 0x7C00u;
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+  bool bad = false;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) bad = bad || (w[k] & e) == e || ((w[k] >> 16) & e) == e;
+  return bad;
+}
+
+template <int PANELS>
+struct TcShape {
+  static constexpr int kSlots = PANELS == 1 ? 5 : 2;
+  static constexpr uint32_t kTileBytes = PANELS * kPanel;
+  static constexpr size_t kSmem = 1024 + (size_t)(1 + kSlots) * kTileBytes;
+};
+
+template <typename T, int PANELS>
+__global__ void __launch_bounds__(kTcThreads, 2)
+    attend_tc_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ TileMaps maps, float sign, float c,
+                     unsigned int* __restrict__ faults) {
+  using S = TcShape<PANELS>;
+  constexpr int DP = 64 * PANELS, NS = S::kSlots;
+  constexpr bool kBf = std::is_same_v<T, __nv_bfloat16>;
+  extern __shared__ uint8_t raw[];
+  __shared__ alignas(8) uint64_t s_bar[2 * NS + 4];
+  __shared__ uint32_t s_tmem;
+  __shared__ unsigned long long s_spoiled;  // new keys whose values are not finite
+  __shared__ uint64_t s_mask[4][kMaxNodes];
+  __shared__ int s_jump[4][kMaxNodes];
+  const uint32_t base = (smem_addr(raw) + 1023u) & ~1023u;
+  uint8_t* const smem = raw + (base - smem_addr(raw));
+  const uint32_t sq = base, ring = base + S::kTileBytes;
+  const uint32_t bars = smem_addr(s_bar);
+  auto full = [&](int s) { return bars + 8 * s; };
+  auto empty = [&](int s) { return bars + 8 * (NS + s); };
+  const uint32_t q_ready = bars + 16 * NS, s_full = q_ready + 8, p_ready = q_ready + 16, o_full = q_ready + 24;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int rows = p.nodes * p.group, tiles_r = (rows + kM - 1) / kM, units = p.kv_heads * tiles_r;
+  const int warps = min(4, (min(rows, kM) + 31) / 32);  // softmax warps that have rows
+  const int D = p.head_dim;
+  if (tid == 0) {
+    for (int s = 0; s < NS; ++s) {
+      mbar_init(full(s), 1);
+      mbar_init(empty(s), 1);
+    }
+    mbar_init(q_ready, warps);
+    mbar_init(s_full, 1);
+    mbar_init(p_ready, warps);
+    mbar_init(o_full, 1);
+  }
+  if (warp == 5) tmem_alloc(smem_addr(&s_tmem), kTmemCols);
+  tmem_fence_before();
+  __syncthreads();
+  tmem_fence_after();
+  const uint32_t tmem = s_tmem;
+  const uint32_t t_s = tmem, t_o = tmem + 128;
+  // this CTA's tiles [w0, w1) of the list
+  const long long W = tile_sum(p) * units;
+  const long long w0 = W * blockIdx.x / gridDim.x, w1 = W * (blockIdx.x + 1) / gridDim.x;
+  bool fine = true;  // no wait gave up
+  if (w0 < w1) {
+    Cursor at = find_tile(p, units, w0);
+    auto next_unit = [&] {
+      at.tile = 0;
+      if (++at.unit == units) {
+        at.unit = 0;
+        at.tiles = ++at.b < p.batch ? tiles_of(p, at.b) : 1;
+      }
+    };
+    if (warp == 4) {
+      // ---- copies
+      if (lane == 0) {
+        tile_prefetch(&maps.kc);
+        tile_prefetch(&maps.vc);
+        int k = 0;  // copies issued
+        for (long long w = w0; w < w1 && fine;) {
+          const int h = at.unit / tiles_r;
+          for (; at.tile < at.tiles && w < w1 && fine; ++at.tile, ++w) {
+            const bool tree = at.tile == at.tiles - 1;
+#pragma unroll 1
+            for (int kv = 0; kv < 2; ++kv, ++k) {
+              const int s = k % NS;
+              if (k >= NS && !mbar_wait_bounded(empty(s), ((k / NS) - 1) & 1)) {
+                fine = false;
+                break;
+              }
+              mbar_expect_tx(full(s), S::kTileBytes);
+              const CUtensorMap* m = tree ? (kv ? &maps.vn : &maps.kn) : (kv ? &maps.vc : &maps.kc);
+              const int y = tree ? 0 : at.tile * kKeys;
+#pragma unroll
+              for (int x = 0; x < PANELS; ++x)
+                tile_load(ring + s * S::kTileBytes + x * kPanel, m, 64 * x, y, h, at.b, full(s));
+            }
+          }
+          next_unit();
+        }
+        // copies still in flight land before the CTA ends
+        for (int j = k > NS ? k - NS : 0; j < k; ++j) fine = mbar_wait_bounded(full(j % NS), (j / NS) & 1) && fine;
+      }
+    } else if (warp == 5) {
+      // ---- products
+      if (lane == 0) {
+        constexpr uint32_t word_s = mma_word(kBf, kM, kKeys, false), word_o = mma_word(kBf, kM, DP, true);
+        int k = 0, t = 0, u = 0;
+        for (long long w = w0; w < w1 && fine; ++u) {
+          fine = mbar_wait_bounded(q_ready, u & 1);
+          bool first = true;
+          for (; at.tile < at.tiles && w < w1 && fine; ++at.tile, ++w, ++t) {
+            const int sk = k % NS;
+            if (!(fine = mbar_wait_bounded(full(sk), (k / NS) & 1))) break;
+            tmem_fence_after();
+            const uint32_t kb = ring + sk * S::kTileBytes;
+#pragma unroll
+            for (int i = 0; i < DP / 16; ++i) {
+              const uint32_t off = (i / 4) * kPanel + (i % 4) * 32;
+              mma_smem(t_s, smem_operand(sq + off, 16), smem_operand(kb + off, 16), word_s, i > 0);
+            }
+            mma_commit(empty(sk));
+            mma_commit(s_full);
+            ++k;
+            const int sv = k % NS;
+            if (!(fine = mbar_wait_bounded(full(sv), (k / NS) & 1) && mbar_wait_bounded(p_ready, t & 1))) break;
+            tmem_fence_after();
+            const uint32_t vb = ring + sv * S::kTileBytes;
+#pragma unroll
+            for (int i = 0; i < kKeys / 16; ++i)
+              mma_tmem(t_o, t_s + 8 * i, smem_operand(vb + 2048 * i, kPanel), word_o, i > 0 || !first);
+            mma_commit(empty(sv));
+            ++k;
+            first = false;
+          }
+          if (fine) mma_commit(o_full);
+          next_unit();
+        }
+      }
+    } else if (warp < warps) {
+      // ---- softmax, one row per thread
+      const uint32_t lanes = (uint32_t)(warp * 32) << 16;
+      int t = 0, u = 0, k = 1, masks_of = -1;  // k: the copy that brings the tile's values
+      for (long long w = w0; w < w1 && fine; ++u) {
+        const int b = at.b, h = at.unit / tiles_r, row = at.unit % tiles_r * kM + tid;
+        const bool mine = row < rows;
+        const int node = row / p.group, qh = h * p.group + row % p.group;
+        if (masks_of != b) {
+          tree_masks(p.parents + (size_t)b * p.nodes, p.nodes, s_mask[warp], s_jump[warp]);
+          masks_of = b;
+        }
+        const uint64_t mask = mine ? s_mask[warp][node] : 0ull;
+        {
+          const T* src = static_cast<const T*>(p.q.data) + b * p.q.batch + qh * p.q.head + node * p.q.row;
+          const uint32_t flip = sign < 0.0f ? 0x80008000u : 0u;  // a negative scale's sign goes to q
+#pragma unroll
+          for (int i = 0; i < DP / 8; ++i) {
+            uint4 v = make_uint4(0, 0, 0, 0);
+            if (mine && 8 * i < D) v = *reinterpret_cast<const uint4*>(src + 8 * i);
+            v.x ^= flip, v.y ^= flip, v.z ^= flip, v.w ^= flip;
+            *reinterpret_cast<uint4*>(smem + (i / 8) * kPanel + tid * 128 + (((i % 8) ^ (tid & 7)) << 4)) = v;
+          }
+        }
+        smem_fence_async();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(q_ready);
+        const int len = length_of(p, b);
+        const int tile0 = at.tile;
+        float m = -INFINITY, l = 0.0f;
+        unsigned long long spoiled = 0ull;
+        for (; at.tile < at.tiles && w < w1; ++at.tile, ++w, ++t, k += 2) {
+          if (!(fine = mbar_wait_bounded(s_full, t & 1))) break;
+          tmem_fence_after();
+          const bool tree = at.tile == at.tiles - 1;
+          const int nk = tree ? p.nodes : min(kKeys, len - at.tile * kKeys);
+          // the values of keys that no row sees are taken out of the product
+          if (tree || nk < kKeys) {
+            if (!(fine = mbar_wait_bounded(full(k % NS), (k / NS) & 1))) break;
+            uint8_t* vs = smem + S::kTileBytes + (k % NS) * S::kTileBytes;
+            if (tree) {
+              if (tid == 0) s_spoiled = 0ull;
+              asm volatile("bar.sync 1, %0;" ::"r"(32 * warps) : "memory");
+              for (int r = tid; r < p.nodes; r += 32 * warps) {
+                bool out = s_mask[warp][r] == 0ull;
+                if (!out) {
+                  bool bad = false;
+                  for (int i = 0; i < DP / 8; ++i)
+                    bad = bad || not_finite<T>(*reinterpret_cast<const uint4*>(
+                                     vs + (i / 8) * kPanel + r * 128 + (((i % 8) ^ (r & 7)) << 4)));
+                  if (bad) atomicOr(&s_spoiled, 1ull << r);
+                  out = bad;
+                }
+                if (out)
+                  for (int i = 0; i < DP / 8; ++i)
+                    *reinterpret_cast<uint4*>(vs + (i / 8) * kPanel + r * 128 + ((i % 8) << 4)) = make_uint4(0, 0, 0, 0);
+              }
+              asm volatile("bar.sync 1, %0;" ::"r"(32 * warps) : "memory");
+              spoiled = s_spoiled;
+            } else {
+              for (int r = nk + tid; r < kKeys; r += 32 * warps)
+                for (int i = 0; i < DP / 8; ++i)
+                  *reinterpret_cast<uint4*>(vs + (i / 8) * kPanel + r * 128 + ((i % 8) << 4)) = make_uint4(0, 0, 0, 0);
+            }
+            smem_fence_async();
+          }
+          uint32_t x[kKeys];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) tmem_load32(t_s + lanes + 32 * i, x + 32 * i);
+          tmem_wait_load();
+          float mx = -INFINITY;
+          if (tree) {
+#pragma unroll
+            for (int i = 0; i < kKeys; ++i)
+              if (i >= kMaxNodes || !(mask >> (i & 63) & 1)) x[i] = __float_as_uint(-INFINITY);
+          } else if (nk < kKeys) {
+#pragma unroll
+            for (int i = 0; i < kKeys; ++i)
+              if (i >= nk) x[i] = __float_as_uint(-INFINITY);
+          }
+#pragma unroll
+          for (int i = 0; i < kKeys; ++i) mx = fmaxf(mx, __uint_as_float(x[i]));
+          const float top = mx == -INFINITY ? mx : mx * c;
+          float f = 1.0f;
+          if (top > m + kSlack || m == -INFINITY) {
+            f = m == -INFINITY ? 0.0f : ex2(m - top);
+            m = top;
+            l *= f;
+          }
+          if (at.tile > tile0 && __any_sync(0xffffffffu, f != 1.0f)) {
+            // the sums so far, on the new reference point
+#pragma unroll 1
+            for (int i = 0; i < DP / 32; ++i) {
+              uint32_t o[32];
+              tmem_load32(t_o + lanes + 32 * i, o);
+              tmem_wait_load();
+#pragma unroll
+              for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
+              tmem_store32(t_o + lanes + 32 * i, o);
+            }
+          }
+          const float ref = m == -INFINITY ? 0.0f : m;
+          float sum = 0.0f;
+#pragma unroll
+          for (int i = 0; i < kKeys; i += 2) {
+            float e0 = ex2(fmaf(__uint_as_float(x[i]), c, -ref)), e1 = ex2(fmaf(__uint_as_float(x[i + 1]), c, -ref));
+            if (c == 0.0f) {  // 0 times -inf is no number
+              if (__uint_as_float(x[i]) == -INFINITY) e0 = 0.0f;
+              if (__uint_as_float(x[i + 1]) == -INFINITY) e1 = 0.0f;
+            }
+            sum += e0 + e1;
+            x[i / 2] = pack2<T>(e0, e1);
+          }
+          l += sum;
+          tmem_store32(t_s + lanes, x);
+          tmem_store32(t_s + lanes + 32, x + 32);
+          tmem_wait_store();
+          tmem_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(p_ready);
+        }
+        if (!fine || !(fine = mbar_wait_bounded(o_full, u & 1))) break;
+        tmem_fence_after();
+        const bool whole = tile0 == 0 && at.tile == at.tiles;
+        const bool seen = mask != 0ull;  // a padding node's row is empty
+        if (whole) {
+          const float inv = l != 0.0f && seen ? 1.0f / l : 0.0f;
+          T* o = mine ? out_row<T>(p, b, node, qh) : nullptr;
+          const unsigned long long hurt = spoiled & mask;
+          for (int i = 0; i < DP / 32; ++i) {
+            uint32_t v[32];
+            tmem_load32(t_o + lanes + 32 * i, v);
+            tmem_wait_load();
+#pragma unroll
+            for (int j = 0; j < 32; j += 8)
+              if (mine && 32 * i + j < D) {
+                float y[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) y[e] = seen ? __uint_as_float(v[j + e]) * inv : 0.0f;
+                *reinterpret_cast<uint4*>(o + 32 * i + j) =
+                    make_uint4(pack2<T>(y[0], y[1]), pack2<T>(y[2], y[3]), pack2<T>(y[4], y[5]), pack2<T>(y[6], y[7]));
+              }
+          }
+          if (mine && hurt) add_spoiled<T>(p, b, h, node, qh, hurt, m, inv, o);
+          if (mine)
+            p.lse[((size_t)b * p.nodes + node) * p.kv_heads * p.group + qh] =
+                l != 0.0f && seen ? kLn2 * (m + log2f(l)) : -INFINITY;
+        } else {
+          // part of a unit: slot 1 holds a unit's beginning, slot 0 what follows
+          float* o = p.part + ((size_t)(2 * blockIdx.x + (tile0 == 0 ? 1 : 0)) * min(rows, kM) + tid) * (DP + 4);
+          for (int i = 0; i < DP / 32; ++i) {
+            uint32_t v[32];
+            tmem_load32(t_o + lanes + 32 * i, v);
+            tmem_wait_load();
+#pragma unroll
+            for (int j = 0; j < 32; j += 4)
+              if (mine) *reinterpret_cast<uint4*>(o + 32 * i + j) = make_uint4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+          }
+          if (mine) {
+            *reinterpret_cast<float4*>(o + DP) =
+                make_float4(m, l, __uint_as_float((uint32_t)spoiled), __uint_as_float((uint32_t)(spoiled >> 32)));
+          }
+        }
+        tmem_fence_before();
+        next_unit();
+      }
+    }
+  }
+  if (!fine && (warp < 4 || lane == 0)) atomicAdd(faults, 1u);
+  tmem_fence_before();
+  __syncthreads();
+  if (warp == 5) {
+    __syncwarp();
+    tmem_free(tmem, kTmemCols);
+  }
+}
+
+// joins the parts of the units that several CTAs share; a warp per row
+template <typename T, int PANELS>
+__global__ void __launch_bounds__(256) join_tc_kernel(const __grid_constant__ AttnParams p, int ctas) {
+  constexpr int DP = 64 * PANELS;
+  __shared__ uint64_t s_mask[8][kMaxNodes];
+  __shared__ int s_jump[8][kMaxNodes];
+  CKKS_PDL_ENTRY();
+  const int rows = p.nodes * p.group, tiles_r = (rows + kM - 1) / kM, units = p.kv_heads * tiles_r;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int per = (rows + 7) / 8;  // CTAs of a (sequence, head)
+  const int bh = blockIdx.x / per, row = blockIdx.x % per * 8 + warp;
+  const int b = bh / p.kv_heads, h = bh % p.kv_heads;
+  if (row >= rows) return;
+  const int unit = h * tiles_r + row / kM, r = row % kM;
+  // this unit's tiles [u0, u1) of the list
+  long long before = 0, all = 0;
+  for (int i = lane; i < p.batch; i += 32) {
+    const int t = tiles_of(p, i);
+    all += t;
+    if (i < b) before += t;
+  }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) {
+    all += __shfl_xor_sync(0xffffffffu, all, o);
+    before += __shfl_xor_sync(0xffffffffu, before, o);
+  }
+  const int tiles = tiles_of(p, b);
+  const long long W = all * units, u0 = before * units + (long long)unit * tiles, u1 = u0 + tiles;
+  const int c0 = (int)((ctas * (u0 + 1) - 1) / W), c1 = (int)((ctas * u1 - 1) / W);
+  if (c0 == c1) return;
+  tree_masks(p.parents + (size_t)b * p.nodes, p.nodes, s_mask[warp], s_jump[warp]);
+  const int node = row / p.group, qh = h * p.group + row % p.group;
+  const uint64_t mask = s_mask[warp][node];
+  const int stride = min(rows, kM);
+  auto part = [&](int i) { return p.part + ((size_t)(2 * i + (i == c0 ? 1 : 0)) * stride + r) * (DP + 4); };
+  float m = -INFINITY;
+  for (int i = c0 + lane; i <= c1; i += 32) m = fmaxf(m, part(i)[DP]);
+#pragma unroll
+  for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  const float ref = m == -INFINITY ? 0.0f : m;
+  float l = 0.0f, x[2 * PANELS];
+  unsigned long long spoiled = 0ull;
+#pragma unroll
+  for (int j = 0; j < 2 * PANELS; ++j) x[j] = 0.0f;
+#pragma unroll 4
+  for (int i = c0; i <= c1; ++i) {
+    const float* o = part(i);
+    const float4 e = *reinterpret_cast<const float4*>(o + DP);
+    const float f = exp2f(e.x - ref);
+    l = fmaf(e.y, f, l);
+    spoiled |= (unsigned long long)__float_as_uint(e.z) | (unsigned long long)__float_as_uint(e.w) << 32;
+#pragma unroll
+    for (int j = 0; j < 2 * PANELS; ++j) x[j] = fmaf(o[lane + 32 * j], f, x[j]);
+  }
+  const bool seen = mask != 0ull;
+  const float inv = l != 0.0f && seen ? 1.0f / l : 0.0f;
+  T* o = out_row<T>(p, b, node, qh);
+#pragma unroll
+  for (int j = 0; j < 2 * PANELS; ++j)
+    if (lane + 32 * j < p.head_dim) o[lane + 32 * j] = from_f32<T>(seen ? x[j] * inv : 0.0f);
+  __syncwarp();
+  if (lane == 0) {
+    if (spoiled & mask) add_spoiled<T>(p, b, h, node, qh, spoiled & mask, m, inv, o);
+    p.lse[((size_t)b * p.nodes + node) * p.kv_heads * p.group + qh] =
+        l != 0.0f && seen ? kLn2 * (m + log2f(l)) : -INFINITY;
+  }
+}
+
 size_t attend_smem(int D) {
   const int D4 = (D + 3) & ~3;
   const size_t run = sizeof(float) * ((size_t)kTile * (D4 + 4) + kTile * D4 + kRows * D4 + kTile * kRows);
@@ -325,10 +811,97 @@ void check_shape(const ckks_draft_attention_args& a) {
   need((long long)a.batch * a.q_heads * a.nodes < (1ll << 31) - 1 && a.capacity < (1 << 30), "sizes too large");
 }
 
+// Tensor-core CTAs: two on each SM, but no fewer than four tiles of keys
+// each at the full capacity (a shorter part is all start-up), and one for
+// each unit where there are fewer units than that
+int tc_ctas(const Context& c, const ckks_draft_attention_args& a) {
+  const long long rows = (long long)a.nodes * (a.q_heads / a.kv_heads);
+  const long long units = (long long)a.batch * a.kv_heads * ((rows + kM - 1) / kM);
+  const long long tiles = units * ((a.capacity + kKeys - 1) / kKeys + 1), slots = 2ll * c.sms;
+  return (int)std::max(1ll, std::min(slots, std::max(tiles / 4, units)));
+}
+
+// one sequence and a CTA for each unit: no unit is shared
+bool tc_alone(const ckks_draft_attention_args& a, int ctas) {
+  const int rows = a.nodes * (a.q_heads / a.kv_heads);
+  return a.batch == 1 && ctas == a.kv_heads * ((rows + kM - 1) / kM);
+}
+
+bool tc_sizes(const ckks_draft_attention_args& a) {
+  return a.dtype != CKKS_FP32 && a.head_dim <= 128 && a.head_dim % 8 == 0;
+}
+
 size_t workspace_of(const Context& c, const ckks_draft_attention_args& a) {
+  if (a.batch == 0) return 0;
   const int s = split_count(c, a);
-  if (s == 1 || a.batch == 0) return 0;
-  return sizeof(float) * (size_t)a.batch * a.q_heads * a.nodes * s * (a.head_dim + 2);
+  size_t n = s == 1 ? 0 : (size_t)a.batch * a.q_heads * a.nodes * s * (a.head_dim + 2);
+  if (tc_sizes(a)) {
+    // tensors whose rows are not aligned pieces take the other kernel
+    const int g = tc_ctas(c, a), rows = std::min(kM, a.nodes * (a.q_heads / a.kv_heads));
+    if (!tc_alone(a, g)) n = std::max(n, (size_t)2 * g * rows * (a.head_dim <= 64 ? 64 + 4 : 128 + 4));
+  }
+  return sizeof(float) * n;
+}
+
+using EncodeTiled = decltype(&cuTensorMapEncodeTiled);
+EncodeTiled encode_tiled() {
+  static const EncodeTiled f = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult r;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &r) != cudaSuccess ||
+        r != cudaDriverEntryPointSuccess)
+      p = nullptr;
+    return reinterpret_cast<EncodeTiled>(p);
+  }();
+  return f;
+}
+
+// [batch][heads][rows][head_dim] in boxes of 128 rows x 64 elements; what a
+// box has outside the tensor reads as 0
+bool tile_map(CUtensorMap* m, const ckks_rows& r, int dtype, int batch, int heads, int rows, int head_dim) {
+  const EncodeTiled f = encode_tiled();
+  if (!f) return false;
+  auto bytes = [](int64_t s, int n) { return n > 1 ? (cuuint64_t)s * 2 : (cuuint64_t)16; };
+  const cuuint64_t dims[4] = {(cuuint64_t)head_dim, (cuuint64_t)rows, (cuuint64_t)heads, (cuuint64_t)batch};
+  const cuuint64_t strides[3] = {bytes(r.row, rows), bytes(r.head, heads), bytes(r.batch, batch)};
+  const cuuint32_t box[4] = {64, (cuuint32_t)kKeys, 1, 1}, ones[4] = {1, 1, 1, 1};
+  return f(m, dtype == CKKS_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, r.data, dims,
+           strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename T, int PANELS>
+void launch_tc(const Context& c, const ckks_draft_attention_args& a, const AttnParams& p, const TileMaps& maps,
+               cudaStream_t st) {
+  using S = TcShape<PANELS>;
+  auto* k = attend_tc_kernel<T, PANELS>;
+  CKKS_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::kSmem));
+  const int ctas = tc_ctas(c, a), rows = p.nodes * p.group;
+  const float factor = std::fabs(p.scale) * kLog2e;
+  k<<<ctas, kTcThreads, S::kSmem, st>>>(p, maps, p.scale < 0.0f ? -1.0f : 1.0f, factor, c.d_faults);
+  CKKS_CUDA(cudaGetLastError());
+  if (!tc_alone(a, ctas))
+    launch_pdl(join_tc_kernel<T, PANELS>, dim3((unsigned)(p.batch * p.kv_heads * ((rows + 7) / 8))), dim3(256), 0, st, p,
+               ctas);
+}
+
+template <typename T>
+bool run_tc(const Context& c, const ckks_draft_attention_args& a, const AttnParams& p, cudaStream_t st) {
+  TileMaps m;
+  if (!tile_map(&m.kn, a.k_new, a.dtype, a.batch, a.kv_heads, a.nodes, a.head_dim) ||
+      !tile_map(&m.vn, a.v_new, a.dtype, a.batch, a.kv_heads, a.nodes, a.head_dim))
+    return false;
+  if (a.capacity == 0) {
+    m.kc = m.kn, m.vc = m.vn;  // not read
+  } else if (!tile_map(&m.kc, a.k_cache, a.dtype, a.batch, a.kv_heads, a.capacity, a.head_dim) ||
+             !tile_map(&m.vc, a.v_cache, a.dtype, a.batch, a.kv_heads, a.capacity, a.head_dim)) {
+    return false;
+  }
+  if (a.head_dim <= 64)
+    launch_tc<T, 1>(c, a, p, m, st);
+  else
+    launch_tc<T, 2>(c, a, p, m, st);
+  return true;
 }
 
 }  // namespace
@@ -355,7 +928,7 @@ extern "C" int ckks_draft_attention(ckks_ctx* ctx, const ckks_draft_attention_ar
     need(args != nullptr, "null argument");
     const ckks_draft_attention_args& a = *args;
     check_shape(a);
-    need(std::isfinite(a.scale), "scale is not finite");
+    need(std::isfinite((float)a.scale), "scale is not finite");
     if (a.batch == 0) return;
     const int e = element_bytes(a.dtype);
     check_rows(a.q, e, "q");
@@ -379,6 +952,7 @@ extern "C" int ckks_draft_attention(ckks_ctx* ctx, const ckks_draft_attention_ar
     p.nodes = a.nodes, p.capacity = a.capacity, p.scale = (float)a.scale;
     p.splits = split_count(c, a);
     p.wide = wide_rows(a.q, a.batch, a.q_heads, a.nodes, a.head_dim, e) &&
+             wide_rows(a.out, a.batch, a.q_heads, a.nodes, a.head_dim, e) &&
              wide_rows(a.k_new, a.batch, a.kv_heads, a.nodes, a.head_dim, e) &&
              wide_rows(a.v_new, a.batch, a.kv_heads, a.nodes, a.head_dim, e) &&
              (a.capacity == 0 || (wide_rows(a.k_cache, a.batch, a.kv_heads, a.capacity, a.head_dim, e) &&
@@ -387,6 +961,8 @@ extern "C" int ckks_draft_attention(ckks_ctx* ctx, const ckks_draft_attention_ar
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     const double bytes = 2.0 * e * a.batch * a.kv_heads * a.capacity * a.head_dim;
     ProfScope ps(c, "draft_attention", bytes, st);
+    if (p.wide && tc_sizes(a) && (a.dtype == CKKS_BF16 ? run_tc<__nv_bfloat16>(c, a, p, st) : run_tc<__half>(c, a, p, st)))
+      return;
     if (a.dtype == CKKS_BF16)
       run_attend<__nv_bfloat16>(p, st);
     else if (a.dtype == CKKS_FP16)
