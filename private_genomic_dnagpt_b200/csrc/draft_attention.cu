@@ -296,22 +296,33 @@ __device__ __noinline__ void add_spoiled(const AttnParams& p, int b, int h, int 
 // The rows of one key/value head (nodes x query heads on it) are the M = 128
 // rows of a tile; a unit of work is (sequence, head, 128 rows), and its keys
 // are tiles of 128: ceil(len / 128) of the cache, then one with the new keys.
-// Scores S = Q K^T go to tensor memory; each row belongs to one thread, which
-// takes its 128 scores into registers, keeps the running maximum and sum, and
-// puts the weights back as the 16-bit A operand of O += P V, O staying in
-// tensor memory.  Both products are issued by one thread; K and V arrive by
-// tiled copies in a ring of slots.  Two CTAs share an SM, so one's products
-// and copies run under the other's exponentials.
+// Scores S = Q K^T go to tensor memory; a thread takes the scores of its row
+// into registers, keeps the running maximum and sum, and puts the weights
+// back as the 16-bit A operand of O += P V, O staying in tensor memory.
 //
-// The lengths are known on the device only, so the CTAs of one wave divide
-// the list of all units' tiles evenly: a CTA may finish one unit, take some
-// whole ones and begin another.  A unit that more than one CTA has part of
-// leaves (m, l, O) in the workspace for the second kernel.
+// One CTA per SM: a thread that copies K and V into a ring of slots (tiled
+// copies), a thread that issues both products, and two groups of four softmax
+// warps that take the unit's tiles in turn, each with its own S and O: one
+// group's products and copies run under the other's exponentials.  K of the
+// next tile comes before V of this one, in the order of the products.
+//
+// With 64 rows or fewer the rows are repeated in the tile (COPIES times), and
+// a copy weighs only its share of a tile's keys, the others' weights being 0:
+// the products cost the same, and the exponentials spread over all warps.
+// The copies and the two groups are parts of the softmax like any split of
+// the keys; they are joined in shared memory when a unit is done.
+//
+// The lengths are known on the device only, so the CTAs divide the list of
+// all units' tiles evenly: a CTA may finish one unit, take some whole ones
+// and begin another.  A unit also counts as kUnitCost tiles for its start and
+// its end.  A unit that more than one CTA has part of leaves (m, l, O) in the
+// workspace for the second kernel.
 //
 // A row's reference point m follows the maximum only when that has grown by
 // more than 2^8 (the weights then stay below 2^8, far inside 16-bit range):
-// O is seldom rescaled.
-constexpr int kM = 128, kKeys = 128, kTcThreads = 192, kTmemCols = 256;
+// O is seldom rescaled.  Weights are rounded to the operands' type for the
+// second product; l sums them before that, in 32 bits.
+constexpr int kM = 128, kKeys = 128, kTcThreads = 320, kTmemCols = 512, kUnitCost = 2;
 constexpr uint32_t kPanel = 128 * 128;  // 128 rows x 64 elements
 constexpr float kSlack = 8.0f;
 
@@ -319,44 +330,56 @@ struct TileMaps {
   CUtensorMap kc, vc, kn, vn;
 };
 
-// the place of tile `w` of the list: sequence, unit within it, tile within it
-struct Cursor {
-  int b, unit, tile, tiles;
-};
-
 __device__ __forceinline__ int tiles_of(const AttnParams& p, int b) { return (length_of(p, b) + kKeys - 1) / kKeys + 1; }
 
-// tiles of one unit of every sequence, summed; by a whole warp
-__device__ __forceinline__ long long tile_sum(const AttnParams& p) {
-  long long s = 0;
-  for (int b = threadIdx.x & 31; b < p.batch; b += 32) s += tiles_of(p, b);
+// A place in the list: sequence, unit within it, tile within that (below 0:
+// the unit's start) and the unit's tiles
+struct Cursor {
+  int b, unit, tile, tiles;
+  __device__ __forceinline__ void next_unit(const AttnParams& p, int units) {
+    tile = -kUnitCost;
+    if (++unit == units) {
+      unit = 0;
+      tiles = ++b < p.batch ? tiles_of(p, b) : 1;
+    }
+  }
+};
+
+// entries of one unit of every sequence, summed; by a whole warp
+__device__ __forceinline__ int entry_sum(const AttnParams& p) {
+  int s = 0;
+  for (int b = threadIdx.x & 31; b < p.batch; b += 32) s += tiles_of(p, b) + kUnitCost;
 #pragma unroll
   for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
   return s;
 }
 
-// by a whole warp
-__device__ __forceinline__ Cursor find_tile(const AttnParams& p, int units, long long w) {
+// entry `w` of the list; by a whole warp
+__device__ __forceinline__ Cursor find_entry(const AttnParams& p, int units, int w) {
   const int lane = threadIdx.x & 31;
-  long long before = 0;
+  int before = 0;
   for (int b0 = 0;; b0 += 32) {
-    const int t = b0 + lane < p.batch ? tiles_of(p, b0 + lane) : 0;
-    long long sum = (long long)t * units;
+    const int t = b0 + lane < p.batch ? tiles_of(p, b0 + lane) + kUnitCost : 0;
+    int sum = t * units;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const long long y = __shfl_up_sync(0xffffffffu, sum, o);
+      const int y = __shfl_up_sync(0xffffffffu, sum, o);
       if (lane >= o) sum += y;
     }
     const uint32_t past = __ballot_sync(0xffffffffu, before + sum > w);
     if (past || b0 + 32 >= p.batch) {
       const int k = past ? __ffs(past) - 1 : 31;
-      const int tk = __shfl_sync(0xffffffffu, t, k);
-      const long long start = before + __shfl_sync(0xffffffffu, sum, k) - (long long)tk * units;
-      const long long off = w - start;
-      return {b0 + k, tk ? (int)(off / tk) : 0, tk ? (int)(off % tk) : 0, tk};
+      const int tk = max(1, __shfl_sync(0xffffffffu, t, k));
+      const int off = w - (before + __shfl_sync(0xffffffffu, sum, k) - tk * units);
+      return {b0 + k, off / tk, off % tk - kUnitCost, tk - kUnitCost};
     }
     before += __shfl_sync(0xffffffffu, sum, 31);
   }
+}
+
+// first entry of part i of n
+__device__ __forceinline__ int part_start(int entries, int i, int n) {
+  return entries / n * i + (int)((unsigned)(entries % n) * (unsigned)i / (unsigned)n);
 }
 
 __device__ __forceinline__ float ex2(float x) {
@@ -383,308 +406,376 @@ __device__ __forceinline__ bool not_finite(uint4 v) {
   const uint32_t w[4] = {v.x, v.y, v.z, v.w};
   bool bad = false;
 #pragma unroll
-  for (int k = 0; k < 4; ++k) bad = bad || (w[k] & e) == e || ((w[k] >> 16) & e) == e;
+  for (int k = 0; k < 4; ++k) bad |= (w[k] & e) == e || ((w[k] >> 16) & e) == e;
   return bad;
+}
+
+__device__ __forceinline__ void group_sync(int id, int threads) {
+  asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
 }
 
 template <int PANELS>
 struct TcShape {
-  static constexpr int kSlots = PANELS == 1 ? 5 : 2;
+  static constexpr int kSlots = PANELS == 1 ? 12 : 6;
   static constexpr uint32_t kTileBytes = PANELS * kPanel;
-  static constexpr size_t kSmem = 1024 + (size_t)(1 + kSlots) * kTileBytes;
+  // behind Q and the ring: (m, l) of every part of a row, ancestor masks, barriers, two words
+  static constexpr uint32_t kExtra = (1 + kSlots) * kTileBytes;
+  static constexpr size_t kSmem = kExtra + 2 * kM * sizeof(float2) + kMaxNodes * 8 + (2 * kSlots + 6) * 8 + 16;
 };
 
-template <typename T, int PANELS>
-__global__ void __launch_bounds__(kTcThreads, 2)
-    attend_tc_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ TileMaps maps, float sign, float c,
+template <typename T, int PANELS, int COPIES>
+__global__ void __launch_bounds__(kTcThreads, 1)
+    attend_tc_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ TileMaps maps, bool negative, float c,
                      unsigned int* __restrict__ faults) {
   using S = TcShape<PANELS>;
-  constexpr int DP = 64 * PANELS, NS = S::kSlots;
+  constexpr int DP = 64 * PANELS, NS = S::kSlots, KQ = kKeys / COPIES, CW = 16 * PANELS;
   constexpr bool kBf = std::is_same_v<T, __nv_bfloat16>;
-  extern __shared__ uint8_t raw[];
-  __shared__ alignas(8) uint64_t s_bar[2 * NS + 4];
-  __shared__ uint32_t s_tmem;
-  __shared__ unsigned long long s_spoiled;  // new keys whose values are not finite
-  __shared__ uint64_t s_mask[4][kMaxNodes];
-  __shared__ int s_jump[4][kMaxNodes];
-  const uint32_t base = (smem_addr(raw) + 1023u) & ~1023u;
-  uint8_t* const smem = raw + (base - smem_addr(raw));
-  const uint32_t sq = base, ring = base + S::kTileBytes;
-  const uint32_t bars = smem_addr(s_bar);
+  extern __shared__ __align__(1024) uint8_t smem[];
+  float2* const s_ml = reinterpret_cast<float2*>(smem + S::kExtra);  // [2][kM]
+  uint64_t* const s_mask = reinterpret_cast<uint64_t*>(s_ml + 2 * kM);
+  uint64_t* const s_bar = s_mask + kMaxNodes;
+  unsigned long long* const s_spoiled = reinterpret_cast<unsigned long long*>(s_bar + 2 * NS + 6);
+  uint32_t* const s_tmem = reinterpret_cast<uint32_t*>(s_spoiled + 1);
+  const uint32_t sq = smem_addr(smem), ring = sq + S::kTileBytes, bars = smem_addr(s_bar);
   auto full = [&](int s) { return bars + 8 * s; };
   auto empty = [&](int s) { return bars + 8 * (NS + s); };
-  const uint32_t q_ready = bars + 16 * NS, s_full = q_ready + 8, p_ready = q_ready + 16, o_full = q_ready + 24;
+  auto s_full = [&](int g) { return bars + 8 * (2 * NS + g); };
+  auto p_ready = [&](int g) { return bars + 8 * (2 * NS + 2 + g); };
+  const uint32_t q_ready = bars + 8 * (2 * NS + 4), o_full = q_ready + 8;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int rows = p.nodes * p.group, tiles_r = (rows + kM - 1) / kM, units = p.kv_heads * tiles_r;
-  const int warps = min(4, (min(rows, kM) + 31) / 32);  // softmax warps that have rows
-  const int D = p.head_dim;
+  asm volatile("griddepcontrol.launch_dependents;");
   if (tid == 0) {
     for (int s = 0; s < NS; ++s) {
       mbar_init(full(s), 1);
       mbar_init(empty(s), 1);
     }
-    mbar_init(q_ready, warps);
-    mbar_init(s_full, 1);
-    mbar_init(p_ready, warps);
+    for (int g = 0; g < 2; ++g) {
+      mbar_init(s_full(g), 1);
+      mbar_init(p_ready(g), 4);
+    }
+    mbar_init(q_ready, 1);
     mbar_init(o_full, 1);
+    *s_spoiled = 0ull;
   }
-  if (warp == 5) tmem_alloc(smem_addr(&s_tmem), kTmemCols);
+  if (warp == 9) tmem_alloc(smem_addr(s_tmem), kTmemCols);
+  // this CTA's entries [w0, w1) of the list
+  const int entries = entry_sum(p) * units;
+  const int w0 = part_start(entries, blockIdx.x, gridDim.x), w1 = part_start(entries, blockIdx.x + 1, gridDim.x);
+  Cursor at = find_entry(p, units, w0);
   tmem_fence_before();
   __syncthreads();
   tmem_fence_after();
-  const uint32_t tmem = s_tmem;
-  const uint32_t t_s = tmem, t_o = tmem + 128;
-  // this CTA's tiles [w0, w1) of the list
-  const long long W = tile_sum(p) * units;
-  const long long w0 = W * blockIdx.x / gridDim.x, w1 = W * (blockIdx.x + 1) / gridDim.x;
+  const uint32_t tmem = *s_tmem;  // S of both groups, then O of both
+  // the tiles of this CTA in the unit at `at`, from tile at.tile on; none
+  // where the CTA has only the unit's start
+  auto tiles_here = [&](int& w) {
+    const int skip = max(0, min(-at.tile, w1 - w));
+    at.tile += skip;
+    w += skip;
+    return max(0, min(at.tiles - at.tile, w1 - w));
+  };
   bool fine = true;  // no wait gave up
-  if (w0 < w1) {
-    Cursor at = find_tile(p, units, w0);
-    auto next_unit = [&] {
-      at.tile = 0;
-      if (++at.unit == units) {
-        at.unit = 0;
-        at.tiles = ++at.b < p.batch ? tiles_of(p, at.b) : 1;
-      }
-    };
-    if (warp == 4) {
-      // ---- copies
-      if (lane == 0) {
-        tile_prefetch(&maps.kc);
-        tile_prefetch(&maps.vc);
-        int k = 0;  // copies issued
-        for (long long w = w0; w < w1 && fine;) {
-          const int h = at.unit / tiles_r;
-          for (; at.tile < at.tiles && w < w1 && fine; ++at.tile, ++w) {
-            const bool tree = at.tile == at.tiles - 1;
-#pragma unroll 1
-            for (int kv = 0; kv < 2; ++kv, ++k) {
-              const int s = k % NS;
-              if (k >= NS && !mbar_wait_bounded(empty(s), ((k / NS) - 1) & 1)) {
-                fine = false;
-                break;
-              }
-              mbar_expect_tx(full(s), S::kTileBytes);
-              const CUtensorMap* m = tree ? (kv ? &maps.vn : &maps.kn) : (kv ? &maps.vc : &maps.kc);
-              const int y = tree ? 0 : at.tile * kKeys;
+  if (warp == 8) {
+    // ---- copies
+    if (lane == 0) {
+      tile_prefetch(&maps.kc);
+      tile_prefetch(&maps.vc);
+      int k = 0;  // copies issued
+      for (int w = w0; w < w1 && fine;) {
+        const int n = tiles_here(w), h = at.unit / tiles_r;
+        auto load = [&](int tile, bool value) {
+          const int s = k % NS;
+          if (k >= NS && !mbar_wait_short(empty(s), ((k / NS) - 1) & 1)) return fine = false;
+          const bool tree = tile == at.tiles - 1;
+          const CUtensorMap* m = tree ? (value ? &maps.vn : &maps.kn) : (value ? &maps.vc : &maps.kc);
+          mbar_expect_tx(full(s), S::kTileBytes);
 #pragma unroll
-              for (int x = 0; x < PANELS; ++x)
-                tile_load(ring + s * S::kTileBytes + x * kPanel, m, 64 * x, y, h, at.b, full(s));
-            }
-          }
-          next_unit();
+          for (int x = 0; x < PANELS; ++x)
+            tile_load(ring + s * S::kTileBytes + x * kPanel, m, 64 * x, tree ? 0 : tile * kKeys, h, at.b, full(s));
+          ++k;
+          return true;
+        };
+        if (n) load(at.tile, false);
+        for (int t = 0; t < n && fine; ++t) {
+          if (t + 1 < n && !load(at.tile + t + 1, false)) break;
+          load(at.tile + t, true);
         }
-        // copies still in flight land before the CTA ends
-        for (int j = k > NS ? k - NS : 0; j < k; ++j) fine = mbar_wait_bounded(full(j % NS), (j / NS) & 1) && fine;
+        w += n;
+        at.next_unit(p, units);
       }
-    } else if (warp == 5) {
-      // ---- products
-      if (lane == 0) {
-        constexpr uint32_t word_s = mma_word(kBf, kM, kKeys, false), word_o = mma_word(kBf, kM, DP, true);
-        int k = 0, t = 0, u = 0;
-        for (long long w = w0; w < w1 && fine; ++u) {
-          fine = mbar_wait_bounded(q_ready, u & 1);
-          bool first = true;
-          for (; at.tile < at.tiles && w < w1 && fine; ++at.tile, ++w, ++t) {
-            const int sk = k % NS;
-            if (!(fine = mbar_wait_bounded(full(sk), (k / NS) & 1))) break;
-            tmem_fence_after();
-            const uint32_t kb = ring + sk * S::kTileBytes;
+      // copies still in flight land before the CTA ends
+      for (int j = k > NS ? k - NS : 0; j < k; ++j) fine = mbar_wait_short(full(j % NS), (j / NS) & 1) && fine;
+    }
+  } else if (warp == 9) {
+    // ---- products
+    if (lane == 0) {
+      constexpr uint32_t word_s = mma_word(kBf, kM, kKeys, false), word_o = mma_word(kBf, kM, DP, true);
+      int k = 0, u = 0;
+      uint32_t phase = 0;  // bit g: parity of group g's next weights
+      for (int w = w0; w < w1 && fine;) {
+        const int n = tiles_here(w);
+        auto scores = [&](int g) {
+          const int s = k % NS;
+          if (!mbar_wait_short(full(s), (k / NS) & 1)) return fine = false;
+          tmem_fence_after();
+          const uint32_t kb = ring + s * S::kTileBytes;
 #pragma unroll
-            for (int i = 0; i < DP / 16; ++i) {
-              const uint32_t off = (i / 4) * kPanel + (i % 4) * 32;
-              mma_smem(t_s, smem_operand(sq + off, 16), smem_operand(kb + off, 16), word_s, i > 0);
-            }
-            mma_commit(empty(sk));
-            mma_commit(s_full);
-            ++k;
-            const int sv = k % NS;
-            if (!(fine = mbar_wait_bounded(full(sv), (k / NS) & 1) && mbar_wait_bounded(p_ready, t & 1))) break;
+          for (int i = 0; i < DP / 16; ++i) {
+            const uint32_t off = (i / 4) * kPanel + (i % 4) * 32;
+            mma_smem(tmem + 128 * g, smem_operand(sq + off, 16), smem_operand(kb + off, 16), word_s, i > 0);
+          }
+          mma_commit(empty(s));
+          mma_commit(s_full(g));
+          ++k;
+          return true;
+        };
+        if (n) {
+          fine = mbar_wait_short(q_ready, u++ & 1) && scores(0);
+          for (int t = 0; t < n && fine; ++t) {
+            if (t + 1 < n && !scores((t + 1) & 1)) break;
+            const int g = t & 1, s = k % NS;
+            if (!(fine = mbar_wait_short(full(s), (k / NS) & 1) && mbar_wait_short(p_ready(g), phase >> g & 1))) break;
+            phase ^= 1u << g;
             tmem_fence_after();
-            const uint32_t vb = ring + sv * S::kTileBytes;
+            const uint32_t vb = ring + s * S::kTileBytes;
 #pragma unroll
             for (int i = 0; i < kKeys / 16; ++i)
-              mma_tmem(t_o, t_s + 8 * i, smem_operand(vb + 2048 * i, kPanel), word_o, i > 0 || !first);
-            mma_commit(empty(sv));
+              mma_tmem(tmem + 256 + 128 * g, tmem + 128 * g + 8 * i, smem_operand(vb + 2048 * i, kPanel), word_o,
+                       i > 0 || t > 1);
+            mma_commit(empty(s));
             ++k;
-            first = false;
           }
           if (fine) mma_commit(o_full);
-          next_unit();
         }
-      }
-    } else if (warp < warps) {
-      // ---- softmax, one row per thread
-      const uint32_t lanes = (uint32_t)(warp * 32) << 16;
-      int t = 0, u = 0, k = 1, masks_of = -1;  // k: the copy that brings the tile's values
-      for (long long w = w0; w < w1 && fine; ++u) {
-        const int b = at.b, h = at.unit / tiles_r, row = at.unit % tiles_r * kM + tid;
-        const bool mine = row < rows;
-        const int node = row / p.group, qh = h * p.group + row % p.group;
-        if (masks_of != b) {
-          tree_masks(p.parents + (size_t)b * p.nodes, p.nodes, s_mask[warp], s_jump[warp]);
-          masks_of = b;
-        }
-        const uint64_t mask = mine ? s_mask[warp][node] : 0ull;
-        {
-          const T* src = static_cast<const T*>(p.q.data) + b * p.q.batch + qh * p.q.head + node * p.q.row;
-          const uint32_t flip = sign < 0.0f ? 0x80008000u : 0u;  // a negative scale's sign goes to q
-#pragma unroll
-          for (int i = 0; i < DP / 8; ++i) {
-            uint4 v = make_uint4(0, 0, 0, 0);
-            if (mine && 8 * i < D) v = *reinterpret_cast<const uint4*>(src + 8 * i);
-            v.x ^= flip, v.y ^= flip, v.z ^= flip, v.w ^= flip;
-            *reinterpret_cast<uint4*>(smem + (i / 8) * kPanel + tid * 128 + (((i % 8) ^ (tid & 7)) << 4)) = v;
-          }
-        }
-        smem_fence_async();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(q_ready);
-        const int len = length_of(p, b);
-        const int tile0 = at.tile;
-        float m = -INFINITY, l = 0.0f;
-        unsigned long long spoiled = 0ull;
-        for (; at.tile < at.tiles && w < w1; ++at.tile, ++w, ++t, k += 2) {
-          if (!(fine = mbar_wait_bounded(s_full, t & 1))) break;
-          tmem_fence_after();
-          const bool tree = at.tile == at.tiles - 1;
-          const int nk = tree ? p.nodes : min(kKeys, len - at.tile * kKeys);
-          // the values of keys that no row sees are taken out of the product
-          if (tree || nk < kKeys) {
-            if (!(fine = mbar_wait_bounded(full(k % NS), (k / NS) & 1))) break;
-            uint8_t* vs = smem + S::kTileBytes + (k % NS) * S::kTileBytes;
-            if (tree) {
-              if (tid == 0) s_spoiled = 0ull;
-              asm volatile("bar.sync 1, %0;" ::"r"(32 * warps) : "memory");
-              for (int r = tid; r < p.nodes; r += 32 * warps) {
-                bool out = s_mask[warp][r] == 0ull;
-                if (!out) {
-                  bool bad = false;
-                  for (int i = 0; i < DP / 8; ++i)
-                    bad = bad || not_finite<T>(*reinterpret_cast<const uint4*>(
-                                     vs + (i / 8) * kPanel + r * 128 + (((i % 8) ^ (r & 7)) << 4)));
-                  if (bad) atomicOr(&s_spoiled, 1ull << r);
-                  out = bad;
-                }
-                if (out)
-                  for (int i = 0; i < DP / 8; ++i)
-                    *reinterpret_cast<uint4*>(vs + (i / 8) * kPanel + r * 128 + ((i % 8) << 4)) = make_uint4(0, 0, 0, 0);
-              }
-              asm volatile("bar.sync 1, %0;" ::"r"(32 * warps) : "memory");
-              spoiled = s_spoiled;
-            } else {
-              for (int r = nk + tid; r < kKeys; r += 32 * warps)
-                for (int i = 0; i < DP / 8; ++i)
-                  *reinterpret_cast<uint4*>(vs + (i / 8) * kPanel + r * 128 + ((i % 8) << 4)) = make_uint4(0, 0, 0, 0);
-            }
-            smem_fence_async();
-          }
-          uint32_t x[kKeys];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) tmem_load32(t_s + lanes + 32 * i, x + 32 * i);
-          tmem_wait_load();
-          float mx = -INFINITY;
-          if (tree) {
-#pragma unroll
-            for (int i = 0; i < kKeys; ++i)
-              if (i >= kMaxNodes || !(mask >> (i & 63) & 1)) x[i] = __float_as_uint(-INFINITY);
-          } else if (nk < kKeys) {
-#pragma unroll
-            for (int i = 0; i < kKeys; ++i)
-              if (i >= nk) x[i] = __float_as_uint(-INFINITY);
-          }
-#pragma unroll
-          for (int i = 0; i < kKeys; ++i) mx = fmaxf(mx, __uint_as_float(x[i]));
-          const float top = mx == -INFINITY ? mx : mx * c;
-          float f = 1.0f;
-          if (top > m + kSlack || m == -INFINITY) {
-            f = m == -INFINITY ? 0.0f : ex2(m - top);
-            m = top;
-            l *= f;
-          }
-          if (at.tile > tile0 && __any_sync(0xffffffffu, f != 1.0f)) {
-            // the sums so far, on the new reference point
-#pragma unroll 1
-            for (int i = 0; i < DP / 32; ++i) {
-              uint32_t o[32];
-              tmem_load32(t_o + lanes + 32 * i, o);
-              tmem_wait_load();
-#pragma unroll
-              for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
-              tmem_store32(t_o + lanes + 32 * i, o);
-            }
-          }
-          const float ref = m == -INFINITY ? 0.0f : m;
-          float sum = 0.0f;
-#pragma unroll
-          for (int i = 0; i < kKeys; i += 2) {
-            float e0 = ex2(fmaf(__uint_as_float(x[i]), c, -ref)), e1 = ex2(fmaf(__uint_as_float(x[i + 1]), c, -ref));
-            if (c == 0.0f) {  // 0 times -inf is no number
-              if (__uint_as_float(x[i]) == -INFINITY) e0 = 0.0f;
-              if (__uint_as_float(x[i + 1]) == -INFINITY) e1 = 0.0f;
-            }
-            sum += e0 + e1;
-            x[i / 2] = pack2<T>(e0, e1);
-          }
-          l += sum;
-          tmem_store32(t_s + lanes, x);
-          tmem_store32(t_s + lanes + 32, x + 32);
-          tmem_wait_store();
-          tmem_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(p_ready);
-        }
-        if (!fine || !(fine = mbar_wait_bounded(o_full, u & 1))) break;
-        tmem_fence_after();
-        const bool whole = tile0 == 0 && at.tile == at.tiles;
-        const bool seen = mask != 0ull;  // a padding node's row is empty
-        if (whole) {
-          const float inv = l != 0.0f && seen ? 1.0f / l : 0.0f;
-          T* o = mine ? out_row<T>(p, b, node, qh) : nullptr;
-          const unsigned long long hurt = spoiled & mask;
-          for (int i = 0; i < DP / 32; ++i) {
-            uint32_t v[32];
-            tmem_load32(t_o + lanes + 32 * i, v);
-            tmem_wait_load();
-#pragma unroll
-            for (int j = 0; j < 32; j += 8)
-              if (mine && 32 * i + j < D) {
-                float y[8];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) y[e] = seen ? __uint_as_float(v[j + e]) * inv : 0.0f;
-                *reinterpret_cast<uint4*>(o + 32 * i + j) =
-                    make_uint4(pack2<T>(y[0], y[1]), pack2<T>(y[2], y[3]), pack2<T>(y[4], y[5]), pack2<T>(y[6], y[7]));
-              }
-          }
-          if (mine && hurt) add_spoiled<T>(p, b, h, node, qh, hurt, m, inv, o);
-          if (mine)
-            p.lse[((size_t)b * p.nodes + node) * p.kv_heads * p.group + qh] =
-                l != 0.0f && seen ? kLn2 * (m + log2f(l)) : -INFINITY;
-        } else {
-          // part of a unit: slot 1 holds a unit's beginning, slot 0 what follows
-          float* o = p.part + ((size_t)(2 * blockIdx.x + (tile0 == 0 ? 1 : 0)) * min(rows, kM) + tid) * (DP + 4);
-          for (int i = 0; i < DP / 32; ++i) {
-            uint32_t v[32];
-            tmem_load32(t_o + lanes + 32 * i, v);
-            tmem_wait_load();
-#pragma unroll
-            for (int j = 0; j < 32; j += 4)
-              if (mine) *reinterpret_cast<uint4*>(o + 32 * i + j) = make_uint4(v[j], v[j + 1], v[j + 2], v[j + 3]);
-          }
-          if (mine) {
-            *reinterpret_cast<float4*>(o + DP) =
-                make_float4(m, l, __uint_as_float((uint32_t)spoiled), __uint_as_float((uint32_t)(spoiled >> 32)));
-          }
-        }
-        tmem_fence_before();
-        next_unit();
+        w += n;
+        at.next_unit(p, units);
       }
     }
+  } else {
+    // ---- softmax: group g, tensor-memory lane L, that is row `row` of the
+    // unit's rows and part `part` of every tile's keys
+    const int g = warp >> 2, quarter = warp & 3, L = quarter * 32 + lane;
+    const int part = COPIES == 4 ? quarter : COPIES == 2 ? quarter >> 1 : 0;
+    const int r0 = COPIES == 4 ? lane : COPIES == 2 ? L & 63 : L;
+    const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+    const uint32_t t_s = tmem + 128 * g + lanes, t_o = tmem + 256 + 128 * g + lanes;
+    int k = 0, u = 0, masks_of = -1;  // k: copies before this unit's
+    uint32_t phase = 0;
+    for (int w = w0; w < w1 && fine;) {
+      const int n = tiles_here(w);
+      if (n == 0) {
+        at.next_unit(p, units);
+        continue;
+      }
+      const int b = at.b, h = at.unit / tiles_r, row = at.unit % tiles_r * kM + r0;
+      const bool mine = row < rows;
+      const int node = mine ? row / p.group : 0, qh = h * p.group + row % p.group;
+      {
+        // each group brings half of the row's 16-byte pieces
+        const T* src = static_cast<const T*>(p.q.data) + b * p.q.batch + qh * p.q.head + node * p.q.row;
+        uint4 v[DP / 16];
+#pragma unroll
+        for (int i = 0; i < DP / 16; ++i) {
+          const int d = 8 * (g * (DP / 16) + i);
+          v[i] = make_uint4(0, 0, 0, 0);
+          if (mine && d < p.head_dim) v[i] = *reinterpret_cast<const uint4*>(src + d);
+        }
+        if (warp == 0 && masks_of != b)
+          tree_masks(p.parents + (size_t)b * p.nodes, p.nodes, s_mask, reinterpret_cast<int*>(s_ml));
+        masks_of = b;
+        const uint32_t flip = negative ? 0x80008000u : 0u;  // a negative scale's sign goes to q
+#pragma unroll
+        for (int i = 0; i < DP / 16; ++i) {
+          const int piece = g * (DP / 16) + i;
+          v[i].x ^= flip, v[i].y ^= flip, v[i].z ^= flip, v[i].w ^= flip;
+          *reinterpret_cast<uint4*>(smem + (piece / 8) * kPanel + L * 128 + (((piece % 8) ^ (L & 7)) << 4)) = v[i];
+        }
+      }
+      smem_fence_async();
+      group_sync(1, 256);
+      if (tid == 0) mbar_arrive(q_ready);
+      const uint64_t mask = mine ? s_mask[node] : 0ull;
+      const int len = length_of(p, b);
+      float m = -INFINITY, l = 0.0f;
+#pragma unroll 1
+      for (int t = g; t < n; t += 2) {
+        const int tile = at.tile + t;
+        const bool tree = tile == at.tiles - 1;
+        const int nk = tree ? p.nodes : min(kKeys, len - tile * kKeys);
+        if (tree || nk < kKeys) {
+          // the values of keys that no row sees are taken out of the product,
+          // and those of new keys that are not finite, which only some see
+          const int kv = k + (t + 1 < n ? 2 * t + 2 : 2 * t + 1);
+          if (!(fine = mbar_wait_short(full(kv % NS), (kv / NS) & 1))) break;
+          uint8_t* vs = smem + (1 + kv % NS) * S::kTileBytes;
+          for (int r = tree ? L : nk + L; r < (tree ? p.nodes : kKeys); r += kM) {
+            bool out = !tree || s_mask[r] == 0ull;
+            if (!out) {
+#pragma unroll
+              for (int i = 0; i < DP / 8; ++i)
+                out |= not_finite<T>(*reinterpret_cast<const uint4*>(vs + (i / 8) * kPanel + r * 128 +
+                                                                     (((i % 8) ^ (r & 7)) << 4)));
+              if (out) atomicOr(s_spoiled, 1ull << r);
+            }
+            if (out)
+#pragma unroll
+              for (int i = 0; i < DP / 8; ++i)
+                *reinterpret_cast<uint4*>(vs + (i / 8) * kPanel + r * 128 + ((i % 8) << 4)) = make_uint4(0, 0, 0, 0);
+          }
+          smem_fence_async();
+        }
+        if (!(fine = mbar_wait_short(s_full(g), phase))) break;
+        phase ^= 1u;
+        tmem_fence_after();
+        uint32_t x[KQ];
+        tmem_load<KQ>(t_s + part * KQ, x);
+        tmem_wait_load();
+        if (tree) {
+          const uint64_t seen = part * KQ < kMaxNodes ? mask >> (part * KQ) : 0ull;
+#pragma unroll
+          for (int i = 0; i < KQ; ++i)
+            if (i >= kMaxNodes || !(seen >> (i & 63) & 1)) x[i] = __float_as_uint(-INFINITY);
+        } else if (nk < kKeys) {
+#pragma unroll
+          for (int i = 0; i < KQ; ++i)
+            if (part * KQ + i >= nk) x[i] = __float_as_uint(-INFINITY);
+        }
+        float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int i = 0; i < KQ; ++i) mx4[i & 3] = fmaxf(mx4[i & 3], __uint_as_float(x[i]));
+        const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
+        const float top = mx == -INFINITY ? mx : mx * c;
+        float f = 1.0f;
+        if (top > m + kSlack || m == -INFINITY) {
+          f = m == -INFINITY ? 0.0f : ex2(m - top);
+          m = top;
+          l *= f;
+        }
+        if (t > 1 && __any_sync(0xffffffffu, f != 1.0f)) {
+          // the sums so far, on the new reference point
+#pragma unroll 1
+          for (int i = 0; i < DP; i += 16) {
+            uint32_t o[16];
+            tmem_load<16>(t_o + i, o);
+            tmem_wait_load();
+#pragma unroll
+            for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
+            tmem_store<16>(t_o + i, o);
+          }
+        }
+        const float ref = m == -INFINITY ? 0.0f : m;
+        float sum[2] = {0.0f, 0.0f};
+#pragma unroll
+        for (int i = 0; i < KQ; i += 2) {
+          float e0 = ex2(fmaf(__uint_as_float(x[i]), c, -ref)), e1 = ex2(fmaf(__uint_as_float(x[i + 1]), c, -ref));
+          sum[0] += e0;
+          sum[1] += e1;
+          x[i / 2] = pack2<T>(e0, e1);
+        }
+        l += sum[0] + sum[1];
+        if constexpr (COPIES == 1) {
+          tmem_store<KQ / 2>(t_s, x);
+        } else {
+          uint32_t zero[KQ / 2];
+#pragma unroll
+          for (int i = 0; i < KQ / 2; ++i) zero[i] = 0u;
+#pragma unroll
+          for (int i = 0; i < COPIES; ++i) {
+            if (i == part)
+              tmem_store<KQ / 2>(t_s + i * (KQ / 2), x);
+            else
+              tmem_store<KQ / 2>(t_s + i * (KQ / 2), zero);
+          }
+        }
+        tmem_wait_store();
+        tmem_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(p_ready(g));
+      }
+      if (!fine || !(fine = mbar_wait_short(o_full, u & 1))) break;
+      ++u;
+      tmem_fence_after();
+      // join the parts of each row: reference point and sum first
+      s_ml[g * kM + L] = make_float2(m, l);
+      group_sync(1, 256);
+      float top = -INFINITY, total = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 2 * COPIES; ++i) top = fmaxf(top, s_ml[(i & 1) * kM + (i >> 1) * (kM / COPIES) + r0].x);
+      const float ref = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+      for (int i = 0; i < 2 * COPIES; ++i) {
+        const float2 e = s_ml[(i & 1) * kM + (i >> 1) * (kM / COPIES) + r0];
+        total = fmaf(e.y, ex2(e.x - ref), total);
+      }
+      const float f = ex2(m - ref);
+      const bool whole = at.tile == 0 && n == at.tiles, seen = mask != 0ull;  // a padding node's row is empty
+      const float inv = total != 0.0f && seen ? 1.0f / total : 0.0f;
+      const unsigned long long spoiled = *s_spoiled;
+      const int share = g * COPIES + part;  // the parts of a row finish its columns in turn
+      T* out = mine ? out_row<T>(p, b, node, qh) : nullptr;
+      // part of a unit: slot 1 holds a unit's beginning, slot 0 what follows
+      float* keep = p.part + ((size_t)(2 * blockIdx.x + (at.tile == 0 ? 1 : 0)) * min(rows, kM) + r0) * (DP + 4);
+      float4* const buf = reinterpret_cast<float4*>(smem);  // [2][kM][CW], 16-byte pieces swizzled
+      auto place = [&](int gg, int ll, int piece) {
+        return (gg * kM + ll) * (CW / 4) + (piece ^ (CW == 32 ? ll & 7 : ll >> 1 & 3));
+      };
+#pragma unroll 1
+      for (int i = 0; i < DP; i += CW) {
+        uint32_t v[CW];
+        tmem_load<CW>(t_o + i, v);
+        tmem_wait_load();
+#pragma unroll
+        for (int j = 0; j < CW / 4; ++j) {
+          float4 e;
+          e.x = f == 0.0f ? 0.0f : __uint_as_float(v[4 * j]) * f;
+          e.y = f == 0.0f ? 0.0f : __uint_as_float(v[4 * j + 1]) * f;
+          e.z = f == 0.0f ? 0.0f : __uint_as_float(v[4 * j + 2]) * f;
+          e.w = f == 0.0f ? 0.0f : __uint_as_float(v[4 * j + 3]) * f;
+          buf[place(g, L, j)] = e;
+        }
+        group_sync(1, 256);
+        if (mine) {
+#pragma unroll
+          for (int j = share; j < CW / 4; j += 2 * COPIES) {
+            float4 e = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+            for (int q = 0; q < 2 * COPIES; ++q) {
+              const float4 y = buf[place(q & 1, (q >> 1) * (kM / COPIES) + r0, j)];
+              e.x += y.x, e.y += y.y, e.z += y.z, e.w += y.w;
+            }
+            if (!whole) {
+              *reinterpret_cast<float4*>(keep + i + 4 * j) = e;
+            } else if (i + 4 * j < p.head_dim) {
+              if (!seen) e = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+              *reinterpret_cast<uint2*>(out + i + 4 * j) =
+                  make_uint2(pack2<T>(e.x * inv, e.y * inv), pack2<T>(e.z * inv, e.w * inv));
+            }
+          }
+        }
+        group_sync(1, 256);
+      }
+      if (mine && share == 0) {
+        if (whole) {
+          if (spoiled & mask) add_spoiled<T>(p, b, h, node, qh, spoiled & mask, top, inv, out);
+          p.lse[((size_t)b * p.nodes + node) * p.kv_heads * p.group + qh] =
+              total != 0.0f && seen ? kLn2 * (top + log2f(total)) : -INFINITY;
+        } else {
+          *reinterpret_cast<float4*>(keep + DP) =
+              make_float4(top, total, __uint_as_float((uint32_t)spoiled), __uint_as_float((uint32_t)(spoiled >> 32)));
+        }
+      }
+      if (tid == 0) *s_spoiled = 0ull;
+      tmem_fence_before();
+      k += 2 * n;
+      w += n;
+      at.next_unit(p, units);
+    }
   }
-  if (!fine && (warp < 4 || lane == 0)) atomicAdd(faults, 1u);
+  if (!fine && (warp < 8 || lane == 0)) atomicAdd(faults, 1u);
   tmem_fence_before();
   __syncthreads();
-  if (warp == 5) {
+  if (warp == 9) {
     __syncwarp();
     tmem_free(tmem, kTmemCols);
   }
@@ -704,10 +795,12 @@ __global__ void __launch_bounds__(256) join_tc_kernel(const __grid_constant__ At
   const int b = bh / p.kv_heads, h = bh % p.kv_heads;
   if (row >= rows) return;
   const int unit = h * tiles_r + row / kM, r = row % kM;
-  // this unit's tiles [u0, u1) of the list
-  long long before = 0, all = 0;
+  // this unit's tiles [u0, u1) of the list, and the CTAs that have the first
+  // and the last: CTA i begins at part_start(i), so w is CTA
+  // floor((ctas (w + 1) - 1) / entries)'s
+  int before = 0, all = 0;
   for (int i = lane; i < p.batch; i += 32) {
-    const int t = tiles_of(p, i);
+    const int t = tiles_of(p, i) + kUnitCost;
     all += t;
     if (i < b) before += t;
   }
@@ -717,16 +810,19 @@ __global__ void __launch_bounds__(256) join_tc_kernel(const __grid_constant__ At
     before += __shfl_xor_sync(0xffffffffu, before, o);
   }
   const int tiles = tiles_of(p, b);
-  const long long W = all * units, u0 = before * units + (long long)unit * tiles, u1 = u0 + tiles;
-  const int c0 = (int)((ctas * (u0 + 1) - 1) / W), c1 = (int)((ctas * u1 - 1) / W);
+  const long long W = (long long)all * units, u0 = (long long)before * units + unit * (tiles + kUnitCost) + kUnitCost;
+  const int c0 = (int)((ctas * (u0 + 1) - 1) / W), c1 = (int)((ctas * (u0 + tiles) - 1) / W);
   if (c0 == c1) return;
   tree_masks(p.parents + (size_t)b * p.nodes, p.nodes, s_mask[warp], s_jump[warp]);
   const int node = row / p.group, qh = h * p.group + row % p.group;
   const uint64_t mask = s_mask[warp][node];
   const int stride = min(rows, kM);
   auto part = [&](int i) { return p.part + ((size_t)(2 * i + (i == c0 ? 1 : 0)) * stride + r) * (DP + 4); };
+  // with fewer entries than CTAs some have none and wrote nothing
+  auto idle = [&](int i) { return W < ctas && part_start((int)W, i, ctas) == part_start((int)W, i + 1, ctas); };
   float m = -INFINITY;
-  for (int i = c0 + lane; i <= c1; i += 32) m = fmaxf(m, part(i)[DP]);
+  for (int i = c0 + lane; i <= c1; i += 32)
+    if (!idle(i)) m = fmaxf(m, part(i)[DP]);
 #pragma unroll
   for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
   const float ref = m == -INFINITY ? 0.0f : m;
@@ -736,6 +832,7 @@ __global__ void __launch_bounds__(256) join_tc_kernel(const __grid_constant__ At
   for (int j = 0; j < 2 * PANELS; ++j) x[j] = 0.0f;
 #pragma unroll 4
   for (int i = c0; i <= c1; ++i) {
+    if (idle(i)) continue;
     const float* o = part(i);
     const float4 e = *reinterpret_cast<const float4*>(o + DP);
     const float f = exp2f(e.x - ref);
@@ -808,16 +905,18 @@ void check_shape(const ckks_draft_attention_args& a) {
   need(a.kv_heads >= 1 && a.q_heads >= 1 && a.q_heads % a.kv_heads == 0,
        "query heads are not a multiple of the key/value heads");
   need(a.head_dim >= 1 && a.head_dim <= kMaxHeadDim, "head_dim outside 1..256");
-  need((long long)a.batch * a.q_heads * a.nodes < (1ll << 31) - 1 && a.capacity < (1 << 30), "sizes too large");
+  need((long long)a.batch * a.q_heads * a.nodes < (1ll << 31) - 1 && a.capacity < (1 << 30) &&
+           (long long)a.batch * a.q_heads * (a.capacity / 128 + 4) < (1ll << 31) - 1,
+       "sizes too large");
 }
 
-// Tensor-core CTAs: two on each SM, but no fewer than four tiles of keys
+// Tensor-core CTAs: one on each SM, but no fewer than four tiles of keys
 // each at the full capacity (a shorter part is all start-up), and one for
 // each unit where there are fewer units than that
 int tc_ctas(const Context& c, const ckks_draft_attention_args& a) {
   const long long rows = (long long)a.nodes * (a.q_heads / a.kv_heads);
   const long long units = (long long)a.batch * a.kv_heads * ((rows + kM - 1) / kM);
-  const long long tiles = units * ((a.capacity + kKeys - 1) / kKeys + 1), slots = 2ll * c.sms;
+  const long long tiles = units * ((a.capacity + kKeys - 1) / kKeys + 1), slots = c.sms;
   return (int)std::max(1ll, std::min(slots, std::max(tiles / 4, units)));
 }
 
@@ -870,19 +969,32 @@ bool tile_map(CUtensorMap* m, const ckks_rows& r, int dtype, int batch, int head
            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <typename T, int PANELS>
+template <typename T, int PANELS, int COPIES>
 void launch_tc(const Context& c, const ckks_draft_attention_args& a, const AttnParams& p, const TileMaps& maps,
                cudaStream_t st) {
   using S = TcShape<PANELS>;
-  auto* k = attend_tc_kernel<T, PANELS>;
+  auto* k = attend_tc_kernel<T, PANELS, COPIES>;
   CKKS_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::kSmem));
   const int ctas = tc_ctas(c, a), rows = p.nodes * p.group;
-  const float factor = std::fabs(p.scale) * kLog2e;
-  k<<<ctas, kTcThreads, S::kSmem, st>>>(p, maps, p.scale < 0.0f ? -1.0f : 1.0f, factor, c.d_faults);
+  // a scale of 0 becomes one that changes no weight: a masked score times 0 would be no number
+  const float factor = std::max(std::fabs(p.scale) * kLog2e, 1e-30f);
+  k<<<ctas, kTcThreads, S::kSmem, st>>>(p, maps, p.scale < 0.0f, factor, c.d_faults);
   CKKS_CUDA(cudaGetLastError());
   if (!tc_alone(a, ctas))
     launch_pdl(join_tc_kernel<T, PANELS>, dim3((unsigned)(p.batch * p.kv_heads * ((rows + 7) / 8))), dim3(256), 0, st, p,
                ctas);
+}
+
+template <typename T, int PANELS>
+void launch_tc(const Context& c, const ckks_draft_attention_args& a, const AttnParams& p, const TileMaps& maps,
+               cudaStream_t st) {
+  const int rows = p.nodes * p.group;
+  if (rows <= 32)
+    launch_tc<T, PANELS, 4>(c, a, p, maps, st);
+  else if (rows <= 64)
+    launch_tc<T, PANELS, 2>(c, a, p, maps, st);
+  else
+    launch_tc<T, PANELS, 1>(c, a, p, maps, st);
 }
 
 template <typename T>

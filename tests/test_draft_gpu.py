@@ -89,6 +89,10 @@ SHAPES = [
     (1, 2, 2, 2, 40, 70, [64], 1, 0),
     (1, 64, 1, 1, 64, 4, [3], 1, 0),           # a chain of 64
     (1, 64, 2, 2, 64, 0, [0], 2, 0),           # a cache without rows
+    (1, 2, 1, 1, 64, 70000, [200], 1, 0),      # far more capacity than keys
+    (3, 3, 2, 1, 128, 40000, [129, 0, 300], 1, 1),
+    (40, 2, 2, 1, 64, 300, [(37 * b) % 301 for b in range(40)], 1, 0),  # many short sequences
+    (70, 33, 2, 2, 64, 140, [(53 * b) % 141 for b in range(70)], 2, 0),
 ]
 
 
