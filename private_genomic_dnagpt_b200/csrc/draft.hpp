@@ -121,43 +121,60 @@ __device__ __forceinline__ T from_f32(float x) {
     return (T)x;
 }
 
-// Ancestor masks of one tree, by one warp: mask[i] gets the bits of node i
-// and of the nodes above it, 0 where i is padding.  Six rounds of pointer
-// doubling cover every depth up to 64.  `jump` is scratch of 64 ints.
-__device__ __forceinline__ void tree_masks(const int32_t* __restrict__ parents, int n, uint64_t* mask, int* jump) {
-  const int lane = threadIdx.x & 31;
+// Ancestor masks of one tree, by one warp, in two steps: the parents into
+// registers, then mask[i] gets the bits of node i and of the nodes above it, 0
+// where i is padding.  Six rounds of pointer doubling cover every depth up to
+// 64.  `jump` is scratch of 64 ints.
+struct TreeReader {
+  int parent[2];
+  __device__ __forceinline__ void read(const int32_t* __restrict__ parents, int n) {
+    const int lane = threadIdx.x & 31;
 #pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    const int i = lane + 32 * k;
-    const int p = i < n ? parents[i] : -2;
-    const bool ok = p >= -1 && p < i;  // a parent comes before its children
-    mask[i] = ok ? 1ull << i : 0ull;
-    jump[i] = ok ? p : -2;
+    for (int k = 0; k < 2; ++k) parent[k] = lane + 32 * k < n ? parents[lane + 32 * k] : -2;
   }
-  __syncwarp();
-#pragma unroll 1
-  for (int r = 0; r < 6; ++r) {
-    uint64_t m[2];
-    int j[2];
+  __device__ __forceinline__ void masks(uint64_t* mask, int* jump) const {
+    const int lane = threadIdx.x & 31;
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
       const int i = lane + 32 * k;
-      const int p = jump[i];
-      m[k] = mask[i] | (p >= 0 ? mask[p] : 0ull);
-      j[k] = p >= 0 ? jump[p] : p;
+      const bool ok = parent[k] >= -1 && parent[k] < i;  // a parent comes before its children
+      mask[i] = ok ? 1ull << i : 0ull;
+      jump[i] = ok ? parent[k] : -2;
     }
     __syncwarp();
+#pragma unroll 1
+    for (int r = 0; r < 6; ++r) {
+      uint64_t m[2];
+      int j[2];
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      mask[lane + 32 * k] = m[k];
-      jump[lane + 32 * k] = j[k];
+      for (int k = 0; k < 2; ++k) {
+        const int i = lane + 32 * k;
+        const int p = jump[i];
+        m[k] = mask[i] | (p >= 0 ? mask[p] : 0ull);
+        j[k] = p >= 0 ? jump[p] : p;
+      }
+      __syncwarp();
+      bool open = false;  // a walk has not reached the root yet
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        mask[lane + 32 * k] = m[k];
+        jump[lane + 32 * k] = j[k];
+        open |= j[k] >= 0;
+      }
+      __syncwarp();
+      if (!__any_sync(0xffffffffu, open)) break;
     }
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+      if (jump[lane + 32 * k] != -1) mask[lane + 32 * k] = 0ull;
     __syncwarp();
   }
-#pragma unroll
-  for (int k = 0; k < 2; ++k)
-    if (jump[lane + 32 * k] != -1) mask[lane + 32 * k] = 0ull;
-  __syncwarp();
+};
+
+__device__ __forceinline__ void tree_masks(const int32_t* __restrict__ parents, int n, uint64_t* mask, int* jump) {
+  TreeReader t;
+  t.read(parents, n);
+  t.masks(mask, jump);
 }
 
 }  // namespace draft

@@ -26,6 +26,7 @@ struct AttnParams {
   float* lse;
   float* part;  // [batch * kv_heads][splits][rows][head_dim + 2]
   int batch, kv_heads, group, head_dim, nodes, capacity, splits;
+  int tile_nodes;  // nodes of one 128-row tile
   float scale;
   bool wide;  // every row is whole, aligned 16-byte pieces
 };
@@ -296,6 +297,7 @@ __device__ __noinline__ void add_spoiled(const AttnParams& p, int b, int h, int 
 // The rows of one key/value head (nodes x query heads on it) are the M = 128
 // rows of a tile; a unit of work is (sequence, head, 128 rows), and its keys
 // are tiles of 128: ceil(len / 128) of the cache, then one with the new keys.
+// (A tile holds whole nodes, so it may have a few rows less.)
 // Scores S = Q K^T go to tensor memory; a thread takes the scores of its row
 // into registers, keeps the running maximum and sum, and puts the weights
 // back as the 16-bit A operand of O += P V, O staying in tensor memory.
@@ -314,7 +316,7 @@ __device__ __noinline__ void add_spoiled(const AttnParams& p, int b, int h, int 
 //
 // The lengths are known on the device only, so the CTAs divide the list of
 // all units' tiles evenly: a CTA may finish one unit, take some whole ones
-// and begin another.  A unit also counts as kUnitCost tiles for its start and
+// and begin another.  A unit also counts as some tiles for its start and
 // its end.  A unit that more than one CTA has part of leaves (m, l, O) in the
 // workspace for the second kernel.
 //
@@ -322,12 +324,17 @@ __device__ __noinline__ void add_spoiled(const AttnParams& p, int b, int h, int 
 // more than 2^8 (the weights then stay below 2^8, far inside 16-bit range):
 // O is seldom rescaled.  Weights are rounded to the operands' type for the
 // second product; l sums them before that, in 32 bits.
-constexpr int kM = 128, kKeys = 128, kTcThreads = 320, kTmemCols = 512, kUnitCost = 2;
+constexpr int kM = 128, kKeys = 128, kTcThreads = 320, kTmemCols = 512;
 constexpr uint32_t kPanel = 128 * 128;  // 128 rows x 64 elements
 constexpr float kSlack = 8.0f;
 
+// What a unit's start and end cost, in tiles: measured on trees of 21 over 4001
+// keys of 64 (2 / 3 / 4 / 5 / 6 tiles: 32.7 / 28.4 / 26.9 / 27.8 / 29.0 us) and
+// trees of 32 over 65536 keys of 128 (2 / 4 / 6 / 8: 97.6 / 95.3 / 93.7 / 91.4 us)
+__host__ __device__ __forceinline__ int unit_cost(const AttnParams& p) { return p.head_dim <= 64 ? 4 : 8; }
+
 struct TileMaps {
-  CUtensorMap kc, vc, kn, vn;
+  CUtensorMap q, kc, vc, kn, vn;
 };
 
 __device__ __forceinline__ int tiles_of(const AttnParams& p, int b) { return (length_of(p, b) + kKeys - 1) / kKeys + 1; }
@@ -337,7 +344,7 @@ __device__ __forceinline__ int tiles_of(const AttnParams& p, int b) { return (le
 struct Cursor {
   int b, unit, tile, tiles;
   __device__ __forceinline__ void next_unit(const AttnParams& p, int units) {
-    tile = -kUnitCost;
+    tile = -unit_cost(p);
     if (++unit == units) {
       unit = 0;
       tiles = ++b < p.batch ? tiles_of(p, b) : 1;
@@ -345,21 +352,29 @@ struct Cursor {
   }
 };
 
-// entries of one unit of every sequence, summed; by a whole warp
-__device__ __forceinline__ int entry_sum(const AttnParams& p) {
-  int s = 0;
-  for (int b = threadIdx.x & 31; b < p.batch; b += 32) s += tiles_of(p, b) + kUnitCost;
+// first entry of part i of n
+__device__ __forceinline__ int part_start(int entries, int i, int n) {
+  return entries / n * i + (int)((unsigned)(entries % n) * (unsigned)i / (unsigned)n);
+}
+
+// entries of one unit of every sequence, summed; by a whole warp.  `first`:
+// those of sequence `lane`
+__device__ __forceinline__ int entry_sum(const AttnParams& p, int& first) {
+  const int lane = threadIdx.x & 31;
+  first = lane < p.batch ? tiles_of(p, lane) + unit_cost(p) : 0;
+  int s = first;
+  for (int b = lane + 32; b < p.batch; b += 32) s += tiles_of(p, b) + unit_cost(p);
 #pragma unroll
   for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
   return s;
 }
 
 // entry `w` of the list; by a whole warp
-__device__ __forceinline__ Cursor find_entry(const AttnParams& p, int units, int w) {
+__device__ __forceinline__ Cursor find_entry(const AttnParams& p, int units, int w, int first) {
   const int lane = threadIdx.x & 31;
   int before = 0;
   for (int b0 = 0;; b0 += 32) {
-    const int t = b0 + lane < p.batch ? tiles_of(p, b0 + lane) + kUnitCost : 0;
+    const int t = b0 == 0 ? first : b0 + lane < p.batch ? tiles_of(p, b0 + lane) + unit_cost(p) : 0;
     int sum = t * units;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -371,15 +386,10 @@ __device__ __forceinline__ Cursor find_entry(const AttnParams& p, int units, int
       const int k = past ? __ffs(past) - 1 : 31;
       const int tk = max(1, __shfl_sync(0xffffffffu, t, k));
       const int off = w - (before + __shfl_sync(0xffffffffu, sum, k) - tk * units);
-      return {b0 + k, off / tk, off % tk - kUnitCost, tk - kUnitCost};
+      return {b0 + k, off / tk, off % tk - unit_cost(p), tk - unit_cost(p)};
     }
     before += __shfl_sync(0xffffffffu, sum, 31);
   }
-}
-
-// first entry of part i of n
-__device__ __forceinline__ int part_start(int entries, int i, int n) {
-  return entries / n * i + (int)((unsigned)(entries % n) * (unsigned)i / (unsigned)n);
 }
 
 __device__ __forceinline__ float ex2(float x) {
@@ -416,11 +426,16 @@ __device__ __forceinline__ void group_sync(int id, int threads) {
 
 template <int PANELS>
 struct TcShape {
-  static constexpr int kSlots = PANELS == 1 ? 12 : 6;
+  static constexpr int kSlots = PANELS == 1 ? 9 : 5;
   static constexpr uint32_t kTileBytes = PANELS * kPanel;
-  // behind Q and the ring: (m, l) of every part of a row, ancestor masks, barriers, two words
-  static constexpr uint32_t kExtra = (1 + kSlots) * kTileBytes;
-  static constexpr size_t kSmem = kExtra + 2 * kM * sizeof(float2) + kMaxNodes * 8 + (2 * kSlots + 6) * 8 + 16;
+  // Two buffers for Q, the next unit's arriving early; 2 x 128 x 32 floats in
+  // which a unit's parts meet at its end (with two panels, its own Q); the
+  // ring; (m, l) of one group's rows, the nodes' masks of two units, barriers,
+  // two words
+  static constexpr uint32_t kMeet = PANELS == 1 ? 2 * kPanel : 0, kRing = 4 * kPanel;
+  static constexpr uint32_t kExtra = kRing + kSlots * kTileBytes;
+  static constexpr int kBars = 2 * kSlots + 9;
+  static constexpr size_t kSmem = kExtra + kM * sizeof(float2) + 2 * kMaxNodes * 8 + kBars * 8 + 16;
 };
 
 template <typename T, int PANELS, int COPIES>
@@ -428,22 +443,25 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     attend_tc_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ TileMaps maps, bool negative, float c,
                      unsigned int* __restrict__ faults) {
   using S = TcShape<PANELS>;
-  constexpr int DP = 64 * PANELS, NS = S::kSlots, KQ = kKeys / COPIES, CW = 16 * PANELS;
+  constexpr int DP = 64 * PANELS, NS = S::kSlots, KQ = kKeys / COPIES, CW = 32;
   constexpr bool kBf = std::is_same_v<T, __nv_bfloat16>;
   extern __shared__ __align__(1024) uint8_t smem[];
-  float2* const s_ml = reinterpret_cast<float2*>(smem + S::kExtra);  // [2][kM]
-  uint64_t* const s_mask = reinterpret_cast<uint64_t*>(s_ml + 2 * kM);
-  uint64_t* const s_bar = s_mask + kMaxNodes;
-  unsigned long long* const s_spoiled = reinterpret_cast<unsigned long long*>(s_bar + 2 * NS + 6);
+  float2* const s_ml = reinterpret_cast<float2*>(smem + S::kExtra);  // [kM]
+  uint64_t* const s_mask = reinterpret_cast<uint64_t*>(s_ml + kM);
+  uint64_t* const s_bar = s_mask + 2 * kMaxNodes;
+  unsigned long long* const s_spoiled = reinterpret_cast<unsigned long long*>(s_bar + S::kBars);
   uint32_t* const s_tmem = reinterpret_cast<uint32_t*>(s_spoiled + 1);
-  const uint32_t sq = smem_addr(smem), ring = sq + S::kTileBytes, bars = smem_addr(s_bar);
+  const uint32_t sq = smem_addr(smem), ring = sq + S::kRing, bars = smem_addr(s_bar);
   auto full = [&](int s) { return bars + 8 * s; };
   auto empty = [&](int s) { return bars + 8 * (NS + s); };
   auto s_full = [&](int g) { return bars + 8 * (2 * NS + g); };
   auto p_ready = [&](int g) { return bars + 8 * (2 * NS + 2 + g); };
-  const uint32_t q_ready = bars + 8 * (2 * NS + 4), o_full = q_ready + 8;
+  auto q_full = [&](int i) { return bars + 8 * (2 * NS + 4 + i); };
+  auto q_empty = [&](int i) { return bars + 8 * (2 * NS + 6 + i); };
+  const uint32_t o_full = bars + 8 * (2 * NS + 8);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int rows = p.nodes * p.group, tiles_r = (rows + kM - 1) / kM, units = p.kv_heads * tiles_r;
+  const int tiles_r = (p.nodes + p.tile_nodes - 1) / p.tile_nodes, units = p.kv_heads * tiles_r;
+  const int tile_rows = p.tile_nodes * p.group;
   asm volatile("griddepcontrol.launch_dependents;");
   if (tid == 0) {
     for (int s = 0; s < NS; ++s) {
@@ -453,16 +471,18 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     for (int g = 0; g < 2; ++g) {
       mbar_init(s_full(g), 1);
       mbar_init(p_ready(g), 4);
+      mbar_init(q_full(g), 1);
+      mbar_init(q_empty(g), 1);
     }
-    mbar_init(q_ready, 1);
     mbar_init(o_full, 1);
     *s_spoiled = 0ull;
   }
   if (warp == 9) tmem_alloc(smem_addr(s_tmem), kTmemCols);
   // this CTA's entries [w0, w1) of the list
-  const int entries = entry_sum(p) * units;
+  int first;
+  const int entries = entry_sum(p, first) * units;
   const int w0 = part_start(entries, blockIdx.x, gridDim.x), w1 = part_start(entries, blockIdx.x + 1, gridDim.x);
-  Cursor at = find_entry(p, units, w0);
+  Cursor at = find_entry(p, units, w0, first);
   tmem_fence_before();
   __syncthreads();
   tmem_fence_after();
@@ -479,9 +499,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   if (warp == 8) {
     // ---- copies
     if (lane == 0) {
+      tile_prefetch(&maps.q);
       tile_prefetch(&maps.kc);
       tile_prefetch(&maps.vc);
-      int k = 0;  // copies issued
+      int k = 0, u = 0;  // tiles of keys or values and units whose copies are issued
       for (int w = w0; w < w1 && fine;) {
         const int n = tiles_here(w), h = at.unit / tiles_r;
         auto load = [&](int tile, bool value) {
@@ -496,7 +517,17 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           ++k;
           return true;
         };
-        if (n) load(at.tile, false);
+        if (n) {
+          const int i = u & 1;
+          if (u >= 2 && !(fine = mbar_wait_short(q_empty(i), ((u >> 1) - 1) & 1))) break;
+          ++u;
+          mbar_expect_tx(q_full(i), COPIES * PANELS * tile_rows * 128);
+#pragma unroll
+          for (int x = 0; x < COPIES * PANELS; ++x)
+            tile_load(sq + i * S::kTileBytes + (x % PANELS) * kPanel + (x / PANELS) * (kPanel / COPIES), &maps.q,
+                      64 * (x % PANELS), h * p.group, at.unit % tiles_r * p.tile_nodes, at.b, q_full(i));
+          load(at.tile, false);
+        }
         for (int t = 0; t < n && fine; ++t) {
           if (t + 1 < n && !load(at.tile + t + 1, false)) break;
           load(at.tile + t, true);
@@ -506,6 +537,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       }
       // copies still in flight land before the CTA ends
       for (int j = k > NS ? k - NS : 0; j < k; ++j) fine = mbar_wait_short(full(j % NS), (j / NS) & 1) && fine;
+      for (int j = u > 2 ? u - 2 : 0; j < u; ++j) fine = mbar_wait_short(q_full(j & 1), j >> 1 & 1) && fine;
     }
   } else if (warp == 9) {
     // ---- products
@@ -523,7 +555,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 #pragma unroll
           for (int i = 0; i < DP / 16; ++i) {
             const uint32_t off = (i / 4) * kPanel + (i % 4) * 32;
-            mma_smem(tmem + 128 * g, smem_operand(sq + off, 16), smem_operand(kb + off, 16), word_s, i > 0);
+            mma_smem(tmem + 128 * g, smem_operand(sq + (u & 1) * S::kTileBytes + off, 16), smem_operand(kb + off, 16),
+                     word_s, i > 0);
           }
           mma_commit(empty(s));
           mma_commit(s_full(g));
@@ -531,7 +564,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           return true;
         };
         if (n) {
-          fine = mbar_wait_short(q_ready, u++ & 1) && scores(0);
+          fine = mbar_wait_short(q_full(u & 1), u >> 1 & 1) && scores(0);
           for (int t = 0; t < n && fine; ++t) {
             if (t + 1 < n && !scores((t + 1) & 1)) break;
             const int g = t & 1, s = k % NS;
@@ -547,6 +580,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             ++k;
           }
           if (fine) mma_commit(o_full);
+          ++u;
         }
         w += n;
         at.next_unit(p, units);
@@ -560,42 +594,30 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const int r0 = COPIES == 4 ? lane : COPIES == 2 ? L & 63 : L;
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
     const uint32_t t_s = tmem + 128 * g + lanes, t_o = tmem + 256 + 128 * g + lanes;
-    int k = 0, u = 0, masks_of = -1;  // k: copies before this unit's
+    int k = 0, u = 0;  // k: tiles of keys and values before this unit's
     uint32_t phase = 0;
+    // The parents of the next unit's nodes are read before this unit's tiles
+    // and become masks at its end: a read among the copies' traffic takes
+    // thousands of cycles.
+    TreeReader reader;
+    if (warp == 0 && w0 < w1) {
+      reader.read(p.parents + (size_t)at.b * p.nodes, p.nodes);
+      reader.masks(s_mask, reinterpret_cast<int*>(s_ml));
+    }
     for (int w = w0; w < w1 && fine;) {
       const int n = tiles_here(w);
-      if (n == 0) {
-        at.next_unit(p, units);
-        continue;
-      }
-      const int b = at.b, h = at.unit / tiles_r, row = at.unit % tiles_r * kM + r0;
-      const bool mine = row < rows;
-      const int node = mine ? row / p.group : 0, qh = h * p.group + row % p.group;
-      {
-        // each group brings half of the row's 16-byte pieces
-        const T* src = static_cast<const T*>(p.q.data) + b * p.q.batch + qh * p.q.head + node * p.q.row;
-        uint4 v[DP / 16];
-#pragma unroll
-        for (int i = 0; i < DP / 16; ++i) {
-          const int d = 8 * (g * (DP / 16) + i);
-          v[i] = make_uint4(0, 0, 0, 0);
-          if (mine && d < p.head_dim) v[i] = *reinterpret_cast<const uint4*>(src + d);
-        }
-        if (warp == 0 && masks_of != b)
-          tree_masks(p.parents + (size_t)b * p.nodes, p.nodes, s_mask, reinterpret_cast<int*>(s_ml));
-        masks_of = b;
-        const uint32_t flip = negative ? 0x80008000u : 0u;  // a negative scale's sign goes to q
-#pragma unroll
-        for (int i = 0; i < DP / 16; ++i) {
-          const int piece = g * (DP / 16) + i;
-          v[i].x ^= flip, v[i].y ^= flip, v[i].z ^= flip, v[i].w ^= flip;
-          *reinterpret_cast<uint4*>(smem + (piece / 8) * kPanel + L * 128 + (((piece % 8) ^ (L & 7)) << 4)) = v[i];
-        }
-      }
-      smem_fence_async();
+      if (n == 0) break;  // only a unit's start is left
+      const int b = at.b, h = at.unit / tiles_r, node0 = at.unit % tiles_r * p.tile_nodes;
+      const int here = min(p.tile_nodes, p.nodes - node0) * p.group;  // rows of this unit
+      const bool mine = r0 < here;
+      const int node = mine ? node0 + r0 / p.group : 0, qh = h * p.group + (mine ? r0 % p.group : 0);
+      uint64_t* const masks = s_mask + (u & 1) * kMaxNodes;
+      Cursor then = at;
+      then.next_unit(p, units);
+      const bool more = w + n < w1;
+      if (warp == 0 && more) reader.read(p.parents + (size_t)then.b * p.nodes, p.nodes);
       group_sync(1, 256);
-      if (tid == 0) mbar_arrive(q_ready);
-      const uint64_t mask = mine ? s_mask[node] : 0ull;
+      const uint64_t mask = mine ? masks[node] : 0ull;
       const int len = length_of(p, b);
       float m = -INFINITY, l = 0.0f;
 #pragma unroll 1
@@ -608,9 +630,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           // and those of new keys that are not finite, which only some see
           const int kv = k + (t + 1 < n ? 2 * t + 2 : 2 * t + 1);
           if (!(fine = mbar_wait_short(full(kv % NS), (kv / NS) & 1))) break;
-          uint8_t* vs = smem + (1 + kv % NS) * S::kTileBytes;
+          uint8_t* vs = smem + S::kRing + (kv % NS) * S::kTileBytes;
           for (int r = tree ? L : nk + L; r < (tree ? p.nodes : kKeys); r += kM) {
-            bool out = !tree || s_mask[r] == 0ull;
+            bool out = !tree || masks[r] == 0ull;
             if (!out) {
 #pragma unroll
               for (int i = 0; i < DP / 8; ++i)
@@ -631,6 +653,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         uint32_t x[KQ];
         tmem_load<KQ>(t_s + part * KQ, x);
         tmem_wait_load();
+        if (negative) {  // scores of -q
+#pragma unroll
+          for (int i = 0; i < KQ; ++i) x[i] ^= 0x80000000u;
+        }
         if (tree) {
           const uint64_t seen = part * KQ < kMaxNodes ? mask >> (part * KQ) : 0ull;
 #pragma unroll
@@ -694,82 +720,90 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         if (lane == 0) mbar_arrive(p_ready(g));
       }
       if (!fine || !(fine = mbar_wait_short(o_full, u & 1))) break;
-      ++u;
       tmem_fence_after();
       // join the parts of each row: reference point and sum first
-      s_ml[g * kM + L] = make_float2(m, l);
+      // [2][kM][CW], 16-byte pieces swizzled; before that the second group's (m, l)
+      float4* const buf = reinterpret_cast<float4*>(smem + (PANELS == 1 ? S::kMeet : (u & 1) * S::kTileBytes));
+      float2* const ml[2] = {s_ml, reinterpret_cast<float2*>(buf)};
+      ml[g][L] = make_float2(m, l);
       group_sync(1, 256);
       float top = -INFINITY, total = 0.0f;
 #pragma unroll
-      for (int i = 0; i < 2 * COPIES; ++i) top = fmaxf(top, s_ml[(i & 1) * kM + (i >> 1) * (kM / COPIES) + r0].x);
+      for (int i = 0; i < 2 * COPIES; ++i) top = fmaxf(top, ml[i & 1][(i >> 1) * (kM / COPIES) + r0].x);
       const float ref = top == -INFINITY ? 0.0f : top;
 #pragma unroll
       for (int i = 0; i < 2 * COPIES; ++i) {
-        const float2 e = s_ml[(i & 1) * kM + (i >> 1) * (kM / COPIES) + r0];
+        const float2 e = ml[i & 1][(i >> 1) * (kM / COPIES) + r0];
         total = fmaf(e.y, ex2(e.x - ref), total);
       }
       const float f = ex2(m - ref);
       const bool whole = at.tile == 0 && n == at.tiles, seen = mask != 0ull;  // a padding node's row is empty
       const float inv = total != 0.0f && seen ? 1.0f / total : 0.0f;
       const unsigned long long spoiled = *s_spoiled;
-      const int share = g * COPIES + part;  // the parts of a row finish its columns in turn
-      T* out = mine ? out_row<T>(p, b, node, qh) : nullptr;
       // part of a unit: slot 1 holds a unit's beginning, slot 0 what follows
-      float* keep = p.part + ((size_t)(2 * blockIdx.x + (at.tile == 0 ? 1 : 0)) * min(rows, kM) + r0) * (DP + 4);
-      float4* const buf = reinterpret_cast<float4*>(smem);  // [2][kM][CW], 16-byte pieces swizzled
-      auto place = [&](int gg, int ll, int piece) {
-        return (gg * kM + ll) * (CW / 4) + (piece ^ (CW == 32 ? ll & 7 : ll >> 1 & 3));
-      };
+      float* const keep = p.part + (size_t)(2 * blockIdx.x + (at.tile == 0 ? 1 : 0)) * tile_rows * (DP + 4);
+      const bool leads = g == 0 && part == 0 && mine;  // one thread of each row
+      group_sync(1, 256);
+      // every row's factor, 0 for one that sees nothing, in the place of its first part's m
+      if (leads) s_ml[r0] = make_float2(whole ? inv : 1.0f, seen || !whole ? 1.0f : 0.0f);
+      auto place = [&](int gg, int ll, int piece) { return (gg * kM + ll) * (CW / 4) + (piece ^ (ll & 7)); };
 #pragma unroll 1
       for (int i = 0; i < DP; i += CW) {
-        uint32_t v[CW];
-        tmem_load<CW>(t_o + i, v);
+        uint32_t o[CW];
+        tmem_load<CW>(t_o + i, o);
         tmem_wait_load();
 #pragma unroll
         for (int j = 0; j < CW / 4; ++j) {
           float4 e;
-          e.x = f == 0.0f ? 0.0f : __uint_as_float(v[4 * j]) * f;
-          e.y = f == 0.0f ? 0.0f : __uint_as_float(v[4 * j + 1]) * f;
-          e.z = f == 0.0f ? 0.0f : __uint_as_float(v[4 * j + 2]) * f;
-          e.w = f == 0.0f ? 0.0f : __uint_as_float(v[4 * j + 3]) * f;
+          e.x = f == 0.0f ? 0.0f : __uint_as_float(o[4 * j]) * f;
+          e.y = f == 0.0f ? 0.0f : __uint_as_float(o[4 * j + 1]) * f;
+          e.z = f == 0.0f ? 0.0f : __uint_as_float(o[4 * j + 2]) * f;
+          e.w = f == 0.0f ? 0.0f : __uint_as_float(o[4 * j + 3]) * f;
           buf[place(g, L, j)] = e;
         }
         group_sync(1, 256);
-        if (mine) {
+        // neighbouring threads take neighbouring pieces of a row
+        for (int x = tid; x < here * (CW / 4); x += 256) {
+          const int r = x / (CW / 4), j = x % (CW / 4), d = i + 4 * j;
+          float4 e = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-          for (int j = share; j < CW / 4; j += 2 * COPIES) {
-            float4 e = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-            for (int q = 0; q < 2 * COPIES; ++q) {
-              const float4 y = buf[place(q & 1, (q >> 1) * (kM / COPIES) + r0, j)];
-              e.x += y.x, e.y += y.y, e.z += y.z, e.w += y.w;
-            }
-            if (!whole) {
-              *reinterpret_cast<float4*>(keep + i + 4 * j) = e;
-            } else if (i + 4 * j < p.head_dim) {
-              if (!seen) e = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-              *reinterpret_cast<uint2*>(out + i + 4 * j) =
-                  make_uint2(pack2<T>(e.x * inv, e.y * inv), pack2<T>(e.z * inv, e.w * inv));
-            }
+          for (int q = 0; q < 2 * COPIES; ++q) {
+            const float4 y = buf[place(q & 1, (q >> 1) * (kM / COPIES) + r, j)];
+            e.x += y.x, e.y += y.y, e.z += y.z, e.w += y.w;
+          }
+          if (!whole) {
+            *reinterpret_cast<float4*>(keep + r * (DP + 4) + d) = e;
+          } else if (d < p.head_dim) {
+            const float2 k2 = s_ml[r];
+            if (k2.y == 0.0f) e = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            T* dst = out_row<T>(p, b, node0 + r / p.group, h * p.group + r % p.group) + d;
+            *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<T>(e.x * k2.x, e.y * k2.x), pack2<T>(e.z * k2.x, e.w * k2.x));
           }
         }
         group_sync(1, 256);
       }
-      if (mine && share == 0) {
+      if (leads) {
         if (whole) {
-          if (spoiled & mask) add_spoiled<T>(p, b, h, node, qh, spoiled & mask, top, inv, out);
+          if (spoiled & mask)
+            add_spoiled<T>(p, b, h, node, qh, spoiled & mask, top, inv, out_row<T>(p, b, node, qh));
           p.lse[((size_t)b * p.nodes + node) * p.kv_heads * p.group + qh] =
               total != 0.0f && seen ? kLn2 * (top + log2f(total)) : -INFINITY;
         } else {
-          *reinterpret_cast<float4*>(keep + DP) =
+          *reinterpret_cast<float4*>(keep + r0 * (DP + 4) + DP) =
               make_float4(top, total, __uint_as_float((uint32_t)spoiled), __uint_as_float((uint32_t)(spoiled >> 32)));
         }
       }
-      if (tid == 0) *s_spoiled = 0ull;
+      if (tid == 0) {
+        *s_spoiled = 0ull;
+        if constexpr (PANELS == 2) smem_fence_async();  // the copy of a later Q follows the sums that met here
+        mbar_arrive(q_empty(u & 1));
+      }
+      ++u;
+      if (warp == 0 && more) reader.masks(s_mask + (u & 1) * kMaxNodes, reinterpret_cast<int*>(s_ml));
       tmem_fence_before();
       k += 2 * n;
       w += n;
-      at.next_unit(p, units);
+      at = then;
     }
   }
   if (!fine && (warp < 8 || lane == 0)) atomicAdd(faults, 1u);
@@ -787,20 +821,23 @@ __global__ void __launch_bounds__(256) join_tc_kernel(const __grid_constant__ At
   constexpr int DP = 64 * PANELS;
   __shared__ uint64_t s_mask[8][kMaxNodes];
   __shared__ int s_jump[8][kMaxNodes];
-  CKKS_PDL_ENTRY();
-  const int rows = p.nodes * p.group, tiles_r = (rows + kM - 1) / kM, units = p.kv_heads * tiles_r;
+  const int rows = p.nodes * p.group;
+  const int tiles_r = (p.nodes + p.tile_nodes - 1) / p.tile_nodes, units = p.kv_heads * tiles_r;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int per = (rows + 7) / 8;  // CTAs of a (sequence, head)
   const int bh = blockIdx.x / per, row = blockIdx.x % per * 8 + warp;
   const int b = bh / p.kv_heads, h = bh % p.kv_heads;
-  if (row >= rows) return;
-  const int unit = h * tiles_r + row / kM, r = row % kM;
+  if (row >= rows) {
+    CKKS_PDL_ENTRY();
+    return;
+  }
+  const int tile_rows = p.tile_nodes * p.group, unit = h * tiles_r + row / tile_rows, r = row % tile_rows;
   // this unit's tiles [u0, u1) of the list, and the CTAs that have the first
   // and the last: CTA i begins at part_start(i), so w is CTA
   // floor((ctas (w + 1) - 1) / entries)'s
   int before = 0, all = 0;
   for (int i = lane; i < p.batch; i += 32) {
-    const int t = tiles_of(p, i) + kUnitCost;
+    const int t = tiles_of(p, i) + unit_cost(p);
     all += t;
     if (i < b) before += t;
   }
@@ -810,14 +847,17 @@ __global__ void __launch_bounds__(256) join_tc_kernel(const __grid_constant__ At
     before += __shfl_xor_sync(0xffffffffu, before, o);
   }
   const int tiles = tiles_of(p, b);
-  const long long W = (long long)all * units, u0 = (long long)before * units + unit * (tiles + kUnitCost) + kUnitCost;
+  const long long W = (long long)all * units, u0 = (long long)before * units + unit * (tiles + unit_cost(p)) + unit_cost(p);
   const int c0 = (int)((ctas * (u0 + 1) - 1) / W), c1 = (int)((ctas * (u0 + tiles) - 1) / W);
-  if (c0 == c1) return;
+  if (c0 == c1) {
+    CKKS_PDL_ENTRY();
+    return;
+  }
   tree_masks(p.parents + (size_t)b * p.nodes, p.nodes, s_mask[warp], s_jump[warp]);
   const int node = row / p.group, qh = h * p.group + row % p.group;
   const uint64_t mask = s_mask[warp][node];
-  const int stride = min(rows, kM);
-  auto part = [&](int i) { return p.part + ((size_t)(2 * i + (i == c0 ? 1 : 0)) * stride + r) * (DP + 4); };
+  CKKS_PDL_ENTRY();  // what is read above no kernel of this call writes
+  auto part = [&](int i) { return p.part + ((size_t)(2 * i + (i == c0 ? 1 : 0)) * tile_rows + r) * (DP + 4); };
   // with fewer entries than CTAs some have none and wrote nothing
   auto idle = [&](int i) { return W < ctas && part_start((int)W, i, ctas) == part_start((int)W, i + 1, ctas); };
   float m = -INFINITY;
@@ -910,24 +950,27 @@ void check_shape(const ckks_draft_attention_args& a) {
        "sizes too large");
 }
 
+bool tc_sizes(const ckks_draft_attention_args& a) {
+  return a.dtype != CKKS_FP32 && a.head_dim <= 128 && a.head_dim % 8 == 0 && a.q_heads / a.kv_heads <= kM;
+}
+
+// nodes whose rows a tile holds
+int tile_nodes(const ckks_draft_attention_args& a) { return std::min(a.nodes, kM / (a.q_heads / a.kv_heads)); }
+
 // Tensor-core CTAs: one on each SM, but no fewer than four tiles of keys
 // each at the full capacity (a shorter part is all start-up), and one for
 // each unit where there are fewer units than that
 int tc_ctas(const Context& c, const ckks_draft_attention_args& a) {
-  const long long rows = (long long)a.nodes * (a.q_heads / a.kv_heads);
-  const long long units = (long long)a.batch * a.kv_heads * ((rows + kM - 1) / kM);
+  const int per = tile_nodes(a);
+  const long long units = (long long)a.batch * a.kv_heads * ((a.nodes + per - 1) / per);
   const long long tiles = units * ((a.capacity + kKeys - 1) / kKeys + 1), slots = c.sms;
   return (int)std::max(1ll, std::min(slots, std::max(tiles / 4, units)));
 }
 
 // one sequence and a CTA for each unit: no unit is shared
 bool tc_alone(const ckks_draft_attention_args& a, int ctas) {
-  const int rows = a.nodes * (a.q_heads / a.kv_heads);
-  return a.batch == 1 && ctas == a.kv_heads * ((rows + kM - 1) / kM);
-}
-
-bool tc_sizes(const ckks_draft_attention_args& a) {
-  return a.dtype != CKKS_FP32 && a.head_dim <= 128 && a.head_dim % 8 == 0;
+  const int per = tile_nodes(a);
+  return a.batch == 1 && ctas == a.kv_heads * ((a.nodes + per - 1) / per);
 }
 
 size_t workspace_of(const Context& c, const ckks_draft_attention_args& a) {
@@ -936,7 +979,7 @@ size_t workspace_of(const Context& c, const ckks_draft_attention_args& a) {
   size_t n = s == 1 ? 0 : (size_t)a.batch * a.q_heads * a.nodes * s * (a.head_dim + 2);
   if (tc_sizes(a)) {
     // tensors whose rows are not aligned pieces take the other kernel
-    const int g = tc_ctas(c, a), rows = std::min(kM, a.nodes * (a.q_heads / a.kv_heads));
+    const int g = tc_ctas(c, a), rows = tile_nodes(a) * (a.q_heads / a.kv_heads);
     if (!tc_alone(a, g)) n = std::max(n, (size_t)2 * g * rows * (a.head_dim <= 64 ? 64 + 4 : 128 + 4));
   }
   return sizeof(float) * n;
@@ -955,16 +998,17 @@ EncodeTiled encode_tiled() {
   return f;
 }
 
-// [batch][heads][rows][head_dim] in boxes of 128 rows x 64 elements; what a
-// box has outside the tensor reads as 0
-bool tile_map(CUtensorMap* m, const ckks_rows& r, int dtype, int batch, int heads, int rows, int head_dim) {
+// [batch][outer][inner][head_dim] in boxes of box_outer x box_inner rows of 64
+// elements; what a box has outside the tensor reads as 0
+bool tile_map(CUtensorMap* m, void* data, int dtype, int head_dim, int inner, int64_t inner_stride, int box_inner,
+              int outer, int64_t outer_stride, int box_outer, int batch, int64_t batch_stride) {
   const EncodeTiled f = encode_tiled();
   if (!f) return false;
   auto bytes = [](int64_t s, int n) { return n > 1 ? (cuuint64_t)s * 2 : (cuuint64_t)16; };
-  const cuuint64_t dims[4] = {(cuuint64_t)head_dim, (cuuint64_t)rows, (cuuint64_t)heads, (cuuint64_t)batch};
-  const cuuint64_t strides[3] = {bytes(r.row, rows), bytes(r.head, heads), bytes(r.batch, batch)};
-  const cuuint32_t box[4] = {64, (cuuint32_t)kKeys, 1, 1}, ones[4] = {1, 1, 1, 1};
-  return f(m, dtype == CKKS_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, r.data, dims,
+  const cuuint64_t dims[4] = {(cuuint64_t)head_dim, (cuuint64_t)inner, (cuuint64_t)outer, (cuuint64_t)batch};
+  const cuuint64_t strides[3] = {bytes(inner_stride, inner), bytes(outer_stride, outer), bytes(batch_stride, batch)};
+  const cuuint32_t box[4] = {64, (cuuint32_t)box_inner, (cuuint32_t)box_outer, 1}, ones[4] = {1, 1, 1, 1};
+  return f(m, dtype == CKKS_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, data, dims,
            strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
@@ -976,6 +1020,7 @@ void launch_tc(const Context& c, const ckks_draft_attention_args& a, const AttnP
   auto* k = attend_tc_kernel<T, PANELS, COPIES>;
   CKKS_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::kSmem));
   const int ctas = tc_ctas(c, a), rows = p.nodes * p.group;
+  static_assert(S::kSmem <= 232448, "shared memory of one block");
   // a scale of 0 becomes one that changes no weight: a masked score times 0 would be no number
   const float factor = std::max(std::fabs(p.scale) * kLog2e, 1e-30f);
   k<<<ctas, kTcThreads, S::kSmem, st>>>(p, maps, p.scale < 0.0f, factor, c.d_faults);
@@ -1000,13 +1045,18 @@ void launch_tc(const Context& c, const ckks_draft_attention_args& a, const AttnP
 template <typename T>
 bool run_tc(const Context& c, const ckks_draft_attention_args& a, const AttnParams& p, cudaStream_t st) {
   TileMaps m;
-  if (!tile_map(&m.kn, a.k_new, a.dtype, a.batch, a.kv_heads, a.nodes, a.head_dim) ||
-      !tile_map(&m.vn, a.v_new, a.dtype, a.batch, a.kv_heads, a.nodes, a.head_dim))
+  // keys and values: 128 rows of one head
+  auto rows_map = [&](CUtensorMap* t, const ckks_rows& r, int rows) {
+    return tile_map(t, r.data, a.dtype, a.head_dim, rows, r.row, kKeys, a.kv_heads, r.head, 1, a.batch, r.batch);
+  };
+  // queries: the heads on one key/value head, of a tile's nodes
+  if (!tile_map(&m.q, a.q.data, a.dtype, a.head_dim, a.q_heads, a.q.head, p.group, a.nodes, a.q.row, p.tile_nodes, a.batch,
+                a.q.batch) ||
+      !rows_map(&m.kn, a.k_new, a.nodes) || !rows_map(&m.vn, a.v_new, a.nodes))
     return false;
   if (a.capacity == 0) {
     m.kc = m.kn, m.vc = m.vn;  // not read
-  } else if (!tile_map(&m.kc, a.k_cache, a.dtype, a.batch, a.kv_heads, a.capacity, a.head_dim) ||
-             !tile_map(&m.vc, a.v_cache, a.dtype, a.batch, a.kv_heads, a.capacity, a.head_dim)) {
+  } else if (!rows_map(&m.kc, a.k_cache, a.capacity) || !rows_map(&m.vc, a.v_cache, a.capacity)) {
     return false;
   }
   if (a.head_dim <= 64)
@@ -1062,7 +1112,7 @@ extern "C" int ckks_draft_attention(ckks_ctx* ctx, const ckks_draft_attention_ar
     p.lens = a.lens, p.parents = a.parents, p.lse = a.lse, p.part = static_cast<float*>(a.workspace);
     p.batch = a.batch, p.kv_heads = a.kv_heads, p.group = a.q_heads / a.kv_heads, p.head_dim = a.head_dim;
     p.nodes = a.nodes, p.capacity = a.capacity, p.scale = (float)a.scale;
-    p.splits = split_count(c, a);
+    p.splits = split_count(c, a), p.tile_nodes = tile_nodes(a);
     p.wide = wide_rows(a.q, a.batch, a.q_heads, a.nodes, a.head_dim, e) &&
              wide_rows(a.out, a.batch, a.q_heads, a.nodes, a.head_dim, e) &&
              wide_rows(a.k_new, a.batch, a.kv_heads, a.nodes, a.head_dim, e) &&
