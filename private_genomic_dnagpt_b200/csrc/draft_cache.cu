@@ -71,9 +71,10 @@ struct AccParams {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kAccKeys = 128, kAccRows = 8;
 
-// CTA = (sequence x head, 128 keys): one key per thread, the accepted rows
-// in shared memory eight at a time; a key's weights are added in the order of
-// the rows, so results do not depend on timing
+// Any stride, size and alignment.  CTA = (sequence x head, 128 keys): one key
+// per thread, the accepted rows in shared memory eight at a time; a key's
+// weights are added in the order of the rows, so results do not depend on
+// timing
 template <typename T>
 __global__ void __launch_bounds__(kAccKeys) accumulate_kernel(AccParams p) {
   __shared__ float sq[kAccRows][kMaxHeadDim], sl[kAccRows];
@@ -117,6 +118,173 @@ __global__ void __launch_bounds__(kAccKeys) accumulate_kernel(AccParams p) {
     if (s < total) {
       float* a = static_cast<float*>(p.acc.data) + b * p.acc.batch + h * p.acc.head + s;
       *a = s < len ? *a + sum : sum;
+    }
+  }
+}
+
+// Rows of whole, aligned 16-byte pieces.  The accepted rows (a few nodes times
+// the query heads on a key/value head) are few, so this streams K once: a warp
+// takes 16 keys at a time as the A operand of 16 x 8 matrix products straight
+// from global memory, with no shared memory between.  The order of the
+// products along head_dim is free as long as both operands have the same one:
+// lane t of a quad reads the 16-byte pieces t, t + 4, ... of its two keys and
+// uses each as two steps' elements, which the q rows in shared memory follow.
+// 16 pieces of a lane are in flight at once (8 KB a warp).  The exponentials
+// of a key lie in one quad, so its sum is two shuffles; a key's weights are
+// added in a fixed order.
+// float32 rows are split in two tensor-float parts, x = hi + lo, and
+// multiplied as hi hi + hi lo + lo hi: products to 2^-21.
+template <typename T>
+struct Pieces {
+  // products of one pair of pieces (keys g and g + 8) with one q piece
+  __device__ __forceinline__ static void mac(float* c, const uint4& a, const uint4& b, const uint4& q) {
+    step(c, a.x, b.x, a.y, b.y, q.x, q.y);
+    step(c, a.z, b.z, a.w, b.w, q.z, q.w);
+  }
+  __device__ __forceinline__ static void step(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                              uint32_t b1) {
+    if constexpr (std::is_same_v<T, __nv_bfloat16>)
+      asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+          : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+          : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    else
+      asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+          : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+          : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  }
+};
+
+template <>
+struct Pieces<float> {
+  __device__ __forceinline__ static uint32_t hi(uint32_t x) {
+    uint32_t y;
+    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(y) : "f"(__uint_as_float(x)));
+    return y;
+  }
+  // of an infinity nothing is left
+  __device__ __forceinline__ static uint32_t lo(uint32_t x) {
+    const float h = __uint_as_float(hi(x));
+    return fabsf(h) == INFINITY ? 0u : hi(__float_as_uint(__uint_as_float(x) - h));
+  }
+  __device__ __forceinline__ static void step(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                              uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  }
+  __device__ __forceinline__ static void both(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                              uint32_t b1) {
+    step(c, lo(a0), lo(a1), lo(a2), lo(a3), hi(b0), hi(b1));
+    step(c, hi(a0), hi(a1), hi(a2), hi(a3), lo(b0), lo(b1));
+    step(c, hi(a0), hi(a1), hi(a2), hi(a3), hi(b0), hi(b1));
+  }
+  __device__ __forceinline__ static void mac(float* c, const uint4& a, const uint4& b, const uint4& q) {
+    both(c, a.x, b.x, a.y, b.y, q.x, q.y);
+    both(c, a.z, b.z, a.w, b.w, q.z, q.w);
+  }
+};
+
+constexpr int kStreamWarps = 8, kStreamRows = 64;  // warps of a CTA; q rows in shared memory at once
+
+// JC: 16-byte pieces of a key's row for each lane of its quad
+template <typename T, int JC>
+__global__ void __launch_bounds__(32 * kStreamWarps, sizeof(T) == 4 || JC > 4 ? 1 : 2)
+    accumulate_stream_kernel(AccParams p, int steps) {
+  constexpr int W = 16 / sizeof(T), U = JC < 8 ? 8 / JC : 1;  // elements of a piece; tiles of 16 keys at once
+  // q in the order of the products: [8 rows][piece][lane]
+  extern __shared__ __align__(16) uint4 s_q[];
+  __shared__ float s_lse[kStreamRows];
+  const int b = blockIdx.x / p.kv_heads, h = blockIdx.x % p.kv_heads;
+  const int32_t* path = p.path + (size_t)b * p.nodes;
+  const int len = p.lens[b], count = p.count[b], D = p.head_dim;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  constexpr int kStep = 16 * U;  // keys of one warp's step
+  const int first = blockIdx.y * steps * kStreamWarps * kStep;
+  if (count <= 0 || !fits(path, count, len, p.nodes, p.capacity) || first >= len + count) return;
+  const int total = len + count, rows = count * p.group;
+  const T* kc = static_cast<const T*>(p.kc.data) + b * p.kc.batch + h * p.kc.head;
+  float* acc = static_cast<float*>(p.acc.data) + b * p.acc.batch + h * p.acc.head;
+  for (int r0 = 0; r0 < rows; r0 += kStreamRows) {
+    const int groups = (min(kStreamRows, rows - r0) + 7) / 8;
+    __syncthreads();
+    for (int i = threadIdx.x; i < groups * JC * 32; i += 32 * kStreamWarps) {
+      const int ln = i & 31, j = (i >> 5) % JC, row = r0 + (i >> 5) / JC * 8 + (ln >> 2), d = ((ln & 3) + 4 * j) * W;
+      uint4 v = make_uint4(0, 0, 0, 0);
+      if (row < rows && d < D) {
+        const int node = path[row / p.group], qh = h * p.group + row % p.group;
+        v = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.q.data) + b * p.q.batch + qh * p.q.head +
+                                            node * p.q.row + d);
+      }
+      s_q[i] = v;
+    }
+    if (threadIdx.x < kStreamRows) {
+      const int row = r0 + threadIdx.x;
+      // a row that is not there weighs nothing
+      s_lse[threadIdx.x] = INFINITY;
+      if (row < rows)
+        s_lse[threadIdx.x] = kLog2e * p.lse[((size_t)b * p.nodes + path[row / p.group]) * p.kv_heads * p.group +
+                                            h * p.group + row % p.group];
+    }
+    __syncthreads();
+    const float c2 = p.scale * kLog2e;
+    for (int it = 0; it < steps; ++it) {
+      const int k0 = first + (it * kStreamWarps + warp) * kStep;
+      if (k0 >= total) break;
+      uint4 a[U][2][JC];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int half = 0; half < 2; ++half)
+#pragma unroll
+          for (int j = 0; j < JC; ++j) {
+            const int s = k0 + 16 * u + g + 8 * half, d = (t + 4 * j) * W;
+            a[u][half][j] = s < total && d < D ? *reinterpret_cast<const uint4*>(kc + s * p.kc.row + d)
+                                               : make_uint4(0, 0, 0, 0);
+          }
+      float sum[U][2];
+#pragma unroll
+      for (int u = 0; u < U; ++u) sum[u][0] = sum[u][1] = 0.0f;
+      for (int gr = 0; gr < groups; ++gr) {
+        float c[U][4];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) c[u][e] = 0.0f;
+#pragma unroll
+        for (int j = 0; j < JC; ++j) {
+          const uint4 q = s_q[(gr * JC + j) * 32 + lane];
+#pragma unroll
+          for (int u = 0; u < U; ++u) Pieces<T>::mac(c[u], a[u][0][j], a[u][1][j], q);
+        }
+        const int row = gr * 8 + 2 * t;  // the lane's two rows
+        const float l0 = s_lse[row], l1 = s_lse[row + 1];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          float e[4] = {exp2f(fmaf(c[u][0], c2, -l0)), exp2f(fmaf(c[u][1], c2, -l1)), exp2f(fmaf(c[u][2], c2, -l0)),
+                        exp2f(fmaf(c[u][3], c2, -l1))};
+          const int s = k0 + 16 * u + g;
+          if (k0 + kStep > len || r0 + gr * 8 + 8 > rows) {
+            // among the appended keys a row sees those up to its own
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              const int rr = r0 + row + (x & 1);
+              if (rr >= rows || s + 8 * (x >> 1) > len + rr / p.group) e[x] = 0.0f;
+            }
+          }
+          sum[u][0] += e[0] + e[1];
+          sum[u][1] += e[2] + e[3];
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          float x = sum[u][half];
+          x += __shfl_xor_sync(0xffffffffu, x, 1);
+          x += __shfl_xor_sync(0xffffffffu, x, 2);
+          const int s = k0 + 16 * u + g + 8 * half;
+          if (t == 0 && s < total) acc[s] = r0 > 0 || s < len ? acc[s] + x : x;
+        }
     }
   }
 }
@@ -247,6 +415,32 @@ __global__ void __launch_bounds__(256) gather_kernel(EvictParams p) {
   }
 }
 
+template <typename T, int JC>
+void launch_stream(const Context& c, const AccParams& p, cudaStream_t st) {
+  // keys of one step of a CTA; as many steps as leave four CTAs for each SM
+  constexpr int kKeys = kStreamWarps * 16 * (JC < 8 ? 8 / JC : 1);
+  const long long heads = (long long)p.batch * p.kv_heads, all = (p.capacity + kKeys - 1) / kKeys;
+  const int steps = (int)std::max(1ll, std::min(all, heads * all / (4ll * c.sms)));
+  const long long y = (all + steps - 1) / steps;
+  const size_t smem = (size_t)(std::min(kStreamRows, p.nodes * p.group) + 7) / 8 * JC * 32 * sizeof(uint4);
+  need(y <= 65535, "sizes too large");
+  accumulate_stream_kernel<T, JC><<<dim3((unsigned)heads, (unsigned)y), 32 * kStreamWarps, smem, st>>>(p, steps);
+  CKKS_CUDA(cudaGetLastError());
+}
+
+template <typename T>
+void run_stream(const Context& c, const AccParams& p, cudaStream_t st) {
+  const int pieces = (p.head_dim * (int)sizeof(T) / 16 + 3) / 4;
+  if (pieces <= 2)
+    launch_stream<T, 2>(c, p, st);
+  else if (pieces <= 4)
+    launch_stream<T, 4>(c, p, st);
+  else if (sizeof(T) == 2 || pieces <= 8)
+    launch_stream<T, 8>(c, p, st);
+  else if constexpr (sizeof(T) == 4)
+    launch_stream<T, 16>(c, p, st);
+}
+
 void check_cache(int dtype, int batch, int kv_heads, int head_dim, int capacity) {
   need(dtype == CKKS_BF16 || dtype == CKKS_FP16 || dtype == CKKS_FP32,
        "caches are CKKS_BF16, CKKS_FP16 or CKKS_FP32");
@@ -333,6 +527,16 @@ extern "C" int ckks_draft_accumulate(ckks_ctx* ctx, const ckks_draft_accumulate_
     OnDevice dev(c);
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     ProfScope ps(c, "draft_accumulate", (double)e * a.batch * a.kv_heads * a.capacity * a.head_dim, st);
+    if (wide_rows(a.q, a.batch, a.q_heads, a.nodes, a.head_dim, e) &&
+        wide_rows(a.k_cache, a.batch, a.kv_heads, a.capacity, a.head_dim, e)) {
+      if (a.dtype == CKKS_BF16)
+        run_stream<__nv_bfloat16>(c, p, st);
+      else if (a.dtype == CKKS_FP16)
+        run_stream<__half>(c, p, st);
+      else
+        run_stream<float>(c, p, st);
+      return;
+    }
     const dim3 grid((unsigned)(a.batch * a.kv_heads), (unsigned)std::min(65535, (a.capacity + kAccKeys - 1) / kAccKeys));
     if (a.dtype == CKKS_BF16)
       accumulate_kernel<__nv_bfloat16><<<grid, kAccKeys, 0, st>>>(p);
