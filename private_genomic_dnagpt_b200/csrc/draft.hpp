@@ -121,6 +121,60 @@ __device__ __forceinline__ T from_f32(float x) {
     return (T)x;
 }
 
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// A list of work whose length only the device knows: sequence b has `units`
+// units of entries_of(b) entries each, one after the other.  CTA i of n takes
+// the entries from list_start(i) to list_start(i + 1).
+__device__ __forceinline__ int list_start(int entries, int i, int n) {
+  return entries / n * i + (int)((unsigned)(entries % n) * (unsigned)i / (unsigned)n);
+}
+
+// entries of one unit of every sequence, summed; by a whole warp.  `first`:
+// those of sequence `lane`
+template <class F>
+__device__ __forceinline__ int list_sum(int batch, F entries_of, int& first) {
+  const int lane = threadIdx.x & 31;
+  first = lane < batch ? entries_of(lane) : 0;
+  int s = first;
+  for (int b = lane + 32; b < batch; b += 32) s += entries_of(b);
+#pragma unroll
+  for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  return s;
+}
+
+struct ListPlace {
+  int b, unit, entry, entries;  // sequence, its unit, the entry within that, the unit's entries
+};
+
+// entry `w` of the list; by a whole warp
+template <class F>
+__device__ __forceinline__ ListPlace list_find(int batch, int units, int w, int first, F entries_of) {
+  const int lane = threadIdx.x & 31;
+  int before = 0;
+  for (int b0 = 0;; b0 += 32) {
+    const int t = b0 == 0 ? first : b0 + lane < batch ? entries_of(b0 + lane) : 0;
+    int sum = t * units;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, sum, o);
+      if (lane >= o) sum += y;
+    }
+    const uint32_t past = __ballot_sync(0xffffffffu, before + sum > w);
+    if (past || b0 + 32 >= batch) {
+      const int k = past ? __ffs(past) - 1 : 31;
+      const int tk = max(1, __shfl_sync(0xffffffffu, t, k));
+      const int off = w - (before + __shfl_sync(0xffffffffu, sum, k) - tk * units);
+      return {b0 + k, off / tk, off % tk, tk};
+    }
+    before += __shfl_sync(0xffffffffu, sum, 31);
+  }
+}
+
 // Ancestor masks of one tree, by one warp, in two steps: the parents into
 // registers, then mask[i] gets the bits of node i and of the nodes above it, 0
 // where i is padding.  Six rounds of pointer doubling cover every depth up to

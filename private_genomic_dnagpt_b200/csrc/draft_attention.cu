@@ -352,52 +352,6 @@ struct Cursor {
   }
 };
 
-// first entry of part i of n
-__device__ __forceinline__ int part_start(int entries, int i, int n) {
-  return entries / n * i + (int)((unsigned)(entries % n) * (unsigned)i / (unsigned)n);
-}
-
-// entries of one unit of every sequence, summed; by a whole warp.  `first`:
-// those of sequence `lane`
-__device__ __forceinline__ int entry_sum(const AttnParams& p, int& first) {
-  const int lane = threadIdx.x & 31;
-  first = lane < p.batch ? tiles_of(p, lane) + unit_cost(p) : 0;
-  int s = first;
-  for (int b = lane + 32; b < p.batch; b += 32) s += tiles_of(p, b) + unit_cost(p);
-#pragma unroll
-  for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-  return s;
-}
-
-// entry `w` of the list; by a whole warp
-__device__ __forceinline__ Cursor find_entry(const AttnParams& p, int units, int w, int first) {
-  const int lane = threadIdx.x & 31;
-  int before = 0;
-  for (int b0 = 0;; b0 += 32) {
-    const int t = b0 == 0 ? first : b0 + lane < p.batch ? tiles_of(p, b0 + lane) + unit_cost(p) : 0;
-    int sum = t * units;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int y = __shfl_up_sync(0xffffffffu, sum, o);
-      if (lane >= o) sum += y;
-    }
-    const uint32_t past = __ballot_sync(0xffffffffu, before + sum > w);
-    if (past || b0 + 32 >= p.batch) {
-      const int k = past ? __ffs(past) - 1 : 31;
-      const int tk = max(1, __shfl_sync(0xffffffffu, t, k));
-      const int off = w - (before + __shfl_sync(0xffffffffu, sum, k) - tk * units);
-      return {b0 + k, off / tk, off % tk - unit_cost(p), tk - unit_cost(p)};
-    }
-    before += __shfl_sync(0xffffffffu, sum, 31);
-  }
-}
-
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
 template <typename T>
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
   if constexpr (std::is_same_v<T, __nv_bfloat16>) {
@@ -480,9 +434,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   if (warp == 9) tmem_alloc(smem_addr(s_tmem), kTmemCols);
   // this CTA's entries [w0, w1) of the list
   int first;
-  const int entries = entry_sum(p, first) * units;
-  const int w0 = part_start(entries, blockIdx.x, gridDim.x), w1 = part_start(entries, blockIdx.x + 1, gridDim.x);
-  Cursor at = find_entry(p, units, w0, first);
+  auto entries_of = [&](int b) { return tiles_of(p, b) + unit_cost(p); };
+  const int entries = list_sum(p.batch, entries_of, first) * units;
+  const int w0 = list_start(entries, blockIdx.x, gridDim.x), w1 = list_start(entries, blockIdx.x + 1, gridDim.x);
+  const ListPlace begin = list_find(p.batch, units, w0, first, entries_of);
+  Cursor at = {begin.b, begin.unit, begin.entry - unit_cost(p), begin.entries - unit_cost(p)};
   tmem_fence_before();
   __syncthreads();
   tmem_fence_after();
@@ -833,7 +789,7 @@ __global__ void __launch_bounds__(256) join_tc_kernel(const __grid_constant__ At
   }
   const int tile_rows = p.tile_nodes * p.group, unit = h * tiles_r + row / tile_rows, r = row % tile_rows;
   // this unit's tiles [u0, u1) of the list, and the CTAs that have the first
-  // and the last: CTA i begins at part_start(i), so w is CTA
+  // and the last: CTA i begins at list_start(i), so w is CTA
   // floor((ctas (w + 1) - 1) / entries)'s
   int before = 0, all = 0;
   for (int i = lane; i < p.batch; i += 32) {
@@ -859,7 +815,7 @@ __global__ void __launch_bounds__(256) join_tc_kernel(const __grid_constant__ At
   CKKS_PDL_ENTRY();  // what is read above no kernel of this call writes
   auto part = [&](int i) { return p.part + ((size_t)(2 * i + (i == c0 ? 1 : 0)) * tile_rows + r) * (DP + 4); };
   // with fewer entries than CTAs some have none and wrote nothing
-  auto idle = [&](int i) { return W < ctas && part_start((int)W, i, ctas) == part_start((int)W, i + 1, ctas); };
+  auto idle = [&](int i) { return W < ctas && list_start((int)W, i, ctas) == list_start((int)W, i + 1, ctas); };
   float m = -INFINITY;
   for (int i = c0 + lane; i <= c1; i += 32)
     if (!idle(i)) m = fmaxf(m, part(i)[DP]);

@@ -186,105 +186,149 @@ struct Pieces<float> {
 
 constexpr int kStreamWarps = 8, kStreamRows = 64;  // warps of a CTA; q rows in shared memory at once
 
-// JC: 16-byte pieces of a key's row for each lane of its quad
+// 16-byte pieces of a key's row for each lane of its quad -> tiles of 16 keys a warp reads at once
+constexpr int stream_tiles(int jc) { return jc <= 2 ? 2 : 1; }
+
+// keys of sequence b that get weight: none where nothing is accepted
+__device__ __forceinline__ int weighed_keys(const AccParams& p, int b) {
+  const int len = p.lens[b], count = p.count[b];
+  return count > 0 && fits(p.path + (size_t)b * p.nodes, count, len, p.nodes, p.capacity) ? len + count : 0;
+}
+
+// The CTAs divide the list of all heads' keys evenly (their number is known
+// on the device only), in entries of one step of a CTA.
 template <typename T, int JC>
 __global__ void __launch_bounds__(32 * kStreamWarps, sizeof(T) == 4 || JC > 4 ? 1 : 2)
-    accumulate_stream_kernel(AccParams p, int steps) {
-  constexpr int W = 16 / sizeof(T), U = JC < 8 ? 8 / JC : 1;  // elements of a piece; tiles of 16 keys at once
+    accumulate_stream_kernel(AccParams p) {
+  constexpr int W = 16 / sizeof(T), U = stream_tiles(JC);
+  constexpr int kWarpKeys = 16 * U, kStep = kStreamWarps * kWarpKeys;
   // q in the order of the products: [8 rows][piece][lane]
   extern __shared__ __align__(16) uint4 s_q[];
   __shared__ float s_lse[kStreamRows];
-  const int b = blockIdx.x / p.kv_heads, h = blockIdx.x % p.kv_heads;
-  const int32_t* path = p.path + (size_t)b * p.nodes;
-  const int len = p.lens[b], count = p.count[b], D = p.head_dim;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  constexpr int kStep = 16 * U;  // keys of one warp's step
-  const int first = blockIdx.y * steps * kStreamWarps * kStep;
-  if (count <= 0 || !fits(path, count, len, p.nodes, p.capacity) || first >= len + count) return;
-  const int total = len + count, rows = count * p.group;
-  const T* kc = static_cast<const T*>(p.kc.data) + b * p.kc.batch + h * p.kc.head;
-  float* acc = static_cast<float*>(p.acc.data) + b * p.acc.batch + h * p.acc.head;
-  for (int r0 = 0; r0 < rows; r0 += kStreamRows) {
-    const int groups = (min(kStreamRows, rows - r0) + 7) / 8;
-    __syncthreads();
-    for (int i = threadIdx.x; i < groups * JC * 32; i += 32 * kStreamWarps) {
-      const int ln = i & 31, j = (i >> 5) % JC, row = r0 + (i >> 5) / JC * 8 + (ln >> 2), d = ((ln & 3) + 4 * j) * W;
-      uint4 v = make_uint4(0, 0, 0, 0);
-      if (row < rows && d < D) {
-        const int node = path[row / p.group], qh = h * p.group + row % p.group;
-        v = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.q.data) + b * p.q.batch + qh * p.q.head +
-                                            node * p.q.row + d);
-      }
-      s_q[i] = v;
-    }
-    if (threadIdx.x < kStreamRows) {
-      const int row = r0 + threadIdx.x;
-      // a row that is not there weighs nothing
-      s_lse[threadIdx.x] = INFINITY;
-      if (row < rows)
-        s_lse[threadIdx.x] = kLog2e * p.lse[((size_t)b * p.nodes + path[row / p.group]) * p.kv_heads * p.group +
-                                            h * p.group + row % p.group];
-    }
-    __syncthreads();
-    const float c2 = p.scale * kLog2e;
-    for (int it = 0; it < steps; ++it) {
-      const int k0 = first + (it * kStreamWarps + warp) * kStep;
-      if (k0 >= total) break;
-      uint4 a[U][2][JC];
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-#pragma unroll
-        for (int half = 0; half < 2; ++half)
-#pragma unroll
-          for (int j = 0; j < JC; ++j) {
-            const int s = k0 + 16 * u + g + 8 * half, d = (t + 4 * j) * W;
-            a[u][half][j] = s < total && d < D ? *reinterpret_cast<const uint4*>(kc + s * p.kc.row + d)
-                                               : make_uint4(0, 0, 0, 0);
-          }
-      float sum[U][2];
-#pragma unroll
-      for (int u = 0; u < U; ++u) sum[u][0] = sum[u][1] = 0.0f;
-      for (int gr = 0; gr < groups; ++gr) {
-        float c[U][4];
+  const int D = p.head_dim, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const float c2 = p.scale * kLog2e;
+  auto entries_of = [&](int b) { return (weighed_keys(p, b) + kStep - 1) / kStep; };
+  int first;
+  const int entries = list_sum(p.batch, entries_of, first) * p.kv_heads;
+  const int w0 = list_start(entries, blockIdx.x, gridDim.x), w1 = list_start(entries, blockIdx.x + 1, gridDim.x);
+  if (w0 >= w1) return;
+  ListPlace at = list_find(p.batch, p.kv_heads, w0, first, entries_of);
+  for (int w = w0; w < w1;) {
+    const int steps = min(at.entries - at.entry, w1 - w);
+    const int b = at.b, h = at.unit, len = p.lens[b], count = p.count[b], total = len + count, rows = count * p.group;
+    const int32_t* path = p.path + (size_t)b * p.nodes;
+    const T* kc = static_cast<const T*>(p.kc.data) + b * p.kc.batch + h * p.kc.head;
+    float* acc = static_cast<float*>(p.acc.data) + b * p.acc.batch + h * p.acc.head;
+    for (int r0 = 0; r0 < rows; r0 += kStreamRows) {
+      const int groups = (min(kStreamRows, rows - r0) + 7) / 8;
+      uint4 next[U][2][JC];
+      // the lane's pieces of its keys in step i
+      auto read = [&](int i) {
+        const int k0 = (at.entry + i) * kStep + warp * kWarpKeys;
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) c[u][e] = 0.0f;
+          for (int half = 0; half < 2; ++half)
 #pragma unroll
-        for (int j = 0; j < JC; ++j) {
-          const uint4 q = s_q[(gr * JC + j) * 32 + lane];
-#pragma unroll
-          for (int u = 0; u < U; ++u) Pieces<T>::mac(c[u], a[u][0][j], a[u][1][j], q);
-        }
-        const int row = gr * 8 + 2 * t;  // the lane's two rows
-        const float l0 = s_lse[row], l1 = s_lse[row + 1];
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-          float e[4] = {exp2f(fmaf(c[u][0], c2, -l0)), exp2f(fmaf(c[u][1], c2, -l1)), exp2f(fmaf(c[u][2], c2, -l0)),
-                        exp2f(fmaf(c[u][3], c2, -l1))};
-          const int s = k0 + 16 * u + g;
-          if (k0 + kStep > len || r0 + gr * 8 + 8 > rows) {
-            // among the appended keys a row sees those up to its own
-#pragma unroll
-            for (int x = 0; x < 4; ++x) {
-              const int rr = r0 + row + (x & 1);
-              if (rr >= rows || s + 8 * (x >> 1) > len + rr / p.group) e[x] = 0.0f;
+            for (int j = 0; j < JC; ++j) {
+              const int s = k0 + 16 * u + g + 8 * half, d = (t + 4 * j) * W;
+              next[u][half][j] = i < steps && s < total && d < D
+                                     ? *reinterpret_cast<const uint4*>(kc + s * p.kc.row + d)
+                                     : make_uint4(0, 0, 0, 0);
             }
-          }
-          sum[u][0] += e[0] + e[1];
-          sum[u][1] += e[2] + e[3];
+      };
+      read(0);
+      __syncthreads();
+      for (int i = threadIdx.x; i < groups * JC * 32; i += 32 * kStreamWarps) {
+        const int ln = i & 31, j = (i >> 5) % JC, row = r0 + (i >> 5) / JC * 8 + (ln >> 2), d = ((ln & 3) + 4 * j) * W;
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (row < rows && d < D) {
+          const int node = path[row / p.group], qh = h * p.group + row % p.group;
+          v = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.q.data) + b * p.q.batch + qh * p.q.head +
+                                              node * p.q.row + d);
         }
+        s_q[i] = v;
       }
+      if (threadIdx.x < kStreamRows) {
+        const int row = r0 + threadIdx.x;
+        // a row that is not there weighs nothing
+        s_lse[threadIdx.x] = INFINITY;
+        if (row < rows)
+          s_lse[threadIdx.x] = kLog2e * p.lse[((size_t)b * p.nodes + path[row / p.group]) * p.kv_heads * p.group +
+                                              h * p.group + row % p.group];
+      }
+      __syncthreads();
+      for (int i = 0; i < steps; ++i) {
+        const int k0 = (at.entry + i) * kStep + warp * kWarpKeys;
+        if (k0 >= total) break;
+        uint4 a[U][2][JC];
 #pragma unroll
-      for (int u = 0; u < U; ++u)
+        for (int u = 0; u < U; ++u)
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          float x = sum[u][half];
-          x += __shfl_xor_sync(0xffffffffu, x, 1);
-          x += __shfl_xor_sync(0xffffffffu, x, 2);
-          const int s = k0 + 16 * u + g + 8 * half;
-          if (t == 0 && s < total) acc[s] = r0 > 0 || s < len ? acc[s] + x : x;
+          for (int half = 0; half < 2; ++half)
+#pragma unroll
+            for (int j = 0; j < JC; ++j) a[u][half][j] = next[u][half][j];
+        read(i + 1);
+        // the weights so far of the keys whose sums this lane will write
+        float old[U][2], sum[U][2];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const int s = k0 + 16 * u + g + 8 * half;
+            old[u][half] = t == 0 && s < (r0 > 0 ? total : len) ? acc[s] : 0.0f;
+            sum[u][half] = 0.0f;
+          }
+        for (int gr = 0; gr < groups; ++gr) {
+          float c[U][4];
+#pragma unroll
+          for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) c[u][e] = 0.0f;
+#pragma unroll
+          for (int j = 0; j < JC; ++j) {
+            const uint4 q = s_q[(gr * JC + j) * 32 + lane];
+#pragma unroll
+            for (int u = 0; u < U; ++u) Pieces<T>::mac(c[u], a[u][0][j], a[u][1][j], q);
+          }
+          const int row = gr * 8 + 2 * t;  // the lane's two rows
+          const float2 l = *reinterpret_cast<const float2*>(s_lse + row);
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            float e[4] = {ex2(fmaf(c[u][0], c2, -l.x)), ex2(fmaf(c[u][1], c2, -l.y)), ex2(fmaf(c[u][2], c2, -l.x)),
+                          ex2(fmaf(c[u][3], c2, -l.y))};
+            const int s = k0 + 16 * u + g;
+            if (k0 + kWarpKeys > len || r0 + gr * 8 + 8 > rows) {
+              // among the appended keys a row sees those up to its own
+#pragma unroll
+              for (int x = 0; x < 4; ++x) {
+                const int rr = r0 + row + (x & 1);
+                if (rr >= rows || s + 8 * (x >> 1) > len + rr / p.group) e[x] = 0.0f;
+              }
+            }
+            sum[u][0] += e[0] + e[1];
+            sum[u][1] += e[2] + e[3];
+          }
         }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            float x = sum[u][half];
+            x += __shfl_xor_sync(0xffffffffu, x, 1);
+            x += __shfl_xor_sync(0xffffffffu, x, 2);
+            const int s = k0 + 16 * u + g + 8 * half;
+            if (t == 0 && s < total) acc[s] = old[u][half] + x;
+          }
+      }
+    }
+    w += steps;
+    at.entry = 0;
+    if (++at.unit == p.kv_heads) {
+      at.unit = 0;
+      do {
+        at.entries = ++at.b < p.batch ? entries_of(at.b) : 1;
+      } while (at.entries == 0);
     }
   }
 }
@@ -417,14 +461,13 @@ __global__ void __launch_bounds__(256) gather_kernel(EvictParams p) {
 
 template <typename T, int JC>
 void launch_stream(const Context& c, const AccParams& p, cudaStream_t st) {
-  // keys of one step of a CTA; as many steps as leave four CTAs for each SM
-  constexpr int kKeys = kStreamWarps * 16 * (JC < 8 ? 8 / JC : 1);
-  const long long heads = (long long)p.batch * p.kv_heads, all = (p.capacity + kKeys - 1) / kKeys;
-  const int steps = (int)std::max(1ll, std::min(all, heads * all / (4ll * c.sms)));
-  const long long y = (all + steps - 1) / steps;
+  constexpr int kKeys = kStreamWarps * 16 * stream_tiles(JC);  // of one entry
+  const long long entries = (long long)p.batch * p.kv_heads * ((p.capacity + kKeys - 1) / kKeys);
+  const unsigned ctas = (unsigned)std::min(entries, (sizeof(T) == 4 || JC > 4 ? 1ll : 2ll) * c.sms);
   const size_t smem = (size_t)(std::min(kStreamRows, p.nodes * p.group) + 7) / 8 * JC * 32 * sizeof(uint4);
-  need(y <= 65535, "sizes too large");
-  accumulate_stream_kernel<T, JC><<<dim3((unsigned)heads, (unsigned)y), 32 * kStreamWarps, smem, st>>>(p, steps);
+  auto* k = accumulate_stream_kernel<T, JC>;
+  if (smem > 48 << 10) CKKS_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  k<<<ctas, 32 * kStreamWarps, smem, st>>>(p);
   CKKS_CUDA(cudaGetLastError());
 }
 
@@ -447,7 +490,7 @@ void check_cache(int dtype, int batch, int kv_heads, int head_dim, int capacity)
   need(batch >= 0 && capacity >= 0, "negative batch or capacity");
   need(kv_heads >= 1 && kv_heads <= 65535, "key/value head count out of range");
   need(head_dim >= 1 && head_dim <= kMaxHeadDim, "head_dim outside 1..256");
-  need((long long)batch * kv_heads < (1ll << 31) - 1 && capacity < (1 << 30), "sizes too large");
+  need((long long)batch * kv_heads * (capacity / 128 + 1) < (1ll << 31) - 1 && capacity < (1 << 30), "sizes too large");
 }
 
 bool disjoint(const void* a0, const void* a1, const void* b0, const void* b1) { return a1 <= b0 || b1 <= a0; }
