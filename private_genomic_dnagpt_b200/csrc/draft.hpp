@@ -101,6 +101,42 @@ inline const char* end_of(const ckks_rows& r, int batch, int heads, int rows, in
   return static_cast<const char*>(r.data) + last * bytes;
 }
 
+// `clusters` clusters of C CTAs
+template <int C, class P>
+void launch_cluster(void (*kernel)(P), int clusters, int threads, cudaStream_t st, const P& params) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)clusters * C);
+  cfg.blockDim = dim3(threads);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = C;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  CKKS_CUDA(cudaLaunchKernelEx(&cfg, kernel, params));
+}
+
+// all CTAs of the cluster, and a value in CTA `rank`'s shared memory
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t cluster_addr(const void* p, int rank) {
+  uint32_t a;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(rank));
+  return a;
+}
+__device__ __forceinline__ int cluster_read(const int* p, int rank) {
+  int v;
+  asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(cluster_addr(p, rank)) : "memory");
+  return v;
+}
+__device__ __forceinline__ double cluster_read(const double* p, int rank) {
+  double v;
+  asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(v) : "r"(cluster_addr(p, rank)) : "memory");
+  return v;
+}
+
 template <typename T>
 __device__ __forceinline__ float to_f32(T x) {
   if constexpr (std::is_same_v<T, __nv_bfloat16>)

@@ -350,108 +350,215 @@ __device__ __forceinline__ uint32_t order_of(float x) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-constexpr int kSelThreads = 1024;
+constexpr int kSelThreads = 512, kSelWarps = kSelThreads / 32, kSelHeld = 16;
 
-// CTA = (sequence, head): the rows to keep, in order.  Four passes over the
-// weights narrow the smallest weight kept down to its 32 bits (histograms of
-// 8 bits); a last one lists the rows above it and the first of those at it.
-__global__ void __launch_bounds__(kSelThreads) select_kernel(EvictParams p) {
-  __shared__ int s_hist[256];
-  __shared__ uint32_t s_prefix;
-  __shared__ int s_left, s_warp[kSelThreads / 32][2];
-  const int b = blockIdx.x / p.kv_heads, h = blockIdx.x % p.kv_heads, tid = threadIdx.x;
+// exclusive prefix sums over the CTA's threads of two counts, and the sums;
+// `scratch` holds 2 kSelWarps ints
+__device__ __forceinline__ int2 counts_before(int gt, int eq, int* scratch, int2& all) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int a = gt, b = eq;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int x = __shfl_up_sync(0xffffffffu, a, o), y = __shfl_up_sync(0xffffffffu, b, o);
+    if (lane >= o) a += x, b += y;
+  }
+  __syncthreads();
+  if (lane == 31) scratch[2 * warp] = a, scratch[2 * warp + 1] = b;
+  __syncthreads();
+  int2 before = make_int2(a - gt, b - eq);
+  all = make_int2(0, 0);
+#pragma unroll
+  for (int w = 0; w < kSelWarps; ++w) {
+    const int x = scratch[2 * w], y = scratch[2 * w + 1];
+    if (w < warp) before.x += x, before.y += y;
+    all.x += x, all.y += y;
+  }
+  return before;
+}
+
+// Cluster of C CTAs = (sequence, head): the rows to keep, in order.  Each CTA
+// has a contiguous share of the weights in blocks of 16 for each thread; the
+// first block stays in registers (a longer cache's others are read again in
+// each pass), so that one read of the weights serves four passes over 8 bits
+// that narrow the smallest weight kept down to its 32 bits: histograms in
+// shared memory (one for every fourth lane, since most weights share their
+// high bits), added across the cluster by each CTA from its neighbours'
+// memory, and a suffix sum over the 256 bins by one warp.  Then the rows above
+// that weight and the first of those at it are listed by prefix sums.
+template <int C>
+__global__ void __launch_bounds__(kSelThreads, 2) select_kernel(EvictParams p) {
+  __shared__ int s_hist[4][256], s_total[256], s_scratch[2 * kSelWarps];
+  __shared__ int s_digit, s_left, s_count[2];
+  const unsigned rank = C > 1 ? blockIdx.x % C : 0;
+  const int head = blockIdx.x / C, b = head / p.kv_heads, h = head % p.kv_heads;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int len = min(max(p.lens[b], 0), p.capacity);
   const int kept = min(len, p.budget), recent = min(p.recent, kept);
   const int older = len - recent, pick = kept - recent;
   const float* acc = static_cast<const float*>(p.acc.data) + b * p.acc.batch + h * p.acc.head;
-  float* ao = static_cast<float*>(p.ao.data) + b * p.ao.batch + h * p.ao.head;
-  int32_t* index = p.index + (size_t)blockIdx.x * p.budget;
-  if (h == 0 && tid == 0) p.lens_out[b] = kept;
-  for (int i = kept + tid; i < p.budget; i += kSelThreads) index[i] = -1;
-  for (int i = tid; i < recent; i += kSelThreads) {
-    index[pick + i] = older + i;
-    ao[pick + i] = acc[older + i];
-  }
-  if (pick == 0) return;
-  if (pick == older) {
-    for (int i = tid; i < pick; i += kSelThreads) {
-      index[i] = i;
-      ao[i] = acc[i];
-    }
+  int32_t* index = p.index + (size_t)head * p.budget;
+  const int all = C * kSelThreads, me = rank * kSelThreads + tid;  // of the cluster's threads
+  if (h == 0 && me == 0) p.lens_out[b] = kept;
+  for (int i = kept + me; i < p.budget; i += all) index[i] = -1;
+  for (int i = me; i < recent; i += all) index[pick + i] = older + i;
+  if (pick == 0 || pick == older) {  // alike in the whole cluster
+    for (int i = me; i < pick; i += all) index[i] = i;
     return;
   }
-  if (tid == 0) {
-    s_prefix = 0;
-    s_left = pick;
-  }
+  // this CTA's weights [lo, hi), whole blocks but for the last
+  constexpr int kBlock = kSelThreads * kSelHeld;
+  const int share = ((older + C - 1) / C + kSelHeld - 1) / kSelHeld * kSelHeld;
+  const int lo = min(older, (int)rank * share), hi = min(older, lo + share), blocks = (hi - lo + kBlock - 1) / kBlock;
+  const bool wide = reinterpret_cast<uintptr_t>(acc) % 16 == 0;  // lo is a multiple of 16
+  auto read = [&](int block, uint32_t* u) {
+    const int i0 = lo + block * kBlock + tid * kSelHeld;
+    float x[kSelHeld];
+    if (wide && i0 + kSelHeld <= hi) {
+#pragma unroll
+      for (int k = 0; k < kSelHeld; k += 4) *reinterpret_cast<float4*>(x + k) = *reinterpret_cast<const float4*>(acc + i0 + k);
+    } else {
+#pragma unroll
+      for (int k = 0; k < kSelHeld; ++k) x[k] = i0 + k < hi ? acc[i0 + k] : 0.0f;
+    }
+#pragma unroll
+    for (int k = 0; k < kSelHeld; ++k) u[k] = order_of(x[k]);
+    return max(0, min(kSelHeld, hi - i0));  // those that are there
+  };
+  uint32_t held[kSelHeld];
+  const int mine = read(0, held);
+  uint32_t prefix = 0;
+  int left = pick;
   for (int shift = 24; shift >= 0; shift -= 8) {
-    if (tid < 256) s_hist[tid] = 0;
+    for (int i = tid; i < 4 * 256; i += kSelThreads) (&s_hist[0][0])[i] = 0;
     __syncthreads();
-    const uint32_t prefix = s_prefix;
-    for (int i = tid; i < older; i += kSelThreads) {
-      const uint32_t u = order_of(acc[i]);
-      if (shift == 24 || u >> (shift + 8) == prefix >> (shift + 8)) atomicAdd(&s_hist[u >> shift & 255], 1);
+    auto add = [&](const uint32_t* u, int n) {
+#pragma unroll
+      for (int k = 0; k < kSelHeld; ++k)
+        if (k < n && (shift == 24 || u[k] >> (shift + 8) == prefix >> (shift + 8)))
+          atomicAdd(&s_hist[lane & 3][u[k] >> shift & 255], 1);
+    };
+    add(held, mine);
+    for (int k = 1; k < blocks; ++k) {
+      uint32_t u[kSelHeld];
+      const int n = read(k, u);
+      add(u, n);
     }
     __syncthreads();
-    if (tid == 0) {
-      int left = s_left, d = 255;
-      while (d > 0 && s_hist[d] < left) left -= s_hist[d--];
-      s_left = left;
-      s_prefix = prefix | (uint32_t)d << shift;
-    }
-    __syncthreads();
-  }
-  const uint32_t edge = s_prefix;
-  const int ties = s_left;  // rows at the edge weight that are kept, the first ones
-  int above = 0, at_edge = 0;  // counts before this round
-  for (int base = 0; base < older; base += kSelThreads) {
-    const int i = base + tid;
-    const uint32_t u = i < older ? order_of(acc[i]) : 0u;
-    const bool gt = i < older && u > edge, eq = i < older && u == edge;
-    const uint32_t mg = __ballot_sync(0xffffffffu, gt), me = __ballot_sync(0xffffffffu, eq);
-    const int lane = tid & 31, warp = tid >> 5;
-    if (lane == 0) {
-      s_warp[warp][0] = __popc(mg);
-      s_warp[warp][1] = __popc(me);
-    }
-    __syncthreads();
-    int bg = above, be = at_edge;
-    for (int w = 0; w < kSelThreads / 32; ++w) {
-      if (w < warp) {
-        bg += s_warp[w][0];
-        be += s_warp[w][1];
+    if (tid < 256) s_total[tid] = s_hist[0][tid] + s_hist[1][tid] + s_hist[2][tid] + s_hist[3][tid];
+    if constexpr (C > 1) {
+      cluster_sync();
+      if (tid < 256) {
+        int n = 0;
+#pragma unroll
+        for (int r = 0; r < C; ++r) n += cluster_read(&s_total[tid], r);
+        s_hist[0][tid] = n;
       }
-      above += s_warp[w][0];
-      at_edge += s_warp[w][1];
-    }
-    const uint32_t below = (1u << lane) - 1u;
-    bg += __popc(mg & below);
-    be += __popc(me & below);
-    if (gt || (eq && be < ties)) {
-      const int slot = bg + min(be, ties);
-      index[slot] = i;
-      ao[slot] = acc[i];
+    } else if (tid < 256) {
+      s_hist[0][tid] = s_total[tid];
     }
     __syncthreads();
+    if (warp == 0) {
+      // the highest digits first: lane 0 has bins 255 .. 248
+      int n[8], sum = 0;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) sum += n[k] = s_hist[0][255 - 8 * lane - k];
+      int upto = sum;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += y;
+      }
+      const uint32_t past = __ballot_sync(0xffffffffu, upto >= left);
+      if (lane == __ffs(past) - 1) {
+        int above = upto - sum, k = 0;
+        while (k < 7 && above + n[k] < left) above += n[k++];
+        s_digit = 255 - 8 * lane - k;
+        s_left = left - above;
+      }
+    }
+    __syncthreads();
+    prefix |= (uint32_t)s_digit << shift;
+    left = s_left;
+    // the neighbours have read this CTA's counts before they are written again
+    if constexpr (C > 1) cluster_sync();
   }
+  // `left` rows at the edge weight are kept, the first ones
+  const uint32_t edge = prefix;
+  auto count = [&](const uint32_t* u, int n, int& gt, int& eq) {
+#pragma unroll
+    for (int k = 0; k < kSelHeld; ++k) {
+      gt += k < n && u[k] > edge;
+      eq += k < n && u[k] == edge;
+    }
+  };
+  int gt = 0, eq = 0;
+  count(held, mine, gt, eq);
+  int2 sum;
+  int2 before = counts_before(gt, eq, s_scratch, sum);
+  int above = 0, at_edge = 0;  // of the CTAs before this one
+  if constexpr (C > 1) {
+    int g2 = 0, e2 = 0;
+    for (int k = 1; k < blocks; ++k) {
+      uint32_t u[kSelHeld];
+      const int n = read(k, u);
+      count(u, n, g2, e2);
+    }
+    int2 more = make_int2(0, 0);
+    if (blocks > 1) counts_before(g2, e2, s_scratch, more);
+    if (tid == 0) s_count[0] = sum.x + more.x, s_count[1] = sum.y + more.y;
+    cluster_sync();
+#pragma unroll
+    for (int r = 0; r < C; ++r)
+      if (r < (int)rank) {
+        above += cluster_read(&s_count[0], r);
+        at_edge += cluster_read(&s_count[1], r);
+      }
+  }
+  auto list = [&](const uint32_t* u, int n, int i0) {
+    int bg = above + before.x, be = at_edge + before.y;
+#pragma unroll
+    for (int k = 0; k < kSelHeld; ++k) {
+      const bool is_gt = k < n && u[k] > edge, is_eq = k < n && u[k] == edge;
+      if (is_gt || (is_eq && be < left)) index[bg + min(be, left)] = i0 + k;
+      bg += is_gt;
+      be += is_eq;
+    }
+    above += sum.x;
+    at_edge += sum.y;
+  };
+  list(held, mine, lo + tid * kSelHeld);
+  for (int k = 1; k < blocks; ++k) {
+    uint32_t u[kSelHeld];
+    const int n = read(k, u);
+    gt = eq = 0;
+    count(u, n, gt, eq);
+    before = counts_before(gt, eq, s_scratch, sum);
+    list(u, n, lo + k * kBlock + tid * kSelHeld);
+  }
+  if constexpr (C > 1) cluster_sync();  // no CTA ends while another may read its counts
 }
 
-// copies the rows listed in index, in pieces of V elements: CTA.x = (sequence
+// copies the rows listed in index and their weights, rows in pieces of V
+// elements: CTA.x = (sequence
 // x head), CTA.y strides over the budget
 template <typename T, typename V>
 __global__ void __launch_bounds__(256) gather_kernel(EvictParams p) {
   constexpr int W = sizeof(V) / sizeof(T);
+  CKKS_PDL_ENTRY();
   const int b = blockIdx.x / p.kv_heads, h = blockIdx.x % p.kv_heads;
   const int kept = min(min(max(p.lens[b], 0), p.capacity), p.budget);
   const int per = p.head_dim / W;
   const int32_t* index = p.index + (size_t)blockIdx.x * p.budget;
   const T* kc = static_cast<const T*>(p.kc.data) + b * p.kc.batch + h * p.kc.head;
   const T* vc = static_cast<const T*>(p.vc.data) + b * p.vc.batch + h * p.vc.head;
+  const float* acc = static_cast<const float*>(p.acc.data) + b * p.acc.batch + h * p.acc.head;
+  float* ao = static_cast<float*>(p.ao.data) + b * p.ao.batch + h * p.ao.head;
   T* ko = static_cast<T*>(p.ko.data) + b * p.ko.batch + h * p.ko.head;
   T* vo = static_cast<T*>(p.vo.data) + b * p.vo.batch + h * p.vo.head;
   const long long n = (long long)kept * per;
   for (long long i = (long long)blockIdx.y * blockDim.x + threadIdx.x; i < n; i += (long long)gridDim.y * blockDim.x) {
     const int r = (int)(i / per), d = (int)(i % per) * W, s = index[r];
+    if (d == 0) ao[r] = acc[s];
     const V k = *reinterpret_cast<const V*>(kc + s * p.kc.row + d);
     const V v = *reinterpret_cast<const V*>(vc + s * p.vc.row + d);
     *reinterpret_cast<V*>(ko + r * p.ko.row + d) = k;
@@ -651,14 +758,20 @@ extern "C" int ckks_draft_evict(ckks_ctx* ctx, const ckks_draft_evict_args* args
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     const int heads = a.batch * a.kv_heads;
     ProfScope ps(c, "draft_evict", heads * (4.0 * a.capacity + a.budget * (4.0 * e * a.head_dim + 8.0)), st);
-    select_kernel<<<heads, kSelThreads, 0, st>>>(p);
-    CKKS_CUDA(cudaGetLastError());
+    // a CTA for each 4096 weights, eight at most
+    if (a.capacity <= 4096)
+      launch_cluster<1>(select_kernel<1>, heads, kSelThreads, st, p);
+    else if (a.capacity <= 8192)
+      launch_cluster<2>(select_kernel<2>, heads, kSelThreads, st, p);
+    else if (a.capacity <= 16384)
+      launch_cluster<4>(select_kernel<4>, heads, kSelThreads, st, p);
+    else
+      launch_cluster<8>(select_kernel<8>, heads, kSelThreads, st, p);
     by_piece(e, wide, [&](auto t, auto v) {
       const long long pieces = (long long)a.budget * a.head_dim * e / (long long)sizeof(v);
       const long long most = std::max(1ll, 16ll * c.sms / heads);
       const unsigned y = (unsigned)std::min({(pieces + 255) / 256, most, 65535ll});
-      gather_kernel<decltype(t), decltype(v)><<<dim3(heads, y), 256, 0, st>>>(p);
+      launch_pdl(gather_kernel<decltype(t), decltype(v)>, dim3(heads, y), dim3(256), 0, st, p);
     });
-    CKKS_CUDA(cudaGetLastError());
   });
 }

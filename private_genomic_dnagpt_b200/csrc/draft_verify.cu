@@ -5,17 +5,26 @@
 // With children c drawn from the draft's row q, child c with token x is kept
 // when u_c q(x) < p(x), and each child refused replaces the target's row p by
 // max(p - q, 0) / Z, Z = sum max(p - q, 0): the tokens kept, and the one drawn
-// from what p is at the end, are distributed as the target's.  Only the rows
-// of the last node reached are needed whole; every other node takes two
-// values.  All sums are in float64: a token is decided by comparing a running
-// sum over the vocabulary with u times the whole one.
+// from what p is at the end, are distributed as the target's.  After any
+// number of refusals p is max(p0 - a q, 0) / S for the row p0 given, with
+// a = 0, S = 1 at first, and a refusal makes of them
+//   a' = a + S,  S' = sum max(p0 - a' q, 0)
+// (max(p - q, 0) = max(max(p0 - a q, 0) - S q, 0) / S), so a refusal is one
+// multiply-add for each entry, however many came before.
+//
+// Only the rows of the nodes at which a child is refused, or the walk ends,
+// are needed whole; every other node takes two values.  All of it is in
+// float64: a token is decided by comparing a running sum over the vocabulary
+// with u times the whole one.
+#include <algorithm>
+
 #include "draft.hpp"
 
 namespace ckks {
 namespace draft {
 namespace {
 
-constexpr int kThreads = 1024, kWarps = kThreads / 32;
+constexpr int kThreads = 512, kWarps = kThreads / 32;
 
 struct VerifyParams {
   ckks_rows target, draft;
@@ -34,28 +43,31 @@ __device__ __forceinline__ double warp_sum(double x) {
   return x;
 }
 
-// p(x) after the refusals so far: `refused` normalisers in z
-__device__ __forceinline__ double remaining(double t, double q, const double* z, int refused) {
-  double r = t > 0.0 ? t : 0.0;
-  const double d = q > 0.0 ? q : 0.0;
-  for (int k = 0; k < refused; ++k) {
-    r -= d;
-    r = r > 0.0 ? r / z[k] : 0.0;
-  }
-  return r;
+// a probability; what is not above 0 (NaN among it) is 0
+__device__ __forceinline__ double weight(float x) { return (double)fmaxf(x, 0.0f); }
+__device__ __forceinline__ double weight(double x) { return x > 0.0 ? x : 0.0; }
+
+// what is left of p(x), times S: max(p - a q, 0).  The comparison looks at the
+// sign bit: float64 instructions are the scarce ones here
+__device__ __forceinline__ double left_of(double p, double q, double a) {
+  const double r = fma(-a, q, p);
+  return __double2hiint(r) < 0 ? 0.0 : r;
 }
 
-// One CTA per sequence.  The walk needs p and q at the drafts' tokens only,
-// which the threads fetch for all nodes at once, each in its parent's row; a
-// refusal costs one pass over that row for Z.  The last token is found by
-// descending radix 32: the warps sum 32 pieces of the row, the piece in which
-// the running sum passes u Z is cut into 32 again, down to single entries.
-template <typename TT, typename TD>
-__global__ void __launch_bounds__(kThreads) verify_kernel(VerifyParams p) {
-  __shared__ double s_p[kMaxNodes], s_q[kMaxNodes], s_u[kMaxNodes + 1], s_z[kMaxNodes], s_sum[kWarps];
-  __shared__ int s_parent[kMaxNodes];
-  __shared__ int s_last[kWarps];
-  const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+// A cluster of C CTAs per sequence, each with a contiguous share of the
+// vocabulary and each warp with a contiguous part of that; a thread keeps the
+// first kHeld of its entries of the row at hand in registers, so refusals at
+// one node and the last draw read the row once (larger vocabularies read the
+// rest again, from L2).  Every CTA walks the tree alike: the walk needs p and
+// q at the drafts' tokens only, which the threads fetch for all nodes at once,
+// each in its parent's row.  Sums add the CTAs' parts in their order.
+template <typename TT, typename TD, int C>
+__global__ void __launch_bounds__(kThreads, sizeof(TT) + sizeof(TD) == 8 ? 2 : 1) verify_kernel(VerifyParams p) {
+  constexpr int kHeld = sizeof(TT) + sizeof(TD) == 8 ? 16 : 8;
+  __shared__ double s_p[kMaxNodes], s_q[kMaxNodes], s_u[kMaxNodes + 1], s_sum[kWarps], s_part[2];
+  __shared__ int s_parent[kMaxNodes], s_last[kWarps], s_tail;
+  const int b = blockIdx.x / C, rank = C > 1 ? blockIdx.x % C : 0;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const TT* target = static_cast<const TT*>(p.target.data) + b * p.target.batch;
   const TD* draft = static_cast<const TD*>(p.draft.data) + b * p.draft.batch;
   const int n = p.nodes, V = p.vocab;
@@ -65,100 +77,192 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(VerifyParams p) {
     if (par < -1 || par >= tid) par = -2;
     s_parent[tid] = par;
     const bool known = par >= -1 && x >= 0 && x < V;
-    s_p[tid] = known ? (double)target[(par + 1) * p.target.row + x] : 0.0;
-    s_q[tid] = known ? (double)draft[(par + 1) * p.draft.row + x] : 0.0;
+    s_p[tid] = known ? weight(target[(par + 1) * p.target.row + x]) : 0.0;
+    s_q[tid] = known ? weight(draft[(par + 1) * p.draft.row + x]) : 0.0;
   }
-  if (tid <= n) s_u[tid] = p.uniforms[(size_t)b * (n + 1) + tid];
+  if (tid >= kThreads - 128 && tid - (kThreads - 128) <= n)
+    s_u[tid - (kThreads - 128)] = p.uniforms[(size_t)b * (n + 1) + tid - (kThreads - 128)];
+  // this warp's entries [x0, x1)
+  const int share = (V + C - 1) / C, lo = min(V, rank * share), hi = min(V, lo + share);
+  const int part = (share + kWarps - 1) / kWarps, x0 = min(hi, lo + warp * part), x1 = min(hi, x0 + part);
   __syncthreads();
-  int at = -1, kept = 0, refused = 0;
-  for (int i = 0; i < n; ++i) {
-    if (s_parent[i] != at) continue;
+  TT hp[kHeld];
+  TD hq[kHeld];
+  int row = -2, at = -1, kept = 0, flip = 0;
+  auto hold = [&] {
+    if (row == at) return;
+    row = at;
     const TT* t = target + (at + 1) * p.target.row;
     const TD* q = draft + (at + 1) * p.draft.row;
-    const double px = remaining(s_p[i], s_q[i], s_z, refused), qx = s_q[i] > 0.0 ? s_q[i] : 0.0;
-    if (s_u[i] * qx < px) {
-      if (tid == 0) p.path[(size_t)b * n + kept] = i;
+#pragma unroll
+    for (int k = 0; k < kHeld; ++k) {
+      const int x = x0 + 32 * k + lane;
+      hp[k] = x < x1 ? t[x] : (TT)0;
+      hq[k] = x < x1 ? q[x] : (TD)0;
+    }
+  };
+  // f(x, what is left of p(x)) for this thread's entries
+  auto each = [&](double a, auto&& f) {
+#pragma unroll
+    for (int k = 0; k < kHeld; ++k) f(x0 + 32 * k + lane, left_of(weight(hp[k]), weight(hq[k]), a));
+    const TT* t = target + (at + 1) * p.target.row;
+    const TD* q = draft + (at + 1) * p.draft.row;
+    for (int x = x0 + 32 * kHeld + lane; x < x1; x += 32 * 8) {
+      TT tp[8];
+      TD tq[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        tp[k] = x + 32 * k < x1 ? t[x + 32 * k] : (TT)0;
+        tq[k] = x + 32 * k < x1 ? q[x + 32 * k] : (TD)0;
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) f(x + 32 * k, left_of(weight(tp[k]), weight(tq[k]), a));
+    }
+  };
+  // sums over the warp, the CTA (s_sum[warp] holds the warps') and the cluster
+  auto sum_all = [&](double a, double* before) {
+    double s = 0.0;
+    each(a, [&](int, double r) { s += r; });
+    s = warp_sum(s);
+    __syncthreads();
+    if (lane == 0) s_sum[warp] = s;
+    __syncthreads();
+    s = 0.0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) s += s_sum[w];
+    if (before) *before = 0.0;
+    if constexpr (C > 1) {
+      // two places in turn: a CTA may be one sum ahead of one that still reads
+      flip ^= 1;
+      if (tid == 0) s_part[flip] = s;
+      cluster_sync();
+      double all = 0.0;
+#pragma unroll
+      for (int r = 0; r < C; ++r) {
+        if (before && r == rank) *before = all;
+        all += cluster_read(&s_part[flip], r);
+      }
+      s = all;
+    }
+    return s;
+  };
+  double a = 0.0, S = 1.0;
+  for (int i = 0; i < n; ++i) {
+    if (s_parent[i] != at) continue;
+    if (s_u[i] * s_q[i] < left_of(s_p[i], s_q[i], a) / S) {
+      if (tid == 0 && rank == 0) p.path[(size_t)b * n + kept] = i;
       ++kept;
       at = i;
-      refused = 0;
-      __syncthreads();  // s_z is written anew
+      a = 0.0, S = 1.0;
       continue;
     }
-    // the refused child's normaliser
-    double z = 0.0;
-    for (int x = tid; x < V; x += kThreads) {
-      const double d = q[x] > 0 ? (double)q[x] : 0.0;
-      const double r = remaining((double)t[x], d, s_z, refused) - d;
-      z += r > 0.0 ? r : 0.0;
-    }
-    z = warp_sum(z);
-    if (lane == 0) s_sum[warp] = z;
-    __syncthreads();
-    z = 0.0;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) z += s_sum[w];
-    if (z > 0.0) {
-      if (tid == 0) s_z[refused] = z;
-      ++refused;
-    }
-    __syncthreads();
+    hold();
+    const double z = sum_all(a + S, nullptr);
+    if (z > 0.0) a += S, S = z;
   }
-  if (tid >= kept && tid < n) p.path[(size_t)b * n + tid] = -1;
-  if (tid == 0) p.count[b] = kept;
-  // the next token, from p as it stands
-  const TT* t = target + (at + 1) * p.target.row;
-  const TD* q = draft + (at + 1) * p.draft.row;
-  auto value = [&](int x) { return remaining((double)t[x], refused ? (double)q[x] : 0.0, s_z, refused); };
-  int lo = 0, size = V;  // the piece searched
-  double before = 0.0, goal = -1.0;
-  int last = 0;  // the last entry above 0, for a goal that rounding put at the whole sum
-  while (true) {
-    const int piece = (size + kWarps - 1) / kWarps;
-    const int w0 = lo + min(size, warp * piece), w1 = lo + min(size, (warp + 1) * piece);
+  if (rank == 0) {
+    if (tid >= kept && tid < n) p.path[(size_t)b * n + tid] = -1;
+    if (tid == 0) p.count[b] = kept;
+  }
+  // the next token, from p as it stands: the CTA, the warp in it and the
+  // entry at which the running sum passes u times the whole one
+  hold();
+  double before;
+  const double goal = s_u[n] * sum_all(a, &before);
+  int last = -1;  // the last entry above 0, for a goal that rounding put at the whole sum
+  each(a, [&](int x, double r) {
+    if (x < x1 && r > 0.0) last = x;
+  });
+  last = __reduce_max_sync(0xffffffffu, last);
+  if (lane == 0) s_last[warp] = last;
+  __syncthreads();
+  double run = before;
+  int hit = -1, tail = -1;
+  double start = 0.0;
+  for (int w = 0; w < kWarps; ++w) {
+    tail = max(tail, s_last[w]);
+    const double next = run + s_sum[w];
+    if (hit < 0 && next > goal) hit = w, start = run;
+    run = next;
+  }
+  // of the CTAs that pass the goal the first is the one
+  bool mine = hit >= 0, none = !mine;
+  if constexpr (C > 1) {
+    flip ^= 1;
+    if (tid == 0) s_part[flip] = hit >= 0 ? 1.0 : 0.0, s_tail = tail;
+    cluster_sync();
+#pragma unroll
+    for (int r = 0; r < C; ++r) {
+      const bool theirs = cluster_read(&s_part[flip], r) != 0.0;
+      if (r < rank && theirs) mine = false;
+      none = none && !theirs;
+      tail = max(tail, cluster_read(&s_tail, r));
+    }
+  }
+  if (none) {
+    if (tid == 0 && rank == 0) p.token[b] = max(tail, 0);
+  } else if (mine) {
+    // the warps cut the part of the warp that passed the goal into theirs,
+    // and the one that passes it there walks its few entries
+    const TT* t = target + (at + 1) * p.target.row;
+    const TD* q = draft + (at + 1) * p.draft.row;
+    const int h0 = min(hi, lo + hit * part), h1 = min(hi, h0 + part), cut = (h1 - h0 + kWarps - 1) / kWarps;
+    const int y0 = min(h1, h0 + warp * cut), y1 = min(h1, y0 + cut);
     double s = 0.0;
-    int mine = -1;
-    for (int x = w0 + lane; x < w1; x += 32) {
-      const double v = value(x);
-      s += v;
-      if (v > 0.0) mine = x;
+    last = -1;
+    for (int x = y0 + lane; x < y1; x += 32) {
+      const double r = left_of(weight(t[x]), weight(q[x]), a);
+      s += r;
+      if (r > 0.0) last = x;
     }
     s = warp_sum(s);
-    mine = __reduce_max_sync(0xffffffffu, mine);
-    if (lane == 0) {
-      s_sum[warp] = s;
-      s_last[warp] = mine;
-    }
+    last = __reduce_max_sync(0xffffffffu, last);
     __syncthreads();
-    if (goal < 0.0) {
-      double all = 0.0;
-      for (int w = 0; w < kWarps; ++w) {
-        all += s_sum[w];
-        if (s_last[w] >= 0) last = s_last[w];
-      }
-      goal = s_u[n] * all;
-    }
-    // the first piece that passes the goal, else none
-    int hit = -1;
-    double run = before;
-    for (int w = 0; w < kWarps; ++w) {
-      const double next = run + s_sum[w];
-      if (next > goal) {
+    if (lane == 0) s_sum[warp] = s, s_last[warp] = last;
+    __syncthreads();
+    double base = start;
+    hit = tail = -1;
+    for (int w = 0; w < kWarps && hit < 0; ++w) {
+      tail = max(tail, s_last[w]);
+      if (base + s_sum[w] > goal)
         hit = w;
-        break;
+      else
+        base += s_sum[w];
+    }
+    if (warp == max(hit, 0)) {
+      int found = -1;
+      for (int x = y0; hit >= 0 && x < y1 && found < 0; x += 32) {
+        const double own = x + lane < y1 ? left_of(weight(t[x + lane]), weight(q[x + lane]), a) : 0.0;
+        double v = own;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const double y = __shfl_up_sync(0xffffffffu, v, o);
+          if (lane >= o) v += y;
+        }
+        const uint32_t past = __ballot_sync(0xffffffffu, own > 0.0 && base + v > goal);
+        if (past) found = x + __ffs(past) - 1;
+        base += __shfl_sync(0xffffffffu, v, 31);
       }
-      run = next;
+      // another order of the same sum may end just below the goal
+      if (lane == 0) p.token[b] = found >= 0 ? found : tail;
     }
-    __syncthreads();
-    if (hit < 0) {
-      lo = last;
-      break;
-    }
-    before = run;
-    lo += min(size, hit * piece);
-    if (piece == 1) break;
-    size = min(piece, V - lo);
   }
-  if (tid == 0) p.token[b] = lo;
+  if constexpr (C > 1) cluster_sync();  // no CTA ends while another may read its parts
+}
+
+template <typename TT, typename TD>
+void run_verify(const Context& c, const VerifyParams& p, cudaStream_t st) {
+  // as many CTAs as the SMs take at once (two on each), none with less than
+  // 1024 entries
+  const int most = std::min(2 * c.sms / std::max(1, p.batch), p.vocab / 1024);
+  if (most >= 8)
+    launch_cluster<8>(verify_kernel<TT, TD, 8>, p.batch, kThreads, st, p);
+  else if (most >= 4)
+    launch_cluster<4>(verify_kernel<TT, TD, 4>, p.batch, kThreads, st, p);
+  else if (most >= 2)
+    launch_cluster<2>(verify_kernel<TT, TD, 2>, p.batch, kThreads, st, p);
+  else
+    launch_cluster<1>(verify_kernel<TT, TD, 1>, p.batch, kThreads, st, p);
 }
 
 void check_rows2(const ckks_rows& r, int dtype, const char* what) {
@@ -198,13 +302,12 @@ extern "C" int ckks_draft_verify(ckks_ctx* ctx, const ckks_draft_verify_args* ar
                  (double)a.batch * a.vocab * (element_bytes(a.target_dtype) + element_bytes(a.draft_dtype)), st);
     const bool td = a.target_dtype == CKKS_FP64, dd = a.draft_dtype == CKKS_FP64;
     if (td && dd)
-      verify_kernel<double, double><<<a.batch, kThreads, 0, st>>>(p);
+      run_verify<double, double>(c, p, st);
     else if (td)
-      verify_kernel<double, float><<<a.batch, kThreads, 0, st>>>(p);
+      run_verify<double, float>(c, p, st);
     else if (dd)
-      verify_kernel<float, double><<<a.batch, kThreads, 0, st>>>(p);
+      run_verify<float, double>(c, p, st);
     else
-      verify_kernel<float, float><<<a.batch, kThreads, 0, st>>>(p);
-    CKKS_CUDA(cudaGetLastError());
+      run_verify<float, float>(c, p, st);
   });
 }

@@ -285,7 +285,8 @@ def check_verify(cc, x):
                                    (torch.float64, torch.float32), (torch.float32, torch.float64)])
 @pytest.mark.parametrize("B,n,V,branch,pad", [(1, 5, 4103, 1, 0), (9, 31, 1000, 2, 2), (7, 12, 33, 4, 0),
                                               (5, 1, 1, 1, 0), (6, 64, 7, 8, 1), (4, 8, 1024, 8, 0),
-                                              (2, 3, 40001, 1, 0), (3, 20, 32, 64, 0), (3, 6, 1025, 2, 0)])
+                                              (2, 3, 40001, 1, 0), (3, 20, 32, 64, 0), (3, 6, 1025, 2, 0),
+                                              (2, 5, 128256, 2, 0), (1, 4, 300007, 1, 0), (40, 7, 8200, 2, 0)])
 def test_verify(cc, tt, td, B, n, V, branch, pad):
     counts = []
     for seed in range(4):
