@@ -38,10 +38,18 @@ _ACCUMULATE = struct.Struct("8id12q4q")
 _EVICT = struct.Struct("8i24q5q")
 
 
+_entries: dict = {}  # the library's entry points by name, looked up once
+_current_stream = None
+
+
 def _torch():
     import torch
+    global _current_stream
     if not _DTYPES:
         _DTYPES.update({torch.bfloat16: 0, torch.float16: 1, torch.float32: 2, torch.float64: 3})
+        # the handle of torch's current stream, without a Stream object where torch offers that
+        _current_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+            lambda index: torch.cuda.current_stream(index).cuda_stream)
     return torch
 
 
@@ -49,8 +57,10 @@ def _refuse(name, why):
     raise ValueError(f"{name}: {why}")
 
 
-def _tensor(t, name, shape, dtype, device, contiguous=False):
-    """Checks one argument and returns it."""
+def _complain(t, name, shape, dtype, device, small):
+    """Says what is wrong with an argument that did not pass."""
+    if not isinstance(t, _torch().Tensor):
+        _refuse(name, f"expected a tensor, got {type(t).__name__}")
     if t.shape != shape:
         _refuse(name, f"expected the shape {tuple(shape)}, got {tuple(t.shape)}")
     if t.dtype is not dtype:
@@ -59,39 +69,64 @@ def _tensor(t, name, shape, dtype, device, contiguous=False):
         _refuse(name, f"expected a tensor of {device}, the context's device, got {t.device}")
     if t.requires_grad and _torch().is_grad_enabled():
         _refuse(name, "requires a gradient, which this operator does not have (call it under torch.no_grad)")
-    if contiguous and not t.is_contiguous():
-        _refuse(name, "must be contiguous")
-    if t.shape and t.shape[-1] > 1 and t.stride(-1) != 1 and t.numel():
-        _refuse(name, "its last dimension must be contiguous")
-    return t
+    _refuse(name, "must be contiguous" if small else "its last dimension must be contiguous")
 
 
-def _writable(t, name):
+# The checks of a call take about as long as its launch, so each tensor's
+# attributes are read once: _strides and _small return what the packed
+# arguments need.
+
+def _strides(t, name, shape, dtype, device, where, grad):
+    """Checks a tensor of rows and returns its strides."""
+    if t.shape != shape or t.dtype is not dtype or t.get_device() != where or (grad and t.requires_grad):
+        _complain(t, name, shape, dtype, device, False)
+    s = t.stride()
+    if s[-1] != 1 and shape[-1] > 1 and t.numel():
+        _complain(t, name, shape, dtype, device, False)
+    return s
+
+
+def _small(t, name, shape, dtype, device, where, grad):
+    """Checks a contiguous tensor and returns its address."""
+    if (t.shape != shape or t.dtype is not dtype or t.get_device() != where or not t.is_contiguous()
+            or (grad and t.requires_grad)):
+        _complain(t, name, shape, dtype, device, True)
+    return t.data_ptr()
+
+
+def _writable(name, shape, strides):
     """Refuses a tensor of which two elements share memory."""
-    for n, s in zip(t.shape, t.stride()):
-        if n > 1 and s == 0:
-            _refuse(name, "is written, but some of its elements share memory")
-    return t
+    if 0 in strides:
+        for n, s in zip(shape, strides):
+            if n > 1 and s == 0:
+                _refuse(name, "is written, but some of its elements share memory")
 
 
-def _device(cc):
+def _setting(cc):
+    """torch, the context's device, its index and whether gradients are on."""
+    torch = _torch()
     d = cc._draft_device
     if d is None:
-        d = cc._draft_device = _torch().device("cuda", cc.params.device)
-    return d
+        d = cc._draft_device = torch.device("cuda", cc.params.device)
+    return torch, d, -1 if d.index is None else d.index, torch.is_grad_enabled()
 
 
-def _call(cc, name, args, device):
-    from . import _check, lib
-    stream = _torch().cuda.current_stream(device).cuda_stream
-    _check(getattr(lib(), name)(cc.h, args, stream))
+def _call(cc, name, args, where):
+    f = _entries.get(name)
+    if f is None:
+        from . import lib
+        f = _entries[name] = getattr(lib(), name)
+    rc = f(cc.h, args, _current_stream(where))
+    if rc:
+        from . import _check
+        _check(rc)
 
 
 def _workspace(cc, name, layout, head, key, device):
     """A workspace for one call; its size is looked up once for each set of
     sizes."""
     sizes = cc._draft_sizes
-    n = sizes.get((name, key))
+    n = sizes.get(key)
     if n is None:
         from . import CKKSError, lib
         n = getattr(lib(), name + "_workspace")(cc.h, layout.pack(*head, 0, 0))
@@ -99,23 +134,17 @@ def _workspace(cc, name, layout, head, key, device):
             raise CKKSError(1, lib().ckks_last_error().decode())
         if len(sizes) >= 256:
             sizes.clear()
-        sizes[(name, key)] = n
+        sizes[key] = n
     if n == 0:
         return None
     torch = _torch()
     return torch.empty(n, dtype=torch.uint8, device=device)
 
 
-def _by_head(t):
-    """(address, batch, head, row strides) of a [batch, heads, rows, ...] tensor."""
-    s = t.stride()
-    return t.data_ptr(), s[0], s[1], s[2]
-
-
-def _by_node(t):
-    """The same of a [batch, rows, heads, ...] tensor."""
-    s = t.stride()
-    return t.data_ptr(), s[0], s[2], s[1]
+def _four(t, name):
+    if t.dim() != 4:
+        _refuse(name, "expected four dimensions")
+    return t.shape
 
 
 def _cache_type(t, name):
@@ -135,32 +164,30 @@ def attention(cc, q, k_cache, v_cache, lens, k_new, v_new, parents, scale=None):
     last dimension.  scale defaults to 1 / sqrt(D).  Returns out [B, n, Hq, D]
     in q's type and lse [B, n, Hq] float32, the log of each row's sum.  A
     padding node's row is 0, its lse -inf."""
-    torch, device = _torch(), _device(cc)
-    if q.dim() != 4 or k_cache.dim() != 4:
-        _refuse("q" if q.dim() != 4 else "k_cache", "expected four dimensions")
-    b, n, hq, d = q.shape
-    hk, cap = k_cache.shape[1], k_cache.shape[2]
-    t = q.dtype
-    code = _cache_type(q, "q")
-    _tensor(q, "q", (b, n, hq, d), t, device)
-    _tensor(k_cache, "k_cache", (b, hk, cap, d), t, device)
-    _tensor(v_cache, "v_cache", (b, hk, cap, d), t, device)
-    _tensor(k_new, "k_new", (b, n, hk, d), t, device)
-    _tensor(v_new, "v_new", (b, n, hk, d), t, device)
-    _tensor(lens, "lens", (b,), torch.int32, device, True)
-    _tensor(parents, "parents", (b, n), torch.int32, device, True)
-    out = torch.empty((b, n, hq, d), dtype=t, device=device)
-    lse = torch.empty((b, n, hq), dtype=torch.float32, device=device)
+    torch, device, where, grad = _setting(cc)
+    shape, cache = _four(q, "q"), _four(k_cache, "k_cache")
+    b, n, hq, d = shape
+    hk, cap = cache[1], cache[2]
+    t, code = q.dtype, _cache_type(q, "q")
+    rows, rest, new, i32 = (b, hk, cap, d), (t, device, where, grad), (b, n, hk, d), torch.int32
+    sq = _strides(q, "q", shape, *rest)
+    sk, sv = _strides(k_cache, "k_cache", rows, *rest), _strides(v_cache, "v_cache", rows, *rest)
+    nk, nv = _strides(k_new, "k_new", new, *rest), _strides(v_new, "v_new", new, *rest)
+    len_at = _small(lens, "lens", (b,), i32, device, where, grad)
+    parents_at = _small(parents, "parents", (b, n), i32, device, where, grad)
+    out = q.new_empty(shape)
+    lse = q.new_empty((b, n, hq), dtype=torch.float32)
     if b == 0:
         return out, lse
-    key = (code, b, hq, hk, d, n, cap)
-    head = (code, b, hq, hk, d, n, cap, 0, 1.0 / math.sqrt(d) if scale is None else float(scale), *_by_node(q),
-            *_by_head(k_cache), *_by_head(v_cache), *_by_node(k_new), *_by_node(v_new), *_by_node(out),
-            lens.data_ptr(), parents.data_ptr(), lse.data_ptr())
-    name = "ckks_draft_attention"
-    ws = _workspace(cc, name, _ATTENTION, head, key, device)
-    _call(cc, name, _ATTENTION.pack(*head, ws.data_ptr() if ws is not None else 0, ws.numel() if ws is not None else 0),
-          device)
+    key = ("attention", code, b, hq, hk, d, n, cap)
+    row = hq * d
+    head = (code, b, hq, hk, d, n, cap, 0, 1.0 / math.sqrt(d) if scale is None else float(scale),
+            q.data_ptr(), sq[0], sq[2], sq[1], k_cache.data_ptr(), sk[0], sk[1], sk[2],
+            v_cache.data_ptr(), sv[0], sv[1], sv[2], k_new.data_ptr(), nk[0], nk[2], nk[1],
+            v_new.data_ptr(), nv[0], nv[2], nv[1], out.data_ptr(), n * row, d, row, len_at, parents_at, lse.data_ptr())
+    ws = _workspace(cc, "ckks_draft_attention", _ATTENTION, head, key, device)
+    args = _ATTENTION.pack(*head, 0, 0) if ws is None else _ATTENTION.pack(*head, ws.data_ptr(), ws.numel())
+    _call(cc, "ckks_draft_attention", args, where)
     return out, lse
 
 
@@ -176,28 +203,27 @@ def verify(cc, target, draft, tokens, parents, uniforms):
     uniforms[n].  Drafts drawn from ``draft`` give tokens distributed as
     ``target``'s.  Returns path [B, n] int32 (accepted nodes from the root on,
     then -1), count [B] int32 and token [B] int32.  Computed in float64."""
-    torch, device = _torch(), _device(cc)
+    torch, device, where, grad = _setting(cc)
     if target.dim() != 3 or target.shape[1] < 1:
         _refuse("target", "expected [batch, nodes + 1, vocabulary]")
-    b, n, v = target.shape[0], target.shape[1] - 1, target.shape[2]
-    codes = []
-    for x, name in ((target, "target"), (draft, "draft")):
-        codes.append(_DTYPES.get(x.dtype, 0))
-        if codes[-1] < 2:
+    shape = target.shape
+    b, n, v = shape[0], shape[1] - 1, shape[2]
+    tc, dc = _DTYPES.get(target.dtype, 0), _DTYPES.get(draft.dtype, 0)
+    for code, x, name in ((tc, target, "target"), (dc, draft, "draft")):
+        if code < 2:
             _refuse(name, f"expected float32 or float64, got {x.dtype}")
-        _tensor(x, name, (b, n + 1, v), x.dtype, device)
-    _tensor(tokens, "tokens", (b, n), torch.int32, device, True)
-    _tensor(parents, "parents", (b, n), torch.int32, device, True)
-    _tensor(uniforms, "uniforms", (b, n + 1), torch.float64, device, True)
-    path = torch.empty((b, n), dtype=torch.int32, device=device)
-    both = torch.empty((2, b), dtype=torch.int32, device=device)
-    count, token = both[0], both[1]
+    ts = _strides(target, "target", shape, target.dtype, device, where, grad)
+    ds = _strides(draft, "draft", shape, draft.dtype, device, where, grad)
+    rest = (torch.int32, device, where, grad)
+    tokens_at, parents_at = _small(tokens, "tokens", (b, n), *rest), _small(parents, "parents", (b, n), *rest)
+    uniforms_at = _small(uniforms, "uniforms", (b, n + 1), torch.float64, device, where, grad)
+    path, both = torch.empty_like(tokens), tokens.new_empty((2, b))
+    count, token = both.unbind()
     if b:
-        ts, ds = target.stride(), draft.stride()
+        at = both.data_ptr()
         _call(cc, "ckks_draft_verify", _VERIFY.pack(
-            codes[0], codes[1], b, n, v, 0, target.data_ptr(), ts[0], 0, ts[1], draft.data_ptr(), ds[0], 0, ds[1],
-            tokens.data_ptr(), parents.data_ptr(), uniforms.data_ptr(), path.data_ptr(), count.data_ptr(),
-            token.data_ptr()), device)
+            tc, dc, b, n, v, 0, target.data_ptr(), ts[0], 0, ts[1], draft.data_ptr(), ds[0], 0, ds[1],
+            tokens_at, parents_at, uniforms_at, path.data_ptr(), at, at + 4 * b), where)
     return path, count, token
 
 
@@ -206,24 +232,23 @@ def commit(cc, k_cache, v_cache, lens, k_new, v_new, path, count):
     the new lengths [B] int32; arguments as for ``attention`` and as ``verify``
     returns them.  A sequence that does not fit its cache is left as it is;
     the next ``cc.Synchronize()`` behind this stream reports it."""
-    torch, device = _torch(), _device(cc)
-    if k_cache.dim() != 4 or k_new.dim() != 4:
-        _refuse("k_cache" if k_cache.dim() != 4 else "k_new", "expected four dimensions")
-    b, hk, cap, d = k_cache.shape
-    n, t = k_new.shape[1], k_cache.dtype
-    code = _cache_type(k_cache, "k_cache")
-    for x, name in ((k_cache, "k_cache"), (v_cache, "v_cache")):
-        _writable(_tensor(x, name, (b, hk, cap, d), t, device), name)
-    _tensor(k_new, "k_new", (b, n, hk, d), t, device)
-    _tensor(v_new, "v_new", (b, n, hk, d), t, device)
-    _tensor(lens, "lens", (b,), torch.int32, device, True)
-    _tensor(path, "path", (b, n), torch.int32, device, True)
-    _tensor(count, "count", (b,), torch.int32, device, True)
-    out = torch.empty((b,), dtype=torch.int32, device=device)
+    torch, device, where, grad = _setting(cc)
+    rows, new = _four(k_cache, "k_cache"), _four(k_new, "k_new")
+    b, hk, cap, d = rows
+    n, t, code = new[1], k_cache.dtype, _cache_type(k_cache, "k_cache")
+    rest, new, ints = (t, device, where, grad), (b, n, hk, d), (torch.int32, device, where, grad)
+    sk, sv = _strides(k_cache, "k_cache", rows, *rest), _strides(v_cache, "v_cache", rows, *rest)
+    _writable("k_cache", rows, sk)
+    _writable("v_cache", rows, sv)
+    nk, nv = _strides(k_new, "k_new", new, *rest), _strides(v_new, "v_new", new, *rest)
+    len_at, path_at = _small(lens, "lens", (b,), *ints), _small(path, "path", (b, n), *ints)
+    count_at = _small(count, "count", (b,), *ints)
+    out = torch.empty_like(lens)
     if b:
         _call(cc, "ckks_draft_commit", _COMMIT.pack(
-            code, b, hk, d, n, cap, *_by_head(k_cache), *_by_head(v_cache), *_by_node(k_new), *_by_node(v_new),
-            lens.data_ptr(), path.data_ptr(), count.data_ptr(), out.data_ptr()), device)
+            code, b, hk, d, n, cap, k_cache.data_ptr(), sk[0], sk[1], sk[2], v_cache.data_ptr(), sv[0], sv[1], sv[2],
+            k_new.data_ptr(), nk[0], nk[2], nk[1], v_new.data_ptr(), nv[0], nv[2], nv[1],
+            len_at, path_at, count_at, out.data_ptr()), where)
     return out
 
 
@@ -232,25 +257,24 @@ def accumulate(cc, q, lse, k_cache, lens, path, count, acc, scale=None):
     attention weights of the accepted nodes, summed over the query heads of a
     key: q and lse as ``attention`` took and returned them, k_cache after the
     commit, lens before it.  The keys behind lens start from 0."""
-    torch, device = _torch(), _device(cc)
-    if q.dim() != 4 or k_cache.dim() != 4:
-        _refuse("q" if q.dim() != 4 else "k_cache", "expected four dimensions")
-    b, n, hq, d = q.shape
-    hk, cap = k_cache.shape[1], k_cache.shape[2]
+    torch, device, where, grad = _setting(cc)
+    shape, cache = _four(q, "q"), _four(k_cache, "k_cache")
+    b, n, hq, d = shape
+    hk, cap = cache[1], cache[2]
     code = _cache_type(q, "q")
-    _tensor(q, "q", (b, n, hq, d), q.dtype, device)
-    _tensor(k_cache, "k_cache", (b, hk, cap, d), q.dtype, device)
-    _tensor(lse, "lse", (b, n, hq), torch.float32, device, True)
-    _tensor(lens, "lens", (b,), torch.int32, device, True)
-    _tensor(path, "path", (b, n), torch.int32, device, True)
-    _tensor(count, "count", (b,), torch.int32, device, True)
-    _writable(_tensor(acc, "acc", (b, hk, cap), torch.float32, device), "acc")
+    ints = (torch.int32, device, where, grad)
+    sq = _strides(q, "q", shape, q.dtype, device, where, grad)
+    sk = _strides(k_cache, "k_cache", (b, hk, cap, d), q.dtype, device, where, grad)
+    lse_at = _small(lse, "lse", (b, n, hq), torch.float32, device, where, grad)
+    len_at, path_at = _small(lens, "lens", (b,), *ints), _small(path, "path", (b, n), *ints)
+    count_at = _small(count, "count", (b,), *ints)
+    sa = _strides(acc, "acc", (b, hk, cap), torch.float32, device, where, grad)
+    _writable("acc", (b, hk, cap), sa)
     if b and cap:
-        s = acc.stride()
         _call(cc, "ckks_draft_accumulate", _ACCUMULATE.pack(
-            code, b, hq, hk, d, n, cap, 0, 1.0 / math.sqrt(d) if scale is None else float(scale), *_by_node(q),
-            *_by_head(k_cache), acc.data_ptr(), s[0], s[1], 0, lse.data_ptr(), lens.data_ptr(), path.data_ptr(),
-            count.data_ptr()), device)
+            code, b, hq, hk, d, n, cap, 0, 1.0 / math.sqrt(d) if scale is None else float(scale),
+            q.data_ptr(), sq[0], sq[2], sq[1], k_cache.data_ptr(), sk[0], sk[1], sk[2], acc.data_ptr(), sa[0], sa[1], 0,
+            lse_at, len_at, path_at, count_at), where)
     return acc
 
 
@@ -263,39 +287,36 @@ def evict(cc, k_cache, v_cache, acc, lens, budget, recent, out=None):
     ``budget`` rows, zero behind the last one, when it is not given.  Returns
     k, v, acc, index [B, Hkv, budget] int32 (the rows kept, then -1) and the
     new lengths [B] int32."""
-    torch, device = _torch(), _device(cc)
-    if k_cache.dim() != 4:
-        _refuse("k_cache", "expected four dimensions")
-    b, hk, cap, d = k_cache.shape
-    t = k_cache.dtype
-    code = _cache_type(k_cache, "k_cache")
-    _tensor(k_cache, "k_cache", (b, hk, cap, d), t, device)
-    _tensor(v_cache, "v_cache", (b, hk, cap, d), t, device)
-    _tensor(acc, "acc", (b, hk, cap), torch.float32, device)
-    _tensor(lens, "lens", (b,), torch.int32, device, True)
+    torch, device, where, grad = _setting(cc)
+    rows = _four(k_cache, "k_cache")
+    b, hk, cap, d = rows
+    t, code, f32 = k_cache.dtype, _cache_type(k_cache, "k_cache"), torch.float32
+    rest = (device, where, grad)
+    sk, sv = _strides(k_cache, "k_cache", rows, t, *rest), _strides(v_cache, "v_cache", rows, t, *rest)
+    sa = _strides(acc, "acc", (b, hk, cap), f32, *rest)
+    len_at = _small(lens, "lens", (b,), torch.int32, *rest)
     if budget < 1 or not 0 <= recent <= budget:
         _refuse("budget", f"need budget >= 1 and 0 <= recent <= budget, got {budget} and {recent}")
     if out is None:
         out = (torch.zeros((b, hk, budget, d), dtype=t, device=device),
                torch.zeros((b, hk, budget, d), dtype=t, device=device),
-               torch.zeros((b, hk, budget), dtype=torch.float32, device=device))
+               torch.zeros((b, hk, budget), dtype=f32, device=device))
     k2, v2, a2 = out
-    if k2.dim() != 4:
-        _refuse("out", "expected (k, v, acc) with four, four and three dimensions")
-    rows = k2.shape[2]
-    if rows < budget:
-        _refuse("out", f"{rows} rows are fewer than the budget of {budget}")
-    for x, shape, kind in ((k2, (b, hk, rows, d), t), (v2, (b, hk, rows, d), t), (a2, (b, hk, rows), torch.float32)):
-        _writable(_tensor(x, "out", shape, kind, device), "out")
-    index = torch.empty((b, hk, budget), dtype=torch.int32, device=device)
-    new = torch.empty((b,), dtype=torch.int32, device=device)
+    kept = _four(k2, "out")[2]
+    if kept < budget:
+        _refuse("out", f"{kept} rows are fewer than the budget of {budget}")
+    sk2, sv2 = _strides(k2, "out", (b, hk, kept, d), t, *rest), _strides(v2, "out", (b, hk, kept, d), t, *rest)
+    sa2 = _strides(a2, "out", (b, hk, kept), f32, *rest)
+    _writable("out", (b, hk, kept, d), sk2)
+    _writable("out", (b, hk, kept, d), sv2)
+    _writable("out", (b, hk, kept), sa2)
+    index, new = lens.new_empty((b, hk, budget)), torch.empty_like(lens)
     if b:
-        s, s2 = acc.stride(), a2.stride()
-        head = (code, b, hk, d, cap, rows, budget, recent, *_by_head(k_cache), *_by_head(v_cache), acc.data_ptr(),
-                s[0], s[1], 0, *_by_head(k2), *_by_head(v2), a2.data_ptr(), s2[0], s2[1], 0, lens.data_ptr(),
-                index.data_ptr(), new.data_ptr())
-        name = "ckks_draft_evict"
-        ws = _workspace(cc, name, _EVICT, head, (b, hk, cap, budget), device)
-        _call(cc, name, _EVICT.pack(*head, ws.data_ptr() if ws is not None else 0, ws.numel() if ws is not None else 0),
-              device)
+        head = (code, b, hk, d, cap, kept, budget, recent, k_cache.data_ptr(), sk[0], sk[1], sk[2],
+                v_cache.data_ptr(), sv[0], sv[1], sv[2], acc.data_ptr(), sa[0], sa[1], 0,
+                k2.data_ptr(), sk2[0], sk2[1], sk2[2], v2.data_ptr(), sv2[0], sv2[1], sv2[2],
+                a2.data_ptr(), sa2[0], sa2[1], 0, len_at, index.data_ptr(), new.data_ptr())
+        ws = _workspace(cc, "ckks_draft_evict", _EVICT, head, ("evict", b, hk, cap, budget), device)
+        args = _EVICT.pack(*head, 0, 0) if ws is None else _EVICT.pack(*head, ws.data_ptr(), ws.numel())
+        _call(cc, "ckks_draft_evict", args, where)
     return k2, v2, a2, index, new
