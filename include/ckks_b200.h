@@ -332,12 +332,13 @@ int ckks_block_mlp_chunks(const ckks_block* b);
 int ckks_block_state_get(ckks_block* b, int kind, int group, ckks_ct* out);
 int ckks_block_state_set(ckks_block* b, int kind, int group, const ckks_ct* in);
 
-/* The last n tokens (0 <= n <= 64, n <= the block's tokens) of the following
- * forwards are a tree of drafted tokens: parents[i] (host) is -1 or an
- * earlier node.  The owner's softmax then lets node i see the tokens before
- * the drafts, itself and its ancestors; all other tokens stay causal.  n = 0
+/* Tokens first .. first + n - 1 (0 <= n <= 64) of the following forwards are
+ * a tree of drafted tokens: parents[i] (host) is -1 or an earlier node of the
+ * tree.  The owner's softmax then lets node i see the tokens before `first`,
+ * itself and its ancestors; all other tokens stay causal (those behind the
+ * tree see all of it: rows that only fill the block's token count).  n = 0
  * makes every token causal again. */
-int ckks_block_set_drafts(ckks_block* b, const int* parents, int n);
+int ckks_block_set_drafts(ckks_block* b, const int* parents, int n, int first);
 
 /* drop the block's encoded BSGS diagonals and masks (about 26 GB per block
  * at N = 2^16); the next forward encodes them again on the device */

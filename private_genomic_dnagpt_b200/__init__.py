@@ -191,7 +191,7 @@ _SIGS = [
     ("ckks_draft_accumulate", ctypes.c_int, [_vp, ctypes.c_char_p, _vp]),
     ("ckks_draft_evict", ctypes.c_int, [_vp, ctypes.c_char_p, _vp]),
     ("ckks_draft_evict_workspace", ctypes.c_longlong, [_vp, ctypes.c_char_p]),
-    ("ckks_block_set_drafts", ctypes.c_int, [_vp, ctypes.POINTER(ctypes.c_int), ctypes.c_int]),
+    ("ckks_block_set_drafts", ctypes.c_int, [_vp, ctypes.POINTER(ctypes.c_int), ctypes.c_int, ctypes.c_int]),
 ]
 
 _lib = None
@@ -819,6 +819,15 @@ class EncryptedBlock:
         _check(lib().ckks_block_forward(self.h, _f64(x), x.shape[0], _f64(y)))
         return y
 
+    def set_drafts(self, parents=(), first: int | None = None):
+        """Makes tokens first .. first + len(parents) - 1 (default: the last
+        ones) of the following forwards a tree of drafted tokens: a node sees
+        the tokens before the tree, itself and its ancestors.  No parents:
+        every token is causal again."""
+        n = len(parents)
+        _check(lib().ckks_block_set_drafts(self.h, (ctypes.c_int * max(1, n))(*[int(p) for p in parents]), n,
+                                           self.tokens - n if first is None else first))
+
     def report(self) -> dict:
         import json
         n = lib().ckks_block_report(self.h, None, 0)
@@ -984,8 +993,20 @@ class EncryptedModel:
             s |= set(self.head.rotation_indices())
         return sorted(s)
 
-    def forward(self, x: np.ndarray):
-        """Returns (hidden [tokens, D] of the last block, head margin or None)."""
+    def forward(self, x: np.ndarray, parents=(), first: int | None = None):
+        """Returns (hidden [tokens, D] of the last block, head margin or None).
+        With ``parents``, tokens first .. first + len(parents) - 1 (default:
+        the last ones) are a tree of drafted tokens, all evaluated in this one
+        forward: row first + i is the hidden state of node i behind the tokens
+        before the tree and its ancestors."""
+        if len(parents):
+            for b in self.blocks:
+                b.set_drafts(parents, first)
+            try:
+                return self.forward(x)
+            finally:
+                for b in self.blocks:
+                    b.set_drafts()
         x = np.ascontiguousarray(x, np.float64)
         hidden = np.zeros_like(x)
         m = np.zeros(1, np.float64)
@@ -994,6 +1015,33 @@ class EncryptedModel:
         _check(lib().ckks_model_forward(hs, n, self.head.h if self.head is not None else None, _f64(x),
                                         x.shape[0], self.cached_blocks, _f64(hidden), _f64(m)))
         return hidden, (float(m[0]) if self.head is not None else None)
+
+    def verify_drafts(self, x: np.ndarray, drafts: np.ndarray, tokens, parents, draft, uniforms, readout):
+        """One encrypted forward over the context x [m, D] (m >= 1) and the
+        drafts' embeddings [n, D] (m + n <= tokens; the last row fills the
+        rest), and the owner's acceptance of the drafts by its probabilities
+        softmax(hidden @ readout.T) in float64, readout [vocabulary, D].
+        ``tokens``, ``parents`` (n ints), ``draft`` [n + 1, vocabulary] and
+        ``uniforms`` [n + 1] are those of ``draft_verify`` for one sequence.
+        Returns (accepted nodes from the root on, next token)."""
+        import torch
+        x, drafts = np.asarray(x, np.float64), np.asarray(drafts, np.float64)
+        m, n = x.shape[0], drafts.shape[0]
+        if m < 1 or n < 1 or m + n > self.tokens:
+            raise ValueError(f"a context of {m} tokens and {n} drafts do not fit the model's {self.tokens} tokens")
+        fill = np.repeat(drafts[-1:], self.tokens - m - n, axis=0)
+        hidden, _ = self.forward(np.concatenate([x, drafts, fill]), parents, m)
+        device = torch.device("cuda", self.cc.params.device)
+        rows = torch.from_numpy(hidden[m - 1:m + n]).to(device)
+        target = torch.softmax(rows @ torch.as_tensor(readout, dtype=torch.float64, device=device).T, -1)
+
+        def one(v, t):
+            return torch.as_tensor(v, dtype=t, device=device)[None].contiguous()
+
+        draft = torch.as_tensor(draft, device=device)[None]
+        path, count, token = self.cc.draft_verify(target[None], draft, one(tokens, torch.int32),
+                                                  one(parents, torch.int32), one(uniforms, torch.float64))
+        return path[0, :int(count[0])].tolist(), int(token[0])
 
 
 def schedule_active_shifts(tokens: int, batch: int, qg: int, kg: int) -> list[int]:

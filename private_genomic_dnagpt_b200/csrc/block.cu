@@ -507,17 +507,17 @@ __global__ void score_gather_kernel(const double* __restrict__ vals, const Score
   scores[((size_t)q * H + h) * T + k] = vals[(size_t)tg.v * slots + (size_t)f * B + ql];
 }
 
-// the tree of drafted tokens that the last n tokens form: bit j of mask[i] is
-// set where drafted token i sees drafted token j (n = 0: every token causal)
+// the tree that tokens first .. first + n - 1 form: bit j of mask[i] is set
+// where node i sees node j (n = 0: every token causal)
 struct DraftTree {
   unsigned long long mask[64];
-  int n;
+  int n, first;
 };
 
-// whether token q sees token k <= q of T
-__device__ __forceinline__ bool draft_sees(const DraftTree& tree, int T, int q, int k) {
-  const int first = T - tree.n;
-  return q < first || k < first || (tree.mask[q - first] >> (k - first) & 1);
+// whether token q sees token k <= q
+__device__ __forceinline__ bool draft_sees(const DraftTree& tree, int q, int k) {
+  const int i = q - tree.first, j = k - tree.first;
+  return i < 0 || i >= tree.n || j < 0 || (tree.mask[i] >> j & 1);
 }
 
 // stable softmax of row (q, h) over the drafted tokens' ancestors and the
@@ -532,12 +532,12 @@ __global__ void softmax_tree_kernel(const double* __restrict__ scores, double* _
   double mx = -INFINITY;
   for (int k = 0; k <= q; ++k) {
     if (!isfinite(row[k])) atomicExch(bad, 1);
-    if (draft_sees(tree, T, q, k)) mx = fmax(mx, row[k]);
+    if (draft_sees(tree, q, k)) mx = fmax(mx, row[k]);
   }
   double den = 0.0;
   for (int k = 0; k <= q; ++k)
-    if (draft_sees(tree, T, q, k)) den += exp(row[k] - mx);
-  for (int k = 0; k < T; ++k) out[k] = k <= q && draft_sees(tree, T, q, k) ? exp(row[k] - mx) / den : 0.0;
+    if (draft_sees(tree, q, k)) den += exp(row[k] - mx);
+  for (int k = 0; k < T; ++k) out[k] = k <= q && draft_sees(tree, q, k) ? exp(row[k] - mx) / den : 0.0;
 }
 
 // stable causal softmax of row (q, h) over k <= q; a missing score poisons the row
@@ -1838,14 +1838,16 @@ int ckks_head_forward(ckks_block* h, const double* x_last, double* margin) {
   });
 }
 
-int ckks_block_set_drafts(ckks_block* b, const int* parents, int n) {
+int ckks_block_set_drafts(ckks_block* b, const int* parents, int n, int first) {
   return bguard([&] {
     if (!b || (n && !parents)) throw ckks::Error(CKKS_EARG, "null argument");
     if (b->orphaned) throw ckks::Error(CKKS_ESTATE, "the block's context was destroyed");
     if (b->d_head) throw ckks::Error(CKKS_EARG, "a head evaluates one token");
-    if (n < 0 || n > 64 || n > b->s.T) throw ckks::Error(CKKS_EARG, "draft count outside 0..64 or above the token count");
+    if (n < 0 || n > 64 || first < 0 || first > b->s.T - n)
+      throw ckks::Error(CKKS_EARG, "more than 64 drafted tokens, or drafted tokens outside the block's");
     blk::DraftTree t{};
     t.n = n;
+    t.first = first;
     for (int i = 0; i < n; ++i) {
       if (parents[i] < -1 || parents[i] >= i)
         throw ckks::Error(CKKS_EARG, "a drafted token's parent is -1 or an earlier drafted token");

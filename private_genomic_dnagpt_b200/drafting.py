@@ -320,3 +320,97 @@ def evict(cc, k_cache, v_cache, acc, lens, budget, recent, out=None):
         args = _EVICT.pack(*head, 0, 0) if ws is None else _EVICT.pack(*head, ws.data_ptr(), ws.numel())
         _call(cc, "ckks_draft_evict", args, where)
     return k2, v2, a2, index, new
+
+
+class DraftModel:
+    """The data owner's plain draft model: blocks of the weights that
+    ``EncryptedBlock`` takes (bias-free pre-LN, tanh-GELU), evaluated on the
+    context's GPU over a key/value cache of ``capacity`` rows per block.
+
+    ``forward`` evaluates a tree of drafted nodes behind the cached tokens,
+    ``accept`` appends the nodes that the target confirmed, ``prefill`` takes
+    a prompt.  With ``budget``, the cache is cut to its ``recent`` latest and
+    its heaviest keys before it would overflow."""
+
+    def __init__(self, cc, block_weights: list, capacity: int, batch: int = 1, heads: int = 12, dtype=None,
+                 budget: int | None = None, recent: int = 0):
+        torch, device, _, _ = _setting(cc)
+        self.cc, self.heads, self.batch, self.capacity = cc, heads, batch, capacity
+        self.budget, self.recent = budget, recent
+        self.dtype = torch.bfloat16 if dtype is None else dtype
+        if budget is not None and budget + MAX_NODES > capacity:
+            _refuse("budget", f"{budget} rows and a tree of {MAX_NODES} nodes do not fit a capacity of {capacity}")
+        names = ("ln1", "attn_qkv", "attn_proj", "ln2", "mlp_fc", "mlp_proj")
+        self.weights = [{k: torch.as_tensor(w[k]).to(device=device, dtype=torch.float32 if k[:2] == "ln" else self.dtype)
+                         for k in names} for w in block_weights]
+        self.width = self.weights[0]["ln1"].shape[0]
+
+        def caches():
+            rows = (batch, heads, capacity, self.width // heads)
+            return [(torch.zeros(rows, dtype=self.dtype, device=device), torch.zeros(rows, dtype=self.dtype, device=device),
+                     torch.zeros(rows[:3], device=device)) for _ in block_weights]
+
+        self.caches, self._spare = caches(), caches() if budget is not None else None
+        self.lens = torch.zeros(batch, dtype=torch.int32, device=device)
+        self._most = 0  # no sequence has more rows than this
+        self._steps = None
+
+    def forward(self, x, parents):
+        """Hidden states [batch, n, D] (float32) of the nodes with embeddings
+        x [batch, n, D] and parents [batch, n] int32 behind the cached tokens.
+        The nodes' rows are kept for ``accept``."""
+        torch = _torch()
+        b, n, width = x.shape
+        if self._most + n > self.capacity:
+            self._make_room(n)
+        x, steps = x.to(torch.float32), []
+        for w, (k_cache, v_cache, _) in zip(self.weights, self.caches):
+            h = torch.layer_norm(x, (width,), w["ln1"], None, 1e-5).to(self.dtype)
+            q, k, v = (h @ w["attn_qkv"].T).view(b, n, 3, self.heads, width // self.heads).unbind(2)
+            out, lse = attention(self.cc, q, k_cache, v_cache, self.lens, k, v, parents)
+            x = x + (out.reshape(b, n, width) @ w["attn_proj"].T).float()
+            h = torch.layer_norm(x, (width,), w["ln2"], None, 1e-5).to(self.dtype)
+            h = torch.nn.functional.gelu(h @ w["mlp_fc"].T, approximate="tanh")
+            x = x + (h @ w["mlp_proj"].T).float()
+            steps.append((q, lse, k, v))
+        self._steps = steps
+        return x
+
+    def accept(self, path, count):
+        """Appends the nodes path[:, :count] of the last ``forward`` to every
+        block's cache, and their attention weights to its keys'."""
+        if self._steps is None:
+            raise RuntimeError("accept follows a forward")
+        lens = self.lens
+        for (q, lse, k, v), (k_cache, v_cache, acc) in zip(self._steps, self.caches):
+            self.lens = commit(self.cc, k_cache, v_cache, lens, k, v, path, count)
+            if self.budget is not None:
+                accumulate(self.cc, q, lse, k_cache, lens, path, count, acc)
+        self._most = min(self.capacity, self._most + path.shape[1])
+        self._steps = None
+
+    def prefill(self, x):
+        """A prompt's embeddings [batch, m, D], in chains of 64 nodes; returns
+        the hidden states [batch, m, D]."""
+        torch = _torch()
+        got = []
+        for c in x.split(MAX_NODES, dim=1):
+            n = c.shape[1]
+            chain = torch.arange(n, dtype=torch.int32, device=c.device).repeat(self.batch, 1)
+            got.append(self.forward(c, chain - 1))
+            self.accept(chain, torch.full((self.batch,), n, dtype=torch.int32, device=c.device))
+        return torch.cat(got, 1)
+
+    def _make_room(self, n):
+        """Before n more rows: the cache cut to its budget, or, without one,
+        the rows counted exactly."""
+        if self.budget is None:
+            self._most = int(self.lens.max())
+            if self._most + n > self.capacity:
+                raise ValueError(f"{self._most} cached rows and {n} nodes exceed the capacity of {self.capacity}")
+            return
+        lens = self.lens
+        for i, (k, v, acc) in enumerate(self.caches):
+            _, _, _, _, self.lens = evict(self.cc, k, v, acc, lens, self.budget, self.recent, out=self._spare[i])
+        self.caches, self._spare = self._spare, self.caches
+        self._most = min(self._most, self.budget)

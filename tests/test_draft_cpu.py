@@ -110,7 +110,7 @@ def test_c_entry_points_refuse_null():
         assert b"null context" in lib.ckks_last_error()
     for name in ("attention", "evict"):
         assert getattr(lib, f"ckks_draft_{name}_workspace")(None, b"\0" * 512) == -1
-    assert lib.ckks_block_set_drafts(None, None, 0) == 1
+    assert lib.ckks_block_set_drafts(None, None, 0, 0) == 1
 
 
 def test_layouts_match_the_header(tmp_path):
