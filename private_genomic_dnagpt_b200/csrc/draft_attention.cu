@@ -26,12 +26,34 @@ struct AttnParams {
   float* lse;
   float* part;  // [batch * kv_heads][splits][rows][head_dim + 2]
   int batch, kv_heads, group, head_dim, nodes, capacity, splits;
-  int tile_nodes;  // nodes of one 128-row tile
+  // The kernels that divide a list of units among their CTAs: rows of a unit,
+  // keys of a tile, whether the new keys have a tile of their own, and what a
+  // unit's start and end cost in tiles
+  int tile_nodes, tile_rows, tile_keys, new_apart, unit_cost;
   float scale;
   bool wide;  // every row is whole, aligned 16-byte pieces
 };
 
 __device__ __forceinline__ int length_of(const AttnParams& p, int b) { return min(max(p.lens[b], 0), p.capacity); }
+
+// tiles of a unit of sequence b
+__device__ __forceinline__ int tiles_of(const AttnParams& p, int b) {
+  const int len = length_of(p, b);
+  return p.new_apart ? (len + p.tile_keys - 1) / p.tile_keys + 1 : (len + p.nodes + p.tile_keys - 1) / p.tile_keys;
+}
+
+// A place in the list: sequence, unit within it, tile within that (below 0:
+// the unit's start) and the unit's tiles
+struct Cursor {
+  int b, unit, tile, tiles;
+  __device__ __forceinline__ void next_unit(const AttnParams& p, int units) {
+    tile = -p.unit_cost;
+    if (++unit == units) {
+      unit = 0;
+      tiles = ++b < p.batch ? tiles_of(p, b) : 1;
+    }
+  }
+};
 
 // natural exponent through the base-2 one: scores are kept times log2(e)
 constexpr float kLog2e = 1.4426950408889634f;
@@ -328,28 +350,8 @@ constexpr int kM = 128, kKeys = 128, kTcThreads = 320, kTmemCols = 512;
 constexpr uint32_t kPanel = 128 * 128;  // 128 rows x 64 elements
 constexpr float kSlack = 8.0f;
 
-// What a unit's start and end cost, in tiles: measured on trees of 21 over 4001
-// keys of 64 (2 / 3 / 4 / 5 / 6 tiles: 32.7 / 28.4 / 26.9 / 27.8 / 29.0 us) and
-// trees of 32 over 65536 keys of 128 (2 / 4 / 6 / 8: 97.6 / 95.3 / 93.7 / 91.4 us)
-__host__ __device__ __forceinline__ int unit_cost(const AttnParams& p) { return p.head_dim <= 64 ? 4 : 8; }
-
 struct TileMaps {
   CUtensorMap q, kc, vc, kn, vn;
-};
-
-__device__ __forceinline__ int tiles_of(const AttnParams& p, int b) { return (length_of(p, b) + kKeys - 1) / kKeys + 1; }
-
-// A place in the list: sequence, unit within it, tile within that (below 0:
-// the unit's start) and the unit's tiles
-struct Cursor {
-  int b, unit, tile, tiles;
-  __device__ __forceinline__ void next_unit(const AttnParams& p, int units) {
-    tile = -unit_cost(p);
-    if (++unit == units) {
-      unit = 0;
-      tiles = ++b < p.batch ? tiles_of(p, b) : 1;
-    }
-  }
 };
 
 template <typename T>
@@ -415,7 +417,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   const uint32_t o_full = bars + 8 * (2 * NS + 8);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int tiles_r = (p.nodes + p.tile_nodes - 1) / p.tile_nodes, units = p.kv_heads * tiles_r;
-  const int tile_rows = p.tile_nodes * p.group;
+  const int tile_rows = p.tile_rows;
   asm volatile("griddepcontrol.launch_dependents;");
   if (tid == 0) {
     for (int s = 0; s < NS; ++s) {
@@ -434,11 +436,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   if (warp == 9) tmem_alloc(smem_addr(s_tmem), kTmemCols);
   // this CTA's entries [w0, w1) of the list
   int first;
-  auto entries_of = [&](int b) { return tiles_of(p, b) + unit_cost(p); };
+  auto entries_of = [&](int b) { return tiles_of(p, b) + p.unit_cost; };
   const int entries = list_sum(p.batch, entries_of, first) * units;
   const int w0 = list_start(entries, blockIdx.x, gridDim.x), w1 = list_start(entries, blockIdx.x + 1, gridDim.x);
   const ListPlace begin = list_find(p.batch, units, w0, first, entries_of);
-  Cursor at = {begin.b, begin.unit, begin.entry - unit_cost(p), begin.entries - unit_cost(p)};
+  Cursor at = {begin.b, begin.unit, begin.entry - p.unit_cost, begin.entries - p.unit_cost};
   tmem_fence_before();
   __syncthreads();
   tmem_fence_after();
@@ -773,12 +775,12 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 
 // joins the parts of the units that several CTAs share; a warp per row
 template <typename T, int PANELS>
-__global__ void __launch_bounds__(256) join_tc_kernel(const __grid_constant__ AttnParams p, int ctas) {
+__global__ void __launch_bounds__(256) join_list_kernel(const __grid_constant__ AttnParams p, int ctas) {
   constexpr int DP = 64 * PANELS;
   __shared__ uint64_t s_mask[8][kMaxNodes];
   __shared__ int s_jump[8][kMaxNodes];
   const int rows = p.nodes * p.group;
-  const int tiles_r = (p.nodes + p.tile_nodes - 1) / p.tile_nodes, units = p.kv_heads * tiles_r;
+  const int tile_rows = p.tile_rows, tiles_r = (rows + tile_rows - 1) / tile_rows, units = p.kv_heads * tiles_r;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int per = (rows + 7) / 8;  // CTAs of a (sequence, head)
   const int bh = blockIdx.x / per, row = blockIdx.x % per * 8 + warp;
@@ -787,13 +789,13 @@ __global__ void __launch_bounds__(256) join_tc_kernel(const __grid_constant__ At
     CKKS_PDL_ENTRY();
     return;
   }
-  const int tile_rows = p.tile_nodes * p.group, unit = h * tiles_r + row / tile_rows, r = row % tile_rows;
+  const int unit = h * tiles_r + row / tile_rows, r = row % tile_rows;
   // this unit's tiles [u0, u1) of the list, and the CTAs that have the first
   // and the last: CTA i begins at list_start(i), so w is CTA
   // floor((ctas (w + 1) - 1) / entries)'s
   int before = 0, all = 0;
   for (int i = lane; i < p.batch; i += 32) {
-    const int t = tiles_of(p, i) + unit_cost(p);
+    const int t = tiles_of(p, i) + p.unit_cost;
     all += t;
     if (i < b) before += t;
   }
@@ -803,7 +805,7 @@ __global__ void __launch_bounds__(256) join_tc_kernel(const __grid_constant__ At
     before += __shfl_xor_sync(0xffffffffu, before, o);
   }
   const int tiles = tiles_of(p, b);
-  const long long W = (long long)all * units, u0 = (long long)before * units + unit * (tiles + unit_cost(p)) + unit_cost(p);
+  const long long W = (long long)all * units, u0 = (long long)before * units + unit * (tiles + p.unit_cost) + p.unit_cost;
   const int c0 = (int)((ctas * (u0 + 1) - 1) / W), c1 = (int)((ctas * (u0 + tiles) - 1) / W);
   if (c0 == c1) {
     CKKS_PDL_ENTRY();
@@ -848,6 +850,255 @@ __global__ void __launch_bounds__(256) join_tc_kernel(const __grid_constant__ At
     if (spoiled & mask) add_spoiled<T>(p, b, h, node, qh, spoiled & mask, m, inv, o);
     p.lse[((size_t)b * p.nodes + node) * p.kv_heads * p.group + qh] =
         l != 0.0f && seen ? kLn2 * (m + log2f(l)) : -INFINITY;
+  }
+}
+
+// ---- float32: CUDA cores --------------------------------------------------------
+// A unit is (sequence, head, RT rows); the CTAs divide the list of all units'
+// key tiles evenly, as above.  A tile of KT keys (the cached and then the new
+// ones) and its values arrive in one of two stages by asynchronous copies
+// while the other is worked on; three CTAs of 34 to 68 KB share an SM.
+// Scores: a thread has one key and RPT rows, so an element of K from shared
+// memory feeds RPT multiply-adds and those of q are broadcasts.  Values: 16
+// threads across each 64 elements, eight across the tile's keys, each with the
+// sums of all RT rows in registers, which meet when the unit is done.  The
+// products are plain float32 multiply-adds: a 32-bit cache is kept for its
+// accuracy.
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool real) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copies_close() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copies_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+template <int RT, int DC>
+struct F32Shape {
+  static constexpr int KT = DC == 1 ? 64 : DC == 2 ? 32 : 16, DP = 64 * DC, KS = DP + 4;  // K rows: reads without conflicts
+  static constexpr int kStage = KT * KS + KT * DP;                                      // floats
+  static constexpr size_t kSmem = sizeof(float) * (2 * kStage + RT * DP + KT * RT + 3 * RT) + kMaxNodes * 12;
+  static_assert(sizeof(float) * 8 * RT * 64 <= sizeof(float) * 2 * kStage, "a unit's sums meet in the stages");
+};
+
+template <int RT, int DC>
+__global__ void __launch_bounds__(kThreads, DC == 1 ? 3 : 2) attend_f32_kernel(const __grid_constant__ AttnParams p) {
+  using S = F32Shape<RT, DC>;
+  constexpr int KT = S::KT, DP = S::DP, KS = S::KS, KG = kThreads / KT, RPT = RT / KG;  // row groups, rows of a thread
+  extern __shared__ __align__(16) float sm[];
+  float* const sq = sm + 2 * S::kStage;  // [RT][DP]
+  float* const sp = sq + RT * DP;        // [KT][RT]
+  float* const s_m = sp + KT * RT;       // running maximum, sum and this tile's factor of each row
+  float* const s_l = s_m + RT;
+  float* const s_c = s_l + RT;
+  uint64_t* const s_mask = reinterpret_cast<uint64_t*>(s_c + RT);
+  int* const s_jump = reinterpret_cast<int*>(s_mask + kMaxNodes);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int rows = p.nodes * p.group, tiles_r = (rows + RT - 1) / RT, units = p.kv_heads * tiles_r, D = p.head_dim;
+  asm volatile("griddepcontrol.launch_dependents;");
+  int first;
+  auto entries_of = [&](int b) { return tiles_of(p, b) + p.unit_cost; };
+  const int entries = list_sum(p.batch, entries_of, first) * units;
+  const int w0 = list_start(entries, blockIdx.x, gridDim.x), w1 = list_start(entries, blockIdx.x + 1, gridDim.x);
+  if (w0 >= w1) return;
+  const ListPlace begin = list_find(p.batch, units, w0, first, entries_of);
+  Cursor at = {begin.b, begin.unit, begin.entry - p.unit_cost, begin.entries - p.unit_cost};
+  const int key = tid % KT, rg = tid / KT;  // scores: this thread's key of the tile and rows RPT rg ..
+  const int dg = tid & 15, kg = tid >> 4;   // values: this thread's elements and every eighth key
+  int masks_of = -1;
+  for (int w = w0; w < w1;) {
+    const int skip = max(0, min(-at.tile, w1 - w));
+    at.tile += skip;
+    w += skip;
+    const int n = max(0, min(at.tiles - at.tile, w1 - w));
+    if (n == 0) break;  // only a unit's start is left
+    const int b = at.b, h = at.unit / tiles_r, row0 = at.unit % tiles_r * RT;
+    const int len = length_of(p, b), total = len + p.nodes;
+    const float* kc = static_cast<const float*>(p.kc.data) + b * p.kc.batch + h * p.kc.head;
+    const float* vc = static_cast<const float*>(p.vc.data) + b * p.vc.batch + h * p.vc.head;
+    const float* kn = static_cast<const float*>(p.kn.data) + b * p.kn.batch + h * p.kn.head;
+    const float* vn = static_cast<const float*>(p.vn.data) + b * p.vn.batch + h * p.vn.head;
+    auto load = [&](int t, int stage) {
+      const uint32_t k_at = smem_addr(sm + stage * S::kStage), v_at = k_at + 4 * KT * KS;
+#pragma unroll
+      for (int i = tid; i < KT * DP / 4; i += kThreads) {
+        const int r = i / (DP / 4), d = i % (DP / 4) * 4, s = (at.tile + t) * KT + r;
+        const bool cached = s < len, real = d < D && s < total && (cached || s_mask[s - len] != 0ull);
+        const float *k = kc, *v = vc;
+        if (real) {
+          k = (cached ? kc + s * p.kc.row : kn + (s - len) * p.kn.row) + d;
+          v = (cached ? vc + s * p.vc.row : vn + (s - len) * p.vn.row) + d;
+        } else {
+          k = v = static_cast<const float*>(p.q.data);  // not read
+        }
+        copy16(k_at + 4 * (r * KS + d), k, real);
+        copy16(v_at + 4 * (r * DP + d), v, real);
+      }
+      copies_close();
+    };
+    if (masks_of != b && warp == 0) tree_masks(p.parents + (size_t)b * p.nodes, p.nodes, s_mask, s_jump);
+    masks_of = b;
+    if (tid < RT) s_m[tid] = -INFINITY, s_l[tid] = 0.0f;
+    __syncthreads();
+    load(0, 0);
+    for (int i = tid; i < RT * (DP / 4); i += kThreads) {
+      const int r = i / (DP / 4), d = i % (DP / 4) * 4, row = row0 + r;
+      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (row < rows && d < D)
+        x = *reinterpret_cast<const float4*>(static_cast<const float*>(p.q.data) + b * p.q.batch +
+                                             (h * p.group + row % p.group) * p.q.head + (row / p.group) * p.q.row + d);
+      const float c = p.scale * kLog2e;
+      *reinterpret_cast<float4*>(sq + r * DP + d) = make_float4(x.x * c, x.y * c, x.z * c, x.w * c);
+    }
+    float acc[DC][RT][4];
+#pragma unroll
+    for (int c = 0; c < DC; ++c)
+#pragma unroll
+      for (int r = 0; r < RT; ++r)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[c][r][e] = 0.0f;
+    for (int t = 0; t < n; ++t) {
+      const int t0 = (at.tile + t) * KT, nk = min(KT, total - t0);
+      if (t + 1 < n) {
+        load(t + 1, (t + 1) & 1);
+        copies_wait<1>();
+      } else {
+        copies_wait<0>();
+      }
+      __syncthreads();
+      const float* sk = sm + (t & 1) * S::kStage;
+      const float* sv = sk + KT * KS;
+      {
+        float x[RPT];
+#pragma unroll
+        for (int r = 0; r < RPT; ++r) x[r] = 0.0f;
+#pragma unroll 8
+        for (int d = 0; d < DP; d += 4) {
+          const float4 k4 = *reinterpret_cast<const float4*>(sk + key * KS + d);
+#pragma unroll
+          for (int r = 0; r < RPT; ++r) {
+            const float4 q4 = *reinterpret_cast<const float4*>(sq + (RPT * rg + r) * DP + d);
+            x[r] = fmaf(k4.x, q4.x, fmaf(k4.y, q4.y, fmaf(k4.z, q4.z, fmaf(k4.w, q4.w, x[r]))));
+          }
+        }
+        const int s = t0 + key;
+        if (t0 + KT > len) {
+#pragma unroll
+          for (int r = 0; r < RPT; ++r) {
+            const int row = row0 + RPT * rg + r;
+            const uint64_t m = row < rows ? s_mask[row / p.group] : 0ull;
+            if (!(key < nk && m && (s < len || (m >> (s - len) & 1)))) x[r] = -INFINITY;
+          }
+        }
+#pragma unroll
+        for (int r = 0; r < RPT; ++r) sp[key * RT + RPT * rg + r] = x[r];
+      }
+      __syncthreads();
+      // running maximum and sum: a warp has RT / 4 rows
+#pragma unroll
+      for (int j = 0; j < RT / 4; ++j) {
+        const int r = warp * (RT / 4) + j;
+        constexpr int KL = (KT + 31) / 32;
+        float x[KL];
+        float mx = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < KL; ++i) {
+          x[i] = lane + 32 * i < KT ? sp[(lane + 32 * i) * RT + r] : -INFINITY;
+          mx = fmaxf(mx, x[i]);
+        }
+#pragma unroll
+        for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+        const float old = s_m[r], m = fmaxf(old, mx), base = m == -INFINITY ? 0.0f : m;
+        float sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < KL; ++i) {
+          x[i] = exp2f(x[i] - base);
+          sum += x[i];
+          if (lane + 32 * i < KT) sp[(lane + 32 * i) * RT + r] = x[i];
+        }
+#pragma unroll
+        for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if (lane == 0) {
+          const float f = exp2f(old - base);
+          s_m[r] = m;
+          s_l[r] = s_l[r] * f + sum;
+          s_c[r] = f;
+        }
+      }
+      __syncthreads();
+      bool same = true;
+#pragma unroll
+      for (int r = 0; r < RT; ++r) same = same && s_c[r] == 1.0f;
+      if (!same) {
+#pragma unroll
+        for (int r = 0; r < RT; ++r) {
+          const float f = s_c[r];
+#pragma unroll
+          for (int c = 0; c < DC; ++c)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[c][r][e] *= f;
+        }
+      }
+      // among new keys a weight of 0 adds nothing, whatever a value that other rows see holds
+      const bool apart = t0 + KT > len;
+#pragma unroll
+      for (int i = 0; i < KT / 8; ++i) {
+        const int k = kg + 8 * i;
+        float x[RT];
+#pragma unroll
+        for (int r = 0; r < RT; r += 4) *reinterpret_cast<float4*>(x + r) = *reinterpret_cast<const float4*>(sp + k * RT + r);
+#pragma unroll
+        for (int c = 0; c < DC; ++c) {
+          const float4 v4 = *reinterpret_cast<const float4*>(sv + k * DP + c * 64 + dg * 4);
+#pragma unroll
+          for (int r = 0; r < RT; ++r)
+            if (!apart || x[r] != 0.0f) {
+              acc[c][r][0] = fmaf(x[r], v4.x, acc[c][r][0]);
+              acc[c][r][1] = fmaf(x[r], v4.y, acc[c][r][1]);
+              acc[c][r][2] = fmaf(x[r], v4.z, acc[c][r][2]);
+              acc[c][r][3] = fmaf(x[r], v4.w, acc[c][r][3]);
+            }
+        }
+      }
+      __syncthreads();
+    }
+    // the eight key groups' sums meet in the stages, 64 elements at a time
+    const bool whole = at.tile == 0 && n == at.tiles;
+    if (whole && tid < RT && row0 + tid < rows && s_mask[(row0 + tid) / p.group] == 0ull) s_l[tid] = 0.0f;  // padding
+    float* const keep = p.part + (size_t)(2 * blockIdx.x + (at.tile == 0 ? 1 : 0)) * RT * (DP + 4);
+#pragma unroll
+    for (int c = 0; c < DC; ++c) {
+#pragma unroll
+      for (int r = 0; r < RT; ++r)
+        *reinterpret_cast<float4*>(sm + (kg * RT + r) * 64 + dg * 4) =
+            make_float4(acc[c][r][0], acc[c][r][1], acc[c][r][2], acc[c][r][3]);
+      __syncthreads();
+      for (int i = tid; i < RT * 64; i += kThreads) {
+        const int r = i / 64, d = c * 64 + i % 64, row = row0 + r;
+        if (row >= rows) continue;
+        float x = 0.0f;
+#pragma unroll
+        for (int g = 0; g < 8; ++g) x += sm[(g * RT + r) * 64 + i % 64];
+        if (!whole) {
+          keep[r * (DP + 4) + d] = x;
+        } else if (d < D) {
+          const float l = s_l[r];
+          out_row<float>(p, b, row / p.group, h * p.group + row % p.group)[d] = l != 0.0f ? x / l : 0.0f;
+        }
+      }
+      __syncthreads();
+    }
+    if (tid < RT && row0 + tid < rows) {
+      const int row = row0 + tid;
+      if (whole)
+        p.lse[((size_t)b * p.nodes + row / p.group) * p.kv_heads * p.group + h * p.group + row % p.group] =
+            s_l[tid] != 0.0f ? kLn2 * (s_m[tid] + log2f(s_l[tid])) : -INFINITY;
+      else
+        *reinterpret_cast<float4*>(keep + tid * (DP + 4) + DP) = make_float4(s_m[tid], s_l[tid], 0.0f, 0.0f);
+    }
+    __syncthreads();
+    w += n;
+    at.next_unit(p, units);
   }
 }
 
@@ -910,35 +1161,95 @@ bool tc_sizes(const ckks_draft_attention_args& a) {
   return a.dtype != CKKS_FP32 && a.head_dim <= 128 && a.head_dim % 8 == 0 && a.q_heads / a.kv_heads <= kM;
 }
 
-// nodes whose rows a tile holds
+// nodes whose rows a tile of the tensor-core kernel holds
 int tile_nodes(const ckks_draft_attention_args& a) { return std::min(a.nodes, kM / (a.q_heads / a.kv_heads)); }
 
-// Tensor-core CTAs: one on each SM, but no fewer than four tiles of keys
-// each at the full capacity (a shorter part is all start-up), and one for
-// each unit where there are fewer units than that
-int tc_ctas(const Context& c, const ckks_draft_attention_args& a) {
-  const int per = tile_nodes(a);
-  const long long units = (long long)a.batch * a.kv_heads * ((a.nodes + per - 1) / per);
-  const long long tiles = units * ((a.capacity + kKeys - 1) / kKeys + 1), slots = c.sms;
-  return (int)std::max(1ll, std::min(slots, std::max(tiles / 4, units)));
+// how a kernel divides its list of units
+struct Division {
+  int tile_rows, tile_keys, new_apart, unit_cost, ctas;
+  bool alone;  // no unit is shared
+};
+
+// `per_sm` CTAs on each SM, but no fewer than four tiles of keys each at the
+// full capacity (a shorter part is all start-up), and one for each unit where
+// there are fewer units than that
+Division divide(const Context& c, const ckks_draft_attention_args& a, Division d, int per_sm) {
+  const long long rows = (long long)a.nodes * (a.q_heads / a.kv_heads);
+  const long long units = (long long)a.batch * a.kv_heads * ((rows + d.tile_rows - 1) / d.tile_rows);
+  const long long tiles = units * ((a.capacity + d.tile_keys - 1) / d.tile_keys + 1);
+  d.ctas = (int)std::max(1ll, std::min((long long)per_sm * c.sms, std::max(tiles / 4, units)));
+  d.alone = a.batch == 1 && d.ctas == units;  // one sequence and a CTA for each unit
+  return d;
 }
 
-// one sequence and a CTA for each unit: no unit is shared
-bool tc_alone(const ckks_draft_attention_args& a, int ctas) {
-  const int per = tile_nodes(a);
-  return a.batch == 1 && ctas == a.kv_heads * ((a.nodes + per - 1) / per);
+// What a unit's start and end cost, in tiles: measured on trees of 21 over 4001
+// keys of 64 (2 / 3 / 4 / 5 / 6 tiles: 32.7 / 28.4 / 26.9 / 27.8 / 29.0 us) and
+// trees of 32 over 65536 keys of 128 (2 / 4 / 6 / 8: 97.6 / 95.3 / 93.7 / 91.4 us)
+Division tc_division(const Context& c, const ckks_draft_attention_args& a) {
+  const int rows = tile_nodes(a) * (a.q_heads / a.kv_heads);
+  return divide(c, a, Division{rows, kKeys, 1, a.head_dim <= 64 ? 4 : 8, 0, false}, 1);
+}
+
+bool f32_sizes(const ckks_draft_attention_args& a) { return a.dtype == CKKS_FP32 && a.head_dim % 4 == 0; }
+
+// 16 rows in a unit where there are more than 8: K and V come from memory or
+// L2 once for all of them.  Wide heads have no registers for that.
+int f32_rows(const ckks_draft_attention_args& a) {
+  return a.head_dim <= 128 && a.nodes * (a.q_heads / a.kv_heads) > 8 ? 16 : 8;
+}
+
+Division f32_division(const Context& c, const ckks_draft_attention_args& a) {
+  const int dc = (a.head_dim + 63) / 64;
+  return divide(c, a, Division{f32_rows(a), dc == 1 ? 64 : dc == 2 ? 32 : 16, 0, 1, 0, false}, dc == 1 ? 3 : 2);
+}
+
+size_t division_floats(const ckks_draft_attention_args& a, const Division& d) {
+  return d.alone ? 0 : (size_t)2 * d.ctas * d.tile_rows * ((a.head_dim + 63) / 64 * 64 + 4);
 }
 
 size_t workspace_of(const Context& c, const ckks_draft_attention_args& a) {
   if (a.batch == 0) return 0;
+  // the tensors' strides decide which kernel runs
   const int s = split_count(c, a);
   size_t n = s == 1 ? 0 : (size_t)a.batch * a.q_heads * a.nodes * s * (a.head_dim + 2);
-  if (tc_sizes(a)) {
-    // tensors whose rows are not aligned pieces take the other kernel
-    const int g = tc_ctas(c, a), rows = tile_nodes(a) * (a.q_heads / a.kv_heads);
-    if (!tc_alone(a, g)) n = std::max(n, (size_t)2 * g * rows * (a.head_dim <= 64 ? 64 + 4 : 128 + 4));
-  }
+  if (tc_sizes(a)) n = std::max(n, division_floats(a, tc_division(c, a)));
+  if (f32_sizes(a)) n = std::max(n, division_floats(a, f32_division(c, a)));
   return sizeof(float) * n;
+}
+
+AttnParams with(AttnParams p, const Division& d) {
+  p.tile_rows = d.tile_rows, p.tile_keys = d.tile_keys, p.new_apart = d.new_apart, p.unit_cost = d.unit_cost;
+  return p;
+}
+
+template <typename T, int PANELS>
+void join_division(const AttnParams& p, const Division& d, cudaStream_t st) {
+  if (d.alone) return;
+  const int rows = p.nodes * p.group;
+  launch_pdl(join_list_kernel<T, PANELS>, dim3((unsigned)(p.batch * p.kv_heads * ((rows + 7) / 8))), dim3(256), 0, st, p,
+             d.ctas);
+}
+
+template <int RT, int DC>
+void launch_f32(const AttnParams& p, const Division& d, cudaStream_t st) {
+  using S = F32Shape<RT, DC>;
+  auto* k = attend_f32_kernel<RT, DC>;
+  CKKS_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::kSmem));
+  k<<<d.ctas, kThreads, S::kSmem, st>>>(p);
+  CKKS_CUDA(cudaGetLastError());
+  join_division<float, DC>(p, d, st);
+}
+
+void run_f32(const Context& c, const ckks_draft_attention_args& a, const AttnParams& base, cudaStream_t st) {
+  const Division d = f32_division(c, a);
+  const AttnParams p = with(base, d);
+  const bool many = d.tile_rows == 16;
+  switch ((a.head_dim + 63) / 64) {
+    case 1: many ? launch_f32<16, 1>(p, d, st) : launch_f32<8, 1>(p, d, st); break;
+    case 2: many ? launch_f32<16, 2>(p, d, st) : launch_f32<8, 2>(p, d, st); break;
+    case 3: launch_f32<8, 3>(p, d, st); break;
+    default: launch_f32<8, 4>(p, d, st); break;
+  }
 }
 
 using EncodeTiled = decltype(&cuTensorMapEncodeTiled);
@@ -970,32 +1281,30 @@ bool tile_map(CUtensorMap* m, void* data, int dtype, int head_dim, int inner, in
 }
 
 template <typename T, int PANELS, int COPIES>
-void launch_tc(const Context& c, const ckks_draft_attention_args& a, const AttnParams& p, const TileMaps& maps,
-               cudaStream_t st) {
+void launch_tc(const Context& c, const AttnParams& p, const TileMaps& maps, const Division& d, cudaStream_t st) {
   using S = TcShape<PANELS>;
+  static_assert(S::kSmem <= 232448, "shared memory of one block");
   auto* k = attend_tc_kernel<T, PANELS, COPIES>;
   CKKS_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::kSmem));
-  const int ctas = tc_ctas(c, a), rows = p.nodes * p.group;
-  static_assert(S::kSmem <= 232448, "shared memory of one block");
   // a scale of 0 becomes one that changes no weight: a masked score times 0 would be no number
   const float factor = std::max(std::fabs(p.scale) * kLog2e, 1e-30f);
-  k<<<ctas, kTcThreads, S::kSmem, st>>>(p, maps, p.scale < 0.0f, factor, c.d_faults);
+  k<<<d.ctas, kTcThreads, S::kSmem, st>>>(p, maps, p.scale < 0.0f, factor, c.d_faults);
   CKKS_CUDA(cudaGetLastError());
-  if (!tc_alone(a, ctas))
-    launch_pdl(join_tc_kernel<T, PANELS>, dim3((unsigned)(p.batch * p.kv_heads * ((rows + 7) / 8))), dim3(256), 0, st, p,
-               ctas);
+  join_division<T, PANELS>(p, d, st);
 }
 
 template <typename T, int PANELS>
-void launch_tc(const Context& c, const ckks_draft_attention_args& a, const AttnParams& p, const TileMaps& maps,
+void launch_tc(const Context& c, const ckks_draft_attention_args& a, const AttnParams& base, const TileMaps& maps,
                cudaStream_t st) {
+  const Division d = tc_division(c, a);
+  const AttnParams p = with(base, d);
   const int rows = p.nodes * p.group;
   if (rows <= 32)
-    launch_tc<T, PANELS, 4>(c, a, p, maps, st);
+    launch_tc<T, PANELS, 4>(c, p, maps, d, st);
   else if (rows <= 64)
-    launch_tc<T, PANELS, 2>(c, a, p, maps, st);
+    launch_tc<T, PANELS, 2>(c, p, maps, d, st);
   else
-    launch_tc<T, PANELS, 1>(c, a, p, maps, st);
+    launch_tc<T, PANELS, 1>(c, p, maps, d, st);
 }
 
 template <typename T>
@@ -1081,6 +1390,10 @@ extern "C" int ckks_draft_attention(ckks_ctx* ctx, const ckks_draft_attention_ar
     ProfScope ps(c, "draft_attention", bytes, st);
     if (p.wide && tc_sizes(a) && (a.dtype == CKKS_BF16 ? run_tc<__nv_bfloat16>(c, a, p, st) : run_tc<__half>(c, a, p, st)))
       return;
+    if (p.wide && f32_sizes(a)) {
+      run_f32(c, a, p, st);
+      return;
+    }
     if (a.dtype == CKKS_BF16)
       run_attend<__nv_bfloat16>(p, st);
     else if (a.dtype == CKKS_FP16)
