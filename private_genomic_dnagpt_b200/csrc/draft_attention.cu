@@ -498,51 +498,50 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       for (int j = u > 2 ? u - 2 : 0; j < u; ++j) fine = mbar_wait_short(q_full(j & 1), j >> 1 & 1) && fine;
     }
   } else if (warp == 9) {
-    // ---- products
-    if (lane == 0) {
-      constexpr uint32_t word_s = mma_word(kBf, kM, kKeys, false), word_o = mma_word(kBf, kM, DP, true);
-      int k = 0, u = 0;
-      uint32_t phase = 0;  // bit g: parity of group g's next weights
-      for (int w = w0; w < w1 && fine;) {
-        const int n = tiles_here(w);
-        auto scores = [&](int g) {
-          const int s = k % NS;
-          if (!mbar_wait_short(full(s), (k / NS) & 1)) return fine = false;
-          tmem_fence_after();
-          const uint32_t kb = ring + s * S::kTileBytes;
+    // ---- products, by the whole warp in step
+    constexpr uint32_t word_s = mma_word(kBf, kM, kKeys, false), word_o = mma_word(kBf, kM, DP, true);
+    const uint32_t t_base = __shfl_sync(0xffffffffu, tmem, 0);
+    auto wait = [&](uint32_t bar, uint32_t parity) { return (bool)__all_sync(0xffffffffu, mbar_wait_short(bar, parity)); };
+    int k = 0, u = 0;
+    uint32_t phase = 0;  // bit g: parity of group g's next weights
+    for (int w = w0; w < w1 && fine;) {
+      const int n = __shfl_sync(0xffffffffu, tiles_here(w), 0);
+      auto scores = [&](int g) {
+        const int s = k % NS;
+        if (!wait(full(s), (k / NS) & 1)) return fine = false;
+        tmem_fence_after();
+        const uint32_t qb = sq + (u & 1) * S::kTileBytes, kb = ring + s * S::kTileBytes;
 #pragma unroll
-          for (int i = 0; i < DP / 16; ++i) {
-            const uint32_t off = (i / 4) * kPanel + (i % 4) * 32;
-            mma_smem(tmem + 128 * g, smem_operand(sq + (u & 1) * S::kTileBytes + off, 16), smem_operand(kb + off, 16),
-                     word_s, i > 0);
-          }
-          mma_commit(empty(s));
-          mma_commit(s_full(g));
-          ++k;
-          return true;
-        };
-        if (n) {
-          fine = mbar_wait_short(q_full(u & 1), u >> 1 & 1) && scores(0);
-          for (int t = 0; t < n && fine; ++t) {
-            if (t + 1 < n && !scores((t + 1) & 1)) break;
-            const int g = t & 1, s = k % NS;
-            if (!(fine = mbar_wait_short(full(s), (k / NS) & 1) && mbar_wait_short(p_ready(g), phase >> g & 1))) break;
-            phase ^= 1u << g;
-            tmem_fence_after();
-            const uint32_t vb = ring + s * S::kTileBytes;
-#pragma unroll
-            for (int i = 0; i < kKeys / 16; ++i)
-              mma_tmem(tmem + 256 + 128 * g, tmem + 128 * g + 8 * i, smem_operand(vb + 2048 * i, kPanel), word_o,
-                       i > 0 || t > 1);
-            mma_commit(empty(s));
-            ++k;
-          }
-          if (fine) mma_commit(o_full);
-          ++u;
+        for (int i = 0; i < DP / 16; ++i) {
+          const uint32_t off = (i / 4) * kPanel + (i % 4) * 32;
+          mma_smem(t_base + 128 * g, smem_operand(qb + off, 16), smem_operand(kb + off, 16), word_s, i > 0);
         }
-        w += n;
-        at.next_unit(p, units);
+        mma_commit(empty(s));
+        mma_commit(s_full(g));
+        ++k;
+        return true;
+      };
+      if (n) {
+        fine = wait(q_full(u & 1), u >> 1 & 1) && scores(0);
+        for (int t = 0; t < n && fine; ++t) {
+          if (t + 1 < n && !scores((t + 1) & 1)) break;
+          const int g = t & 1, s = k % NS;
+          if (!(fine = wait(full(s), (k / NS) & 1) && wait(p_ready(g), phase >> g & 1))) break;
+          phase ^= 1u << g;
+          tmem_fence_after();
+          const uint32_t vb = ring + s * S::kTileBytes;
+#pragma unroll
+          for (int i = 0; i < kKeys / 16; ++i)
+            mma_tmem(t_base + 256 + 128 * g, t_base + 128 * g + 8 * i, smem_operand(vb + 2048 * i, kPanel), word_o,
+                     i > 0 || t > 1);
+          mma_commit(empty(s));
+          ++k;
+        }
+        if (fine) mma_commit(o_full);
+        ++u;
       }
+      w += n;
+      at.next_unit(p, units);
     }
   } else {
     // ---- softmax: group g, tensor-memory lane L, that is row `row` of the

@@ -103,11 +103,15 @@ __host__ __device__ constexpr uint32_t mma_word(bool bf16, int m, int n, bool b_
          (uint32_t)(m >> 4) << 24;
 }
 
+// The following are called by a whole converged warp, one lane of which issues:
+// the operands are uniform registers, and in a branch that one lane takes
+// alone every product spends about 90 cycles on moving them there.
+
 // D (tensor memory) = A B (+ D), A and B in shared memory
 __device__ __forceinline__ void mma_smem(uint32_t d, uint64_t a, uint64_t b, uint32_t word, bool add) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+      "{\n .reg .pred p, one;\n setp.ne.u32 p, %4, 0;\n elect.sync _|one, 0xffffffff;\n"
+      " @one tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
       "l"(a), "l"(b), "r"(word), "r"((uint32_t)add)
       : "memory");
 }
@@ -115,15 +119,18 @@ __device__ __forceinline__ void mma_smem(uint32_t d, uint64_t a, uint64_t b, uin
 // the same with A in tensor memory
 __device__ __forceinline__ void mma_tmem(uint32_t d, uint32_t a, uint64_t b, uint32_t word, bool add) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
+      "{\n .reg .pred p, one;\n setp.ne.u32 p, %4, 0;\n elect.sync _|one, 0xffffffff;\n"
+      " @one tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
       "r"(a), "l"(b), "r"(word), "r"((uint32_t)add)
       : "memory");
 }
 
-// one arrival on `bar` once every product issued so far by this thread is done
+// one arrival on `bar` once every product that this warp issued so far is done
 __device__ __forceinline__ void mma_commit(uint32_t bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+  asm volatile(
+      "{\n .reg .pred one;\n elect.sync _|one, 0xffffffff;\n"
+      " @one tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(bar)
+      : "memory");
 }
 
 // ---- shared memory ------------------------------------------------------------
