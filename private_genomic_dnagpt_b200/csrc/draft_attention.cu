@@ -582,9 +582,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         const int tile = at.tile + t;
         const bool tree = tile == at.tiles - 1;
         const int nk = tree ? p.nodes : min(kKeys, len - tile * kKeys);
+        if (!(fine = mbar_wait_short(s_full(g), phase))) break;
+        phase ^= 1u;
         if (tree || nk < kKeys) {
           // the values of keys that no row sees are taken out of the product,
-          // and those of new keys that are not finite, which only some see
+          // and those of new keys that are not finite, which only some see.  (The
+          // copy that had the slot before was used ahead of this tile's scores,
+          // so the wait cannot take its arrival for this one's.)
           const int kv = k + (t + 1 < n ? 2 * t + 2 : 2 * t + 1);
           if (!(fine = mbar_wait_short(full(kv % NS), (kv / NS) & 1))) break;
           uint8_t* vs = smem + S::kRing + (kv % NS) * S::kTileBytes;
@@ -604,8 +608,6 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           }
           smem_fence_async();
         }
-        if (!(fine = mbar_wait_short(s_full(g), phase))) break;
-        phase ^= 1u;
         tmem_fence_after();
         uint32_t x[KQ];
         tmem_load<KQ>(t_s + part * KQ, x);
