@@ -17,7 +17,8 @@ namespace {
 __device__ __forceinline__ bool fits(const int32_t* path, int count, int len, int nodes, int capacity) {
   if (count < 0 || count > nodes || len < 0 || len > capacity || count > capacity - len) return false;
   bool ok = true;
-  for (int j = 0; j < count; ++j) ok = ok && path[j] >= 0 && path[j] < nodes;
+#pragma unroll 8
+  for (int j = 0; j < count; ++j) ok &= (unsigned)path[j] < (unsigned)nodes;  // no read waits for another
   return ok;
 }
 
@@ -124,13 +125,13 @@ __global__ void __launch_bounds__(kAccKeys) accumulate_kernel(AccParams p) {
 
 // Rows of whole, aligned 16-byte pieces.  The accepted rows (a few nodes times
 // the query heads on a key/value head) are few, so this streams K once: a warp
-// takes 16 keys at a time as the A operand of 16 x 8 matrix products straight
-// from global memory, with no shared memory between.  The order of the
-// products along head_dim is free as long as both operands have the same one:
+// takes 16 keys at a time as the A operand of 16 x 8 matrix products.  Each
+// lane copies the pieces that it will use itself into its own places of a ring
+// in shared memory, ahead by the ring's steps and without any barrier: a
+// larger register file for loads in flight.  The order of the products along head_dim is free as long as both operands have the same one:
 // lane t of a quad reads the 16-byte pieces t, t + 4, ... of its two keys and
 // uses each as two steps' elements, which the q rows in shared memory follow.
-// 16 pieces of a lane are in flight at once (8 KB a warp).  The exponentials
-// of a key lie in one quad, so its sum is two shuffles; a key's weights are
+// The exponentials of a key lie in one quad, so its sum is two shuffles; a key's weights are
 // added in a fixed order.
 // float32 rows are split in two tensor-float parts, x = hi + lo, and
 // multiplied as hi hi + hi lo + lo hi: products to 2^-21.
@@ -188,6 +189,18 @@ constexpr int kStreamWarps = 8, kStreamRows = 64;  // warps of a CTA; q rows in 
 
 // 16-byte pieces of a key's row for each lane of its quad -> tiles of 16 keys a warp reads at once
 constexpr int stream_tiles(int jc) { return jc <= 2 ? 2 : 1; }
+// CTAs on an SM, and steps of the ring: 64 to 96 KB in flight in each
+constexpr int stream_ctas(int jc) { return jc <= 4 ? 2 : 1; }
+constexpr int stream_ring(int jc) { return jc <= 8 ? 3 : 1; }
+constexpr size_t stream_ring_bytes(int jc) {
+  return (size_t)stream_ring(jc) * kStreamWarps * 32 * 2 * jc * stream_tiles(jc) * 16;
+}
+
+__device__ __forceinline__ void copy16(uint4* dst, const void* src, bool real) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src),
+               "r"(real ? 16 : 0)
+               : "memory");
+}
 
 // keys of sequence b that get weight: none where nothing is accepted
 __device__ __forceinline__ int weighed_keys(const AccParams& p, int b) {
@@ -198,12 +211,13 @@ __device__ __forceinline__ int weighed_keys(const AccParams& p, int b) {
 // The CTAs divide the list of all heads' keys evenly (their number is known
 // on the device only), in entries of one step of a CTA.
 template <typename T, int JC>
-__global__ void __launch_bounds__(32 * kStreamWarps, sizeof(T) == 4 || JC > 4 ? 1 : 2)
-    accumulate_stream_kernel(AccParams p) {
-  constexpr int W = 16 / sizeof(T), U = stream_tiles(JC);
+__global__ void __launch_bounds__(32 * kStreamWarps, stream_ctas(JC)) accumulate_stream_kernel(AccParams p) {
+  constexpr int W = 16 / sizeof(T), U = stream_tiles(JC), R = stream_ring(JC);
   constexpr int kWarpKeys = 16 * U, kStep = kStreamWarps * kWarpKeys;
-  // q in the order of the products: [8 rows][piece][lane]
-  extern __shared__ __align__(16) uint4 s_q[];
+  // the ring, [step][warp][piece of a key][lane], and q in the order of the
+  // products, [8 rows][piece][lane]
+  extern __shared__ __align__(16) uint4 s_ring[];
+  uint4* const s_q = s_ring + stream_ring_bytes(JC) / 16;
   __shared__ float s_lse[kStreamRows];
   const int D = p.head_dim, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const float c2 = p.scale * kLog2e;
@@ -221,9 +235,11 @@ __global__ void __launch_bounds__(32 * kStreamWarps, sizeof(T) == 4 || JC > 4 ? 
     float* acc = static_cast<float*>(p.acc.data) + b * p.acc.batch + h * p.acc.head;
     for (int r0 = 0; r0 < rows; r0 += kStreamRows) {
       const int groups = (min(kStreamRows, rows - r0) + 7) / 8;
-      uint4 next[U][2][JC];
-      // the lane's pieces of its keys in step i
-      auto read = [&](int i) {
+      // the lane's pieces of its keys in step i, into its places
+      auto place = [&](int i, int u, int half, int j) {
+        return s_ring + ((((i % R) * kStreamWarps + warp) * U + u) * 2 + half) * JC * 32 + j * 32 + lane;
+      };
+      auto fetch = [&](int i) {
         const int k0 = (at.entry + i) * kStep + warp * kWarpKeys;
 #pragma unroll
         for (int u = 0; u < U; ++u)
@@ -232,12 +248,13 @@ __global__ void __launch_bounds__(32 * kStreamWarps, sizeof(T) == 4 || JC > 4 ? 
 #pragma unroll
             for (int j = 0; j < JC; ++j) {
               const int s = k0 + 16 * u + g + 8 * half, d = (t + 4 * j) * W;
-              next[u][half][j] = i < steps && s < total && d < D
-                                     ? *reinterpret_cast<const uint4*>(kc + s * p.kc.row + d)
-                                     : make_uint4(0, 0, 0, 0);
+              const bool real = i < steps && s < total && d < D;
+              copy16(place(i, u, half, j), real ? kc + s * p.kc.row + d : kc, real);
             }
+        asm volatile("cp.async.commit_group;" ::: "memory");
       };
-      read(0);
+#pragma unroll
+      for (int i = 0; i < R; ++i) fetch(i);
       __syncthreads();
       for (int i = threadIdx.x; i < groups * JC * 32; i += 32 * kStreamWarps) {
         const int ln = i & 31, j = (i >> 5) % JC, row = r0 + (i >> 5) / JC * 8 + (ln >> 2), d = ((ln & 3) + 4 * j) * W;
@@ -261,14 +278,15 @@ __global__ void __launch_bounds__(32 * kStreamWarps, sizeof(T) == 4 || JC > 4 ? 
       for (int i = 0; i < steps; ++i) {
         const int k0 = (at.entry + i) * kStep + warp * kWarpKeys;
         if (k0 >= total) break;
+        asm volatile("cp.async.wait_group %0;" ::"n"(R - 1) : "memory");
         uint4 a[U][2][JC];
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
           for (int half = 0; half < 2; ++half)
 #pragma unroll
-            for (int j = 0; j < JC; ++j) a[u][half][j] = next[u][half][j];
-        read(i + 1);
+            for (int j = 0; j < JC; ++j) a[u][half][j] = *place(i, u, half, j);
+        fetch(i + R);
         // the weights so far of the keys whose sums this lane will write
         float old[U][2], sum[U][2];
 #pragma unroll
@@ -321,6 +339,7 @@ __global__ void __launch_bounds__(32 * kStreamWarps, sizeof(T) == 4 || JC > 4 ? 
             if (t == 0 && s < total) acc[s] = old[u][half] + x;
           }
       }
+      asm volatile("cp.async.wait_group 0;" ::: "memory");  // before the ring is filled anew
     }
     w += steps;
     at.entry = 0;
@@ -570,10 +589,11 @@ template <typename T, int JC>
 void launch_stream(const Context& c, const AccParams& p, cudaStream_t st) {
   constexpr int kKeys = kStreamWarps * 16 * stream_tiles(JC);  // of one entry
   const long long entries = (long long)p.batch * p.kv_heads * ((p.capacity + kKeys - 1) / kKeys);
-  const unsigned ctas = (unsigned)std::min(entries, (sizeof(T) == 4 || JC > 4 ? 1ll : 2ll) * c.sms);
-  const size_t smem = (size_t)(std::min(kStreamRows, p.nodes * p.group) + 7) / 8 * JC * 32 * sizeof(uint4);
+  const unsigned ctas = (unsigned)std::min(entries, (long long)stream_ctas(JC) * c.sms);
+  const size_t smem = stream_ring_bytes(JC) + (size_t)(std::min(kStreamRows, p.nodes * p.group) + 7) / 8 * JC * 512;
+  static_assert(stream_ctas(JC) * (stream_ring_bytes(JC) + kStreamRows / 8 * JC * 512 + 2048) <= 228 << 10, "fits an SM");
   auto* k = accumulate_stream_kernel<T, JC>;
-  if (smem > 48 << 10) CKKS_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  CKKS_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   k<<<ctas, 32 * kStreamWarps, smem, st>>>(p);
   CKKS_CUDA(cudaGetLastError());
 }
