@@ -919,21 +919,38 @@ __global__ void __launch_bounds__(kThreads, DC == 1 ? 3 : 2) attend_f32_kernel(c
     const float* vc = static_cast<const float*>(p.vc.data) + b * p.vc.batch + h * p.vc.head;
     const float* kn = static_cast<const float*>(p.kn.data) + b * p.kn.batch + h * p.kn.head;
     const float* vn = static_cast<const float*>(p.vn.data) + b * p.vn.batch + h * p.vn.head;
+    // a thread copies the same elements of every RS-th key
+    constexpr int kAcross = DC == 1 ? 16 : DC == 2 ? 32 : 64, RS = kThreads / kAcross;
+    static_assert(KT % RS == 0 && 4 * kAcross >= DP, "whole rounds of whole rows");
+    const int cr = tid / kAcross, cd = tid % kAcross * 4;
     auto load = [&](int t, int stage) {
-      const uint32_t k_at = smem_addr(sm + stage * S::kStage), v_at = k_at + 4 * KT * KS;
+      const int t0 = (at.tile + t) * KT;
+      uint32_t k_at = smem_addr(sm + stage * S::kStage) + 4 * (cr * KS + cd);
+      uint32_t v_at = smem_addr(sm + stage * S::kStage + KT * KS) + 4 * (cr * DP + cd);
+      if (cd >= DP) {
+        // 192 elements: a quarter of the threads has none
+      } else if (t0 + KT <= len) {
+        const float *k = kc + (t0 + cr) * p.kc.row + cd, *v = vc + (t0 + cr) * p.vc.row + cd;
+        const bool real = cd < D;
+        if (!real) k = kc, v = vc;
 #pragma unroll
-      for (int i = tid; i < KT * DP / 4; i += kThreads) {
-        const int r = i / (DP / 4), d = i % (DP / 4) * 4, s = (at.tile + t) * KT + r;
-        const bool cached = s < len, real = d < D && s < total && (cached || s_mask[s - len] != 0ull);
-        const float *k = kc, *v = vc;
-        if (real) {
-          k = (cached ? kc + s * p.kc.row : kn + (s - len) * p.kn.row) + d;
-          v = (cached ? vc + s * p.vc.row : vn + (s - len) * p.vn.row) + d;
-        } else {
-          k = v = static_cast<const float*>(p.q.data);  // not read
+        for (int r = 0; r < KT; r += RS, k_at += 4 * RS * KS, v_at += 4 * RS * DP) {
+          copy16(k_at, k, real);
+          copy16(v_at, v, real);
+          if (real) k += RS * p.kc.row, v += RS * p.vc.row;
         }
-        copy16(k_at + 4 * (r * KS + d), k, real);
-        copy16(v_at + 4 * (r * DP + d), v, real);
+      } else {
+        for (int r = 0; r < KT; r += RS, k_at += 4 * RS * KS, v_at += 4 * RS * DP) {
+          const int s = t0 + cr + r;
+          const bool cached = s < len, real = cd < D && s < total && (cached || s_mask[s - len] != 0ull);
+          const float *k = static_cast<const float*>(p.q.data), *v = k;  // not read where nothing is there
+          if (real) {
+            k = (cached ? kc + s * p.kc.row : kn + (s - len) * p.kn.row) + cd;
+            v = (cached ? vc + s * p.vc.row : vn + (s - len) * p.vn.row) + cd;
+          }
+          copy16(k_at, k, real);
+          copy16(v_at, v, real);
+        }
       }
       copies_close();
     };
