@@ -1057,27 +1057,32 @@ __global__ void __launch_bounds__(kThreads, DC == 1 ? 3 : 2) attend_f32_kernel(c
             for (int e = 0; e < 4; ++e) acc[c][r][e] *= f;
         }
       }
-      // among new keys a weight of 0 adds nothing, whatever a value that other rows see holds
-      const bool apart = t0 + KT > len;
+      auto values = [&](auto apart) {
 #pragma unroll
-      for (int i = 0; i < KT / 8; ++i) {
-        const int k = kg + 8 * i;
-        float x[RT];
+        for (int i = 0; i < KT / 8; ++i) {
+          const int k = kg + 8 * i;
+          float x[RT];
 #pragma unroll
-        for (int r = 0; r < RT; r += 4) *reinterpret_cast<float4*>(x + r) = *reinterpret_cast<const float4*>(sp + k * RT + r);
+          for (int r = 0; r < RT; r += 4) *reinterpret_cast<float4*>(x + r) = *reinterpret_cast<const float4*>(sp + k * RT + r);
 #pragma unroll
-        for (int c = 0; c < DC; ++c) {
-          const float4 v4 = *reinterpret_cast<const float4*>(sv + k * DP + c * 64 + dg * 4);
+          for (int c = 0; c < DC; ++c) {
+            const float4 v4 = *reinterpret_cast<const float4*>(sv + k * DP + c * 64 + dg * 4);
 #pragma unroll
-          for (int r = 0; r < RT; ++r)
-            if (!apart || x[r] != 0.0f) {
-              acc[c][r][0] = fmaf(x[r], v4.x, acc[c][r][0]);
-              acc[c][r][1] = fmaf(x[r], v4.y, acc[c][r][1]);
-              acc[c][r][2] = fmaf(x[r], v4.z, acc[c][r][2]);
-              acc[c][r][3] = fmaf(x[r], v4.w, acc[c][r][3]);
-            }
+            for (int r = 0; r < RT; ++r)
+              if (!decltype(apart)::value || x[r] != 0.0f) {
+                acc[c][r][0] = fmaf(x[r], v4.x, acc[c][r][0]);
+                acc[c][r][1] = fmaf(x[r], v4.y, acc[c][r][1]);
+                acc[c][r][2] = fmaf(x[r], v4.z, acc[c][r][2]);
+                acc[c][r][3] = fmaf(x[r], v4.w, acc[c][r][3]);
+              }
+          }
         }
-      }
+      };
+      // among new keys a weight of 0 adds nothing, whatever a value that other rows see holds
+      if (t0 + KT > len)
+        values(std::true_type{});
+      else
+        values(std::false_type{});
       __syncthreads();
     }
     // the eight key groups' sums meet in the stages, 64 elements at a time
