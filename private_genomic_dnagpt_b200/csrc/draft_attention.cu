@@ -819,26 +819,47 @@ __global__ void __launch_bounds__(256) join_list_kernel(const __grid_constant__ 
   auto part = [&](int i) { return p.part + ((size_t)(2 * i + (i == c0 ? 1 : 0)) * tile_rows + r) * (DP + 4); };
   // with fewer entries than CTAs some have none and wrote nothing
   auto idle = [&](int i) { return W < ctas && list_start((int)W, i, ctas) == list_start((int)W, i + 1, ctas); };
-  float m = -INFINITY;
-  for (int i = c0 + lane; i <= c1; i += 32)
-    if (!idle(i)) m = fmaxf(m, part(i)[DP]);
-#pragma unroll
-  for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  const float ref = m == -INFINITY ? 0.0f : m;
-  float l = 0.0f, x[2 * PANELS];
+  // A lane has the (m, l) of one part; more than 32 parts (one sequence over a
+  // whole wave) come in rounds on a growing reference point.  The parts'
+  // sums are read eight at a time, so that a row waits for memory twice.
+  float m = -INFINITY, l = 0.0f, x[2 * PANELS];
   unsigned long long spoiled = 0ull;
 #pragma unroll
   for (int j = 0; j < 2 * PANELS; ++j) x[j] = 0.0f;
-#pragma unroll 4
-  for (int i = c0; i <= c1; ++i) {
-    if (idle(i)) continue;
-    const float* o = part(i);
-    const float4 e = *reinterpret_cast<const float4*>(o + DP);
-    const float f = exp2f(e.x - ref);
-    l = fmaf(e.y, f, l);
-    spoiled |= (unsigned long long)__float_as_uint(e.z) | (unsigned long long)__float_as_uint(e.w) << 32;
+  for (int i0 = c0; i0 <= c1; i0 += 32) {
+    const int mine = i0 + lane, n = min(32, c1 - i0 + 1);
+    const bool real = mine <= c1 && !idle(mine);
+    const float4 e = real ? *reinterpret_cast<const float4*>(part(mine) + DP) : make_float4(-INFINITY, 0.f, 0.f, 0.f);
+    const uint32_t there = __ballot_sync(0xffffffffu, real);
+    float top = e.x;
 #pragma unroll
-    for (int j = 0; j < 2 * PANELS; ++j) x[j] = fmaf(o[lane + 32 * j], f, x[j]);
+    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    spoiled |= (unsigned long long)__reduce_or_sync(0xffffffffu, __float_as_uint(e.z)) |
+               (unsigned long long)__reduce_or_sync(0xffffffffu, __float_as_uint(e.w)) << 32;
+    const float up = fmaxf(m, top), ref = up == -INFINITY ? 0.0f : up, old = exp2f(m - ref), f = exp2f(e.x - ref);
+    float sum = e.y * f;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    l = fmaf(l, old, sum);
+    m = up;
+#pragma unroll
+    for (int j = 0; j < 2 * PANELS; ++j) x[j] *= old;
+    for (int i = 0; i < n; i += 8) {
+      float y[8][2 * PANELS];
+#pragma unroll
+      for (int q = 0; q < 8; ++q) {
+        const bool is = i + q < 32 && (there >> ((i + q) & 31) & 1);
+        const float* o = part(i0 + i + q);
+#pragma unroll
+        for (int j = 0; j < 2 * PANELS; ++j) y[q][j] = is ? o[lane + 32 * j] : 0.0f;
+      }
+#pragma unroll
+      for (int q = 0; q < 8; ++q) {
+        const float fq = __shfl_sync(0xffffffffu, f, (i + q) & 31);
+#pragma unroll
+        for (int j = 0; j < 2 * PANELS; ++j) x[j] = fmaf(y[q][j], fq, x[j]);
+      }
+    }
   }
   const bool seen = mask != 0ull;
   const float inv = l != 0.0f && seen ? 1.0f / l : 0.0f;
