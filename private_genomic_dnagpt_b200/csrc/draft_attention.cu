@@ -791,6 +791,9 @@ __global__ void __launch_bounds__(256) join_list_kernel(const __grid_constant__ 
     return;
   }
   const int unit = h * tiles_r + row / tile_rows, r = row % tile_rows;
+  // the reads that wait for nothing first: this kernel is a chain of them
+  TreeReader reader;
+  reader.read(p.parents + (size_t)b * p.nodes, p.nodes);
   // this unit's tiles [u0, u1) of the list, and the CTAs that have the first
   // and the last: CTA i begins at list_start(i), so w is CTA
   // floor((ctas (w + 1) - 1) / entries)'s
@@ -812,9 +815,7 @@ __global__ void __launch_bounds__(256) join_list_kernel(const __grid_constant__ 
     CKKS_PDL_ENTRY();
     return;
   }
-  tree_masks(p.parents + (size_t)b * p.nodes, p.nodes, s_mask[warp], s_jump[warp]);
   const int node = row / p.group, qh = h * p.group + row % p.group;
-  const uint64_t mask = s_mask[warp][node];
   CKKS_PDL_ENTRY();  // what is read above no kernel of this call writes
   auto part = [&](int i) { return p.part + ((size_t)(2 * i + (i == c0 ? 1 : 0)) * tile_rows + r) * (DP + 4); };
   // with fewer entries than CTAs some have none and wrote nothing
@@ -831,6 +832,7 @@ __global__ void __launch_bounds__(256) join_list_kernel(const __grid_constant__ 
     const bool real = mine <= c1 && !idle(mine);
     const float4 e = real ? *reinterpret_cast<const float4*>(part(mine) + DP) : make_float4(-INFINITY, 0.f, 0.f, 0.f);
     const uint32_t there = __ballot_sync(0xffffffffu, real);
+    if (i0 == c0) reader.masks(s_mask[warp], s_jump[warp]);  // while the read above is on its way
     float top = e.x;
 #pragma unroll
     for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
@@ -861,6 +863,7 @@ __global__ void __launch_bounds__(256) join_list_kernel(const __grid_constant__ 
       }
     }
   }
+  const uint64_t mask = s_mask[warp][node];
   const bool seen = mask != 0ull;
   const float inv = l != 0.0f && seen ? 1.0f / l : 0.0f;
   T* o = out_row<T>(p, b, node, qh);
