@@ -468,7 +468,9 @@ typedef struct {
  * of itself and its ancestors: out = sum_s softmax(scale q.k)_s v_s, and the
  * natural log of the softmax's sum in lse.  nodes = 1 is the single-token
  * decode step.  The row of a node that is padding is 0 and its lse -inf.
- * Rows of the cache behind lens[b] are not used, whatever they hold.
+ * Rows of the cache behind lens[b] are not used, whatever they hold; an
+ * infinite or NaN value that a row sees makes that element of the row
+ * infinite or NaN.  16-bit tensors round each softmax weight to their type.
  * q_heads / kv_heads query heads share each key/value head. */
 int ckks_draft_attention(ckks_ctx* ctx, const ckks_draft_attention_args* args, void* stream);
 /* workspace bytes for these sizes (the pointers are not looked at), or -1 */
@@ -511,7 +513,8 @@ typedef struct {
 } ckks_draft_commit_args;
 
 /* Appends the new keys and values of nodes path[b][0..count[b]) behind
- * lens[b] and writes the new lengths.  A sequence whose count, path or length
+ * lens[b] and writes the new lengths (the new rows do not overlap the
+ * caches).  A sequence whose count, path or length
  * does not fit (count outside 0..nodes, a node outside 0..nodes-1, more rows
  * than the capacity) is left as it is, with its length unchanged, and is
  * reported as CKKS_ECAPACITY by a ckks_sync that runs after the stream

@@ -1402,7 +1402,8 @@ extern "C" int ckks_draft_attention(ckks_ctx* ctx, const ckks_draft_attention_ar
     need(args != nullptr, "null argument");
     const ckks_draft_attention_args& a = *args;
     check_shape(a);
-    need(std::isfinite((float)a.scale), "scale is not finite");
+    need(a.reserved == 0, "reserved field is not 0");
+    need(std::isfinite((float)a.scale * kLog2e), "scale is not finite");
     if (a.batch == 0) return;
     const int e = element_bytes(a.dtype);
     check_rows(a.q, e, "q");

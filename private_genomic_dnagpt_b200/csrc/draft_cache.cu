@@ -658,6 +658,12 @@ extern "C" int ckks_draft_commit(ckks_ctx* ctx, const ckks_draft_commit_args* ar
     check_ptr(a.count, "count");
     check_ptr(a.lens_out, "lens_out");
     need(disjoint(a.lens, a.lens + a.batch, a.lens_out, a.lens_out + a.batch), "lens_out overlaps lens");
+    if (a.capacity)
+      for (const ckks_rows* cache : {&a.k_cache, &a.v_cache})
+        for (const ckks_rows* fresh : {&a.k_new, &a.v_new})
+          need(disjoint(cache->data, end_of(*cache, a.batch, a.kv_heads, a.capacity, a.head_dim, e), fresh->data,
+                        end_of(*fresh, a.batch, a.kv_heads, a.nodes, a.head_dim, e)),
+               "new rows overlap the cache");
     CommitParams p{a.k_cache, a.v_cache,  a.k_new,    a.v_new, a.lens,    a.path, a.count, a.lens_out,
                    c.d_faults + 1, a.batch, a.kv_heads, a.head_dim, a.nodes, a.capacity};
     const bool wide = a.capacity && wide_rows(a.k_cache, a.batch, a.kv_heads, a.capacity, a.head_dim, e) &&
@@ -682,7 +688,8 @@ extern "C" int ckks_draft_accumulate(ckks_ctx* ctx, const ckks_draft_accumulate_
     check_cache(a.dtype, a.batch, a.kv_heads, a.head_dim, a.capacity);
     need(a.nodes >= 1 && a.nodes <= kMaxNodes, "node count outside 1..64");
     need(a.q_heads >= 1 && a.q_heads % a.kv_heads == 0, "query heads are not a multiple of the key/value heads");
-    need(std::isfinite(a.scale), "scale is not finite");
+    need(a.reserved == 0, "reserved field is not 0");
+    need(std::isfinite((float)a.scale * kLog2e), "scale is not finite");
     if (a.batch == 0 || a.capacity == 0) return;
     const int e = element_bytes(a.dtype);
     check_rows(a.q, e, "q");

@@ -282,6 +282,7 @@ extern "C" int ckks_draft_verify(ckks_ctx* ctx, const ckks_draft_verify_args* ar
     Context& c = context_of(ctx);
     need(args != nullptr, "null argument");
     const ckks_draft_verify_args& a = *args;
+    need(a.reserved == 0, "reserved field is not 0");
     need(a.batch >= 0, "negative batch");
     need(a.nodes >= 1 && a.nodes <= kMaxNodes, "node count outside 1..64");
     need(a.vocab >= 1 && a.vocab < (1 << 30), "vocabulary size out of range");

@@ -562,4 +562,50 @@ def test_refusals(cc):
     with pytest.raises(eng.CKKSError) as e:  # in place
         cc.draft_evict(x["k_cache"], x["v_cache"], acc, x["lens"], 40, 5, out=(x["k_cache"], x["v_cache"], acc))
     assert "overlaps" in str(e.value)
+    path, count = i32([[0, 1, 2]] * 2), i32([1, 1])
+    with pytest.raises(eng.CKKSError, match="overlap the cache"):
+        new = x["k_cache"][:, :, 40:43].transpose(1, 2)
+        cc.draft_commit(x["k_cache"], x["v_cache"], x["lens"], new, x["v_new"], path, count)
+    with pytest.raises(eng.CKKSError):
+        cc.draft_accumulate(x["q"], torch.zeros(2, 3, 4, device="cuda"), x["k_cache"], x["lens"], path, count, acc, 1e39)
+    v = verify_inputs(2, 3, 10, 1, torch.float32, torch.float32, 1)
+    with pytest.raises(eng.CKKSError):  # a tree without nodes
+        cc.draft_verify(v["target"][:, :1], v["draft"][:, :1], v["tokens"][:, :0], v["parents"][:, :0],
+                        v["uniforms"][:, :1].contiguous())
+    cc.Synchronize()
+
+
+def test_refused_structs(cc):
+    """What the packed arguments of Python never hold, at the C entry points."""
+    import ctypes
+    from private_genomic_dnagpt_b200 import drafting as d
+    lib, buf = eng.lib(), torch.zeros(4096, device="cuda")
+    at = buf.data_ptr()
+
+    def attention(**change):
+        f = dict(dtype=0, batch=1, q_heads=2, kv_heads=1, head_dim=16, nodes=2, capacity=4, reserved=0, scale=1.0)
+        rows = {n: [at, 64, 16, 16] for n in ("q", "k_cache", "v_cache", "k_new", "v_new", "out")}
+        last = dict(lens=at, parents=at, lse=at, workspace=at, workspace_bytes=1 << 14)
+        for k, v in change.items():
+            if k in f:
+                f[k] = v
+            elif k in rows:
+                rows[k] = v
+            else:
+                last[k] = v
+        args = d._ATTENTION.pack(*f.values(), *[x for r in rows.values() for x in r], *last.values())
+        return lib.ckks_draft_attention(cc.h, args, None)
+
+    assert attention(batch=0) == 0
+    for change in (dict(dtype=3), dict(dtype=9), dict(dtype=-1), dict(batch=-1), dict(q_heads=3, kv_heads=2),
+                   dict(q_heads=0), dict(kv_heads=0), dict(head_dim=0), dict(head_dim=257), dict(nodes=0),
+                   dict(nodes=65), dict(capacity=-1), dict(capacity=1 << 30), dict(reserved=1),
+                   dict(scale=float("inf")), dict(q=[0, 64, 16, 16]), dict(q=[at + 1, 64, 16, 16]),
+                   dict(k_cache=[at, -64, 16, 16]), dict(out=[0, 64, 16, 16]), dict(lens=0), dict(lens=at + 2),
+                   dict(parents=0), dict(lse=0), dict(workspace=at + 4), dict(batch=1 << 30, q_heads=64, kv_heads=1)):
+        assert attention(**change) == 1, change
+        assert lib.ckks_last_error()
+    assert attention(nodes=64, q_heads=8, capacity=4000, workspace_bytes=16) == 1  # too small
+    assert lib.ckks_draft_attention(cc.h, None, None) == 1
+    assert ctypes.sizeof(ctypes.c_void_p) == 8
     cc.Synchronize()
