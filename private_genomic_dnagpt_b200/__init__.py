@@ -183,14 +183,14 @@ _SIGS = [
                                         ctypes.POINTER(_vp)]),
     ("ckks_lane_shift", ctypes.c_int, [_vp, ctypes.POINTER(_vp), ctypes.c_int, ctypes.POINTER(ctypes.c_int),
                                        ctypes.c_int, ctypes.c_int, ctypes.POINTER(_vp)]),
-    # the argument structs of the drafted-decoding operators are packed by drafting.py
-    ("ckks_draft_attention", ctypes.c_int, [_vp, ctypes.c_char_p, _vp]),
-    ("ckks_draft_attention_workspace", ctypes.c_longlong, [_vp, ctypes.c_char_p]),
-    ("ckks_draft_verify", ctypes.c_int, [_vp, ctypes.c_char_p, _vp]),
-    ("ckks_draft_commit", ctypes.c_int, [_vp, ctypes.c_char_p, _vp]),
-    ("ckks_draft_accumulate", ctypes.c_int, [_vp, ctypes.c_char_p, _vp]),
-    ("ckks_draft_evict", ctypes.c_int, [_vp, ctypes.c_char_p, _vp]),
-    ("ckks_draft_evict_workspace", ctypes.c_longlong, [_vp, ctypes.c_char_p]),
+    # the drafted-decoding operators on torch tensors go through csrc/torch_draft.cpp
+    ("ckks_draft_attention", ctypes.c_int, [_vp, _vp, _vp]),
+    ("ckks_draft_attention_workspace", ctypes.c_longlong, [_vp, _vp]),
+    ("ckks_draft_verify", ctypes.c_int, [_vp, _vp, _vp]),
+    ("ckks_draft_commit", ctypes.c_int, [_vp, _vp, _vp]),
+    ("ckks_draft_accumulate", ctypes.c_int, [_vp, _vp, _vp]),
+    ("ckks_draft_evict", ctypes.c_int, [_vp, _vp, _vp]),
+    ("ckks_draft_evict_workspace", ctypes.c_longlong, [_vp, _vp]),
     ("ckks_block_set_drafts", ctypes.c_int, [_vp, ctypes.POINTER(ctypes.c_int), ctypes.c_int, ctypes.c_int]),
 ]
 
@@ -338,8 +338,6 @@ class Diagonals:
 class CryptoContext:
     """GenCryptoContext result: parameters, device tables and keys."""
 
-    _draft_device = None  # torch device of the drafted-decoding operators, made on their first use
-
     def __init__(self, params: CCParams):
         p = ckks_params(params.ring_dim_log, params.limbs, params.dnum, params.first_mod_bits,
                         params.scale_mod_bits, params.special_mod_bits, params.seed, params.device)
@@ -357,7 +355,6 @@ class CryptoContext:
         m = np.zeros(self.L + self.K, np.uint64)
         _check(lib().ckks_ctx_moduli(h, _u64(m), m.size))
         self.moduli = m
-        self._draft_sizes = {}
 
     def __del__(self):
         try:

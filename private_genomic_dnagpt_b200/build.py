@@ -2,8 +2,10 @@
 
 ``python -m private_genomic_dnagpt_b200.build`` (or ``build()``) compiles every
 ``csrc/*.cu`` translation unit in parallel and links
-``private_genomic_dnagpt_b200/libckks_b200.so``.  Only stale objects are
-rebuilt.
+``private_genomic_dnagpt_b200/libckks_b200.so``, and compiles
+``csrc/torch_draft.cpp`` against the installed torch into
+``private_genomic_dnagpt_b200/_draft.so`` (the drafted-decoding operators on
+torch tensors).  Only stale objects are rebuilt.
 """
 
 from __future__ import annotations
@@ -19,6 +21,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OBJ = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "libckks_b200.so")
+BINDING = os.path.join(HERE, "_draft.so")
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-lineinfo", "-std=c++17", "--expt-relaxed-constexpr",
@@ -62,6 +65,32 @@ def _compile(src: str, verbose: bool) -> str:
     return obj
 
 
+def build_binding() -> str:
+    """The torch binding; needs the engine's library and torch."""
+    src = os.path.join(CSRC, "torch_draft.cpp")
+    deps = [src, os.path.join(HERE, "..", "include", "ckks_b200.h")]
+    if os.path.exists(BINDING) and all(os.path.getmtime(d) <= os.path.getmtime(BINDING) for d in deps):
+        return BINDING
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension
+    libs = os.path.join(os.path.dirname(torch.__file__), "lib")
+    cuda = os.environ.get("CUDA_HOME", "/usr/local/cuda")
+    gxx = "/usr/bin/g++" if os.path.exists("/usr/bin/g++") else (shutil.which("g++") or "g++")
+    include = [f"-I{p}" for p in (*cpp_extension.include_paths(), sysconfig.get_path("include"),
+                                  os.path.join(cuda, "include"))]
+    cmd = [gxx, "-O2", "-std=c++17", "-fPIC", "-shared", *include, "-DTORCH_EXTENSION_NAME=_draft",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", src, "-o", BINDING, f"-L{libs}",
+           "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda", f"-L{HERE}",
+           "-l:libckks_b200.so", f"-Wl,-rpath,{libs}",
+           "-Wl,-rpath,$ORIGIN"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"g++ failed for {src}:\n{r.stdout}\n{r.stderr}")
+    return BINDING
+
+
 def build(verbose: bool = False) -> str:
     os.makedirs(OBJ, exist_ok=True)
     srcs = sorted(glob.glob(os.path.join(CSRC, "*.cu")))
@@ -72,6 +101,11 @@ def build(verbose: bool = False) -> str:
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
             raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
+    try:
+        import torch  # noqa: F401
+    except ImportError:
+        return LIB  # the engine itself needs no torch
+    build_binding()
     return LIB
 
 

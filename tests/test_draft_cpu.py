@@ -16,19 +16,22 @@ from private_genomic_dnagpt_b200 import drafting  # noqa: E402
 import draft_reference as ref  # noqa: E402
 
 
-class Reached(Exception):
-    pass
-
-
 @pytest.fixture
-def cc(monkeypatch):
-    """A context whose device is the CPU and whose library calls are caught."""
-    def call(cc, name, args, where):
-        raise Reached(name)
+def cc():
+    """A context that is not there, on the CPU: good arguments pass the checks
+    and are refused by the C entry point."""
+    return SimpleNamespace(h=SimpleNamespace(value=0), params=SimpleNamespace(device=-1))
 
-    monkeypatch.setattr(drafting, "_call", call)
-    monkeypatch.setattr(drafting, "_workspace", lambda *a: None)
-    return SimpleNamespace(h=None, params=SimpleNamespace(device=0), _draft_device=torch.device("cpu"), _draft_sizes={})
+
+class Reached:
+    """A call that passes the checks ends at the null context."""
+
+    def __enter__(self):
+        self.inner = pytest.raises(eng.CKKSError, match="null context")
+        return self.inner.__enter__()
+
+    def __exit__(self, *e):
+        return self.inner.__exit__(*e)
 
 
 def args(op, t=torch.float32):
@@ -54,7 +57,7 @@ OPS = ["attention", "verify", "commit", "accumulate", "evict"]
 @pytest.mark.parametrize("op", OPS)
 @pytest.mark.parametrize("t", [torch.bfloat16, torch.float16, torch.float32])
 def test_good_arguments_reach_the_library(cc, op, t):
-    with pytest.raises(Reached):
+    with Reached():
         getattr(drafting, op)(cc, **args(op, t))
 
 
@@ -78,7 +81,7 @@ def test_every_tensor_is_checked(cc, op):
 
 @pytest.mark.parametrize("op", OPS)
 def test_tensors_of_another_device_are_refused(cc, op):
-    cc._draft_device = torch.device("cuda", 0)
+    cc.params.device = 0
     with pytest.raises(ValueError, match="the context's device"):
         getattr(drafting, op)(cc, **args(op))
 
@@ -99,31 +102,18 @@ def test_written_tensors_have_their_own_memory(cc):
 def test_evict_outputs(cc):
     for rows, ok in ((5, True), (9, True), (4, False)):
         out = (torch.zeros(2, 2, rows, 8), torch.zeros(2, 2, rows, 8), torch.zeros(2, 2, rows))
-        with pytest.raises(Reached if ok else ValueError):
+        with Reached() if ok else pytest.raises(ValueError):
             drafting.evict(cc, **args("evict"), out=out)
 
 
 def test_c_entry_points_refuse_null():
     lib = eng.lib()
     for name in ("attention", "verify", "commit", "accumulate", "evict"):
-        assert getattr(lib, "ckks_draft_" + name)(None, b"\0" * 512, None) == 1
+        assert getattr(lib, "ckks_draft_" + name)(None, ctypes.create_string_buffer(512), None) == 1
         assert b"null context" in lib.ckks_last_error()
     for name in ("attention", "evict"):
-        assert getattr(lib, f"ckks_draft_{name}_workspace")(None, b"\0" * 512) == -1
+        assert getattr(lib, f"ckks_draft_{name}_workspace")(None, ctypes.create_string_buffer(512)) == -1
     assert lib.ckks_block_set_drafts(None, None, 0, 0) == 1
-
-
-def test_layouts_match_the_header(tmp_path):
-    """The sizes of the packed structs are those of the header's."""
-    import subprocess
-    src = tmp_path / "sizes.c"
-    names = ["attention", "verify", "commit", "accumulate", "evict"]
-    src.write_text('#include <stdio.h>\n#include "%s"\nint main(void) {\n%s return 0; }\n' % (
-        eng.HEADER, "".join(f'printf("%zu\\n", sizeof(ckks_draft_{n}_args));\n' for n in names)))
-    exe = tmp_path / "sizes"
-    subprocess.run(["gcc", str(src), "-o", str(exe)], check=True)
-    got = [int(x) for x in subprocess.run([str(exe)], capture_output=True, text=True, check=True).stdout.split()]
-    assert got == [getattr(drafting, "_" + n.upper()).size for n in names]
 
 
 def test_reference_is_self_consistent():

@@ -10,6 +10,8 @@ doubled by the division through a sum with the same error.  So
 S = sum |q k| scale, and lse is off by half of the second part plus 2^-22 of
 itself."""
 
+import ctypes
+
 import numpy as np
 import pytest
 
@@ -575,37 +577,40 @@ def test_refusals(cc):
     cc.Synchronize()
 
 
+class Rows(ctypes.Structure):
+    _fields_ = [("data", ctypes.c_void_p)] + [(n, ctypes.c_int64) for n in ("batch", "head", "row")]
+
+
+class AttentionArgs(ctypes.Structure):
+    """ckks_draft_attention_args of include/ckks_b200.h."""
+    _fields_ = ([(n, ctypes.c_int32) for n in ("dtype", "batch", "q_heads", "kv_heads", "head_dim", "nodes", "capacity",
+                                               "reserved")] + [("scale", ctypes.c_double)]
+                + [(n, Rows) for n in ("q", "k_cache", "v_cache", "k_new", "v_new", "out")]
+                + [(n, ctypes.c_void_p) for n in ("lens", "parents", "lse", "workspace")]
+                + [("workspace_bytes", ctypes.c_size_t)])
+
+
 def test_refused_structs(cc):
-    """What the packed arguments of Python never hold, at the C entry points."""
-    import ctypes
-    from private_genomic_dnagpt_b200 import drafting as d
+    """What torch tensors never hold, at the C entry points."""
     lib, buf = eng.lib(), torch.zeros(4096, device="cuda")
     at = buf.data_ptr()
 
     def attention(**change):
-        f = dict(dtype=0, batch=1, q_heads=2, kv_heads=1, head_dim=16, nodes=2, capacity=4, reserved=0, scale=1.0)
-        rows = {n: [at, 64, 16, 16] for n in ("q", "k_cache", "v_cache", "k_new", "v_new", "out")}
-        last = dict(lens=at, parents=at, lse=at, workspace=at, workspace_bytes=1 << 14)
-        for k, v in change.items():
-            if k in f:
-                f[k] = v
-            elif k in rows:
-                rows[k] = v
-            else:
-                last[k] = v
-        args = d._ATTENTION.pack(*f.values(), *[x for r in rows.values() for x in r], *last.values())
-        return lib.ckks_draft_attention(cc.h, args, None)
+        f = dict(dtype=0, batch=1, q_heads=2, kv_heads=1, head_dim=16, nodes=2, capacity=4, reserved=0, scale=1.0,
+                 lens=at, parents=at, lse=at, workspace=at, workspace_bytes=1 << 14)
+        f |= {n: Rows(at, 64, 16, 16) for n in ("q", "k_cache", "v_cache", "k_new", "v_new", "out")}
+        a = AttentionArgs(**(f | change))
+        return lib.ckks_draft_attention(cc.h, ctypes.byref(a), None)
 
     assert attention(batch=0) == 0
     for change in (dict(dtype=3), dict(dtype=9), dict(dtype=-1), dict(batch=-1), dict(q_heads=3, kv_heads=2),
                    dict(q_heads=0), dict(kv_heads=0), dict(head_dim=0), dict(head_dim=257), dict(nodes=0),
                    dict(nodes=65), dict(capacity=-1), dict(capacity=1 << 30), dict(reserved=1),
-                   dict(scale=float("inf")), dict(q=[0, 64, 16, 16]), dict(q=[at + 1, 64, 16, 16]),
-                   dict(k_cache=[at, -64, 16, 16]), dict(out=[0, 64, 16, 16]), dict(lens=0), dict(lens=at + 2),
+                   dict(scale=float("inf")), dict(q=Rows(0, 64, 16, 16)), dict(q=Rows(at + 1, 64, 16, 16)),
+                   dict(k_cache=Rows(at, -64, 16, 16)), dict(out=Rows(0, 64, 16, 16)), dict(lens=0), dict(lens=at + 2),
                    dict(parents=0), dict(lse=0), dict(workspace=at + 4), dict(batch=1 << 30, q_heads=64, kv_heads=1)):
         assert attention(**change) == 1, change
         assert lib.ckks_last_error()
     assert attention(nodes=64, q_heads=8, capacity=4000, workspace_bytes=16) == 1  # too small
     assert lib.ckks_draft_attention(cc.h, None, None) == 1
-    assert ctypes.sizeof(ctypes.c_void_p) == 8
     cc.Synchronize()
