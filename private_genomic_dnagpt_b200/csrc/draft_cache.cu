@@ -208,10 +208,14 @@ __device__ __forceinline__ int weighed_keys(const AccParams& p, int b) {
   return count > 0 && fits(p.path + (size_t)b * p.nodes, count, len, p.nodes, p.capacity) ? len + count : 0;
 }
 
-// The CTAs divide the list of all heads' keys evenly (their number is known
-// on the device only), in entries of one step of a CTA.
+// each > 0: CTA (x, y) takes `each` steps of head x from step y each on, if the
+// head has that many.  Otherwise the CTAs divide the list of all heads' keys
+// evenly (their number is known on the device only), in entries of one step:
+// long caches of unequal lengths then end together, but a CTA reads the whole
+// batch's lengths first and may begin a second head, which short ones feel
+// (4001 keys: 13.9 us divided by heads, 16.6 us as a list; 65536 keys: 58 and 50).
 template <typename T, int JC>
-__global__ void __launch_bounds__(32 * kStreamWarps, stream_ctas(JC)) accumulate_stream_kernel(AccParams p) {
+__global__ void __launch_bounds__(32 * kStreamWarps, stream_ctas(JC)) accumulate_stream_kernel(AccParams p, int each) {
   constexpr int W = 16 / sizeof(T), U = stream_tiles(JC), R = stream_ring(JC);
   constexpr int kWarpKeys = 16 * U, kStep = kStreamWarps * kWarpKeys;
   // the ring, [step][warp][piece of a key][lane], and q in the order of the
@@ -222,11 +226,19 @@ __global__ void __launch_bounds__(32 * kStreamWarps, stream_ctas(JC)) accumulate
   const int D = p.head_dim, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const float c2 = p.scale * kLog2e;
   auto entries_of = [&](int b) { return (weighed_keys(p, b) + kStep - 1) / kStep; };
-  int first;
-  const int entries = list_sum(p.batch, entries_of, first) * p.kv_heads;
-  const int w0 = list_start(entries, blockIdx.x, gridDim.x), w1 = list_start(entries, blockIdx.x + 1, gridDim.x);
+  int w0 = 0, w1;
+  ListPlace at;
+  if (each > 0) {
+    at.b = blockIdx.x / p.kv_heads, at.unit = blockIdx.x % p.kv_heads, at.entry = blockIdx.y * each;
+    at.entries = entries_of(at.b);
+    w1 = min(each, at.entries - at.entry);
+  } else {
+    int first;
+    const int entries = list_sum(p.batch, entries_of, first) * p.kv_heads;
+    w0 = list_start(entries, blockIdx.x, gridDim.x), w1 = list_start(entries, blockIdx.x + 1, gridDim.x);
+    if (w0 < w1) at = list_find(p.batch, p.kv_heads, w0, first, entries_of);
+  }
   if (w0 >= w1) return;
-  ListPlace at = list_find(p.batch, p.kv_heads, w0, first, entries_of);
   for (int w = w0; w < w1;) {
     const int steps = min(at.entries - at.entry, w1 - w);
     const int b = at.b, h = at.unit, len = p.lens[b], count = p.count[b], total = len + count, rows = count * p.group;
@@ -342,6 +354,7 @@ __global__ void __launch_bounds__(32 * kStreamWarps, stream_ctas(JC)) accumulate
       asm volatile("cp.async.wait_group 0;" ::: "memory");  // before the ring is filled anew
     }
     w += steps;
+    if (w >= w1) break;
     at.entry = 0;
     if (++at.unit == p.kv_heads) {
       at.unit = 0;
@@ -588,13 +601,20 @@ __global__ void __launch_bounds__(256) gather_kernel(EvictParams p) {
 template <typename T, int JC>
 void launch_stream(const Context& c, const AccParams& p, cudaStream_t st) {
   constexpr int kKeys = kStreamWarps * 16 * stream_tiles(JC);  // of one entry
-  const long long entries = (long long)p.batch * p.kv_heads * ((p.capacity + kKeys - 1) / kKeys);
-  const unsigned ctas = (unsigned)std::min(entries, (long long)stream_ctas(JC) * c.sms);
+  const long long heads = (long long)p.batch * p.kv_heads, steps = (p.capacity + kKeys - 1) / kKeys;
+  const long long entries = heads * steps, ctas = (long long)stream_ctas(JC) * c.sms;
+  // one wave when the caches are three quarters full: 12 heads of 8 sequences
+  // over 4001 keys take 18.9 / 13.9 / 17.5 us with 3 / 4 / 6 steps each, one
+  // sequence over 2000 keys 7.2 / 10.8 with 2 / 4
+  const int each = (int)((3 * entries + 4 * ctas - 1) / (4 * ctas));
+  const bool by_head = each <= 8;
+  const dim3 grid = by_head ? dim3((unsigned)heads, (unsigned)((steps + each - 1) / each))
+                            : dim3((unsigned)std::min(entries, ctas));
   const size_t smem = stream_ring_bytes(JC) + (size_t)(std::min(kStreamRows, p.nodes * p.group) + 7) / 8 * JC * 512;
   static_assert(stream_ctas(JC) * (stream_ring_bytes(JC) + kStreamRows / 8 * JC * 512 + 2048) <= 228 << 10, "fits an SM");
   auto* k = accumulate_stream_kernel<T, JC>;
   CKKS_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-  k<<<ctas, 32 * kStreamWarps, smem, st>>>(p);
+  k<<<grid, 32 * kStreamWarps, smem, st>>>(p, by_head ? each : 0);
   CKKS_CUDA(cudaGetLastError());
 }
 
