@@ -223,6 +223,7 @@ __global__ void __launch_bounds__(32 * kStreamWarps, stream_ctas(JC)) accumulate
   extern __shared__ __align__(16) uint4 s_ring[];
   uint4* const s_q = s_ring + stream_ring_bytes(JC) / 16;
   __shared__ float s_lse[kStreamRows];
+  __shared__ int s_last[kStreamRows];  // the last key that a row sees; -1 for a row that is not there
   const int D = p.head_dim, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const float c2 = p.scale * kLog2e;
   auto entries_of = [&](int b) { return (weighed_keys(p, b) + kStep - 1) / kStep; };
@@ -252,17 +253,18 @@ __global__ void __launch_bounds__(32 * kStreamWarps, stream_ctas(JC)) accumulate
         return s_ring + ((((i % R) * kStreamWarps + warp) * U + u) * 2 + half) * JC * 32 + j * 32 + lane;
       };
       auto fetch = [&](int i) {
-        const int k0 = (at.entry + i) * kStep + warp * kWarpKeys;
+        const int k0 = (at.entry + i) * kStep + warp * kWarpKeys + g;
+        const T* key = kc + k0 * p.kc.row + t * W;
+        const bool whole = i < steps && k0 + kWarpKeys - 8 < total;  // all of this lane's keys are there
 #pragma unroll
-        for (int u = 0; u < U; ++u)
+        for (int u = 0; u < 2 * U; ++u, key += 8 * p.kc.row) {
+          const bool there = whole || (i < steps && k0 + 8 * u < total);
 #pragma unroll
-          for (int half = 0; half < 2; ++half)
-#pragma unroll
-            for (int j = 0; j < JC; ++j) {
-              const int s = k0 + 16 * u + g + 8 * half, d = (t + 4 * j) * W;
-              const bool real = i < steps && s < total && d < D;
-              copy16(place(i, u, half, j), real ? kc + s * p.kc.row + d : kc, real);
-            }
+          for (int j = 0; j < JC; ++j) {
+            const bool real = there && (t + 4 * j) * W < D;
+            copy16(place(i, u >> 1, u & 1, j), real ? key + 4 * j * W : kc, real);
+          }
+        }
         asm volatile("cp.async.commit_group;" ::: "memory");
       };
 #pragma unroll
@@ -282,6 +284,7 @@ __global__ void __launch_bounds__(32 * kStreamWarps, stream_ctas(JC)) accumulate
         const int row = r0 + threadIdx.x;
         // a row that is not there weighs nothing
         s_lse[threadIdx.x] = INFINITY;
+        s_last[threadIdx.x] = row < rows ? len + row / p.group : -1;
         if (row < rows)
           s_lse[threadIdx.x] = kLog2e * p.lse[((size_t)b * p.nodes + path[row / p.group]) * p.kv_heads * p.group +
                                               h * p.group + row % p.group];
@@ -323,19 +326,16 @@ __global__ void __launch_bounds__(32 * kStreamWarps, stream_ctas(JC)) accumulate
           }
           const int row = gr * 8 + 2 * t;  // the lane's two rows
           const float2 l = *reinterpret_cast<const float2*>(s_lse + row);
+          const int2 last = *reinterpret_cast<const int2*>(s_last + row);
 #pragma unroll
           for (int u = 0; u < U; ++u) {
             float e[4] = {ex2(fmaf(c[u][0], c2, -l.x)), ex2(fmaf(c[u][1], c2, -l.y)), ex2(fmaf(c[u][2], c2, -l.x)),
                           ex2(fmaf(c[u][3], c2, -l.y))};
             const int s = k0 + 16 * u + g;
-            if (k0 + kWarpKeys > len || r0 + gr * 8 + 8 > rows) {
-              // among the appended keys a row sees those up to its own
-#pragma unroll
-              for (int x = 0; x < 4; ++x) {
-                const int rr = r0 + row + (x & 1);
-                if (rr >= rows || s + 8 * (x >> 1) > len + rr / p.group) e[x] = 0.0f;
-              }
-            }
+            e[0] = s <= last.x ? e[0] : 0.0f;
+            e[1] = s <= last.y ? e[1] : 0.0f;
+            e[2] = s + 8 <= last.x ? e[2] : 0.0f;
+            e[3] = s + 8 <= last.y ? e[3] : 0.0f;
             sum[u][0] += e[0] + e[1];
             sum[u][1] += e[2] + e[3];
           }
