@@ -289,6 +289,17 @@ __global__ void __launch_bounds__(32 * kStreamWarps, stream_ctas(JC)) accumulate
           s_lse[threadIdx.x] = kLog2e * p.lse[((size_t)b * p.nodes + path[row / p.group]) * p.kv_heads * p.group +
                                               h * p.group + row % p.group];
       }
+      // the weights so far of the keys of step i whose sums this lane will write
+      float soon[U][2];
+      auto weights = [&](int i) {
+        const int s0 = (at.entry + i) * kStep + warp * kWarpKeys + g, end = i < steps && t == 0 ? r0 > 0 ? total : len : 0;
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int half = 0; half < 2; ++half)
+            soon[u][half] = s0 + 16 * u + 8 * half < end ? acc[s0 + 16 * u + 8 * half] : 0.0f;
+      };
+      weights(0);
       __syncthreads();
       for (int i = 0; i < steps; ++i) {
         const int k0 = (at.entry + i) * kStep + warp * kWarpKeys;
@@ -302,16 +313,12 @@ __global__ void __launch_bounds__(32 * kStreamWarps, stream_ctas(JC)) accumulate
 #pragma unroll
             for (int j = 0; j < JC; ++j) a[u][half][j] = *place(i, u, half, j);
         fetch(i + R);
-        // the weights so far of the keys whose sums this lane will write
         float old[U][2], sum[U][2];
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            const int s = k0 + 16 * u + g + 8 * half;
-            old[u][half] = t == 0 && s < (r0 > 0 ? total : len) ? acc[s] : 0.0f;
-            sum[u][half] = 0.0f;
-          }
+          for (int half = 0; half < 2; ++half) old[u][half] = soon[u][half], sum[u][half] = 0.0f;
+        weights(i + 1);
         for (int gr = 0; gr < groups; ++gr) {
           float c[U][4];
 #pragma unroll
