@@ -211,9 +211,8 @@ __device__ __forceinline__ int weighed_keys(const AccParams& p, int b) {
 // each > 0: CTA (x, y) takes `each` steps of head x from step y each on, if the
 // head has that many.  Otherwise the CTAs divide the list of all heads' keys
 // evenly (their number is known on the device only), in entries of one step:
-// long caches of unequal lengths then end together, but a CTA reads the whole
-// batch's lengths first and may begin a second head, which short ones feel
-// (4001 keys: 13.9 us divided by heads, 16.6 us as a list; 65536 keys: 58 and 50).
+// caches of unequal lengths then end together, but a CTA reads the whole
+// batch's lengths first and may begin a second head.
 template <typename T, int JC>
 __global__ void __launch_bounds__(32 * kStreamWarps, stream_ctas(JC)) accumulate_stream_kernel(AccParams p, int each) {
   constexpr int W = 16 / sizeof(T), U = stream_tiles(JC), R = stream_ring(JC);
@@ -610,11 +609,14 @@ void launch_stream(const Context& c, const AccParams& p, cudaStream_t st) {
   constexpr int kKeys = kStreamWarps * 16 * stream_tiles(JC);  // of one entry
   const long long heads = (long long)p.batch * p.kv_heads, steps = (p.capacity + kKeys - 1) / kKeys;
   const long long entries = heads * steps, ctas = (long long)stream_ctas(JC) * c.sms;
-  // one wave when the caches are three quarters full: 12 heads of 8 sequences
-  // over 4001 keys take 18.9 / 13.9 / 17.5 us with 3 / 4 / 6 steps each, one
-  // sequence over 2000 keys 7.2 / 10.8 with 2 / 4
+  // By heads: one wave when the caches are three quarters full (12 heads of 8
+  // sequences over 4001 keys took 18.9 / 13.9 / 17.5 us with 3 / 4 / 6 steps
+  // each).  As a list where a CTA's share is long against what the heads that
+  // it begins cost, about 16 steps each: by heads / as a list, 12 heads over
+  // 4001 keys 10.8 / 12.5 us with 8 sequences, over 8000 keys 30.3 / 43.7 with
+  // 16, 8 wider heads over 65536 keys 61.1 / 44.4 with 2.
   const int each = (int)((3 * entries + 4 * ctas - 1) / (4 * ctas));
-  const bool by_head = each <= 8;
+  const bool by_head = entries < 16 * (heads + ctas);
   const dim3 grid = by_head ? dim3((unsigned)heads, (unsigned)((steps + each - 1) / each))
                             : dim3((unsigned)std::min(entries, ctas));
   const size_t smem = stream_ring_bytes(JC) + (size_t)(std::min(kStreamRows, p.nodes * p.group) + 7) / 8 * JC * 512;
