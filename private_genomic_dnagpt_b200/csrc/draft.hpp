@@ -123,7 +123,8 @@ __device__ __forceinline__ void cluster_sync() {
 }
 __device__ __forceinline__ uint32_t cluster_addr(const void* p, int rank) {
   uint32_t a;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(rank));
+  const uint32_t own = (uint32_t)__cvta_generic_to_shared(p);
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(own), "r"(rank));
   return a;
 }
 __device__ __forceinline__ int cluster_read(const int* p, int rank) {
