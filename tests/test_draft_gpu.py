@@ -92,6 +92,12 @@ SHAPES = [
     (1, 64, 1, 1, 64, 4, [3], 1, 0),           # a chain of 64
     (1, 64, 2, 2, 64, 0, [0], 2, 0),           # a cache without rows
     (1, 2, 1, 1, 64, 70000, [200], 1, 0),      # far more capacity than keys
+    (5, 1, 1, 1, 64, 50000, [0] * 5, 1, 0),
+    (1, 3, 130, 1, 64, 150, [140], 1, 0),      # more heads on a key than a tile has rows
+    (1, 2, 128, 1, 128, 150, [129], 1, 0),
+    (2, 64, 6, 2, 64, 260, [257, 3], 3, 1),    # tiles of 126 rows
+    (1, 5, 96, 2, 32, 140, [133], 2, 0),
+    (1, 12, 8, 1, 80, 900, [897], 2, 0),       # 96 rows
     (3, 3, 2, 1, 128, 40000, [129, 0, 300], 1, 1),
     (40, 2, 2, 1, 64, 300, [(37 * b) % 301 for b in range(40)], 1, 0),  # many short sequences
     (70, 33, 2, 2, 64, 140, [(53 * b) % 141 for b in range(70)], 2, 0),
@@ -220,9 +226,10 @@ def test_attention_repeats_exactly(cc, dtype):
     assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
 
 
-def test_attention_on_other_streams_and_in_graphs(cc):
+@pytest.mark.parametrize("dtype,D", [(torch.bfloat16, 64), (torch.float16, 128), (torch.float32, 64), (torch.float32, 33)])
+def test_attention_on_other_streams_and_in_graphs(cc, dtype, D):
     """Two captured calls replayed side by side, and one on another stream."""
-    xs = [inputs(torch.bfloat16, 1, 5, 4, 4, 64, 6000, [5999 - s], [tree(5, 1)], seed=11 + s) for s in range(2)]
+    xs = [inputs(dtype, 1, 5, 4, 4, D, 6000, [5999 - s], [tree(5, 1)], seed=11 + s) for s in range(2)]
     want = [cc.draft_attention(**x) for x in xs]
     torch.cuda.synchronize()
     s = torch.cuda.Stream()
@@ -411,7 +418,9 @@ def test_commit_leaves_what_does_not_fit(cc):
 @pytest.mark.parametrize("shape", [(1, 1, 12, 12, 64, 128, [103], [1]), (3, 9, 8, 2, 128, 700, [500, 0, 691], [4, 9, 5]),
                                    (2, 64, 4, 4, 64, 400, [129, 336], [64, 3]), (2, 5, 6, 3, 80, 300, [290, 128], [5, 0]),
                                    (1, 3, 2, 1, 33, 70, [60], [2]), (1, 2, 8, 1, 256, 3000, [2998], [2]),
-                                   (2, 16, 16, 2, 96, 260, [240, 3], [16, 16])])
+                                   (2, 16, 16, 2, 96, 260, [240, 3], [16, 16]),
+                                   (3, 4, 4, 2, 8, 620000, [300000, 0, 619996], [3, 0, 4]),  # divided as a list
+                                   (1, 3, 2, 1, 8, 1500000, [1499990], [2])])
 def test_accumulate(cc, dtype, shape):
     """A weight is exp of a score off by (D + 8) 2^-24 S and an lse off by
     2^-24 of itself; the sum over the rows adds their number of roundings."""
@@ -468,7 +477,8 @@ def check_evict(x, acc, budget, recent, got, before):
 @pytest.mark.parametrize("shape", [(1, 3, 64, 2100, [2100], 1000, 100), (4, 2, 128, 300, [300, 0, 64, 65], 64, 8),
                                    (2, 2, 33, 90, [90, 41], 41, 41), (1, 1, 80, 50, [50], 1, 0), (1, 1, 64, 50, [50], 1, 1),
                                    (2, 1, 1, 5000, [5000, 4097], 4096, 5), (1, 2, 96, 70000, [70000], 9000, 300),
-                                   (3, 2, 40, 30, [40, -4, 30], 29, 3)])
+                                   (3, 2, 40, 30, [40, -4, 30], 29, 3), (1, 2, 16, 12000, [12000], 5000, 100),
+                                   (2, 1, 8, 200000, [200000, 131073], 40000, 0)])
 def test_evict(cc, dtype, shape):
     B, Hk, D, cap, lens, budget, recent = shape
     x = inputs(dtype, B, 1, Hk, Hk, D, cap, lens, [[-1]] * B, seed=16)
@@ -531,6 +541,9 @@ def test_cache_strides_and_streams(cc):
     s.synchronize()
     assert all(torch.equal(p, q) for p, q in zip(want, got))
     assert torch.equal(wide[:, :, 100:600], a) and not wide[:, :, :100].any() and not wide[:, :, 600:].any()
+    odd = torch.zeros(2, 2, 700, device="cuda")  # weights off every wide boundary
+    got = step(mixed["k_cache"], mixed["v_cache"], odd[:, :, 101:601])
+    assert all(torch.equal(p, q) for p, q in zip(want, got))
     g = torch.cuda.CUDAGraph()
     a.zero_()
     with torch.cuda.graph(g):

@@ -124,6 +124,37 @@ def test_draft_model_keeps_to_its_budget(model):
     model.cc.Synchronize()
 
 
+def test_draft_model_of_a_batch(model):
+    """Two sequences side by side, with trees of different sizes and other
+    accepted nodes, as two models of one."""
+    ws = [weights(60), weights(61)]
+    x = torch.from_numpy(np.stack([plain_block.synthetic_input(s, 100, d=D) for s in (62, 63)])).float().cuda()
+    both = DraftModel(model.cc, ws, capacity=164, batch=2, heads=HEADS, dtype=torch.float32, budget=100, recent=10)
+    ones = [DraftModel(model.cc, ws, capacity=164, heads=HEADS, dtype=torch.float32, budget=100, recent=10)
+            for _ in range(2)]
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    parents, path, count = [[-1, 0, 0, 1], [-1, -1, -2, 2]], [[0, 1, 3, -1], [1, -1, -1, -1]], [3, 1]
+    both.prefill(x[:, :60])
+    for m, s in zip(ones, x):
+        m.prefill(s[None, :60])
+    for step in range(4):
+        rows = x[:, 60 + 4 * step:64 + 4 * step]
+        got = both.forward(rows, i32(parents))
+        both.accept(i32(path), i32(count))
+        for b, m in enumerate(ones):
+            want = m.forward(rows[b:b + 1], i32(parents[b:b + 1]))
+            real = 4 if b == 0 else 2
+            assert (got[b, :real] - want[0, :real]).abs().max() <= 1e-5 * want.abs().max()
+            m.accept(i32(path[b:b + 1]), i32(count[b:b + 1]))
+    assert both.lens.tolist() == [72, 64] == [int(m.lens[0]) for m in ones]
+    for (k, v, acc), pairs in zip(both.caches, zip(ones[0].caches, ones[1].caches)):
+        for b, (k1, v1, a1) in enumerate(pairs):
+            n = int(both.lens[b])
+            for t, t1 in ((k, k1), (v, v1), (acc, a1)):
+                assert (t[b, :, :n] - t1[0, :, :n]).abs().max() <= 1e-4 * t1[0, :, :n].abs().max()
+    model.cc.Synchronize()
+
+
 def test_drafts_confirmed_by_the_encrypted_model(model):
     """The whole round: the draft model proposes a tree of greedy tokens, the
     encrypted model evaluates it in one forward, the accepted nodes enter the
