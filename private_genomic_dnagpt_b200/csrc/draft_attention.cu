@@ -527,8 +527,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           const uint32_t off = (i / 4) * kPanel + (i % 4) * 32;
           mma_smem(t_base + 128 * g, smem_operand(qb + off, 16), smem_operand(kb + off, 16), word_s, i > 0);
         }
-        mma_commit(empty(s));
         mma_commit(s_full(g));
+        mma_commit(empty(s));
         ++k;
         return true;
       };
