@@ -350,7 +350,7 @@ __device__ __noinline__ void add_spoiled(const AttnParams& p, int b, int h, int 
 // O is seldom rescaled.  Weights are rounded to the operands' type for the
 // second product; l sums them before that, in 32 bits.
 //
-// Measured: 32 nodes x 4 heads over 65536 keys of 128 (470 MB) 92.8 us, of it
+// Measured: 32 nodes x 4 heads over 65536 keys of 128 (470 MB) 91.5 us, of it
 // the tiles at 98 % of the copy rate and about 15 us of set-up, unit ends and
 // joining; 21 nodes over 4001 keys of 64, eight ragged sequences, 25.7 us: a
 // tile's products and waits take one warp 1250 cycles, its bytes 1420 of an
@@ -1247,10 +1247,11 @@ Division divide(const Context& c, const ckks_draft_attention_args& a, Division d
 
 // What a unit's start and end cost, in tiles: measured on trees of 21 over 4001
 // keys of 64 (2 / 3 / 4 / 5 / 6 tiles: 32.7 / 28.4 / 26.9 / 27.8 / 29.0 us) and
-// trees of 32 over 65536 keys of 128 (2 / 4 / 6 / 8: 97.6 / 95.3 / 93.7 / 91.4 us)
+// trees of 32 over 65536 keys of 128 (2 / 4 / 6 / 8 tiles: 97.6 / 95.3 / 93.7 /
+// 91.4 us), later 8 / 10: 92.2 / 90.1 us
 Division tc_division(const Context& c, const ckks_draft_attention_args& a) {
   const int rows = tile_nodes(a) * (a.q_heads / a.kv_heads);
-  return divide(c, a, Division{rows, kKeys, 1, a.head_dim <= 64 ? 4 : 8, 0, false}, 1);
+  return divide(c, a, Division{rows, kKeys, 1, a.head_dim <= 64 ? 4 : 10, 0, false}, 1);
 }
 
 bool f32_sizes(const ckks_draft_attention_args& a) { return a.dtype == CKKS_FP32 && a.head_dim % 4 == 0; }
