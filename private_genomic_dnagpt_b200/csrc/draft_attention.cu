@@ -73,9 +73,9 @@ __device__ __forceinline__ T* out_row(const AttnParams& p, int b, int node, int 
 // across head_dim (4 elements each, looping over larger ones), 8 across the
 // keys of the tile, each with the sums of all 8 rows in registers; the 8
 // partial sums meet once, at the end.  Products and sums are in 32 bits.  What
-// the two kernels below do not take comes here: unaligned rows, 16-bit heads
-// over 128, odd head sizes.  Loads are not overlapped within a CTA (5 float32
-// rows over 6000 keys took it 87 us, against 39 below).
+// the two kernels below do not take comes here: unaligned rows, odd head sizes.
+// Loads are not overlapped within a CTA (5 float32 rows over 6000 keys took it
+// 87 us, against 39 below).
 constexpr int kRows = 8, kTile = 64, kThreads = 128;
 
 template <typename T>
@@ -331,7 +331,8 @@ __device__ __noinline__ void add_spoiled(const AttnParams& p, int b, int h, int 
 // copies), a thread that issues both products, and two groups of four softmax
 // warps that take the unit's tiles in turn, each with its own S and O: one
 // group's products and copies run under the other's exponentials.  K of the
-// next tile comes before V of this one, in the order of the products.
+// next tile comes before V of this one, in the order of the products.  (Over
+// 128 elements there is one group, whose scores and weights share their place.)
 //
 // With 64 rows or fewer the rows are repeated in the tile (COPIES times), and
 // a copy weighs only its share of a tile's keys, the others' weights being 0:
@@ -354,8 +355,10 @@ __device__ __noinline__ void add_spoiled(const AttnParams& p, int b, int h, int 
 // the tiles at 98 % of the copy rate and about 15 us of set-up, unit ends and
 // joining; 21 nodes over 4001 keys of 64, eight ragged sequences, 25.7 us: a
 // tile's products and waits take one warp 1250 cycles, its bytes 1420 of an
-// SM's share of HBM, and set-up, unit ends and joining some 9 us.
-constexpr int kM = 128, kKeys = 128, kTcThreads = 320, kTmemCols = 512;
+// SM's share of HBM, and set-up, unit ends and joining some 9 us.  Four
+// sequences over 8000 keys of 256: 8 nodes and 8 heads 60 us (floor 33), 32
+// nodes x 4 heads on each of 4 heads 50 us (6560 on the CUDA cores above).
+constexpr int kM = 128, kKeys = 128, kTmemCols = 512;
 constexpr uint32_t kPanel = 128 * 128;  // 128 rows x 64 elements
 constexpr float kSlack = 8.0f;
 
@@ -389,26 +392,31 @@ __device__ __forceinline__ void group_sync(int id, int threads) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
 }
 
+// by panels of 64 elements of head_dim
 template <int PANELS>
 struct TcShape {
-  static constexpr int kSlots = PANELS == 1 ? 9 : 5;
+  // over 128 elements tensor memory has room for one group's O, and shared
+  // memory for one Q
+  static constexpr int kGroups = PANELS <= 2 ? 2 : 1, kThreads = 32 * (4 * kGroups + 2);
+  static constexpr int kSlots = PANELS == 1 ? 9 : PANELS == 2 ? 5 : PANELS == 3 ? 3 : 2;
   static constexpr uint32_t kTileBytes = PANELS * kPanel;
-  // Two buffers for Q, the next unit's arriving early; 2 x 128 x 32 floats in
-  // which a unit's parts meet at its end (with two panels, its own Q); the
-  // ring; (m, l) of one group's rows, the nodes' masks of two units, barriers,
-  // two words
-  static constexpr uint32_t kMeet = PANELS == 1 ? 2 * kPanel : 0, kRing = 4 * kPanel;
+  // A buffer for Q for each group, the next unit's arriving early; 32 floats of
+  // each group's 128 rows, in which a unit's parts meet at its end (but for one
+  // panel its own Q); the ring; (m, l) of one group's rows, the nodes' masks of
+  // two units, barriers, two words
+  static constexpr uint32_t kMeet = PANELS == 1 ? 2 * kPanel : 0;
+  static constexpr uint32_t kRing = PANELS == 1 ? 4 * kPanel : kGroups * kTileBytes;
   static constexpr uint32_t kExtra = kRing + kSlots * kTileBytes;
   static constexpr int kBars = 2 * kSlots + 9;
   static constexpr size_t kSmem = kExtra + kM * sizeof(float2) + 2 * kMaxNodes * 8 + kBars * 8 + 16;
 };
 
 template <typename T, int PANELS, int COPIES>
-__global__ void __launch_bounds__(kTcThreads, 1)
+__global__ void __launch_bounds__(TcShape<PANELS>::kThreads, 1)
     attend_tc_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ TileMaps maps, bool negative, float c,
                      unsigned int* __restrict__ faults) {
   using S = TcShape<PANELS>;
-  constexpr int DP = 64 * PANELS, NS = S::kSlots, KQ = kKeys / COPIES, CW = 32;
+  constexpr int DP = 64 * PANELS, NS = S::kSlots, KQ = kKeys / COPIES, CW = 32, GR = S::kGroups;
   constexpr bool kBf = std::is_same_v<T, __nv_bfloat16>;
   extern __shared__ __align__(1024) uint8_t smem[];
   float2* const s_ml = reinterpret_cast<float2*>(smem + S::kExtra);  // [kM]
@@ -442,7 +450,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     mbar_init(o_full, 1);
     *s_spoiled = 0ull;
   }
-  if (warp == 9) tmem_alloc(smem_addr(s_tmem), kTmemCols);
+  if (warp == 4 * GR + 1) tmem_alloc(smem_addr(s_tmem), kTmemCols);
   // this CTA's entries [w0, w1) of the list
   int first;
   auto entries_of = [&](int b) { return tiles_of(p, b) + p.unit_cost; };
@@ -453,7 +461,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   tmem_fence_before();
   __syncthreads();
   tmem_fence_after();
-  const uint32_t tmem = *s_tmem;  // S of both groups, then O of both
+  const uint32_t tmem = *s_tmem;  // S of every group, then O of every group
   // the tiles of this CTA in the unit at `at`, from tile at.tile on; none
   // where the CTA has only the unit's start
   auto tiles_here = [&](int& w) {
@@ -463,7 +471,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     return max(0, min(at.tiles - at.tile, w1 - w));
   };
   bool fine = true;  // no wait gave up
-  if (warp == 8) {
+  if (warp == 4 * GR) {
     // ---- copies
     if (lane == 0) {
       tile_prefetch(&maps.q);
@@ -485,8 +493,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           return true;
         };
         if (n) {
-          const int i = u & 1;
-          if (u >= 2 && !(fine = mbar_wait_short(q_empty(i), ((u >> 1) - 1) & 1))) break;
+          const int i = u % GR;
+          if (u >= GR && !(fine = mbar_wait_short(q_empty(i), (u / GR - 1) & 1))) break;
           ++u;
           mbar_expect_tx(q_full(i), COPIES * PANELS * tile_rows * 128);
 #pragma unroll
@@ -495,18 +503,19 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                       64 * (x % PANELS), h * p.group, at.unit % tiles_r * p.tile_nodes, at.b, q_full(i));
           load(at.tile, false);
         }
+        // in the order of the products
         for (int t = 0; t < n && fine; ++t) {
-          if (t + 1 < n && !load(at.tile + t + 1, false)) break;
-          load(at.tile + t, true);
+          if (GR == 2 && t + 1 < n && !load(at.tile + t + 1, false)) break;
+          if (load(at.tile + t, true) && GR == 1 && t + 1 < n) load(at.tile + t + 1, false);
         }
         w += n;
         at.next_unit(p, units);
       }
       // copies still in flight land before the CTA ends
       for (int j = k > NS ? k - NS : 0; j < k; ++j) fine = mbar_wait_short(full(j % NS), (j / NS) & 1) && fine;
-      for (int j = u > 2 ? u - 2 : 0; j < u; ++j) fine = mbar_wait_short(q_full(j & 1), j >> 1 & 1) && fine;
+      for (int j = u > GR ? u - GR : 0; j < u; ++j) fine = mbar_wait_short(q_full(j % GR), j / GR & 1) && fine;
     }
-  } else if (warp == 9) {
+  } else if (warp == 4 * GR + 1) {
     // ---- products, by the whole warp in step
     constexpr uint32_t word_s = mma_word(kBf, kM, kKeys, false), word_o = mma_word(kBf, kM, DP, true);
     const uint32_t t_base = __shfl_sync(0xffffffffu, tmem, 0);
@@ -521,7 +530,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         const int s = k % NS;
         if (!wait(full(s), (k / NS) & 1)) return fine = false;
         tmem_fence_after();
-        const uint32_t qb = sq + (u & 1) * S::kTileBytes, kb = ring + s * S::kTileBytes;
+        const uint32_t qb = sq + (u % GR) * S::kTileBytes, kb = ring + s * S::kTileBytes;
 #pragma unroll
         for (int i = 0; i < DP / 16; ++i) {
           const uint32_t off = (i / 4) * kPanel + (i % 4) * 32;
@@ -533,20 +542,22 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         return true;
       };
       if (n) {
-        fine = wait(q_full(u & 1), u >> 1 & 1) && scores(0);
+        fine = wait(q_full(u % GR), u / GR & 1) && scores(0);
         for (int t = 0; t < n && fine; ++t) {
-          if (t + 1 < n && !scores((t + 1) & 1)) break;
-          const int g = t & 1, s = k % NS;
+          // one group's next scores take the place of this tile's weights
+          if (GR == 2 && t + 1 < n && !scores((t + 1) & 1)) break;
+          const int g = t % GR, s = k % NS;
           if (!(fine = wait(full(s), (k / NS) & 1) && wait(p_ready(g), phase >> g & 1))) break;
           phase ^= 1u << g;
           tmem_fence_after();
           const uint32_t vb = ring + s * S::kTileBytes;
 #pragma unroll
           for (int i = 0; i < kKeys / 16; ++i)
-            mma_tmem(t_base + 256 + 128 * g, t_base + 128 * g + 8 * i, smem_operand(vb + 2048 * i, kPanel), word_o,
-                     i > 0 || t > 1);
+            mma_tmem(t_base + 128 * (GR + g), t_base + 128 * g + 8 * i, smem_operand(vb + 2048 * i, kPanel), word_o,
+                     i > 0 || t >= GR);
           mma_commit(empty(s));
           ++k;
+          if (GR == 1 && t + 1 < n && !scores(0)) break;
         }
         if (fine) mma_commit(o_full);
         ++u;
@@ -561,7 +572,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const int part = COPIES == 4 ? quarter : COPIES == 2 ? quarter >> 1 : 0;
     const int r0 = COPIES == 4 ? lane : COPIES == 2 ? L & 63 : L;
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
-    const uint32_t t_s = tmem + 128 * g + lanes, t_o = tmem + 256 + 128 * g + lanes;
+    const uint32_t t_s = tmem + 128 * g + lanes, t_o = tmem + 128 * (GR + g) + lanes;
     int k = 0, u = 0;  // k: tiles of keys and values before this unit's
     uint32_t phase = 0;
     // The parents of the next unit's nodes are read before this unit's tiles
@@ -584,12 +595,12 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       then.next_unit(p, units);
       const bool more = w + n < w1;
       if (warp == 0 && more) reader.read(p.parents + (size_t)then.b * p.nodes, p.nodes);
-      group_sync(1, 256);
+      group_sync(1, 128 * GR);
       const uint64_t mask = mine ? masks[node] : 0ull;
       const int len = length_of(p, b);
       float m = -INFINITY, l = 0.0f;
 #pragma unroll 1
-      for (int t = g; t < n; t += 2) {
+      for (int t = g; t < n; t += GR) {
         const int tile = at.tile + t;
         const bool tree = tile == at.tiles - 1;
         const int nk = tree ? p.nodes : min(kKeys, len - tile * kKeys);
@@ -600,7 +611,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           // and those of new keys that are not finite, which only some see.  (The
           // copy that had the slot before was used ahead of this tile's scores,
           // so the wait cannot take its arrival for this one's.)
-          const int kv = k + (t + 1 < n ? 2 * t + 2 : 2 * t + 1);
+          const int kv = k + (GR == 2 && t + 1 < n ? 2 * t + 2 : 2 * t + 1);
           if (!(fine = mbar_wait_short(full(kv % NS), (kv / NS) & 1))) break;
           uint8_t* vs = smem + S::kRing + (kv % NS) * S::kTileBytes;
           for (int r = tree ? L : nk + L; r < (tree ? p.nodes : kKeys); r += kM) {
@@ -648,7 +659,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           m = top;
           l *= f;
         }
-        if (t > 1 && __any_sync(0xffffffffu, f != 1.0f)) {
+        if (t >= GR && __any_sync(0xffffffffu, f != 1.0f)) {
           // the sums so far, on the new reference point
 #pragma unroll 1
           for (int i = 0; i < DP; i += 16) {
@@ -692,18 +703,18 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       if (!fine || !(fine = mbar_wait_short(o_full, u & 1))) break;
       tmem_fence_after();
       // join the parts of each row: reference point and sum first
-      // [2][kM][CW], 16-byte pieces swizzled; before that the second group's (m, l)
-      float4* const buf = reinterpret_cast<float4*>(smem + (PANELS == 1 ? S::kMeet : (u & 1) * S::kTileBytes));
+      // [GR][kM][CW], 16-byte pieces swizzled; before that the second group's (m, l)
+      float4* const buf = reinterpret_cast<float4*>(smem + (PANELS == 1 ? S::kMeet : (u % GR) * S::kTileBytes));
       float2* const ml[2] = {s_ml, reinterpret_cast<float2*>(buf)};
       ml[g][L] = make_float2(m, l);
-      group_sync(1, 256);
+      group_sync(1, 128 * GR);
       float top = -INFINITY, total = 0.0f;
 #pragma unroll
-      for (int i = 0; i < 2 * COPIES; ++i) top = fmaxf(top, ml[i & 1][(i >> 1) * (kM / COPIES) + r0].x);
+      for (int i = 0; i < GR * COPIES; ++i) top = fmaxf(top, ml[i % GR][i / GR * (kM / COPIES) + r0].x);
       const float ref = top == -INFINITY ? 0.0f : top;
 #pragma unroll
-      for (int i = 0; i < 2 * COPIES; ++i) {
-        const float2 e = ml[i & 1][(i >> 1) * (kM / COPIES) + r0];
+      for (int i = 0; i < GR * COPIES; ++i) {
+        const float2 e = ml[i % GR][i / GR * (kM / COPIES) + r0];
         total = fmaf(e.y, ex2(e.x - ref), total);
       }
       const float f = ex2(m - ref);
@@ -713,7 +724,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       // part of a unit: slot 1 holds a unit's beginning, slot 0 what follows
       float* const keep = p.part + (size_t)(2 * blockIdx.x + (at.tile == 0 ? 1 : 0)) * tile_rows * (DP + 4);
       const bool leads = g == 0 && part == 0 && mine;  // one thread of each row
-      group_sync(1, 256);
+      group_sync(1, 128 * GR);
       // every row's factor, 0 for one that sees nothing, in the place of its first part's m
       if (leads) s_ml[r0] = make_float2(whole ? inv : 1.0f, seen || !whole ? 1.0f : 0.0f);
       auto place = [&](int gg, int ll, int piece) { return (gg * kM + ll) * (CW / 4) + (piece ^ (ll & 7)); };
@@ -731,14 +742,14 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           e.w = f == 0.0f ? 0.0f : __uint_as_float(o[4 * j + 3]) * f;
           buf[place(g, L, j)] = e;
         }
-        group_sync(1, 256);
+        group_sync(1, 128 * GR);
         // neighbouring threads take neighbouring pieces of a row
-        for (int x = tid; x < here * (CW / 4); x += 256) {
+        for (int x = tid; x < here * (CW / 4); x += 128 * GR) {
           const int r = x / (CW / 4), j = x % (CW / 4), d = i + 4 * j;
           float4 e = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-          for (int q = 0; q < 2 * COPIES; ++q) {
-            const float4 y = buf[place(q & 1, (q >> 1) * (kM / COPIES) + r, j)];
+          for (int q = 0; q < GR * COPIES; ++q) {
+            const float4 y = buf[place(q % GR, q / GR * (kM / COPIES) + r, j)];
             e.x += y.x, e.y += y.y, e.z += y.z, e.w += y.w;
           }
           if (!whole) {
@@ -751,7 +762,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 make_uint2(pack2<T>(e.x * k2.x, e.y * k2.x), pack2<T>(e.z * k2.x, e.w * k2.x));
           }
         }
-        group_sync(1, 256);
+        group_sync(1, 128 * GR);
       }
       if (leads) {
         if (whole) {
@@ -766,8 +777,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       }
       if (tid == 0) {
         *s_spoiled = 0ull;
-        if constexpr (PANELS == 2) smem_fence_async();  // the copy of a later Q follows the sums that met here
-        mbar_arrive(q_empty(u & 1));
+        if constexpr (PANELS > 1) smem_fence_async();  // the copy of a later Q follows the sums that met here
+        mbar_arrive(q_empty(u % GR));
       }
       ++u;
       if (warp == 0 && more) reader.masks(s_mask + (u & 1) * kMaxNodes, reinterpret_cast<int*>(s_ml));
@@ -777,10 +788,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       at = then;
     }
   }
-  if (!fine && (warp < 8 || lane == 0)) atomicAdd(faults, 1u);
+  if (!fine && (warp < 4 * GR || lane == 0)) atomicAdd(faults, 1u);
   tmem_fence_before();
   __syncthreads();
-  if (warp == 9) {
+  if (warp == 4 * GR + 1) {
     __syncwarp();
     tmem_free(tmem, kTmemCols);
   }
@@ -1221,7 +1232,7 @@ void check_shape(const ckks_draft_attention_args& a) {
 }
 
 bool tc_sizes(const ckks_draft_attention_args& a) {
-  return a.dtype != CKKS_FP32 && a.head_dim <= 128 && a.head_dim % 8 == 0 && a.q_heads / a.kv_heads <= kM;
+  return a.dtype != CKKS_FP32 && a.head_dim % 8 == 0 && a.q_heads / a.kv_heads <= kM;
 }
 
 // nodes whose rows a tile of the tensor-core kernel holds
@@ -1352,7 +1363,7 @@ void launch_tc(const Context& c, const AttnParams& p, const TileMaps& maps, cons
   CKKS_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::kSmem));
   // a scale of 0 becomes one that changes no weight: a masked score times 0 would be no number
   const float factor = std::max(std::fabs(p.scale) * kLog2e, 1e-30f);
-  k<<<d.ctas, kTcThreads, S::kSmem, st>>>(p, maps, p.scale < 0.0f, factor, c.d_faults);
+  k<<<d.ctas, S::kThreads, S::kSmem, st>>>(p, maps, p.scale < 0.0f, factor, c.d_faults);
   CKKS_CUDA(cudaGetLastError());
   join_division<T, PANELS>(p, d, st);
 }
@@ -1388,10 +1399,12 @@ bool run_tc(const Context& c, const ckks_draft_attention_args& a, const AttnPara
   } else if (!rows_map(&m.kc, a.k_cache, a.capacity) || !rows_map(&m.vc, a.v_cache, a.capacity)) {
     return false;
   }
-  if (a.head_dim <= 64)
-    launch_tc<T, 1>(c, a, p, m, st);
-  else
-    launch_tc<T, 2>(c, a, p, m, st);
+  switch ((a.head_dim + 63) / 64) {
+    case 1: launch_tc<T, 1>(c, a, p, m, st); break;
+    case 2: launch_tc<T, 2>(c, a, p, m, st); break;
+    case 3: launch_tc<T, 3>(c, a, p, m, st); break;
+    default: launch_tc<T, 4>(c, a, p, m, st); break;
+  }
   return true;
 }
 

@@ -98,6 +98,11 @@ SHAPES = [
     (2, 64, 6, 2, 64, 260, [257, 3], 3, 1),    # tiles of 126 rows
     (1, 5, 96, 2, 32, 140, [133], 2, 0),
     (1, 12, 8, 1, 80, 900, [897], 2, 0),       # 96 rows
+    (2, 40, 8, 2, 256, 900, [897, 300], 2, 1),
+    (3, 64, 4, 1, 160, 700, [700, 0, 129], 3, 2),
+    (2, 17, 3, 3, 136, 1000, [999, 640], 2, 0),
+    (1, 33, 2, 1, 192, 2000, [1999], 1, 0),
+    (70, 9, 2, 2, 248, 260, [(53 * b) % 261 for b in range(70)], 2, 0),
     (3, 3, 2, 1, 128, 40000, [129, 0, 300], 1, 1),
     (40, 2, 2, 1, 64, 300, [(37 * b) % 301 for b in range(40)], 1, 0),  # many short sequences
     (70, 33, 2, 2, 64, 140, [(53 * b) % 141 for b in range(70)], 2, 0),
@@ -114,7 +119,8 @@ def test_attention(cc, dtype, shape):
 
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("shape", [(2, 13, 8, 2, 128, 9000, [8999, 4097], 3), (1, 1, 4, 4, 64, 20000, [19999], 1),
-                                   (1, 40, 4, 1, 64, 5000, [4999], 2)])
+                                   (1, 40, 4, 1, 64, 5000, [4999], 2),
+                                   (2, 21, 4, 1, 256, 9000, [8999, 4097], 3)])
 def test_attention_over_long_caches(cc, dtype, shape):
     B, n, Hq, Hk, D, cap, lens, branch = shape
     x = inputs(dtype, B, n, Hq, Hk, D, cap, lens, [tree(n, branch)] * B, seed=1)
@@ -129,11 +135,13 @@ def test_attention_sharp_rows(cc, dtype):
     check_attention(x, *cc.draft_attention(**x, scale=0.5), scale=0.5)
     check_attention(x, *cc.draft_attention(**x, scale=-0.01), scale=-0.01)
     check_attention(x, *cc.draft_attention(**x, scale=0.0), scale=0.0)
+    x = inputs(dtype, 2, 6, 4, 2, 200, 600, [600, 321], [tree(6, 2)] * 2, seed=2, spread=6.0)
+    check_attention(x, *cc.draft_attention(**x))
 
 
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
-@pytest.mark.parametrize("D", [64, 128, 40])
+@pytest.mark.parametrize("D", [64, 128, 40, 256])
 def test_attention_ignores_what_is_masked(cc, dtype, bad, D):
     """Rows behind the length and padding nodes hold NaN and infinities."""
     lens = [130, 0, 257]
@@ -150,7 +158,7 @@ def test_attention_ignores_what_is_masked(cc, dtype, bad, D):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("D", [64, 128, 40])
+@pytest.mark.parametrize("D", [64, 128, 40, 256])
 @pytest.mark.parametrize("G", [1, 4])
 def test_attention_keeps_siblings_apart(cc, dtype, D, G):
     """A node whose key and value are NaN or infinite spoils its own row and
