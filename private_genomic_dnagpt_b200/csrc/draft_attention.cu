@@ -1241,7 +1241,8 @@ int tile_nodes(const ckks_draft_attention_args& a) { return std::min(a.nodes, kM
 // how a kernel divides its list of units
 struct Division {
   int tile_rows, tile_keys, new_apart, unit_cost, ctas;
-  bool alone;  // no unit is shared
+  bool alone;   // no unit is shared
+  bool listed;  // the list of full caches has fewer than 2^31 - 1 entries
 };
 
 // `per_sm` CTAs on each SM, but no fewer than four tiles of keys each at the
@@ -1251,6 +1252,9 @@ Division divide(const Context& c, const ckks_draft_attention_args& a, Division d
   const long long rows = (long long)a.nodes * (a.q_heads / a.kv_heads);
   const long long units = (long long)a.batch * a.kv_heads * ((rows + d.tile_rows - 1) / d.tile_rows);
   const long long tiles = units * ((a.capacity + d.tile_keys - 1) / d.tile_keys + 1);
+  // the kernels count the list's entries in 32 bits
+  const long long keys = (long long)a.capacity + (d.new_apart ? 0 : a.nodes);
+  d.listed = units * ((keys + d.tile_keys - 1) / d.tile_keys + (d.new_apart ? 1 : 0) + d.unit_cost) < (1ll << 31) - 1;
   d.ctas = (int)std::max(1ll, std::min((long long)per_sm * c.sms, std::max(tiles / 4, units)));
   d.alone = a.batch == 1 && d.ctas == units;  // one sequence and a CTA for each unit
   return d;
@@ -1262,7 +1266,7 @@ Division divide(const Context& c, const ckks_draft_attention_args& a, Division d
 // 91.4 us), later 8 / 10: 92.2 / 90.1 us
 Division tc_division(const Context& c, const ckks_draft_attention_args& a) {
   const int rows = tile_nodes(a) * (a.q_heads / a.kv_heads);
-  return divide(c, a, Division{rows, kKeys, 1, a.head_dim <= 64 ? 4 : 10, 0, false}, 1);
+  return divide(c, a, Division{rows, kKeys, 1, a.head_dim <= 64 ? 4 : 10, 0, false, false}, 1);
 }
 
 bool f32_sizes(const ckks_draft_attention_args& a) { return a.dtype == CKKS_FP32 && a.head_dim % 4 == 0; }
@@ -1275,11 +1279,18 @@ int f32_rows(const ckks_draft_attention_args& a) {
 
 Division f32_division(const Context& c, const ckks_draft_attention_args& a) {
   const int dc = (a.head_dim + 63) / 64;
-  return divide(c, a, Division{f32_rows(a), dc == 1 ? 64 : dc == 2 ? 32 : 16, 0, 1, 0, false}, dc == 1 ? 3 : 2);
+  return divide(c, a, Division{f32_rows(a), dc == 1 ? 64 : dc == 2 ? 32 : 16, 0, 1, 0, false, false}, dc == 1 ? 3 : 2);
 }
 
 size_t division_floats(const ckks_draft_attention_args& a, const Division& d) {
   return d.alone ? 0 : (size_t)2 * d.ctas * d.tile_rows * ((a.head_dim + 63) / 64 * 64 + 4);
+}
+
+// which of the kernels that divide a list takes these sizes; a list whose
+// entries 32 bits do not hold is left to the plain kernel, which has none
+bool takes_tc(const Context& c, const ckks_draft_attention_args& a) { return tc_sizes(a) && tc_division(c, a).listed; }
+bool takes_f32(const Context& c, const ckks_draft_attention_args& a) {
+  return f32_sizes(a) && f32_division(c, a).listed;
 }
 
 size_t workspace_of(const Context& c, const ckks_draft_attention_args& a) {
@@ -1287,8 +1298,8 @@ size_t workspace_of(const Context& c, const ckks_draft_attention_args& a) {
   // the tensors' strides decide which kernel runs
   const int s = split_count(c, a);
   size_t n = s == 1 ? 0 : (size_t)a.batch * a.q_heads * a.nodes * s * (a.head_dim + 2);
-  if (tc_sizes(a)) n = std::max(n, division_floats(a, tc_division(c, a)));
-  if (f32_sizes(a)) n = std::max(n, division_floats(a, f32_division(c, a)));
+  if (takes_tc(c, a)) n = std::max(n, division_floats(a, tc_division(c, a)));
+  if (takes_f32(c, a)) n = std::max(n, division_floats(a, f32_division(c, a)));
   return sizeof(float) * n;
 }
 
@@ -1467,10 +1478,10 @@ extern "C" int ckks_draft_attention(ckks_ctx* ctx, const ckks_draft_attention_ar
     const double bytes = 2.0 * e * a.batch * a.kv_heads * a.capacity * a.head_dim;
     ProfScope ps(c, "draft_attention", bytes, st);
     // strides that no tensor map holds are left to the plain kernel
-    if (p.wide && tc_sizes(a)) {
+    if (p.wide && takes_tc(c, a)) {
       if (a.dtype == CKKS_BF16 ? run_tc<__nv_bfloat16>(c, a, p, st) : run_tc<__half>(c, a, p, st)) return;
     }
-    if (p.wide && f32_sizes(a)) {
+    if (p.wide && takes_f32(c, a)) {
       run_f32(c, a, p, st);
       return;
     }

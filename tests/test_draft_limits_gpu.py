@@ -1,0 +1,41 @@
+"""Limits of the drafted-decoding operators that no ordinary call comes near,
+and waits that run out."""
+
+import ctypes
+
+import pytest
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+import private_genomic_dnagpt_b200 as eng  # noqa: E402
+
+from test_draft_gpu import AttentionArgs  # noqa: E402
+
+
+@pytest.fixture(scope="module")
+def cc():
+    return eng.GenCryptoContext(eng.CCParams(ring_dim_log=10, limbs=3, dnum=1, seed=3))
+
+
+def attention_workspace(cc, **sizes):
+    """No pointer is looked at and nothing is launched."""
+    a = AttentionArgs(**(dict(scale=1.0) | sizes))
+    return eng.lib().ckks_draft_attention_workspace(cc.h, ctypes.byref(a))
+
+
+@pytest.mark.parametrize("sizes,last,step", [
+    # float32 heads of 256: 512 x 128 units of 8 rows, tiles of 16 keys and one entry for a unit's start;
+    # 32767 entries a unit are the most
+    (dict(dtype=2, batch=512, q_heads=16, kv_heads=1, head_dim=256, nodes=64), 32766 * 16 - 64, 16),
+    # float32 heads of 64: 512 x 64 units of 16 rows, tiles of 64 keys
+    (dict(dtype=2, batch=512, q_heads=16, kv_heads=1, head_dim=64, nodes=64), 65534 * 64 - 64, 64),
+    # 16-bit heads of 64: 2^20 units, tiles of 128 keys, one more for the new keys and four entries for the start
+    (dict(dtype=0, batch=1 << 20, q_heads=1, kv_heads=1, head_dim=64, nodes=64), 2042 * 128, 128)])
+def test_attention_list_fits_32_bits(cc, sizes, last, step):
+    """The kernels that divide a list of tiles need a workspace for the parts
+    of units; from the first size on at which the list would pass 2^31 entries
+    the call goes to the kernel without one, which here divides no keys."""
+    assert attention_workspace(cc, capacity=last, **sizes) > 0
+    assert attention_workspace(cc, capacity=last + 1, **sizes) == 0
+    assert attention_workspace(cc, capacity=last + step, **sizes) == 0
