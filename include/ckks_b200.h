@@ -569,6 +569,11 @@ long long ckks_draft_evict_workspace(ckks_ctx* ctx, const ckks_draft_evict_args*
  * intact.  starve = 1: the barrier expects more bytes than are copied, the
  * wait gives up after one second, and ckks_sync's CKKS_ECUDA is returned. */
 int ckks_selftest_bulk_wait(ckks_ctx* ctx, int starve);
+/* The same for warps that meet at a barrier after their waits, as in
+ * ckks_draft_attention: eight warps wait, one thread of warp `starved` (0..7)
+ * for an arrival that does not come.  All leave together and ckks_sync's
+ * CKKS_ECUDA is returned; CKKS_OK with starved = -1. */
+int ckks_selftest_group_wait(ckks_ctx* ctx, int starved);
 
 #ifdef __cplusplus
 }

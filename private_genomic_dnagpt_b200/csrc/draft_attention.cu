@@ -392,6 +392,23 @@ __device__ __forceinline__ void group_sync(int id, int threads) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
 }
 
+// The barriers above wait without limit, so warps that meet there go on or
+// leave together: a wait on an mbarrier counts for the whole warp (which then
+// runs the collective tensor-memory instructions or does not), and the warps'
+// results are joined at a barrier that all of them reach, whatever theirs is.
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity) {
+  return (bool)__all_sync(0xffffffffu, mbar_wait_short(bar, parity));
+}
+__device__ __forceinline__ bool group_all(int id, int threads, bool ok) {
+  uint32_t all;
+  asm volatile(
+      "{\n .reg .pred p, q;\n setp.ne.u32 p, %3, 0;\n bar.red.and.pred q, %1, %2, p;\n selp.u32 %0, 1, 0, q;\n}\n"
+      : "=r"(all)
+      : "r"(id), "r"(threads), "r"((uint32_t)ok)
+      : "memory");
+  return all != 0;
+}
+
 // by panels of 64 elements of head_dim
 template <int PANELS>
 struct TcShape {
@@ -519,16 +536,13 @@ __global__ void __launch_bounds__(TcShape<PANELS>::kThreads, 1)
     // ---- products, by the whole warp in step
     constexpr uint32_t word_s = mma_word(kBf, kM, kKeys, false), word_o = mma_word(kBf, kM, DP, true);
     const uint32_t t_base = __shfl_sync(0xffffffffu, tmem, 0);
-    auto wait = [&](uint32_t bar, uint32_t parity) {
-      return (bool)__all_sync(0xffffffffu, mbar_wait_short(bar, parity));
-    };
     int k = 0, u = 0;
     uint32_t phase = 0;  // bit g: parity of group g's next weights
     for (int w = w0; w < w1 && fine;) {
       const int n = __shfl_sync(0xffffffffu, tiles_here(w), 0);
       auto scores = [&](int g) {
         const int s = k % NS;
-        if (!wait(full(s), (k / NS) & 1)) return fine = false;
+        if (!warp_wait(full(s), (k / NS) & 1)) return fine = false;
         tmem_fence_after();
         const uint32_t qb = sq + (u % GR) * S::kTileBytes, kb = ring + s * S::kTileBytes;
 #pragma unroll
@@ -542,12 +556,12 @@ __global__ void __launch_bounds__(TcShape<PANELS>::kThreads, 1)
         return true;
       };
       if (n) {
-        fine = wait(q_full(u % GR), u / GR & 1) && scores(0);
+        fine = warp_wait(q_full(u % GR), u / GR & 1) && scores(0);
         for (int t = 0; t < n && fine; ++t) {
           // one group's next scores take the place of this tile's weights
           if (GR == 2 && t + 1 < n && !scores((t + 1) & 1)) break;
           const int g = t % GR, s = k % NS;
-          if (!(fine = wait(full(s), (k / NS) & 1) && wait(p_ready(g), phase >> g & 1))) break;
+          if (!(fine = warp_wait(full(s), (k / NS) & 1) && warp_wait(p_ready(g), phase >> g & 1))) break;
           phase ^= 1u << g;
           tmem_fence_after();
           const uint32_t vb = ring + s * S::kTileBytes;
@@ -604,7 +618,7 @@ __global__ void __launch_bounds__(TcShape<PANELS>::kThreads, 1)
         const int tile = at.tile + t;
         const bool tree = tile == at.tiles - 1;
         const int nk = tree ? p.nodes : min(kKeys, len - tile * kKeys);
-        if (!(fine = mbar_wait_short(s_full(g), phase))) break;
+        if (!(fine = warp_wait(s_full(g), phase))) break;
         phase ^= 1u;
         if (tree || nk < kKeys) {
           // the values of keys that no row sees are taken out of the product,
@@ -612,7 +626,7 @@ __global__ void __launch_bounds__(TcShape<PANELS>::kThreads, 1)
           // copy that had the slot before was used ahead of this tile's scores,
           // so the wait cannot take its arrival for this one's.)
           const int kv = k + (GR == 2 && t + 1 < n ? 2 * t + 2 : 2 * t + 1);
-          if (!(fine = mbar_wait_short(full(kv % NS), (kv / NS) & 1))) break;
+          if (!(fine = warp_wait(full(kv % NS), (kv / NS) & 1))) break;
           uint8_t* vs = smem + S::kRing + (kv % NS) * S::kTileBytes;
           for (int r = tree ? L : nk + L; r < (tree ? p.nodes : kKeys); r += kM) {
             bool out = !tree || masks[r] == 0ull;
@@ -700,14 +714,14 @@ __global__ void __launch_bounds__(TcShape<PANELS>::kThreads, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive(p_ready(g));
       }
-      if (!fine || !(fine = mbar_wait_short(o_full, u & 1))) break;
+      fine = fine && warp_wait(o_full, u & 1);
       tmem_fence_after();
       // join the parts of each row: reference point and sum first
       // [GR][kM][CW], 16-byte pieces swizzled; before that the second group's (m, l)
       float4* const buf = reinterpret_cast<float4*>(smem + (PANELS == 1 ? S::kMeet : (u % GR) * S::kTileBytes));
       float2* const ml[2] = {s_ml, reinterpret_cast<float2*>(buf)};
       ml[g][L] = make_float2(m, l);
-      group_sync(1, 128 * GR);
+      if (!(fine = group_all(1, 128 * GR, fine))) break;
       float top = -INFINITY, total = 0.0f;
 #pragma unroll
       for (int i = 0; i < GR * COPIES; ++i) top = fmaxf(top, ml[i % GR][i / GR * (kM / COPIES) + r0].x);
@@ -794,6 +808,25 @@ __global__ void __launch_bounds__(TcShape<PANELS>::kThreads, 1)
   if (warp == 4 * GR + 1) {
     __syncwarp();
     tmem_free(tmem, kTmemCols);
+  }
+}
+
+// Eight warps meet after waits of which one lane's, in warp `starved`, can only
+// run out: seen[w] is 1 where warp w went on and 2 where it left.
+__global__ void group_wait_probe_kernel(int starved, int* __restrict__ seen, unsigned int* __restrict__ faults) {
+  __shared__ alignas(8) uint64_t s_bar[2];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t bars = smem_addr(s_bar);
+  if (threadIdx.x == 0) {
+    mbar_init(bars, 1);
+    mbar_init(bars + 8, 1);
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) mbar_arrive(bars);
+  const bool ok = group_all(1, blockDim.x, warp_wait(bars + (warp == starved && lane == 5 ? 8 : 0), 0));
+  if (lane == 0) {
+    seen[warp] = ok ? 1 : 2;
+    if (!ok) atomicAdd(faults, 1u);
   }
 }
 
@@ -1491,5 +1524,25 @@ extern "C" int ckks_draft_attention(ckks_ctx* ctx, const ckks_draft_attention_ar
       run_attend<__half>(p, st);
     else
       run_attend<float>(p, st);
+  });
+}
+
+extern "C" int ckks_selftest_group_wait(ckks_ctx* ctx, int starved) {
+  return guard([&] {
+    Context& c = context_of(ctx);
+    constexpr int kWarps = 8;
+    int seen[kWarps] = {};
+    OnDevice dev(c);
+    int* d = (int*)c.alloc(sizeof(seen));
+    CKKS_CUDA(cudaMemsetAsync(d, 0, sizeof(seen), c.stream));
+    group_wait_probe_kernel<<<1, 32 * kWarps, 0, c.stream>>>(starved, d, c.d_faults);
+    CKKS_CUDA(cudaGetLastError());
+    CKKS_CUDA(cudaMemcpyAsync(seen, d, sizeof(seen), cudaMemcpyDeviceToHost, c.stream));
+    CKKS_CUDA(cudaStreamSynchronize(c.stream));
+    c.release(d);
+    const unsigned int faults = take_device_faults(c);
+    for (int w = 1; w < kWarps; ++w)
+      if (seen[w] != seen[0]) throw Error(CKKS_ESTATE, "warps that met after a wait did not go on or leave together");
+    if (seen[0] != 1 || faults) throw Error(CKKS_ECUDA, "bounded wait of a group of warps gave up");
   });
 }

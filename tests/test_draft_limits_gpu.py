@@ -39,3 +39,16 @@ def test_attention_list_fits_32_bits(cc, sizes, last, step):
     assert attention_workspace(cc, capacity=last, **sizes) > 0
     assert attention_workspace(cc, capacity=last + 1, **sizes) == 0
     assert attention_workspace(cc, capacity=last + step, **sizes) == 0
+
+
+def test_warps_that_meet_leave_together(cc):
+    """The waits of the attention kernel's softmax warps: one thread whose wait
+    runs out takes all warps out with it (none is left at the barrier where
+    they meet), the fault is reported once and the context stays usable."""
+    lib = eng.lib()
+    assert lib.ckks_selftest_group_wait(cc.h, -1) == 0
+    for starved in (0, 6):
+        assert lib.ckks_selftest_group_wait(cc.h, starved) == 3
+        assert b"gave up" in lib.ckks_last_error()
+    assert lib.ckks_selftest_group_wait(cc.h, -1) == 0
+    cc.Synchronize()
