@@ -470,7 +470,9 @@ typedef struct {
  * decode step.  The row of a node that is padding is 0 and its lse -inf.
  * Rows of the cache behind lens[b] are not used, whatever they hold; an
  * infinite or NaN value that a row sees makes that element of the row
- * infinite or NaN.  16-bit tensors round each softmax weight to their type.
+ * infinite or NaN.  Products and sums are in 32 bits; between the two
+ * products a softmax weight keeps at least 16 bits with bfloat16 tensors, 22
+ * with float16 and 24 with float32 ones.
  * q_heads / kv_heads query heads share each key/value head. */
 int ckks_draft_attention(ckks_ctx* ctx, const ckks_draft_attention_args* args, void* stream);
 /* workspace bytes for these sizes (the pointers are not looked at), or -1 */
