@@ -472,7 +472,8 @@ typedef struct {
  * infinite or NaN value that a row sees makes that element of the row
  * infinite or NaN.  Products and sums are in 32 bits; between the two
  * products a softmax weight keeps at least 16 bits with bfloat16 tensors, 22
- * with float16 and 24 with float32 ones.
+ * with float16 (in steps of 2^-31 of the row's largest at the finest) and 24
+ * with float32 ones.
  * q_heads / kv_heads query heads share each key/value head. */
 int ckks_draft_attention(ckks_ctx* ctx, const ckks_draft_attention_args* args, void* stream);
 /* workspace bytes for these sizes (the pointers are not looked at), or -1 */

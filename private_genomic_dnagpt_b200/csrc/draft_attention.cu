@@ -347,7 +347,7 @@ __device__ __noinline__ void add_spoiled(const AttnParams& p, int b, int h, int 
 // workspace for the second kernel.
 //
 // A row's reference point m follows the maximum only when that has grown by
-// more than 2^8 (the weights then stay below 2^8, far inside 16-bit range):
+// more than 2^8 (the weights then stay below 2^8, 2^15 in float16, which the types hold):
 // O is seldom rescaled.  l sums the weights in 32 bits.  For the second
 // product each weight is two numbers of the operands' type, so that the result
 // is as far from the exact one as its own rounding takes it.  With one number
@@ -365,6 +365,11 @@ __device__ __noinline__ void add_spoiled(const AttnParams& p, int b, int h, int 
 constexpr int kM = 128, kKeys = 128, kTmemCols = 512;
 constexpr uint32_t kPanel = 128 * 128;  // 128 rows x 64 elements
 constexpr float kSlack = 8.0f;
+// float16 weights end at 2^-24, far above the smallest ones beside a heavy key,
+// so their reference point lies 2^7 below the maximum: the largest weight is
+// between 2^7 and 2^15
+template <typename T>
+constexpr float kBelow = std::is_same_v<T, __half> ? 7.0f : 0.0f;
 
 struct TileMaps {
   CUtensorMap q, kc, vc, kn, vn;
@@ -407,7 +412,7 @@ __device__ __forceinline__ float2 sub2(float2 a, float2 b) {
 // Two positive weights as the sum of two pairs of the type: `hi` has their
 // leading bits (cut, so that what is left is exact: one byte permutation in
 // bfloat16), `lo` what is left, rounded: 16 bits of each weight in bfloat16, 22
-// in float16, there in multiples of 2^-24 at the finest.
+// in float16, there in multiples of 2^-24 at the finest (2^-31 of the largest weight).
 template <typename T>
 __device__ __forceinline__ void split2(float2 e, uint32_t& hi, uint32_t& lo) {
   constexpr uint32_t keep = std::is_same_v<T, __nv_bfloat16> ? 0xFFFF0000u : 0xFFFFE000u;
@@ -711,7 +716,7 @@ __global__ void __launch_bounds__(TcShape<PANELS>::kThreads, 1)
 #pragma unroll
         for (int i = 0; i < KQ; ++i) mx4[i & 3] = fmaxf(mx4[i & 3], __uint_as_float(x[i]));
         const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
-        const float top = mx == -INFINITY ? mx : mx * c;
+        const float top = mx == -INFINITY ? mx : fmaf(mx, c, -kBelow<T>);
         float f = 1.0f;
         if (top > m + kSlack || m == -INFINITY) {
           f = m == -INFINITY ? 0.0f : ex2(m - top);
