@@ -77,6 +77,7 @@ __device__ __forceinline__ T* out_row(const AttnParams& p, int b, int node, int 
 // Loads are not overlapped within a CTA (5 float32 rows over 6000 keys took it
 // 87 us, against 39 below).
 constexpr int kRows = 8, kTile = 64, kThreads = 128;
+constexpr uint32_t kUnseen = 0x80000000u;  // -0: the weight of a key that a row does not see (others are +0 and more)
 
 template <typename T>
 __device__ __forceinline__ void load_row4(float* dst, const T* src, int d, int D, bool wide) {
@@ -105,7 +106,7 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(AttnParams p) {
   float* sq = sv + kTile * D4;          // [kRows][D4]
   float* sp = sq + kRows * D4;          // [kTile][kRows]
   __shared__ float s_m[kRows], s_l[kRows], s_c[kRows];
-  __shared__ uint64_t s_mask[kMaxNodes];
+  __shared__ uint64_t s_mask[kMaxNodes], s_row[kRows];  // of the nodes, and of the rows here
   __shared__ int s_jump[kMaxNodes];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int rows = p.nodes * p.group, tiles_r = (rows + kRows - 1) / kRows;
@@ -115,7 +116,10 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(AttnParams p) {
   // this split's keys [k0, k1) of the cached and then the new ones
   const int per = ((total + p.splits - 1) / p.splits + kTile - 1) / kTile * kTile;
   const int k0 = min(total, (int)blockIdx.y * per), k1 = min(total, k0 + per);
-  if (warp == 0) tree_masks(p.parents + (size_t)b * p.nodes, p.nodes, s_mask, s_jump);
+  if (warp == 0) {
+    tree_masks(p.parents + (size_t)b * p.nodes, p.nodes, s_mask, s_jump);
+    if (lane < kRows) s_row[lane] = rt * kRows + lane < rows ? s_mask[(rt * kRows + lane) / p.group] : 0ull;
+  }
   for (int i = tid; i < kRows * (D4 / 4); i += kThreads) {
     const int r = i / (D4 / 4), d = i % (D4 / 4) * 4, row = rt * kRows + r;
     float x[4] = {0.f, 0.f, 0.f, 0.f};
@@ -197,8 +201,9 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(AttnParams p) {
       float sum = ea + ec;
 #pragma unroll
       for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      sp[lane * kRows + r] = ea;
-      sp[(lane + 32) * kRows + r] = ec;
+      auto sees = [&](int at) { return at < len || (at < k1 && (s_row[r] >> (at - len) & 1)); };
+      sp[lane * kRows + r] = sees(t0 + lane) ? ea : __uint_as_float(kUnseen);
+      sp[(lane + 32) * kRows + r] = sees(t0 + lane + 32) ? ec : __uint_as_float(kUnseen);
       if (lane == 0) {
         s_m[r] = m;
         s_l[r] = s_l[r] * f + sum;
@@ -225,9 +230,9 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(AttnParams p) {
         const float4 v4 = *reinterpret_cast<const float4*>(sv + k * D4 + d);
 #pragma unroll
         for (int r = 0; r < kRows; ++r) {
-          // a weight of 0 adds nothing, whatever a value that other rows see holds
+          // a new key's values, whatever they hold, reach the rows that see it only
           const float x = w[r];
-          if (x != 0.0f) {
+          if (__float_as_uint(x) != kUnseen) {
             acc[c][r][0] = fmaf(x, v4.x, acc[c][r][0]);
             acc[c][r][1] = fmaf(x, v4.y, acc[c][r][1]);
             acc[c][r][2] = fmaf(x, v4.z, acc[c][r][2]);
@@ -301,7 +306,7 @@ __global__ void __launch_bounds__(kThreads) join_kernel(AttnParams p) {
 
 // Adds to one finished row the new keys whose values are not finite, which
 // the product left out so that they do not reach the rows that may not see
-// them: what they add is infinite or no number, unless their weight is 0.
+// them: what those elements add is infinite or no number, whatever the weight.
 template <typename T>
 __device__ __noinline__ void add_spoiled(const AttnParams& p, int b, int h, int node, int qh, unsigned long long which,
                                          float m, float inv, T* out) {
@@ -313,7 +318,6 @@ __device__ __noinline__ void add_spoiled(const AttnParams& p, int b, int h, int 
     float s = 0.0f;
     for (int d = 0; d < p.head_dim; ++d) s = fmaf(to_f32(q[d]), to_f32(k[d]), s);
     const float w = exp2f(s * (p.scale * kLog2e) - m) * inv;
-    if (w == 0.0f) continue;
     for (int d = 0; d < p.head_dim; ++d) out[d] = from_f32<T>(fmaf(w, to_f32(v[d]), to_f32(out[d])));
   }
 }
@@ -784,6 +788,7 @@ __global__ void __launch_bounds__(TcShape<PANELS>::kThreads, 1)
         total = fmaf(e.y, ex2(e.x - ref), total);
       }
       const float f = ex2(m - ref);
+      const bool some = g < n;  // a group without a tile has no sums
       const bool whole = at.tile == 0 && n == at.tiles, seen = mask != 0ull;  // a padding node's row is empty
       const float inv = total != 0.0f && seen ? 1.0f / total : 0.0f;
       const unsigned long long spoiled = *s_spoiled;
@@ -802,10 +807,10 @@ __global__ void __launch_bounds__(TcShape<PANELS>::kThreads, 1)
 #pragma unroll
         for (int j = 0; j < CW / 4; ++j) {
           float4 e;
-          e.x = f == 0.0f ? 0.0f : __uint_as_float(o[4 * j]) * f;
-          e.y = f == 0.0f ? 0.0f : __uint_as_float(o[4 * j + 1]) * f;
-          e.z = f == 0.0f ? 0.0f : __uint_as_float(o[4 * j + 2]) * f;
-          e.w = f == 0.0f ? 0.0f : __uint_as_float(o[4 * j + 3]) * f;
+          e.x = some ? __uint_as_float(o[4 * j]) * f : 0.0f;
+          e.y = some ? __uint_as_float(o[4 * j + 1]) * f : 0.0f;
+          e.z = some ? __uint_as_float(o[4 * j + 2]) * f : 0.0f;
+          e.w = some ? __uint_as_float(o[4 * j + 3]) * f : 0.0f;
           buf[place(g, L, j)] = e;
         }
         group_sync(1, 128 * GR);
@@ -1013,7 +1018,7 @@ struct F32Shape {
   static constexpr int KT = DC == 1 ? 64 : DC == 2 ? 32 : 16, DP = 64 * DC;
   static constexpr int KS = DP + 4;                  // stride of K's rows: reads without conflicts
   static constexpr int kStage = KT * KS + KT * DP;  // floats
-  static constexpr size_t kSmem = sizeof(float) * (2 * kStage + RT * DP + KT * RT + 3 * RT) + kMaxNodes * 12;
+  static constexpr size_t kSmem = sizeof(float) * (2 * kStage + RT * DP + KT * RT + 3 * RT) + kMaxNodes * 12 + RT * 8;
   static_assert(sizeof(float) * 8 * RT * 64 <= sizeof(float) * 2 * kStage, "a unit's sums meet in the stages");
 };
 
@@ -1028,7 +1033,8 @@ __global__ void __launch_bounds__(kThreads, DC == 1 ? 3 : 2) attend_f32_kernel(c
   float* const s_l = s_m + RT;
   float* const s_c = s_l + RT;
   uint64_t* const s_mask = reinterpret_cast<uint64_t*>(s_c + RT);
-  int* const s_jump = reinterpret_cast<int*>(s_mask + kMaxNodes);
+  uint64_t* const s_row = s_mask + kMaxNodes;  // the masks of a unit's rows
+  int* const s_jump = reinterpret_cast<int*>(s_row + RT);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int rows = p.nodes * p.group, tiles_r = (rows + RT - 1) / RT, units = p.kv_heads * tiles_r, D = p.head_dim;
   asm volatile("griddepcontrol.launch_dependents;");
@@ -1093,6 +1099,7 @@ __global__ void __launch_bounds__(kThreads, DC == 1 ? 3 : 2) attend_f32_kernel(c
     masks_of = b;
     if (tid < RT) s_m[tid] = -INFINITY, s_l[tid] = 0.0f;
     __syncthreads();
+    if (tid < RT) s_row[tid] = row0 + tid < rows ? s_mask[(row0 + tid) / p.group] : 0ull;  // used behind a barrier
     load(0, 0);
     for (int i = tid; i < RT * (DP / 4); i += kThreads) {
       const int r = i / (DP / 4), d = i % (DP / 4) * 4, row = row0 + r;
@@ -1138,8 +1145,7 @@ __global__ void __launch_bounds__(kThreads, DC == 1 ? 3 : 2) attend_f32_kernel(c
         if (t0 + KT > len) {
 #pragma unroll
           for (int r = 0; r < RPT; ++r) {
-            const int row = row0 + RPT * rg + r;
-            const uint64_t m = row < rows ? s_mask[row / p.group] : 0ull;
+            const uint64_t m = s_row[RPT * rg + r];
             if (!(key < nk && m && (s < len || (m >> (s - len) & 1)))) x[r] = -INFINITY;
           }
         }
@@ -1165,8 +1171,10 @@ __global__ void __launch_bounds__(kThreads, DC == 1 ? 3 : 2) attend_f32_kernel(c
         float sum = 0.0f;
 #pragma unroll
         for (int i = 0; i < KL; ++i) {
+          const int at = t0 + lane + 32 * i;
           x[i] = exp2f(x[i] - base);
           sum += x[i];
+          if (at >= len && !(at < total && (s_row[r] >> (at - len) & 1))) x[i] = __uint_as_float(kUnseen);
           if (lane + 32 * i < KT) sp[(lane + 32 * i) * RT + r] = x[i];
         }
 #pragma unroll
@@ -1205,7 +1213,7 @@ __global__ void __launch_bounds__(kThreads, DC == 1 ? 3 : 2) attend_f32_kernel(c
             const float4 v4 = *reinterpret_cast<const float4*>(sv + k * DP + c * 64 + dg * 4);
 #pragma unroll
             for (int r = 0; r < RT; ++r)
-              if (!decltype(apart)::value || x[r] != 0.0f) {
+              if (!decltype(apart)::value || __float_as_uint(x[r]) != kUnseen) {
                 acc[c][r][0] = fmaf(x[r], v4.x, acc[c][r][0]);
                 acc[c][r][1] = fmaf(x[r], v4.y, acc[c][r][1]);
                 acc[c][r][2] = fmaf(x[r], v4.z, acc[c][r][2]);
@@ -1214,7 +1222,7 @@ __global__ void __launch_bounds__(kThreads, DC == 1 ? 3 : 2) attend_f32_kernel(c
           }
         }
       };
-      // among new keys a weight of 0 adds nothing, whatever a value that other rows see holds
+      // a new key's values, whatever they hold, reach the rows that see it only
       if (t0 + KT > len)
         values(std::true_type{});
       else
