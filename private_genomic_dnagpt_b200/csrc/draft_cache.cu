@@ -139,7 +139,9 @@ __global__ void __launch_bounds__(kAccKeys) accumulate_kernel(AccParams p) {
 // over 4001 keys of 64, eight sequences, 10.9 us, where the chain of reads
 // (lengths, accepted nodes, their rows) shows.
 // float32 rows are split in two tensor-float parts, x = hi + lo, and
-// multiplied as hi hi + hi lo + lo hi: products to 2^-21.
+// multiplied as hi hi + hi lo + lo hi: products to 2^-21.  What is infinite or
+// no number has no such parts: a score that is not finite is computed anew by
+// `score_of`.
 template <typename T>
 struct Pieces {
   // products of one pair of pieces (keys g and g + 8) with one q piece
@@ -189,6 +191,14 @@ struct Pieces<float> {
     both(c, a.z, b.z, a.w, b.w, q.z, q.w);
   }
 };
+
+// q . k in the order of the elements
+template <typename T>
+__device__ __noinline__ float score_of(const T* q, const T* k, int D) {
+  float s = 0.0f;
+  for (int d = 0; d < D; ++d) s = fmaf(to_f32(q[d]), to_f32(k[d]), s);
+  return s;
+}
 
 constexpr int kStreamWarps = 8, kStreamRows = 64;  // warps of a CTA; q rows in shared memory at once
 
@@ -340,9 +350,19 @@ __global__ void __launch_bounds__(32 * kStreamWarps, stream_ctas(JC)) accumulate
           const int2 last = *reinterpret_cast<const int2*>(s_last + row);
 #pragma unroll
           for (int u = 0; u < U; ++u) {
+            const int s = k0 + 16 * u + g;
+            if constexpr (std::is_same_v<T, float>) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const int key = s + (e < 2 ? 0 : 8), r = r0 + row + (e & 1);
+                if (!(fabsf(c[u][e]) < INFINITY) && key <= (e & 1 ? last.y : last.x))
+                  c[u][e] = score_of(static_cast<const T*>(p.q.data) + b * p.q.batch +
+                                         (h * p.group + r % p.group) * p.q.head + path[r / p.group] * p.q.row,
+                                     kc + key * p.kc.row, D);
+              }
+            }
             float e[4] = {ex2(fmaf(c[u][0], c2, -l.x)), ex2(fmaf(c[u][1], c2, -l.y)), ex2(fmaf(c[u][2], c2, -l.x)),
                           ex2(fmaf(c[u][3], c2, -l.y))};
-            const int s = k0 + 16 * u + g;
             e[0] = s <= last.x ? e[0] : 0.0f;
             e[1] = s <= last.y ? e[1] : 0.0f;
             e[2] = s + 8 <= last.x ? e[2] : 0.0f;
