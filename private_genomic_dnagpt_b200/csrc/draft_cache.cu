@@ -138,12 +138,22 @@ __global__ void __launch_bounds__(kAccKeys) accumulate_kernel(AccParams p) {
 // 16 accepted rows over 65536 keys of 128 take 44.3 us, 86 % of the copy rate; 4
 // over 4001 keys of 64, eight sequences, 10.9 us, where the chain of reads
 // (lengths, accepted nodes, their rows) shows.
-// float32 rows are split in two tensor-float parts, x = hi + lo, and
-// multiplied as hi hi + hi lo + lo hi: products to 2^-21.  What is infinite or
-// no number has no such parts: a score that is not finite is computed anew by
-// `score_of`.
+// A float32 element is three bfloat16 numbers of 8 bits each (cut, so their sum
+// is the element), and a product of two elements eight of the nine products of
+// these, to 2^-30 of it; sums are in 32 bits, the smaller products' apart from
+// the largest ones'.  What is infinite or no number has no such parts: a score
+// that is not finite is computed anew by `score_of`.
+// (Two tensor-float parts and three products, to 2^-22, took 118 us where this
+// takes 84: 16 rows over 30000 keys of 128, two sequences of 8 heads.)
 template <typename T>
 struct Pieces {
+  struct Sums {
+    float c[4];
+    __device__ __forceinline__ float total(int e) const { return c[e]; }
+  };
+  __device__ __forceinline__ static void mac(Sums& s, const uint4& a, const uint4& b, const uint4& q) {
+    mac(s.c, a, b, q);
+  }
   // products of one pair of pieces (keys g and g + 8) with one q piece
   __device__ __forceinline__ static void mac(float* c, const uint4& a, const uint4& b, const uint4& q) {
     step(c, a.x, b.x, a.y, b.y, q.x, q.y);
@@ -164,31 +174,41 @@ struct Pieces {
 
 template <>
 struct Pieces<float> {
-  __device__ __forceinline__ static uint32_t hi(uint32_t x) {
-    uint32_t y;
-    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(y) : "f"(__uint_as_float(x)));
-    return y;
-  }
-  // of an infinity nothing is left
-  __device__ __forceinline__ static uint32_t lo(uint32_t x) {
-    const float h = __uint_as_float(hi(x));
-    return fabsf(h) == INFINITY ? 0u : hi(__float_as_uint(__uint_as_float(x) - h));
-  }
-  __device__ __forceinline__ static void step(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                              uint32_t b1) {
-    asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-  }
-  __device__ __forceinline__ static void both(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                              uint32_t b1) {
-    step(c, lo(a0), lo(a1), lo(a2), lo(a3), hi(b0), hi(b1));
-    step(c, hi(a0), hi(a1), hi(a2), hi(a3), lo(b0), lo(b1));
-    step(c, hi(a0), hi(a1), hi(a2), hi(a3), hi(b0), hi(b1));
-  }
-  __device__ __forceinline__ static void mac(float* c, const uint4& a, const uint4& b, const uint4& q) {
-    both(c, a.x, b.x, a.y, b.y, q.x, q.y);
-    both(c, a.z, b.z, a.w, b.w, q.z, q.w);
+  struct Sums {
+    float c[4], rest[4];
+    __device__ __forceinline__ float total(int e) const { return c[e] + rest[e]; }
+  };
+  // four elements as pairs of their parts
+  struct Parts {
+    uint32_t p[3][2];
+    __device__ __forceinline__ static uint32_t upper(float x) { return __float_as_uint(x) & 0xFFFF0000u; }
+    __device__ __forceinline__ explicit Parts(const uint4& v) {
+      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        float x = __uint_as_float(w[2 * k]), y = __uint_as_float(w[2 * k + 1]);
+#pragma unroll
+        for (int i = 0; i < 3; ++i) {
+          p[i][k] = __byte_perm(__float_as_uint(x), __float_as_uint(y), 0x7632);
+          x -= __uint_as_float(upper(x));
+          y -= __uint_as_float(upper(y));
+        }
+      }
+    }
+  };
+  __device__ __forceinline__ static void mac(Sums& s, const uint4& a, const uint4& b, const uint4& q) {
+    const Parts x(a), y(b), z(q);
+    auto step = [&](float* c, int i, int j) {
+      Pieces<__nv_bfloat16>::step(c, x.p[i][0], y.p[i][0], x.p[i][1], y.p[i][1], z.p[j][0], z.p[j][1]);
+    };
+    step(s.rest, 1, 2);
+    step(s.rest, 2, 1);
+    step(s.rest, 0, 2);
+    step(s.rest, 2, 0);
+    step(s.rest, 1, 1);
+    step(s.rest, 0, 1);
+    step(s.rest, 1, 0);
+    step(s.c, 0, 0);
   }
 };
 
@@ -334,16 +354,12 @@ __global__ void __launch_bounds__(32 * kStreamWarps, stream_ctas(JC)) accumulate
           for (int half = 0; half < 2; ++half) old[u][half] = soon[u][half], sum[u][half] = 0.0f;
         weights(i + 1);
         for (int gr = 0; gr < groups; ++gr) {
-          float c[U][4];
-#pragma unroll
-          for (int u = 0; u < U; ++u)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) c[u][e] = 0.0f;
+          typename Pieces<T>::Sums sums[U] = {};
 #pragma unroll
           for (int j = 0; j < JC; ++j) {
             const uint4 q = s_q[(gr * JC + j) * 32 + lane];
 #pragma unroll
-            for (int u = 0; u < U; ++u) Pieces<T>::mac(c[u], a[u][0][j], a[u][1][j], q);
+            for (int u = 0; u < U; ++u) Pieces<T>::mac(sums[u], a[u][0][j], a[u][1][j], q);
           }
           const int row = gr * 8 + 2 * t;  // the lane's two rows
           const float2 l = *reinterpret_cast<const float2*>(s_lse + row);
@@ -351,18 +367,20 @@ __global__ void __launch_bounds__(32 * kStreamWarps, stream_ctas(JC)) accumulate
 #pragma unroll
           for (int u = 0; u < U; ++u) {
             const int s = k0 + 16 * u + g;
-            if constexpr (std::is_same_v<T, float>) {
+            float c[4];
 #pragma unroll
-              for (int e = 0; e < 4; ++e) {
+            for (int e = 0; e < 4; ++e) {
+              c[e] = sums[u].total(e);
+              if constexpr (std::is_same_v<T, float>) {
                 const int key = s + (e < 2 ? 0 : 8), r = r0 + row + (e & 1);
-                if (!(fabsf(c[u][e]) < INFINITY) && key <= (e & 1 ? last.y : last.x))
-                  c[u][e] = score_of(static_cast<const T*>(p.q.data) + b * p.q.batch +
-                                         (h * p.group + r % p.group) * p.q.head + path[r / p.group] * p.q.row,
-                                     kc + key * p.kc.row, D);
+                if (!(fabsf(c[e]) < INFINITY) && key <= (e & 1 ? last.y : last.x))
+                  c[e] = score_of(static_cast<const T*>(p.q.data) + b * p.q.batch +
+                                      (h * p.group + r % p.group) * p.q.head + path[r / p.group] * p.q.row,
+                                  kc + key * p.kc.row, D);
               }
             }
-            float e[4] = {ex2(fmaf(c[u][0], c2, -l.x)), ex2(fmaf(c[u][1], c2, -l.y)), ex2(fmaf(c[u][2], c2, -l.x)),
-                          ex2(fmaf(c[u][3], c2, -l.y))};
+            float e[4] = {ex2(fmaf(c[0], c2, -l.x)), ex2(fmaf(c[1], c2, -l.y)), ex2(fmaf(c[2], c2, -l.x)),
+                          ex2(fmaf(c[3], c2, -l.y))};
             e[0] = s <= last.x ? e[0] : 0.0f;
             e[1] = s <= last.y ? e[1] : 0.0f;
             e[2] = s + 8 <= last.x ? e[2] : 0.0f;

@@ -11,7 +11,7 @@ pytestmark = pytest.mark.gpu
 
 import private_genomic_dnagpt_b200 as eng  # noqa: E402
 
-from test_draft_gpu import HALF, f64, inputs, tree  # noqa: E402
+from test_draft_gpu import HALF, f64, i32, inputs, tree  # noqa: E402
 
 
 @pytest.fixture(scope="module")
@@ -76,3 +76,22 @@ def test_attention_beside_a_heavy_key(cc, D, nodes, ahead):
     room += 2.0 ** -31 * values[:, None] + 2.0 ** -25
     assert (np.abs(f64(out) - want) / room).max() <= 1.0
     assert (np.abs(f64(lse) - wlse) <= 0.5 * noise + 2.0 ** -22 * (1 + np.abs(wlse))).all()
+
+
+@pytest.mark.parametrize("D", [4, 8, 16])
+def test_float32_weights_take_whole_products(cc, D):
+    """Every element is 1 + 2^-11 - 2^-22 times a power of two, whose square
+    lies 2^-22 of itself above what elements cut to twice 11 bits give without
+    the product of their second parts.  With scale 1 the score S is off by two
+    roundings of 2^-24 and the log-sum times log2(e) by one, ex2 by 2^-21 of
+    the weight: the weight is off by 3 2^-24 S + 2^-21 of itself."""
+    x = inputs(torch.float32, 1, 1, 1, 1, D, 200, [190], [[-1]], seed=32)
+    v = 1 + 2.0 ** -11 - 2.0 ** -22
+    x["q"].fill_(v * 1024 / D)
+    x["k_cache"].fill_(v)
+    S = D * float(x["q"][0, 0, 0, 0]) * float(x["k_cache"][0, 0, 0, 0])
+    lse = torch.full((1, 1, 1), S, device="cuda")
+    want = np.exp(S - float(lse[0, 0, 0]))
+    got = f64(cc.draft_accumulate(x["q"], lse, x["k_cache"], x["lens"], i32([[0]]), i32([1]),
+                                  torch.zeros(1, 1, 200, device="cuda"), 1.0))[0, 0, :191]
+    assert np.abs(got - want).max() <= (3 * 2.0 ** -24 * S + 2.0 ** -21) * want
