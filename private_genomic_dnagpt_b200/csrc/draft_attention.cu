@@ -1280,7 +1280,9 @@ template <typename T, int DC>
 void launch_attend(const AttnParams& p, cudaStream_t st) {
   const size_t smem = attend_smem(p.head_dim);
   auto* k = attend_kernel<T, DC>;
-  CKKS_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  // the most that any call asks for: calls of other sizes from other threads
+  // may come between this and the launch
+  CKKS_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)attend_smem(64 * DC)));
   const int rows = p.nodes * p.group;
   const dim3 grid((unsigned)(p.batch * p.kv_heads * ((rows + kRows - 1) / kRows)), p.splits);
   k<<<grid, kThreads, smem, st>>>(p);

@@ -665,9 +665,12 @@ void launch_stream(const Context& c, const AccParams& p, cudaStream_t st) {
   const dim3 grid = by_head ? dim3((unsigned)heads, (unsigned)((steps + each - 1) / each))
                             : dim3((unsigned)std::min(entries, ctas));
   const size_t smem = stream_ring_bytes(JC) + (size_t)(std::min(kStreamRows, p.nodes * p.group) + 7) / 8 * JC * 512;
-  static_assert(stream_ctas(JC) * (stream_ring_bytes(JC) + kStreamRows / 8 * JC * 512 + 2048) <= 228 << 10, "fits an SM");
+  constexpr size_t most = stream_ring_bytes(JC) + kStreamRows / 8 * JC * 512;
+  static_assert(stream_ctas(JC) * (most + 2048) <= 228 << 10, "fits an SM");
   auto* k = accumulate_stream_kernel<T, JC>;
-  CKKS_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  // the most that any call asks for: calls of other sizes from other threads
+  // may come between this and the launch
+  CKKS_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most));
   k<<<grid, 32 * kStreamWarps, smem, st>>>(p, by_head ? each : 0);
   CKKS_CUDA(cudaGetLastError());
 }

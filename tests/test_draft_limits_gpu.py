@@ -2,6 +2,7 @@
 and waits that run out."""
 
 import ctypes
+import threading
 
 import pytest
 
@@ -10,7 +11,7 @@ pytestmark = pytest.mark.gpu
 
 import private_genomic_dnagpt_b200 as eng  # noqa: E402
 
-from test_draft_gpu import AttentionArgs  # noqa: E402
+from test_draft_gpu import AttentionArgs, Rows  # noqa: E402
 
 
 @pytest.fixture(scope="module")
@@ -52,3 +53,45 @@ def test_warps_that_meet_leave_together(cc):
         assert b"gave up" in lib.ckks_last_error()
     assert lib.ckks_selftest_group_wait(cc.h, -1) == 0
     cc.Synchronize()
+
+
+class AccumulateArgs(ctypes.Structure):
+    """ckks_draft_accumulate_args of include/ckks_b200.h."""
+    _fields_ = ([(n, ctypes.c_int32) for n in ("dtype", "batch", "q_heads", "kv_heads", "head_dim", "nodes", "capacity",
+                                               "reserved")] + [("scale", ctypes.c_double)]
+                + [(n, Rows) for n in ("q", "k_cache", "acc")]
+                + [(n, ctypes.c_void_p) for n in ("lse", "lens", "path", "count")])
+
+
+def test_contexts_of_two_threads_share_no_launch_setting():
+    """Two host threads, each with a context and a stream of its own, whose
+    calls of one kernel take different amounts of shared memory."""
+    lib, calls = eng.lib(), 2000
+    buf = torch.zeros(1 << 20, device="cuda")  # lengths, counts and parents of 0 among them
+    outs = [torch.zeros(1 << 20, device="cuda") for _ in range(2)]
+    failed = []
+
+    def work(i):
+        cc = eng.GenCryptoContext(eng.CCParams(ring_dim_log=10, limbs=3, dnum=1, seed=3))
+        stream, at, out = torch.cuda.Stream(), buf.data_ptr(), outs[i].data_ptr()
+        group, D = (64, 63) if i else (1, 33)
+        acc = AccumulateArgs(dtype=0, batch=1, q_heads=group, kv_heads=1, head_dim=64, nodes=1, capacity=64, scale=1.0,
+                             q=Rows(at, 1 << 14, 64, 64), k_cache=Rows(at, 4096, 4096, 64), acc=Rows(out, 64, 64, 0),
+                             lse=at, lens=at, path=at, count=at)
+        att = AttentionArgs(dtype=2, batch=1, q_heads=1, kv_heads=1, head_dim=D, nodes=1, capacity=1, scale=1.0,
+                            lens=at, parents=at, lse=out, **{n: Rows(at, 64, 64, 64) for n in
+                                                            ("q", "k_cache", "v_cache", "k_new", "v_new")},
+                            out=Rows(out + 4096, 64, 64, 64))
+        for _ in range(calls):
+            for call, a in ((lib.ckks_draft_accumulate, acc), (lib.ckks_draft_attention, att)):
+                if call(cc.h, ctypes.byref(a), stream.cuda_stream):
+                    failed.append(lib.ckks_last_error())
+                    return
+        stream.synchronize()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed, failed
