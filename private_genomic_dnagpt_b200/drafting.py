@@ -117,8 +117,10 @@ class DraftModel:
 
     ``forward`` evaluates a tree of drafted nodes behind the cached tokens,
     ``accept`` appends the nodes that the target confirmed, ``prefill`` takes
-    a prompt.  With ``budget``, the cache is cut to its ``recent`` latest and
-    its heaviest keys before it would overflow."""
+    a prompt.  With ``budget``, a tree that would not fit behind the longest
+    sequence's rows has every sequence cut to its ``recent`` latest and its
+    heaviest keys first.  Where it might not fit, ``forward`` reads the lengths
+    back (it waits for the GPU then)."""
 
     def __init__(self, cc, block_weights: list, capacity: int, batch: int = 1, heads: int = 12, dtype=None,
                  budget: int | None = None, recent: int = 0):
@@ -191,13 +193,14 @@ class DraftModel:
         return torch.cat(got, 1)
 
     def _make_room(self, n):
-        """Before n more rows: the cache cut to its budget, or, without one,
-        the rows counted exactly."""
-        if self.budget is None:
-            self._most = int(self.lens.max())
-            if self._most + n > self.capacity:
-                raise ValueError(f"{self._most} cached rows and {n} nodes exceed the capacity of {self.capacity}")
+        """Before n more rows than `_most` leaves room for: the rows counted
+        exactly (`accept` only knows how many there are at most) and, where
+        they would not fit, the cache cut to its budget."""
+        self._most = int(self.lens.max())
+        if self._most + n <= self.capacity:
             return
+        if self.budget is None:
+            raise ValueError(f"{self._most} cached rows and {n} nodes exceed the capacity of {self.capacity}")
         lens = self.lens
         for i, (k, v, acc) in enumerate(self.caches):
             _, _, _, _, self.lens = evict(self.cc, k, v, acc, lens, self.budget, self.recent, out=self._spare[i])
