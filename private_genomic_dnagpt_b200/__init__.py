@@ -998,9 +998,9 @@ class EncryptedModel:
         forward: row first + i is the hidden state of node i behind the tokens
         before the tree and its ancestors."""
         if len(parents):
-            for b in self.blocks:
-                b.set_drafts(parents, first)
             try:
+                for b in self.blocks:
+                    b.set_drafts(parents, first)
                 return self.forward(x)
             finally:
                 for b in self.blocks:

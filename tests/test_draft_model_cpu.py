@@ -8,6 +8,7 @@ import pytest
 
 torch = pytest.importorskip("torch")
 
+import private_genomic_dnagpt_b200 as eng  # noqa: E402
 from private_genomic_dnagpt_b200 import drafting  # noqa: E402
 
 
@@ -77,3 +78,21 @@ def test_draft_model_without_a_budget_refuses(operators):
         step(m, 20, [1])
     with pytest.raises(ValueError, match="74 cached rows and 27 nodes"):
         step(m, 27, [1])
+
+
+def test_a_refused_tree_leaves_no_block_with_drafts():
+    """The second block refuses the tree: the first one is causal again."""
+    class Block:
+        def __init__(self, refuses):
+            self.refuses, self.tree = refuses, ()
+
+        def set_drafts(self, parents=(), first=None):
+            if self.refuses and len(parents):
+                raise eng.CKKSError(2, "the block's context was destroyed")
+            self.tree = tuple(parents)
+
+    model = eng.EncryptedModel.__new__(eng.EncryptedModel)
+    model.blocks = [Block(False), Block(True)]
+    with pytest.raises(eng.CKKSError):
+        model.forward(np.zeros((4, 8)), [-1, 0])
+    assert model.blocks[0].tree == ()
