@@ -48,6 +48,12 @@ int cache_type(const Tensor& t, const char* name) {
   return code;
 }
 
+// a size in an argument struct
+int32_t size32(int64_t n, const char* what) {
+  TORCH_CHECK_VALUE(n <= INT32_MAX, what, ": ", n, " is more than the entry points take");
+  return (int32_t)n;
+}
+
 void four(const Tensor& t, const char* name) { TORCH_CHECK_VALUE(t.dim() == 4, name, ": expected four dimensions"); }
 
 void check(const Call& c, const Tensor& t, const char* name, at::IntArrayRef shape, at::ScalarType type) {
@@ -115,8 +121,9 @@ std::tuple<Tensor, Tensor> attention(uintptr_t ctx, int device, const Tensor& q,
   a.parents = small<const int32_t>(c, parents, "parents", {b, n}, at::kInt);
   Tensor out = at::empty({b, n, hq, d}, q.options()), lse = at::empty({b, n, hq}, q.options().dtype(at::kFloat));
   if (b == 0) return {out, lse};
-  a.dtype = code, a.batch = b, a.q_heads = hq, a.kv_heads = hk, a.head_dim = d, a.nodes = n, a.capacity = cap;
-  a.scale = scale_of(scale, d);
+  a.dtype = code, a.batch = size32(b, "batch"), a.q_heads = size32(hq, "query heads");
+  a.kv_heads = size32(hk, "key/value heads"), a.head_dim = size32(d, "head size"), a.nodes = size32(n, "nodes");
+  a.capacity = size32(cap, "capacity"), a.scale = scale_of(scale, d);
   a.q = by_node(q), a.k_cache = by_head(k_cache), a.v_cache = by_head(v_cache);
   a.k_new = by_node(k_new), a.v_new = by_node(v_new), a.out = by_node(out);
   a.lse = lse.data_ptr<float>();
@@ -145,7 +152,7 @@ std::tuple<Tensor, Tensor, Tensor> verify(uintptr_t ctx, int device, const Tenso
   Tensor path = at::empty({b, n}, tokens.options()), count = at::empty({b}, tokens.options()),
          token = at::empty({b}, tokens.options());
   if (b) {
-    a.batch = b, a.nodes = n, a.vocab = v;
+    a.batch = size32(b, "batch"), a.nodes = size32(n, "nodes"), a.vocab = size32(v, "vocabulary");
     a.path = path.data_ptr<int32_t>(), a.count = count.data_ptr<int32_t>(), a.token = token.data_ptr<int32_t>();
     c.done(ckks_draft_verify(c.ctx, &a, c.stream()));
   }
@@ -172,7 +179,8 @@ Tensor commit(uintptr_t ctx, int device, const Tensor& k_cache, const Tensor& v_
   a.count = small<const int32_t>(c, count, "count", {b}, at::kInt);
   Tensor out = at::empty({b}, lens.options());
   if (b) {
-    a.batch = b, a.kv_heads = hk, a.head_dim = d, a.nodes = n, a.capacity = cap;
+    a.batch = size32(b, "batch"), a.kv_heads = size32(hk, "key/value heads"), a.head_dim = size32(d, "head size");
+    a.nodes = size32(n, "nodes"), a.capacity = size32(cap, "capacity");
     a.k_cache = by_head(k_cache), a.v_cache = by_head(v_cache), a.k_new = by_node(k_new), a.v_new = by_node(v_new);
     a.lens_out = out.data_ptr<int32_t>();
     c.done(ckks_draft_commit(c.ctx, &a, c.stream()));
@@ -197,7 +205,8 @@ Tensor accumulate(uintptr_t ctx, int device, const Tensor& q, const Tensor& lse,
   check_rows(c, acc, "acc", {b, hk, cap}, at::kFloat);
   check_written(acc, "acc");
   if (b && cap) {
-    a.batch = b, a.q_heads = hq, a.kv_heads = hk, a.head_dim = d, a.nodes = n, a.capacity = cap;
+    a.batch = size32(b, "batch"), a.q_heads = size32(hq, "query heads"), a.kv_heads = size32(hk, "key/value heads");
+    a.head_dim = size32(d, "head size"), a.nodes = size32(n, "nodes"), a.capacity = size32(cap, "capacity");
     a.scale = scale_of(scale, d);
     a.q = by_node(q), a.k_cache = by_head(k_cache), a.acc = by_head(acc);
     c.done(ckks_draft_accumulate(c.ctx, &a, c.stream()));
@@ -235,8 +244,8 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> evict(uintptr_t ctx, int devi
   for (const Tensor* x : {&k2, &v2, &a2}) check_written(*x, "out");
   Tensor index = at::empty({b, hk, budget}, lens.options()), lens_out = at::empty({b}, lens.options());
   if (b) {
-    a.batch = b, a.kv_heads = hk, a.head_dim = d, a.capacity = cap;
-    a.out_capacity = rows, a.budget = budget, a.recent = recent;
+    a.batch = size32(b, "batch"), a.kv_heads = size32(hk, "key/value heads"), a.head_dim = size32(d, "head size");
+    a.capacity = size32(cap, "capacity"), a.out_capacity = size32(rows, "out"), a.budget = budget, a.recent = recent;
     a.k_cache = by_head(k_cache), a.v_cache = by_head(v_cache), a.acc = by_head(acc);
     a.k_out = by_head(k2), a.v_out = by_head(v2), a.acc_out = by_head(a2);
     a.index = index.data_ptr<int32_t>(), a.lens_out = lens_out.data_ptr<int32_t>();
