@@ -23,6 +23,7 @@ struct Call {
   ckks_ctx* ctx;
   int device;
   bool grad = at::GradMode::is_enabled();
+  bool forward_grad = c10::AutogradState::get_tls_state().get_fw_grad_mode();
   void* stream() const { return device < 0 ? nullptr : (void*)c10::cuda::getCurrentCUDAStream(device).stream(); }
   void done(int rc) const {
     if (rc == CKKS_OK) return;
@@ -63,6 +64,8 @@ void check(const Call& c, const Tensor& t, const char* name, at::IntArrayRef sha
                     ": expected a tensor of the context's device, cuda:", c.device, ", got ", t.device());
   TORCH_CHECK_VALUE(!(c.grad && t.requires_grad()), name,
                     ": requires a gradient, which this operator does not have (call it under torch.no_grad)");
+  TORCH_CHECK_VALUE(!(c.forward_grad && t._fw_grad(/*level=*/0).defined()), name,
+                    ": carries a forward-mode gradient, which this operator does not have");
 }
 
 // a tensor of rows: any strides, the last dimension contiguous

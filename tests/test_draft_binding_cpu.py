@@ -19,3 +19,17 @@ def test_sizes_past_32_bits(cc):  # noqa: F811
         a[name] = a[name][:, :, :1].expand(2, 2, 2 ** 32 + 10, 8)
     with pytest.raises(ValueError, match="capacity: 4294967306"):
         drafting.attention(cc, **a)
+
+
+@pytest.mark.parametrize("op", OPS)
+def test_forward_mode_gradients_are_refused(cc, op):  # noqa: F811
+    """A tangent would be dropped without a word, also under no_grad."""
+    import torch.autograd.forward_ad as fwd
+    for name, t in args(op).items():
+        if isinstance(t, torch.Tensor) and t.is_floating_point():
+            with fwd.dual_level(), torch.no_grad():
+                a = args(op) | {name: fwd.make_dual(t, torch.ones_like(t))}
+                with pytest.raises(ValueError, match="forward-mode"):
+                    getattr(drafting, op)(cc, **a)
+                with fwd._set_fwd_grad_enabled(False), Reached():
+                    getattr(drafting, op)(cc, **a)
