@@ -66,6 +66,7 @@ void check(const Call& c, const Tensor& t, const char* name, at::IntArrayRef sha
                     ": requires a gradient, which this operator does not have (call it under torch.no_grad)");
   TORCH_CHECK_VALUE(!(c.forward_grad && t._fw_grad(/*level=*/0).defined()), name,
                     ": carries a forward-mode gradient, which this operator does not have");
+  TORCH_CHECK_VALUE(!t.is_neg(), name, ": a view whose memory holds the negated values (resolve_neg makes a copy)");
 }
 
 // a tensor of rows: any strides, the last dimension contiguous

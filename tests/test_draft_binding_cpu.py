@@ -33,3 +33,13 @@ def test_forward_mode_gradients_are_refused(cc, op):  # noqa: F811
                     getattr(drafting, op)(cc, **a)
                 with fwd._set_fwd_grad_enabled(False), Reached():
                     getattr(drafting, op)(cc, **a)
+
+
+@pytest.mark.parametrize("op", OPS)
+def test_negated_views_are_refused(cc, op):  # noqa: F811
+    """The imaginary part of a conjugate is such a view."""
+    assert torch.zeros(3, dtype=torch.complex64).conj().imag.is_neg()
+    for name, t in args(op).items():
+        if isinstance(t, torch.Tensor) and t.is_floating_point():
+            with pytest.raises(ValueError, match="negated"):
+                getattr(drafting, op)(cc, **(args(op) | {name: torch._neg_view(t)}))
