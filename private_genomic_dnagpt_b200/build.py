@@ -51,17 +51,32 @@ def _deps_newer(obj: str, src: str) -> bool:
     return any(os.path.getmtime(s) > t for s in srcs)
 
 
+def _make(cmd: list[str], out: str, what: str) -> str:
+    """Runs the compiler or linker; `out` appears whole or not at all, so that
+    processes started together do not load what another has half written.
+    Returns what it printed."""
+    root, ext = os.path.splitext(out)
+    part = f"{root}.{os.getpid()}{ext}"
+    try:
+        r = subprocess.run([*cmd, "-o", part], capture_output=True, text=True)
+        if r.returncode != 0:
+            raise RuntimeError(f"{what}:\n{r.stdout}\n{r.stderr}")
+        os.replace(part, out)
+    finally:
+        if os.path.exists(part):
+            os.remove(part)
+    return r.stderr
+
+
 def _compile(src: str, verbose: bool) -> str:
     obj = os.path.join(OBJ, os.path.basename(src).replace(".cu", ".o"))
     if _deps_newer(obj, src):
-        cmd = [_nvcc(), *_host_compiler(), *ARCH, *FLAGS, "-c", src, "-o", obj]
+        cmd = [_nvcc(), *_host_compiler(), *ARCH, *FLAGS, "-c", src]
         if verbose:
             cmd += ["-Xptxas", "-v"]
-        r = subprocess.run(cmd, capture_output=True, text=True)
-        if r.returncode != 0:
-            raise RuntimeError(f"nvcc failed for {src}:\n{r.stdout}\n{r.stderr}")
+        printed = _make(cmd, obj, f"nvcc failed for {src}")
         if verbose:
-            sys.stderr.write(r.stderr)
+            sys.stderr.write(printed)
     return obj
 
 
@@ -81,13 +96,11 @@ def build_binding() -> str:
     include = [f"-I{p}" for p in (*cpp_extension.include_paths(), sysconfig.get_path("include"),
                                   os.path.join(cuda, "include"))]
     cmd = [gxx, "-O2", "-std=c++17", "-fPIC", "-shared", *include, "-DTORCH_EXTENSION_NAME=_draft",
-           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", src, "-o", BINDING, f"-L{libs}",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", src, f"-L{libs}",
            "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda", f"-L{HERE}",
            "-l:libckks_b200.so", f"-Wl,-rpath,{libs}",
            "-Wl,-rpath,$ORIGIN"]
-    r = subprocess.run(cmd, capture_output=True, text=True)
-    if r.returncode != 0:
-        raise RuntimeError(f"g++ failed for {src}:\n{r.stdout}\n{r.stderr}")
+    _make(cmd, BINDING, f"g++ failed for {src}")
     return BINDING
 
 
@@ -97,10 +110,7 @@ def build(verbose: bool = False) -> str:
     with cf.ThreadPoolExecutor(max_workers=min(8, os.cpu_count() or 1)) as ex:
         objs = list(ex.map(lambda s: _compile(s, verbose), srcs))
     if not os.path.exists(LIB) or any(os.path.getmtime(o) > os.path.getmtime(LIB) for o in objs):
-        cmd = [_nvcc(), *_host_compiler(), *ARCH, "-shared", "-o", LIB, *objs, "-lcudart"]
-        r = subprocess.run(cmd, capture_output=True, text=True)
-        if r.returncode != 0:
-            raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
+        _make([_nvcc(), *_host_compiler(), *ARCH, "-shared", *objs, "-lcudart"], LIB, "link failed")
     try:
         import torch  # noqa: F401
     except ImportError:
