@@ -996,7 +996,8 @@ __global__ void __launch_bounds__(256) join_list_kernel(const __grid_constant__ 
 // A unit is (sequence, head, RT rows); the CTAs divide the list of all units'
 // key tiles evenly, as above.  A tile of KT keys (the cached and then the new
 // ones) and its values arrive in one of two stages by asynchronous copies
-// while the other is worked on; three CTAs of 34 to 68 KB share an SM.
+// while the other is worked on; three CTAs share an SM for heads of up to 64
+// elements (71 to 75 KB each), two for wider ones (56 to 76 KB).
 // Scores: a thread has one key and RPT rows, so an element of K from shared
 // memory feeds RPT multiply-adds and those of q are broadcasts.  Values: 16
 // threads across each 64 elements, eight across the tile's keys, each with the
@@ -1018,12 +1019,15 @@ struct F32Shape {
   static constexpr int KT = DC == 1 ? 64 : DC == 2 ? 32 : 16, DP = 64 * DC;
   static constexpr int KS = DP + 4;                  // stride of K's rows: reads without conflicts
   static constexpr int kStage = KT * KS + KT * DP;  // floats
-  static constexpr size_t kSmem = sizeof(float) * (2 * kStage + RT * DP + KT * RT + 3 * RT) + kMaxNodes * 12 + RT * 8;
+  static constexpr int kCtas = DC == 1 ? 3 : 2;  // on an SM
+  static constexpr size_t kSmem = sizeof(float) * (2 * kStage + RT * DP + KT * RT + 3 * RT) + (kMaxNodes + RT) * 8;
+  static_assert(kCtas * (kSmem + 1024) <= 228 << 10, "the CTAs that a launch counts on fit an SM");
+  static_assert(KT * RT >= kMaxNodes, "the masks' scratch fits the scores' place");
   static_assert(sizeof(float) * 8 * RT * 64 <= sizeof(float) * 2 * kStage, "a unit's sums meet in the stages");
 };
 
 template <int RT, int DC>
-__global__ void __launch_bounds__(kThreads, DC == 1 ? 3 : 2) attend_f32_kernel(const __grid_constant__ AttnParams p) {
+__global__ void __launch_bounds__(kThreads, F32Shape<RT, DC>::kCtas) attend_f32_kernel(const __grid_constant__ AttnParams p) {
   using S = F32Shape<RT, DC>;
   constexpr int KT = S::KT, DP = S::DP, KS = S::KS, KG = kThreads / KT, RPT = RT / KG;  // row groups, rows of a thread
   extern __shared__ __align__(16) float sm[];
@@ -1034,7 +1038,6 @@ __global__ void __launch_bounds__(kThreads, DC == 1 ? 3 : 2) attend_f32_kernel(c
   float* const s_c = s_l + RT;
   uint64_t* const s_mask = reinterpret_cast<uint64_t*>(s_c + RT);
   uint64_t* const s_row = s_mask + kMaxNodes;  // the masks of a unit's rows
-  int* const s_jump = reinterpret_cast<int*>(s_row + RT);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int rows = p.nodes * p.group, tiles_r = (rows + RT - 1) / RT, units = p.kv_heads * tiles_r, D = p.head_dim;
   asm volatile("griddepcontrol.launch_dependents;");
@@ -1095,7 +1098,7 @@ __global__ void __launch_bounds__(kThreads, DC == 1 ? 3 : 2) attend_f32_kernel(c
       }
       copies_close();
     };
-    if (masks_of != b && warp == 0) tree_masks(p.parents + (size_t)b * p.nodes, p.nodes, s_mask, s_jump);
+    if (masks_of != b && warp == 0) tree_masks(p.parents + (size_t)b * p.nodes, p.nodes, s_mask, reinterpret_cast<int*>(sp));
     masks_of = b;
     if (tid < RT) s_m[tid] = -INFINITY, s_l[tid] = 0.0f;
     __syncthreads();
