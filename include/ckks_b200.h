@@ -456,7 +456,7 @@ typedef struct {
   ckks_rows v_cache;
   ckks_rows k_new; /* row = node: [batch][nodes][kv_heads][head_dim] */
   ckks_rows v_new;
-  ckks_rows out;          /* as q */
+  ckks_rows out;          /* as q; out and lse overlap none of the inputs */
   const int32_t* lens;    /* [batch] keys in the cache; taken as 0..capacity */
   const int32_t* parents; /* [batch][nodes] */
   float* lse;             /* [batch][nodes][q_heads] out */
@@ -550,19 +550,19 @@ typedef struct {
   int32_t budget, recent;      /* 0 <= recent <= budget, budget >= 1 */
   ckks_rows k_cache, v_cache;  /* inputs */
   ckks_rows acc;               /* float32 weights, as for ckks_draft_accumulate */
-  ckks_rows k_out, v_out;      /* outputs, not overlapping the inputs */
+  ckks_rows k_out, v_out;      /* outputs, not overlapping the inputs or one another */
   ckks_rows acc_out;           /* float32 */
   const int32_t* lens;         /* [batch]; taken as 0..capacity */
   int32_t* index;              /* [batch][kv_heads][budget] out: rows kept, then -1 */
   int32_t* lens_out;           /* [batch] out, not overlapping lens */
-  void* workspace;             /* ckks_draft_evict_workspace bytes, 16-byte aligned */
+  void* workspace;             /* ckks_draft_evict_workspace bytes (none today), 16-byte aligned */
   size_t workspace_bytes;
 } ckks_draft_evict_args;
 
 /* Copies at most `budget` rows of each head's cache, in their order: the
  * last `recent` ones and, of the others, those with the largest weights (the
- * lower index first among equals; a weight that is not a number counts as
- * -inf).  A shorter cache is copied whole.  Output rows behind the last one
+ * lower index first among equals; a weight that is not a number comes behind
+ * all others, -inf among them).  A shorter cache is copied whole.  Output rows behind the last one
  * kept are left as they were. */
 int ckks_draft_evict(ckks_ctx* ctx, const ckks_draft_evict_args* args, void* stream);
 long long ckks_draft_evict_workspace(ckks_ctx* ctx, const ckks_draft_evict_args* args);

@@ -101,7 +101,8 @@ def accumulate(cc, q, lse, k_cache, lens, path, count, acc, scale=None):
 def evict(cc, k_cache, v_cache, acc, lens, budget, recent, out=None):
     """Copies at most ``budget`` rows of each head's cache, in their order:
     the last ``recent`` ones and, of the others, those with the largest weights
-    in acc [B, Hkv, capacity] float32 (the lower index first among equals).
+    in acc [B, Hkv, capacity] float32 (the lower index first among equals, a
+    weight that is not a number behind all others).
     ``out``: (k, v, acc) of at least ``budget`` rows to write into, their rows
     behind the last one kept being left as they were; new tensors of exactly
     ``budget`` rows, zero behind the last one, when it is not given.  Returns

@@ -104,3 +104,12 @@ def test_largest_float32_keys(cc):
     even = 6.0 * np.exp(float(np.float32(3.4e38)) * 2.0 ** -131)
     assert np.abs(got[0, :, 0:288:2] - even).max() <= 1e-5 * even
     assert np.abs(got[0, :, 1:288:2] - 6.0).max() <= 6e-5
+
+
+def test_weights_that_are_no_numbers_are_evicted_first(cc):
+    """The order of eviction by hand: numbers, then -inf, then NaN."""
+    acc = torch.tensor([[[float("nan"), float("-inf"), -1.0, float("nan"), float("inf")]]], device="cuda")
+    k = torch.arange(5.0, device="cuda")[None, None, :, None].clone()
+    for budget, rows in ((1, [4]), (2, [2, 4]), (3, [1, 2, 4]), (4, [0, 1, 2, 4]), (5, [0, 1, 2, 3, 4])):
+        got = cc.draft_evict(k, k.clone(), acc, i32([5]), budget, 0)
+        assert got[3][0, 0].tolist() == rows and got[0][0, 0, :, 0].tolist() == rows
