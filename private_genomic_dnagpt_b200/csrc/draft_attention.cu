@@ -1358,13 +1358,17 @@ Division divide(const Context& c, const ckks_draft_attention_args& a, Division d
   return d;
 }
 
-// What a unit's start and end cost, in tiles: measured on trees of 21 over 4001
-// keys of 64 (2 / 3 / 4 / 5 / 6 tiles: 32.7 / 28.4 / 26.9 / 27.8 / 29.0 us) and
-// trees of 32 over 65536 keys of 128 (2 / 4 / 6 / 8 tiles: 97.6 / 95.3 / 93.7 /
-// 91.4 us), later 8 / 10: 92.2 / 90.1 us
+// What a unit's start and end cost, in tiles of its keys; wider heads have
+// longer tiles.  Measured with 2 / 4 / 6 / 10 tiles (us): heads of 64, 21 rows over
+// 4001 keys, eight ragged sequences of 12: 36.2 / 29.2 / 30.4 / 32.9; 128 rows over
+// 65536, two of 8: 78.5 / 76.5 / 75.8 / 75.8.  Heads of 128, 128 rows over 65536:
+// 102 / 99.4 / 97.8 / 95.8, over 2000, eight of 8: 48.4 / 39.1 / 38.1 / 38.7; 16 rows over
+// 8000, three of 12: 35.6 / 34.3 / 34.7 / 36.0.  Heads of 256, 8 rows over 8000, four of
+// 8: 59.7 / 61.7 / 61.7 / 65.4, over 32000: 99 / 99 / 98 / 100; of 192, 16 rows over
+// 3000: 27.8 / 30.6 / 29.7 / 31.9.
 Division tc_division(const Context& c, const ckks_draft_attention_args& a) {
   const int rows = tile_nodes(a) * (a.q_heads / a.kv_heads);
-  return divide(c, a, Division{rows, kKeys, 1, a.head_dim <= 64 ? 4 : 10, 0, false, false}, 1);
+  return divide(c, a, Division{rows, kKeys, 1, a.head_dim <= 64 ? 4 : a.head_dim <= 128 ? 6 : 2, 0, false, false}, 1);
 }
 
 bool f32_sizes(const ckks_draft_attention_args& a) { return a.dtype == CKKS_FP32 && a.head_dim % 4 == 0; }
