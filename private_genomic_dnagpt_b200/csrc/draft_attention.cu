@@ -75,7 +75,7 @@ __device__ __forceinline__ T* out_row(const AttnParams& p, int b, int node, int 
 // partial sums meet once, at the end.  Products and sums are in 32 bits.  What
 // the two kernels below do not take comes here: unaligned rows, odd head sizes.
 // Loads are not overlapped within a CTA (5 float32 rows over 6000 keys took it
-// 87 us, against 39 below).
+// 87 us, against 40 below).
 constexpr int kRows = 8, kTile = 64, kThreads = 128;
 constexpr uint32_t kUnseen = 0x80000000u;  // -0: the weight of a key that a row does not see (others are +0 and more)
 
@@ -356,16 +356,17 @@ __device__ __noinline__ void add_spoiled(const AttnParams& p, int b, int h, int 
 // product each weight is two numbers of the operands' type, so that the result
 // is as far from the exact one as its own rounding takes it.  With one number
 // the error was 1.1 to 1.4 times that; the second costs half as many products
-// again: 90.8 -> 96.8, 26.9 -> 28.7, 56.6 -> 67.5 and 45.8 -> 51.6 us for the
-// four below.
+// again (91 us instead of 98 for the first case below, 26.9 instead of 27.8).
 //
-// Measured: 32 nodes x 4 heads over 65536 keys of 128 (470 MB) 91.5 us, of it
-// the tiles at 98 % of the copy rate and about 15 us of set-up, unit ends and
-// joining; 21 nodes over 4001 keys of 64, eight ragged sequences, 25.7 us: a
-// tile's products and waits take one warp 1250 cycles, its bytes 1420 of an
-// SM's share of HBM, and set-up, unit ends and joining some 9 us.  Four
-// sequences over 8000 keys of 256: 8 nodes and 8 heads 60 us (floor 33), 32
-// nodes x 4 heads on each of 4 heads 50 us (6560 on the CUDA cores above).
+// Measured: 32 nodes x 4 heads over 65536 keys of 128 (470 MB) 98 us: 49 tiles a
+// CTA at 1.55 us (1.40 with one number a weight, both at 1.65 GHz, where the
+// power limit has the clock), set-up 3, the unit's end 6 and joining 10.  A
+// tile is 24 products of 64 cycles and three looks at barriers in the warp
+// that issues them, against 1.5 us for its bytes.  21 nodes over 4001 keys of
+// 64, eight ragged sequences, 27.8 us: a tile takes that warp 1600 cycles, its
+// bytes would take 1420; set-up, unit ends and joining some 9 us.  Four
+// sequences over 8000 keys of 256: 8 nodes and 8 heads 59 us (floor 33), 32
+// nodes x 4 heads on each of 4 heads 49 us (6560 on the CUDA cores above).
 constexpr int kM = 128, kKeys = 128, kTmemCols = 512;
 constexpr uint32_t kPanel = 128 * 128;  // 128 rows x 64 elements
 constexpr float kSlack = 8.0f;
@@ -1015,8 +1016,8 @@ __global__ void __launch_bounds__(256) join_list_kernel(const __grid_constant__ 
 // threads across each 64 elements, eight across the tile's keys, each with the
 // sums of all RT rows in registers, which meet when the unit is done.  The
 // products are plain float32 multiply-adds: a 32-bit cache is kept for its
-// accuracy.  Bound by issue slots: 5 rows over 6000 keys of 64 take 38.8 us
-// (3.1 TB/s, 1.36 instructions a cycle from 12 warps an SM).
+// accuracy.  Bound by issue slots: 5 rows over 6000 keys of 64 take 40.2 us
+// (3.0 TB/s, 1.34 instructions a cycle from 12 warps an SM).
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool real) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
 }
@@ -1372,12 +1373,12 @@ Division divide(const Context& c, const ckks_draft_attention_args& a, Division d
 
 // What a unit's start and end cost, in tiles of its keys; wider heads have
 // longer tiles.  Measured with 2 / 4 / 6 / 10 tiles (us): heads of 64, 21 rows over
-// 4001 keys, eight ragged sequences of 12: 36.2 / 29.2 / 30.4 / 32.9; 128 rows over
-// 65536, two of 8: 78.5 / 76.5 / 75.8 / 75.8.  Heads of 128, 128 rows over 65536:
-// 102 / 99.4 / 97.8 / 95.8, over 2000, eight of 8: 48.4 / 39.1 / 38.1 / 38.7; 16 rows over
-// 8000, three of 12: 35.6 / 34.3 / 34.7 / 36.0.  Heads of 256, 8 rows over 8000, four of
-// 8: 59.7 / 61.7 / 61.7 / 65.4, over 32000: 99 / 99 / 98 / 100; of 192, 16 rows over
-// 3000: 27.8 / 30.6 / 29.7 / 31.9.
+// 4001 keys, eight ragged sequences of 12: 36.3 / 27.6 / 28.2 / 29.8; 128 rows over
+// 65536, two of 8: 78.0 / 75.7 / 75.5 / 75.5.  Heads of 128, 128 rows over 65536:
+// 104 / 102 / 100 / 98.3, over 2000, eight of 8: 48.3 / 39.0 / 37.4 / 38.2; 16 rows over
+// 4001, eight of 12: 49 / 39 / 38.4 / 45.  Heads of 256, 8 rows over 8000, four of 8:
+// 60.0 / 61.0 / 60.3 / 64.5, over 32000: 99 / 100 / 102 / 101; of 192, 16 rows over
+// 3000: 27.3 / 30.1 / 29.3 / 31.3.
 Division tc_division(const Context& c, const ckks_draft_attention_args& a) {
   const int rows = tile_nodes(a) * (a.q_heads / a.kv_heads);
   return divide(c, a, Division{rows, kKeys, 1, a.head_dim <= 64 ? 4 : a.head_dim <= 128 ? 6 : 2, 0, false, false}, 1);

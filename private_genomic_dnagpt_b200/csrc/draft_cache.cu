@@ -135,8 +135,8 @@ __global__ void __launch_bounds__(kAccKeys) accumulate_kernel(AccParams p) {
 // uses each as two steps' elements, which the q rows in shared memory follow.
 // The exponentials of a key lie in one quad, so its sum is two shuffles; a key's weights are
 // added in a fixed order.
-// 16 accepted rows over 65536 keys of 128 take 44.3 us, 86 % of the copy rate; 4
-// over 4001 keys of 64, eight sequences, 10.9 us, where the chain of reads
+// 16 accepted rows over 65536 keys of 128 take 45.2 us, 84 % of the copy rate; 4
+// over 4001 keys of 64, eight sequences, 12.1 us, where the chain of reads
 // (lengths, accepted nodes, their rows) shows.
 // A float32 element is three bfloat16 numbers of 8 bits each (cut, so their sum
 // is the element), and a product of two elements eight of the nine products of

@@ -63,8 +63,8 @@ __device__ __forceinline__ double left_of(double p, double q, double a) {
 // each in its parent's row.  Sums add the CTAs' parts in their order.
 // Bound by the slowest sequence's chain: each refusal is a row from HBM, two
 // conversions, a multiply-add and an add in float64 for each entry, and a
-// cluster barrier, 3 to 4 us; 64 trees of 31 over 32003 entries take 19.1 us, one
-// chain of 5 over 4103 6.6 us.  (One CTA a sequence took 61 us.)
+// cluster barrier, 3 to 4 us; 64 trees of 31 over 32003 entries take 20.0 us, one
+// chain of 5 over 4103 7.2 us.  (One CTA a sequence took 61 us.)
 template <typename TT, typename TD, int C>
 __global__ void __launch_bounds__(kThreads, sizeof(TT) + sizeof(TD) == 8 ? 2 : 1) verify_kernel(VerifyParams p) {
   constexpr int kHeld = sizeof(TT) + sizeof(TD) == 8 ? 16 : 8;
