@@ -83,7 +83,7 @@ P* small(const Call& c, const Tensor& t, const char* name, at::IntArrayRef shape
   return static_cast<P*>(t.data_ptr());
 }
 
-// refuses a tensor of which two elements share memory
+// refuses a tensor whose elements share memory along an expanded dimension
 void check_written(const Tensor& t, const char* name) {
   for (int64_t i = 0; i < t.dim(); ++i)
     TORCH_CHECK_VALUE(t.size(i) <= 1 || t.stride(i) != 0, name, ": is written, but some of its elements share memory");
