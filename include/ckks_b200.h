@@ -567,6 +567,77 @@ typedef struct {
 int ckks_draft_evict(ckks_ctx* ctx, const ckks_draft_evict_args* args, void* stream);
 long long ckks_draft_evict_workspace(ckks_ctx* ctx, const ckks_draft_evict_args* args);
 
+/* ---- prompts, and caches in 4 bits ------------------------------------------ */
+typedef struct {
+  int32_t dtype; /* CKKS_BF16, CKKS_FP16 or CKKS_FP32: q, k, v, out */
+  int32_t batch, q_heads, kv_heads, head_dim; /* q_heads a multiple of kv_heads; head_dim 1..256 */
+  int32_t tokens;                             /* rows of the packed tensors */
+  double scale;
+  ckks_rows q, k, v; /* row = token: [tokens][heads][head_dim] in any strides, batch unused */
+  ckks_rows out;     /* as q; out and lse overlap none of the inputs */
+  const int32_t* starts; /* [batch + 1] */
+  float* lse;            /* [tokens][q_heads] out */
+} ckks_draft_prompt_args;
+
+/* Causal attention within each of `batch` packed prompts: sequence b has the
+ * rows from starts[b] to starts[b + 1], row i of it sees the rows up to itself.
+ * Each start is taken as 0..tokens and as no less than those before it.  Rows
+ * of no sequence get 0, their lse -inf.  A key or value that a row does not
+ * see does not reach it, whatever it holds; an infinite or NaN value that a
+ * row sees makes that element of the row infinite or NaN.  Products and sums
+ * are in 32 bits; between the two products a softmax weight keeps 8 bits with
+ * bfloat16 tensors, 11 with float16 and 24 with float32 ones.  No workspace. */
+int ckks_draft_prompt(ckks_ctx* ctx, const ckks_draft_prompt_args* args, void* stream);
+
+/* A 4-bit cache holds rows of ckks_draft_row4_bytes(head_dim) bytes on 4-byte
+ * boundaries: the head's elements in groups of 16, each element a 4-bit
+ * floating-point number (bit 3 the sign, the others 0, 0.5, 1, 1.5, 2, 3, 4, 6)
+ * times its group's scale.  First the elements, 8 bytes a group with the even
+ * one in a byte's low half, then a byte for each group's scale (five exponent
+ * bits with bias 15, three of mantissa, no sign), then zeros.  A scale is a
+ * sixth of the group's largest magnitude rounded to three bits (2^-17 at the
+ * finest, 10240 at most: values beyond 61440 become 61440), an element the
+ * nearest number of its scale, both to even in the middle; a group that holds
+ * an infinity or a NaN has the scale 0xFC, and all of it reads as NaN.  All
+ * values are exact in bfloat16 and float16.  In the ckks_rows of such a cache
+ * the strides are in bytes, multiples of 4. */
+int ckks_draft_row4_bytes(int head_dim); /* or -1 */
+
+typedef struct {
+  int32_t dtype; /* CKKS_BF16, CKKS_FP16 or CKKS_FP32: k and v, and a plain cache */
+  int32_t batch, kv_heads, head_dim, tokens, capacity;
+  ckks_rows k_cache, v_cache; /* [batch][kv_heads][capacity] rows */
+  ckks_rows k, v;             /* row = token, batch unused; not overlapping the caches */
+  const int32_t* starts;      /* [batch + 1], as for ckks_draft_prompt */
+  const int32_t* lens;        /* [batch] rows in the caches already */
+  int32_t* lens_out;          /* [batch] out, not overlapping starts or lens */
+} ckks_draft_fill_args;
+
+/* Appends every packed sequence's rows behind lens[b] and writes the new
+ * lengths.  A sequence that does not fit its cache is left as it is, with its
+ * length unchanged, and reported as for ckks_draft_commit. */
+int ckks_draft_fill(ckks_ctx* ctx, const ckks_draft_fill_args* args, void* stream);
+/* the same into 4-bit caches */
+int ckks_draft_fill4(ckks_ctx* ctx, const ckks_draft_fill_args* args, void* stream);
+/* ckks_draft_commit into 4-bit caches (dtype: of k_new and v_new) */
+int ckks_draft_commit4(ckks_ctx* ctx, const ckks_draft_commit_args* args, void* stream);
+
+typedef struct {
+  int32_t dtype; /* of out: CKKS_BF16, CKKS_FP16 or CKKS_FP32 */
+  int32_t batch, kv_heads, head_dim, capacity, reserved;
+  ckks_rows cache;     /* 4-bit rows */
+  ckks_rows out;       /* [batch][kv_heads][capacity][head_dim], not overlapping the cache */
+  const int32_t* lens; /* [batch]; taken as 0..capacity */
+} ckks_draft_read4_args;
+
+/* The values of a 4-bit cache, exactly; 0 behind lens[b]. */
+int ckks_draft_read4(ckks_ctx* ctx, const ckks_draft_read4_args* args, void* stream);
+
+/* ckks_draft_attention over 4-bit caches (dtype: of q, k_new, v_new and out).
+ * Scores and sums are those of the caches' exact values. */
+int ckks_draft_attention4(ckks_ctx* ctx, const ckks_draft_attention_args* args, void* stream);
+long long ckks_draft_attention4_workspace(ckks_ctx* ctx, const ckks_draft_attention_args* args);
+
 /* Diagnostic of the bounded waits: one CTA stages 4 KiB through a bulk copy
  * into shared memory and back.  starve = 0: CKKS_OK when the data came back
  * intact.  starve = 1: the barrier expects more bytes than are copied, the

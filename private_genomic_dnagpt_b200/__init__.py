@@ -192,6 +192,14 @@ _SIGS = [
     ("ckks_draft_accumulate", ctypes.c_int, [_vp, _vp, _vp]),
     ("ckks_draft_evict", ctypes.c_int, [_vp, _vp, _vp]),
     ("ckks_draft_evict_workspace", ctypes.c_longlong, [_vp, _vp]),
+    ("ckks_draft_prompt", ctypes.c_int, [_vp, _vp, _vp]),
+    ("ckks_draft_row4_bytes", ctypes.c_int, [ctypes.c_int]),
+    ("ckks_draft_fill", ctypes.c_int, [_vp, _vp, _vp]),
+    ("ckks_draft_fill4", ctypes.c_int, [_vp, _vp, _vp]),
+    ("ckks_draft_commit4", ctypes.c_int, [_vp, _vp, _vp]),
+    ("ckks_draft_read4", ctypes.c_int, [_vp, _vp, _vp]),
+    ("ckks_draft_attention4", ctypes.c_int, [_vp, _vp, _vp]),
+    ("ckks_draft_attention4_workspace", ctypes.c_longlong, [_vp, _vp]),
     ("ckks_block_set_drafts", ctypes.c_int, [_vp, ctypes.POINTER(ctypes.c_int), ctypes.c_int, ctypes.c_int]),
 ]
 
@@ -767,6 +775,33 @@ class CryptoContext:
         """The cache cut to ``budget`` rows: (k, v, acc, index, lens); see
         ``drafting.evict``."""
         return drafting.evict(self, k_cache, v_cache, acc, lens, budget, recent, out)
+
+    def draft_prompt(self, q, k, v, starts, scale=None):
+        """Causal attention within packed prompts: (out, lse); see
+        ``drafting.prompt``."""
+        return drafting.prompt(self, q, k, v, starts, scale)
+
+    def draft_fill(self, k_cache, v_cache, lens, k, v, starts):
+        """Packed prompts' rows appended to the cache in place: the new
+        lengths; see ``drafting.fill``."""
+        return drafting.fill(self, k_cache, v_cache, lens, k, v, starts)
+
+    def draft_fill4(self, k_cache, v_cache, lens, k, v, starts):
+        """``draft_fill`` into a 4-bit cache; see ``drafting.fill4``."""
+        return drafting.fill4(self, k_cache, v_cache, lens, k, v, starts)
+
+    def draft_commit4(self, k_cache, v_cache, lens, k_new, v_new, path, count):
+        """``draft_commit`` into a 4-bit cache; see ``drafting.commit4``."""
+        return drafting.commit4(self, k_cache, v_cache, lens, k_new, v_new, path, count)
+
+    def draft_read4(self, cache, lens, head_dim, dtype):
+        """The values of a 4-bit cache; see ``drafting.read4``."""
+        return drafting.read4(self, cache, lens, head_dim, dtype)
+
+    def draft_attention4(self, q, k_cache, v_cache, lens, k_new, v_new, parents, scale=None):
+        """``draft_attention`` over a 4-bit cache; see
+        ``drafting.attention4``."""
+        return drafting.attention4(self, q, k_cache, v_cache, lens, k_new, v_new, parents, scale)
 
 
 def GenCryptoContext(params: CCParams) -> CryptoContext:

@@ -665,8 +665,9 @@ int ckks_sync(ckks_ctx* ctx) {
                                   " bounded device wait(s) gave up (a bulk copy into shared memory did not complete); "
                                   "the outputs since the last synchronisation are not valid");
     if (r)
-      throw Error(CKKS_ECAPACITY, std::to_string(r) + " sequence(s) left unchanged by ckks_draft_commit: the count, the "
-                                                      "path or the length does not fit the cache");
+      throw Error(CKKS_ECAPACITY, std::to_string(r) + " sequence(s) left unchanged by ckks_draft_commit, ckks_draft_commit4, "
+                                                      "ckks_draft_fill or ckks_draft_fill4: the count, the path or "
+                                                      "the length does not fit the cache");
   });
 }
 

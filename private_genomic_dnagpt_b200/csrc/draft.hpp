@@ -164,6 +164,34 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+// four elements of a row from element d on, as floats; 0 behind the row's end
+template <typename T>
+__device__ __forceinline__ void load_row4(float* dst, const T* src, int d, int D, bool wide) {
+  if (wide) {
+    if constexpr (sizeof(T) == 4) {
+      *reinterpret_cast<float4*>(dst) = *reinterpret_cast<const float4*>(src + d);
+    } else {
+      const uint2 u = *reinterpret_cast<const uint2*>(src + d);
+      const T* e = reinterpret_cast<const T*>(&u);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) dst[k] = to_f32(e[k]);
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) dst[k] = d + k < D ? to_f32(src[d + k]) : 0.0f;
+  }
+}
+
+// Whether a sequence's count, path and length fit; evaluated alike by every
+// thread of a CTA from `count` entries of path
+__device__ __forceinline__ bool fits(const int32_t* path, int count, int len, int nodes, int capacity) {
+  if (count < 0 || count > nodes || len < 0 || len > capacity || count > capacity - len) return false;
+  bool ok = true;
+#pragma unroll 8
+  for (int j = 0; j < count; ++j) ok &= (unsigned)path[j] < (unsigned)nodes;  // no read waits for another
+  return ok;
+}
+
 // A list of work whose length only the device knows: sequence b has `units`
 // units of entries_of(b) entries each, one after the other.  CTA i of n takes
 // the entries from list_start(i) to list_start(i + 1).

@@ -12,8 +12,8 @@
 #include <algorithm>
 #include <cmath>
 
-#include "draft.hpp"
-#include "tcgen.cuh"
+#include "draft_fp4.cuh"
+#include "draft_tc.cuh"
 
 namespace ckks {
 namespace draft {
@@ -79,26 +79,10 @@ __device__ __forceinline__ T* out_row(const AttnParams& p, int b, int node, int 
 constexpr int kRows = 8, kTile = 64, kThreads = 128;
 constexpr uint32_t kUnseen = 0x80000000u;  // -0: the weight of a key that a row does not see (others are +0 and more)
 
-template <typename T>
-__device__ __forceinline__ void load_row4(float* dst, const T* src, int d, int D, bool wide) {
-  if (wide) {
-    if constexpr (sizeof(T) == 4) {
-      *reinterpret_cast<float4*>(dst) = *reinterpret_cast<const float4*>(src + d);
-    } else {
-      const uint2 u = *reinterpret_cast<const uint2*>(src + d);
-      const T* e = reinterpret_cast<const T*>(&u);
-#pragma unroll
-      for (int k = 0; k < 4; ++k) dst[k] = to_f32(e[k]);
-    }
-  } else {
-#pragma unroll
-    for (int k = 0; k < 4; ++k) dst[k] = d + k < D ? to_f32(src[d + k]) : 0.0f;
-  }
-}
-
-// DC: chunks of 64 elements that cover head_dim
-template <typename T, int DC>
+// DC: chunks of 64 elements that cover head_dim; FOUR: the caches are 4-bit rows
+template <typename T, int DC, bool FOUR>
 __global__ void __launch_bounds__(kThreads) attend_kernel(AttnParams p) {
+  using Cached = std::conditional_t<FOUR, uint8_t, T>;
   extern __shared__ __align__(16) float sm[];
   const int D = p.head_dim, D4 = (D + 3) & ~3, KS = D4 + 4;  // row stride of the keys: 16-byte reads without conflicts
   float* sk = sm;                       // [kTile][KS]
@@ -144,8 +128,8 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(AttnParams p) {
   __syncthreads();
   const int key = tid & 63, rh = tid >> 6;  // scores: this thread's key of the tile and rows 4 rh .. 4 rh + 3
   const int dg = tid & 15, kg = tid >> 4;   // values: this thread's elements and every eighth key
-  const T* kc = static_cast<const T*>(p.kc.data) + b * p.kc.batch + h * p.kc.head;
-  const T* vc = static_cast<const T*>(p.vc.data) + b * p.vc.batch + h * p.vc.head;
+  const Cached* kc = static_cast<const Cached*>(p.kc.data) + b * p.kc.batch + h * p.kc.head;
+  const Cached* vc = static_cast<const Cached*>(p.vc.data) + b * p.vc.batch + h * p.vc.head;
   const T* kn = static_cast<const T*>(p.kn.data) + b * p.kn.batch + h * p.kn.head;
   const T* vn = static_cast<const T*>(p.vn.data) + b * p.vn.batch + h * p.vn.head;
   for (int t0 = k0; t0 < k1; t0 += kTile) {
@@ -155,8 +139,13 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(AttnParams p) {
       float x[4] = {0.f, 0.f, 0.f, 0.f}, y[4] = {0.f, 0.f, 0.f, 0.f};
       if (r < nk) {
         if (s < len) {
-          load_row4(x, kc + s * p.kc.row, d, D, p.wide);
-          load_row4(y, vc + s * p.vc.row, d, D, p.wide);
+          if constexpr (FOUR) {
+            load_row4_4bit(x, kc + s * p.kc.row, d, D);
+            load_row4_4bit(y, vc + s * p.vc.row, d, D);
+          } else {
+            load_row4(x, kc + s * p.kc.row, d, D, p.wide);
+            load_row4(y, vc + s * p.vc.row, d, D, p.wide);
+          }
         } else if (s_mask[s - len]) {
           load_row4(x, kn + (s - len) * p.kn.row, d, D, p.wide);
           load_row4(y, vn + (s - len) * p.vn.row, d, D, p.wide);
@@ -367,52 +356,9 @@ __device__ __noinline__ void add_spoiled(const AttnParams& p, int b, int h, int 
 // bytes would take 1420; set-up, unit ends and joining some 9 us.  Four
 // sequences over 8000 keys of 256: 8 nodes and 8 heads 59 us (floor 33), 32
 // nodes x 4 heads on each of 4 heads 49 us (6560 on the CUDA cores above).
-constexpr int kM = 128, kKeys = 128, kTmemCols = 512;
-constexpr uint32_t kPanel = 128 * 128;  // 128 rows x 64 elements
-constexpr float kSlack = 8.0f;
-// float16 weights end at 2^-24, far above the smallest ones beside a heavy key,
-// so their reference point lies 2^7 below the maximum: the largest weight is
-// between 2^7 and 2^15
-template <typename T>
-constexpr float kBelow = std::is_same_v<T, __half> ? 7.0f : 0.0f;
-
 struct TileMaps {
   CUtensorMap q, kc, vc, kn, vn;
 };
-
-template <typename T>
-__device__ __forceinline__ uint32_t pack2(float a, float b) {
-  if constexpr (std::is_same_v<T, __nv_bfloat16>) {
-    const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&v);
-  } else {
-    const __half2 v = __floats2half2_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&v);
-  }
-}
-
-// two float32 operations in one instruction
-__device__ __forceinline__ unsigned long long pair_of(float2 v) {
-  return (unsigned long long)__float_as_uint(v.y) << 32 | __float_as_uint(v.x);
-}
-__device__ __forceinline__ float2 of_pair(unsigned long long v) {
-  return make_float2(__uint_as_float((uint32_t)v), __uint_as_float((uint32_t)(v >> 32)));
-}
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-  unsigned long long d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(pair_of(a)), "l"(pair_of(b)), "l"(pair_of(c)));
-  return of_pair(d);
-}
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-  unsigned long long d;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(pair_of(a)), "l"(pair_of(b)));
-  return of_pair(d);
-}
-__device__ __forceinline__ float2 sub2(float2 a, float2 b) {
-  unsigned long long d;
-  asm("sub.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(pair_of(a)), "l"(pair_of(b)));
-  return of_pair(d);
-}
 
 // Two positive weights as the sum of two pairs of the type: `hi` has their
 // leading bits (cut, so that what is left is exact: one byte permutation in
@@ -428,50 +374,6 @@ __device__ __forceinline__ void split2(float2 e, uint32_t& hi, uint32_t& lo) {
   else
     hi = pack2<T>(cut.x, cut.y);
   lo = pack2<T>(left.x, left.y);
-}
-
-// any of eight 16-bit elements infinite or NaN
-template <typename T>
-__device__ __forceinline__ bool not_finite(uint4 v) {
-  constexpr uint32_t e = std::is_same_v<T, __nv_bfloat16> ? 0x7F80u : 0x7C00u;
-  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-  bool bad = false;
-#pragma unroll
-  for (int k = 0; k < 4; ++k) bad |= (w[k] & e) == e || ((w[k] >> 16) & e) == e;
-  return bad;
-}
-
-__device__ __forceinline__ void group_sync(int id, int threads) {
-  asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
-}
-
-// The barriers above wait without limit, so warps that meet there go on or
-// leave together: a wait on an mbarrier counts for the whole warp (which then
-// runs the collective tensor-memory instructions or does not), and the warps'
-// results are joined at a barrier that all of them reach, whatever theirs is.
-__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity) {
-  return (bool)__all_sync(0xffffffffu, mbar_wait_short(bar, parity));
-}
-// two such waits; done both, they cost one look (a look takes about 200 cycles of
-// the warp that issues the products: trees of 21 over 4001 keys 29.2 -> 27.6 us)
-__device__ __forceinline__ bool warp_wait_both(uint32_t a, uint32_t pa, uint32_t b, uint32_t pb) {
-  uint32_t done;
-  asm volatile(
-      "{\n .reg .pred p, q;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
-      " mbarrier.try_wait.parity.shared::cta.b64 q, [%3], %4;\n and.pred p, p, q;\n selp.u32 %0, 1, 0, p;\n}\n"
-      : "=r"(done)
-      : "r"(a), "r"(pa), "r"(b), "r"(pb)
-      : "memory");
-  return __all_sync(0xffffffffu, done) || (warp_wait(a, pa) && warp_wait(b, pb));
-}
-__device__ __forceinline__ bool group_all(int id, int threads, bool ok) {
-  uint32_t all;
-  asm volatile(
-      "{\n .reg .pred p, q;\n setp.ne.u32 p, %3, 0;\n bar.red.and.pred q, %1, %2, p;\n selp.u32 %0, 1, 0, q;\n}\n"
-      : "=r"(all)
-      : "r"(id), "r"(threads), "r"((uint32_t)ok)
-      : "memory");
-  return all != 0;
 }
 
 // by panels of 64 elements of head_dim
@@ -1292,10 +1194,10 @@ size_t attend_smem(int D) {
   return run > red ? run : red;
 }
 
-template <typename T, int DC>
+template <typename T, int DC, bool FOUR>
 void launch_attend(const AttnParams& p, cudaStream_t st) {
   const size_t smem = attend_smem(p.head_dim);
-  auto* k = attend_kernel<T, DC>;
+  auto* k = attend_kernel<T, DC, FOUR>;
   // the most that any call asks for: calls of other sizes from other threads
   // may come between this and the launch
   CKKS_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)attend_smem(64 * DC)));
@@ -1305,13 +1207,13 @@ void launch_attend(const AttnParams& p, cudaStream_t st) {
   CKKS_CUDA(cudaGetLastError());
 }
 
-template <typename T>
+template <typename T, bool FOUR>
 void run_attend(const AttnParams& p, cudaStream_t st) {
   switch ((p.head_dim + 63) / 64) {
-    case 1: launch_attend<T, 1>(p, st); break;
-    case 2: launch_attend<T, 2>(p, st); break;
-    case 3: launch_attend<T, 3>(p, st); break;
-    default: launch_attend<T, 4>(p, st); break;
+    case 1: launch_attend<T, 1, FOUR>(p, st); break;
+    case 2: launch_attend<T, 2, FOUR>(p, st); break;
+    case 3: launch_attend<T, 3, FOUR>(p, st); break;
+    default: launch_attend<T, 4, FOUR>(p, st); break;
   }
   if (p.splits > 1) {
     join_kernel<T><<<(unsigned)(p.batch * p.kv_heads * p.nodes * p.group), kThreads, 0, st>>>(p);
@@ -1418,6 +1320,13 @@ size_t workspace_of(const Context& c, const ckks_draft_attention_args& a) {
   return sizeof(float) * n;
 }
 
+// over a 4-bit cache
+size_t workspace4_of(const Context& c, const ckks_draft_attention_args& a) {
+  if (a.batch == 0) return 0;
+  const int s = split_count(c, a);
+  return s == 1 ? 0 : sizeof(float) * (size_t)a.batch * a.q_heads * a.nodes * s * (a.head_dim + 2);
+}
+
 AttnParams with(AttnParams p, const Division& d) {
   p.tile_rows = d.tile_rows, p.tile_keys = d.tile_keys, p.new_apart = d.new_apart, p.unit_cost = d.unit_cost;
   return p;
@@ -1451,34 +1360,6 @@ void run_f32(const Context& c, const ckks_draft_attention_args& a, const AttnPar
     case 3: launch_f32<8, 3>(p, d, st); break;
     default: launch_f32<8, 4>(p, d, st); break;
   }
-}
-
-using EncodeTiled = decltype(&cuTensorMapEncodeTiled);
-EncodeTiled encode_tiled() {
-  static const EncodeTiled f = [] {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult r;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &r) != cudaSuccess ||
-        r != cudaDriverEntryPointSuccess)
-      p = nullptr;
-    return reinterpret_cast<EncodeTiled>(p);
-  }();
-  return f;
-}
-
-// [batch][outer][inner][head_dim] in boxes of box_outer x box_inner rows of 64
-// elements; what a box has outside the tensor reads as 0
-bool tile_map(CUtensorMap* m, void* data, int dtype, int head_dim, int inner, int64_t inner_stride, int box_inner,
-              int outer, int64_t outer_stride, int box_outer, int batch, int64_t batch_stride) {
-  const EncodeTiled f = encode_tiled();
-  if (!f) return false;
-  auto bytes = [](int64_t s, int n) { return n > 1 ? (cuuint64_t)s * 2 : (cuuint64_t)16; };
-  const cuuint64_t dims[4] = {(cuuint64_t)head_dim, (cuuint64_t)inner, (cuuint64_t)outer, (cuuint64_t)batch};
-  const cuuint64_t strides[3] = {bytes(inner_stride, inner), bytes(outer_stride, outer), bytes(batch_stride, batch)};
-  const cuuint32_t box[4] = {64, (cuuint32_t)box_inner, (cuuint32_t)box_outer, 1}, ones[4] = {1, 1, 1, 1};
-  return f(m, dtype == CKKS_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, data, dims,
-           strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 template <typename T, int PANELS, int COPIES>
@@ -1552,7 +1433,10 @@ extern "C" long long ckks_draft_attention_workspace(ckks_ctx* ctx, const ckks_dr
   return n;
 }
 
-extern "C" int ckks_draft_attention(ckks_ctx* ctx, const ckks_draft_attention_args* args, void* stream) {
+namespace {
+// FOUR: the caches are 4-bit rows, strides in bytes
+template <bool FOUR>
+int run(ckks_ctx* ctx, const ckks_draft_attention_args* args, void* stream) {
   return guard([&] {
     Context& c = context_of(ctx);
     need(args != nullptr, "null argument");
@@ -1564,8 +1448,12 @@ extern "C" int ckks_draft_attention(ckks_ctx* ctx, const ckks_draft_attention_ar
     const int e = element_bytes(a.dtype);
     check_rows(a.q, e, "q");
     if (a.capacity) {
-      check_rows(a.k_cache, e, "k_cache");
-      check_rows(a.v_cache, e, "v_cache");
+      check_rows(a.k_cache, FOUR ? 1 : e, "k_cache");
+      check_rows(a.v_cache, FOUR ? 1 : e, "v_cache");
+      if constexpr (FOUR) {
+        check_row4(a.k_cache, a.batch, a.kv_heads, a.capacity, "k_cache");
+        check_row4(a.v_cache, a.batch, a.kv_heads, a.capacity, "v_cache");
+      }
     }
     check_rows(a.k_new, e, "k_new");
     check_rows(a.v_new, e, "v_new");
@@ -1573,7 +1461,7 @@ extern "C" int ckks_draft_attention(ckks_ctx* ctx, const ckks_draft_attention_ar
     check_ptr(a.lens, "lens");
     check_ptr(a.parents, "parents");
     check_ptr(a.lse, "lse");
-    const size_t ws = workspace_of(c, a);
+    const size_t ws = FOUR ? workspace4_of(c, a) : workspace_of(c, a);
     need(a.workspace_bytes >= ws && (ws == 0 || a.workspace), "workspace smaller than ckks_draft_attention_workspace");
     need(reinterpret_cast<uintptr_t>(a.workspace) % 16 == 0, "workspace not aligned to 16 bytes");
     AttnParams p{};
@@ -1585,28 +1473,51 @@ extern "C" int ckks_draft_attention(ckks_ctx* ctx, const ckks_draft_attention_ar
     p.wide = wide_rows(a.q, a.batch, a.q_heads, a.nodes, a.head_dim, e) &&
              wide_rows(a.out, a.batch, a.q_heads, a.nodes, a.head_dim, e) &&
              wide_rows(a.k_new, a.batch, a.kv_heads, a.nodes, a.head_dim, e) &&
-             wide_rows(a.v_new, a.batch, a.kv_heads, a.nodes, a.head_dim, e) &&
-             (a.capacity == 0 || (wide_rows(a.k_cache, a.batch, a.kv_heads, a.capacity, a.head_dim, e) &&
-                                  wide_rows(a.v_cache, a.batch, a.kv_heads, a.capacity, a.head_dim, e)));
+             wide_rows(a.v_new, a.batch, a.kv_heads, a.nodes, a.head_dim, e);
+    if (!FOUR && a.capacity)
+      p.wide = p.wide && wide_rows(a.k_cache, a.batch, a.kv_heads, a.capacity, a.head_dim, e) &&
+               wide_rows(a.v_cache, a.batch, a.kv_heads, a.capacity, a.head_dim, e);
     OnDevice dev(c);
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const double bytes = 2.0 * e * a.batch * a.kv_heads * a.capacity * a.head_dim;
-    ProfScope ps(c, "draft_attention", bytes, st);
-    // strides that no tensor map holds are left to the plain kernel
-    if (p.wide && takes_tc(c, a)) {
-      if (a.dtype == CKKS_BF16 ? run_tc<__nv_bfloat16>(c, a, p, st) : run_tc<__half>(c, a, p, st)) return;
-    }
-    if (p.wide && takes_f32(c, a)) {
-      run_f32(c, a, p, st);
-      return;
+    const double bytes = 2.0 * a.batch * a.kv_heads * a.capacity * (FOUR ? row4_bytes(a.head_dim) : e * a.head_dim);
+    ProfScope ps(c, FOUR ? "draft_attention4" : "draft_attention", bytes, st);
+    if constexpr (!FOUR) {
+      // strides that no tensor map holds are left to the plain kernel
+      if (p.wide && takes_tc(c, a)) {
+        if (a.dtype == CKKS_BF16 ? run_tc<__nv_bfloat16>(c, a, p, st) : run_tc<__half>(c, a, p, st)) return;
+      }
+      if (p.wide && takes_f32(c, a)) {
+        run_f32(c, a, p, st);
+        return;
+      }
     }
     if (a.dtype == CKKS_BF16)
-      run_attend<__nv_bfloat16>(p, st);
+      run_attend<__nv_bfloat16, FOUR>(p, st);
     else if (a.dtype == CKKS_FP16)
-      run_attend<__half>(p, st);
+      run_attend<__half, FOUR>(p, st);
     else
-      run_attend<float>(p, st);
+      run_attend<float, FOUR>(p, st);
   });
+}
+}  // namespace
+
+extern "C" int ckks_draft_attention(ckks_ctx* ctx, const ckks_draft_attention_args* args, void* stream) {
+  return run<false>(ctx, args, stream);
+}
+
+extern "C" long long ckks_draft_attention4_workspace(ckks_ctx* ctx, const ckks_draft_attention_args* a) {
+  long long n = -1;
+  guard([&] {
+    Context& c = context_of(ctx);
+    need(a != nullptr, "null argument");
+    check_shape(*a);
+    n = (long long)workspace4_of(c, *a);
+  });
+  return n;
+}
+
+extern "C" int ckks_draft_attention4(ckks_ctx* ctx, const ckks_draft_attention_args* args, void* stream) {
+  return run<true>(ctx, args, stream);
 }
 
 extern "C" int ckks_selftest_group_wait(ckks_ctx* ctx, int starved) {

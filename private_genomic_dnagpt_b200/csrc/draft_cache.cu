@@ -12,16 +12,6 @@ namespace ckks {
 namespace draft {
 namespace {
 
-// Whether a sequence's count, path and length fit; evaluated alike by every
-// thread of a CTA from `count` entries of path
-__device__ __forceinline__ bool fits(const int32_t* path, int count, int len, int nodes, int capacity) {
-  if (count < 0 || count > nodes || len < 0 || len > capacity || count > capacity - len) return false;
-  bool ok = true;
-#pragma unroll 8
-  for (int j = 0; j < count; ++j) ok &= (unsigned)path[j] < (unsigned)nodes;  // no read waits for another
-  return ok;
-}
-
 // ---- commit --------------------------------------------------------------------
 struct CommitParams {
   ckks_rows kc, vc, kn, vn;

@@ -1,0 +1,102 @@
+// draft_fp4.cuh -- rows of a 4-bit cache.
+//
+// A head's elements in groups of 16: each element x is a 4-bit floating-point
+// number c (sign, two exponent bits, one mantissa bit: 0, 0.5, 1, 1.5, 2, 3, 4,
+// 6) times the group's scale s, an 8-bit one (five exponent bits, three of
+// mantissa, no sign).  A row is the groups' elements, 8 bytes each with the
+// even element in a byte's low half, then the groups' scales, then zeros up to
+// a multiple of four bytes: 9/16 of a byte an element.
+//
+// c s has at most six significant bits and lies in float16's range (s is at
+// most 10240, six of it a float16; 2^-17 at the finest), so bfloat16 and float16
+// hold every value of a row exactly and a product over the cache loses nothing
+// on its way to the tensor cores.  An 8-bit scale without a sign has room for
+// float16's exponents: it is the leading half of a float16 but for the sign,
+// and decoding is one shift.
+#pragma once
+#include <cuda_fp4.h>
+
+#include "draft.hpp"
+
+namespace ckks {
+namespace draft {
+
+constexpr int kGroup4 = 16;
+constexpr uint32_t kScaleTop = 0xE2;   // 10240
+constexpr uint32_t kScaleNone = 0xFC;  // no number: a group that holds an infinity or a NaN
+
+__host__ __device__ constexpr int groups4(int head_dim) { return (head_dim + kGroup4 - 1) / kGroup4; }
+__host__ __device__ constexpr int row4_bytes(int head_dim) { return (9 * groups4(head_dim) + 3) / 4 * 4; }
+
+// a cache's rows start on 4-byte boundaries
+inline void check_row4(const ckks_rows& r, int batch, int heads, int rows, const char* what) {
+  auto fits = [](int64_t s, int n) { return n <= 1 || s % 4 == 0; };
+  if (reinterpret_cast<uintptr_t>(r.data) % 4 || !fits(r.batch, batch) || !fits(r.head, heads) || !fits(r.row, rows))
+    throw Error(CKKS_EARG, std::string(what) + ": a 4-bit row does not start on a 4-byte boundary");
+}
+
+__device__ __forceinline__ __half scale4(uint32_t byte) { return __ushort_as_half((unsigned short)(byte << 7)); }
+
+// A sixth of the group's largest magnitude, rounded to three bits of mantissa
+// (to even in the middle).  The quotient rounded to 24 bits first gives the
+// same result as the exact one: it can only reach a middle m of five bits from
+// 6 m itself, because the float next to 6 m is off by more than half a step of m.
+__device__ __forceinline__ uint32_t scale4_of(float top) {
+  const float a = __fdiv_rn(top, 6.0f);
+  const uint32_t u = __float_as_uint(a);
+  if (a < 6.103515625e-5f) return (uint32_t)__float2int_rn(a * 131072.0f);  // 2^-14 and below: multiples of 2^-17
+  const uint32_t b = ((u + 0x7FFFFu + (u >> 20 & 1u)) >> 20) - (112u << 3);
+  return b < kScaleTop ? b : kScaleTop;
+}
+
+// One group: the 16 codes and the scale.  x / s is rounded to 24 bits, which
+// moves no quotient onto or over the border between two codes (a border times
+// s has at most seven bits, and the float next to it is off by more than half
+// a step of the border).  The quotient is q + r e with q = x r, e = x - q s and
+// r = 1 / s rounded: with r rounded correctly this is x / s rounded correctly
+// (Markstein, "Computation of elementary functions on the IBM RISC System/6000
+// processor", 1990).
+__device__ __forceinline__ uint64_t encode4(const float* x, uint32_t& scale) {
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < kGroup4; ++i) top = max(top, __float_as_uint(x[i]) & 0x7FFFFFFFu);
+  if (top >= 0x7F800000u) {
+    scale = kScaleNone;
+    return 0;
+  }
+  scale = scale4_of(__uint_as_float(top));
+  if (scale == 0) {
+    uint64_t w = 0;  // zeros keep their signs
+#pragma unroll
+    for (int i = 0; i < kGroup4; ++i) w |= (uint64_t)(__float_as_uint(x[i]) >> 31) << (4 * i + 3);
+    return w;
+  }
+  const float s = __half2float(scale4(scale)), r = __frcp_rn(s);
+  uint32_t w[2] = {0, 0};
+#pragma unroll
+  for (int i = 0; i < kGroup4; i += 2) {
+    float t[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const float q = __fmul_rn(x[i + k], r);
+      t[k] = copysignf(__fmaf_rn(__fmaf_rn(-q, s, x[i + k]), r, q), x[i + k]);  // -0 stays
+    }
+    w[i / 8] |= (uint32_t)__nv_cvt_float2_to_fp4x2(make_float2(t[0], t[1]), __NV_E2M1, cudaRoundNearest) << (4 * (i % 8));
+  }
+  return (uint64_t)w[1] << 32 | w[0];
+}
+
+// two elements from a byte, times the scale (in both halves), exactly
+__device__ __forceinline__ __half2 decode4(uint32_t byte, __half2 scale) {
+  return __hmul2(__half2(__nv_cvt_fp4x2_to_halfraw2((__nv_fp4x2_storage_t)byte, __NV_E2M1)), scale);
+}
+
+// elements d .. d + 3 of a row (d a multiple of 4)
+__device__ __forceinline__ void load_row4_4bit(float* dst, const uint8_t* row, int d, int D) {
+  const __half2 s = __half2half2(scale4(row[8 * groups4(D) + d / kGroup4]));
+  const float2 a = __half22float2(decode4(row[d / 2], s)), b = __half22float2(decode4(row[d / 2 + 1], s));
+  dst[0] = a.x, dst[1] = a.y, dst[2] = b.x, dst[3] = b.y;
+}
+
+}  // namespace draft
+}  // namespace ckks

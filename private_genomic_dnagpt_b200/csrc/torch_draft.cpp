@@ -7,6 +7,7 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/extension.h>
 
+#include <algorithm>
 #include <cmath>
 #include <optional>
 #include <tuple>
@@ -55,7 +56,7 @@ int32_t size32(int64_t n, const char* what) {
   return (int32_t)n;
 }
 
-void four(const Tensor& t, const char* name) { TORCH_CHECK_VALUE(t.dim() == 4, name, ": expected four dimensions"); }
+void four_dims(const Tensor& t, const char* name) { TORCH_CHECK_VALUE(t.dim() == 4, name, ": expected four dimensions"); }
 
 void check(const Call& c, const Tensor& t, const char* name, at::IntArrayRef shape, at::ScalarType type) {
   TORCH_CHECK_VALUE(t.sizes() == shape, name, ": expected the shape ", shape, ", got ", t.sizes());
@@ -106,18 +107,29 @@ Tensor workspace(const Call& c, long long bytes, A& a, const Tensor& like) {
 
 double scale_of(std::optional<double> scale, int64_t d) { return scale ? *scale : 1.0 / std::sqrt((double)d); }
 
+// bytes of a row of a 4-bit cache
+int64_t row4_bytes(int64_t d) {
+  const int n = ckks_draft_row4_bytes((int)std::clamp<int64_t>(d, 0, INT32_MAX));
+  TORCH_CHECK_VALUE(n >= 0, "head size: ", ckks_last_error());
+  return n;
+}
+
+// `four`: over a cache in 4 bits
+template <bool four>
 std::tuple<Tensor, Tensor> attention(uintptr_t ctx, int device, const Tensor& q, const Tensor& k_cache,
                                      const Tensor& v_cache, const Tensor& lens, const Tensor& k_new,
                                      const Tensor& v_new, const Tensor& parents, std::optional<double> scale) {
   const Call c{(ckks_ctx*)ctx, device};
-  four(q, "q");
-  four(k_cache, "k_cache");
+  four_dims(q, "q");
+  four_dims(k_cache, "k_cache");
   const int64_t b = q.size(0), n = q.size(1), hq = q.size(2), d = q.size(3), hk = k_cache.size(1), cap = k_cache.size(2);
   const auto t = q.scalar_type();
   const int code = cache_type(q, "q");
   check_rows(c, q, "q", {b, n, hq, d}, t);
-  check_rows(c, k_cache, "k_cache", {b, hk, cap, d}, t);
-  check_rows(c, v_cache, "v_cache", {b, hk, cap, d}, t);
+  const int64_t row = four ? row4_bytes(d) : d;
+  const auto cached = four ? at::kByte : t;
+  check_rows(c, k_cache, "k_cache", {b, hk, cap, row}, cached);
+  check_rows(c, v_cache, "v_cache", {b, hk, cap, row}, cached);
   check_rows(c, k_new, "k_new", {b, n, hk, d}, t);
   check_rows(c, v_new, "v_new", {b, n, hk, d}, t);
   ckks_draft_attention_args a{};
@@ -131,8 +143,9 @@ std::tuple<Tensor, Tensor> attention(uintptr_t ctx, int device, const Tensor& q,
   a.q = by_node(q), a.k_cache = by_head(k_cache), a.v_cache = by_head(v_cache);
   a.k_new = by_node(k_new), a.v_new = by_node(v_new), a.out = by_node(out);
   a.lse = lse.data_ptr<float>();
-  const Tensor ws = workspace(c, ckks_draft_attention_workspace(c.ctx, &a), a, q);
-  c.done(ckks_draft_attention(c.ctx, &a, c.stream()));
+  const Tensor ws =
+      workspace(c, (four ? ckks_draft_attention4_workspace : ckks_draft_attention_workspace)(c.ctx, &a), a, q);
+  c.done((four ? ckks_draft_attention4 : ckks_draft_attention)(c.ctx, &a, c.stream()));
   return {out, lse};
 }
 
@@ -163,17 +176,19 @@ std::tuple<Tensor, Tensor, Tensor> verify(uintptr_t ctx, int device, const Tenso
   return {path, count, token};
 }
 
+template <bool four>
 Tensor commit(uintptr_t ctx, int device, const Tensor& k_cache, const Tensor& v_cache, const Tensor& lens,
               const Tensor& k_new, const Tensor& v_new, const Tensor& path, const Tensor& count) {
   const Call c{(ckks_ctx*)ctx, device};
-  four(k_cache, "k_cache");
-  four(k_new, "k_new");
-  const int64_t b = k_cache.size(0), hk = k_cache.size(1), cap = k_cache.size(2), d = k_cache.size(3), n = k_new.size(1);
-  const auto t = k_cache.scalar_type();
+  four_dims(k_cache, "k_cache");
+  four_dims(k_new, "k_new");
+  const int64_t b = k_cache.size(0), hk = k_cache.size(1), cap = k_cache.size(2), n = k_new.size(1);
+  const int64_t d = (four ? k_new : k_cache).size(3), row = four ? row4_bytes(d) : d;
+  const auto t = (four ? k_new : k_cache).scalar_type(), cached = four ? at::kByte : t;
   ckks_draft_commit_args a{};
-  a.dtype = cache_type(k_cache, "k_cache");
-  check_rows(c, k_cache, "k_cache", {b, hk, cap, d}, t);
-  check_rows(c, v_cache, "v_cache", {b, hk, cap, d}, t);
+  a.dtype = four ? cache_type(k_new, "k_new") : cache_type(k_cache, "k_cache");
+  check_rows(c, k_cache, "k_cache", {b, hk, cap, row}, cached);
+  check_rows(c, v_cache, "v_cache", {b, hk, cap, row}, cached);
   check_written(k_cache, "k_cache");
   check_written(v_cache, "v_cache");
   check_rows(c, k_new, "k_new", {b, n, hk, d}, t);
@@ -187,7 +202,7 @@ Tensor commit(uintptr_t ctx, int device, const Tensor& k_cache, const Tensor& v_
     a.nodes = size32(n, "nodes"), a.capacity = size32(cap, "capacity");
     a.k_cache = by_head(k_cache), a.v_cache = by_head(v_cache), a.k_new = by_node(k_new), a.v_new = by_node(v_new);
     a.lens_out = out.data_ptr<int32_t>();
-    c.done(ckks_draft_commit(c.ctx, &a, c.stream()));
+    c.done((four ? ckks_draft_commit4 : ckks_draft_commit)(c.ctx, &a, c.stream()));
   }
   return out;
 }
@@ -195,8 +210,8 @@ Tensor commit(uintptr_t ctx, int device, const Tensor& k_cache, const Tensor& v_
 Tensor accumulate(uintptr_t ctx, int device, const Tensor& q, const Tensor& lse, const Tensor& k_cache,
                   const Tensor& lens, const Tensor& path, const Tensor& count, Tensor acc, std::optional<double> scale) {
   const Call c{(ckks_ctx*)ctx, device};
-  four(q, "q");
-  four(k_cache, "k_cache");
+  four_dims(q, "q");
+  four_dims(k_cache, "k_cache");
   const int64_t b = q.size(0), n = q.size(1), hq = q.size(2), d = q.size(3), hk = k_cache.size(1), cap = k_cache.size(2);
   ckks_draft_accumulate_args a{};
   a.dtype = cache_type(q, "q");
@@ -224,7 +239,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> evict(uintptr_t ctx, int devi
                                                          const Tensor& v_cache, const Tensor& acc, const Tensor& lens,
                                                          int64_t budget, int64_t recent, std::optional<Caches> out) {
   const Call c{(ckks_ctx*)ctx, device};
-  four(k_cache, "k_cache");
+  four_dims(k_cache, "k_cache");
   const int64_t b = k_cache.size(0), hk = k_cache.size(1), cap = k_cache.size(2), d = k_cache.size(3);
   const auto t = k_cache.scalar_type();
   ckks_draft_evict_args a{};
@@ -239,7 +254,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> evict(uintptr_t ctx, int devi
     out = Caches{at::zeros({b, hk, budget, d}, k_cache.options()), at::zeros({b, hk, budget, d}, k_cache.options()),
                  at::zeros({b, hk, budget}, acc.options())};
   Tensor k2 = std::get<0>(*out), v2 = std::get<1>(*out), a2 = std::get<2>(*out);
-  four(k2, "out");
+  four_dims(k2, "out");
   const int64_t rows = k2.size(2);
   TORCH_CHECK_VALUE(rows >= budget, "out: ", rows, " rows are fewer than the budget of ", budget);
   check_rows(c, k2, "out", {b, hk, rows, d}, t);
@@ -259,12 +274,99 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> evict(uintptr_t ctx, int devi
   return {k2, v2, a2, index, lens_out};
 }
 
+// packed rows [tokens, heads, head size]
+ckks_rows by_token(const Tensor& t) { return {t.data_ptr(), 0, t.stride(1), t.stride(0)}; }
+
+void three(const Tensor& t, const char* name) { TORCH_CHECK_VALUE(t.dim() == 3, name, ": expected three dimensions"); }
+
+const int32_t* starts_of(const Call& c, const Tensor& starts, int64_t batch) {
+  return small<const int32_t>(c, starts, "starts", {batch + 1}, at::kInt);
+}
+
+std::tuple<Tensor, Tensor> prompt(uintptr_t ctx, int device, const Tensor& q, const Tensor& k, const Tensor& v,
+                                  const Tensor& starts, std::optional<double> scale) {
+  const Call c{(ckks_ctx*)ctx, device};
+  three(q, "q");
+  three(k, "k");
+  const int64_t t = q.size(0), hq = q.size(1), d = q.size(2), hk = k.size(1);
+  ckks_draft_prompt_args a{};
+  a.dtype = cache_type(q, "q");
+  check_rows(c, q, "q", {t, hq, d}, q.scalar_type());
+  check_rows(c, k, "k", {t, hk, d}, q.scalar_type());
+  check_rows(c, v, "v", {t, hk, d}, q.scalar_type());
+  TORCH_CHECK_VALUE(starts.dim() == 1 && starts.size(0) >= 1, "starts: expected [sequences + 1]");
+  a.starts = starts_of(c, starts, starts.size(0) - 1);
+  Tensor out = at::empty({t, hq, d}, q.options()), lse = at::empty({t, hq}, q.options().dtype(at::kFloat));
+  if (t == 0) return {out, lse};
+  a.batch = size32(starts.size(0) - 1, "sequences"), a.q_heads = size32(hq, "query heads");
+  a.kv_heads = size32(hk, "key/value heads"), a.head_dim = size32(d, "head size"), a.tokens = size32(t, "tokens");
+  a.scale = scale_of(scale, d);
+  a.q = by_token(q), a.k = by_token(k), a.v = by_token(v), a.out = by_token(out), a.lse = lse.data_ptr<float>();
+  c.done(ckks_draft_prompt(c.ctx, &a, c.stream()));
+  return {out, lse};
+}
+
+template <bool four>
+Tensor fill(uintptr_t ctx, int device, const Tensor& k_cache, const Tensor& v_cache, const Tensor& lens,
+            const Tensor& k, const Tensor& v, const Tensor& starts) {
+  const Call c{(ckks_ctx*)ctx, device};
+  four_dims(k_cache, "k_cache");
+  three(k, "k");
+  const int64_t b = k_cache.size(0), hk = k_cache.size(1), cap = k_cache.size(2), t = k.size(0), d = k.size(2);
+  const int64_t row = four ? row4_bytes(d) : d;
+  const auto cached = four ? at::kByte : k.scalar_type();
+  ckks_draft_fill_args a{};
+  a.dtype = cache_type(k, "k");
+  check_rows(c, k_cache, "k_cache", {b, hk, cap, row}, cached);
+  check_rows(c, v_cache, "v_cache", {b, hk, cap, row}, cached);
+  check_written(k_cache, "k_cache");
+  check_written(v_cache, "v_cache");
+  check_rows(c, k, "k", {t, hk, d}, k.scalar_type());
+  check_rows(c, v, "v", {t, hk, d}, k.scalar_type());
+  a.lens = small<const int32_t>(c, lens, "lens", {b}, at::kInt);
+  a.starts = starts_of(c, starts, b);
+  Tensor out = at::empty({b}, lens.options());
+  if (b) {
+    a.batch = size32(b, "batch"), a.kv_heads = size32(hk, "key/value heads"), a.head_dim = size32(d, "head size");
+    a.tokens = size32(t, "tokens"), a.capacity = size32(cap, "capacity");
+    a.k_cache = by_head(k_cache), a.v_cache = by_head(v_cache), a.k = by_token(k), a.v = by_token(v);
+    a.lens_out = out.data_ptr<int32_t>();
+    c.done((four ? ckks_draft_fill4 : ckks_draft_fill)(c.ctx, &a, c.stream()));
+  }
+  return out;
+}
+
+Tensor read4(uintptr_t ctx, int device, const Tensor& cache, const Tensor& lens, int64_t head_dim,
+             at::ScalarType dtype) {
+  const Call c{(ckks_ctx*)ctx, device};
+  four_dims(cache, "cache");
+  const int64_t b = cache.size(0), hk = cache.size(1), cap = cache.size(2);
+  check_rows(c, cache, "cache", {b, hk, cap, row4_bytes(head_dim)}, at::kByte);
+  ckks_draft_read4_args a{};
+  a.lens = small<const int32_t>(c, lens, "lens", {b}, at::kInt);
+  Tensor out = at::empty({b, hk, cap, head_dim}, cache.options().dtype(dtype));
+  a.dtype = cache_type(out, "dtype");
+  if (b && cap) {
+    a.batch = size32(b, "batch"), a.kv_heads = size32(hk, "key/value heads"), a.head_dim = size32(head_dim, "head size");
+    a.capacity = size32(cap, "capacity"), a.cache = by_head(cache), a.out = by_head(out);
+    c.done(ckks_draft_read4(c.ctx, &a, c.stream()));
+  }
+  return out;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_draft, m) {
-  m.def("attention", &attention);
+  m.def("attention", &attention<false>);
+  m.def("attention4", &attention<true>);
   m.def("verify", &verify);
-  m.def("commit", &commit);
+  m.def("commit", &commit<false>);
+  m.def("commit4", &commit<true>);
   m.def("accumulate", &accumulate);
   m.def("evict", &evict);
+  m.def("prompt", &prompt);
+  m.def("fill", &fill<false>);
+  m.def("fill4", &fill<true>);
+  m.def("read4", &read4);
+  m.def("row4_bytes", &row4_bytes);
 }

@@ -12,6 +12,12 @@ on torch's current stream (``CryptoContext`` offers them as methods):
   draft_commit       the accepted rows appended to the cache
   draft_accumulate   the attention weight they give each cached key
   draft_evict        the cache cut to its latest and heaviest keys
+  draft_prompt       causal attention within packed prompts
+  draft_fill         the prompts' rows appended to the cache
+
+and over a cache in 4 bits (9/16 of a byte an element; ``row4_bytes``)
+``draft_attention4``, ``draft_commit4``, ``draft_fill4`` and ``draft_read4``,
+which gives its values back.
 
 ``DraftModel`` is the plain draft model: blocks of the same weights that
 ``EncryptedBlock`` takes, evaluated with these operators; it stands beside
@@ -109,6 +115,63 @@ def evict(cc, k_cache, v_cache, acc, lens, budget, recent, out=None):
     k, v, acc, index [B, Hkv, budget] int32 (the rows kept, then -1) and the
     new lengths [B] int32."""
     return (_binding or _native()).evict(cc.h.value, cc.params.device, k_cache, v_cache, acc, lens, budget, recent, out)
+
+
+def prompt(cc, q, k, v, starts, scale=None):
+    """Causal attention within packed prompts of different lengths.
+
+    q [T, Hq, D]; k, v [T, Hkv, D]; starts [B + 1] int32: sequence b has the
+    rows from starts[b] to starts[b + 1] (each start taken as 0..T and as no
+    less than those before it).  bfloat16, float16 or float32, Hq a multiple of
+    Hkv, D <= 256, any strides with a contiguous last dimension.  scale defaults
+    to 1 / sqrt(D).  Returns out [T, Hq, D] in q's type and lse [T, Hq] float32,
+    the log of each row's sum; a row of no sequence is 0, its lse -inf."""
+    return (_binding or _native()).prompt(cc.h.value, cc.params.device, q, k, v, starts, scale)
+
+
+def fill(cc, k_cache, v_cache, lens, k, v, starts):
+    """Appends packed prompts' rows, k and v [T, Hkv, D] with ``starts`` as for
+    ``prompt``, to the caches [B, Hkv, capacity, D] behind lens [B] int32 (in
+    place) and returns the new lengths.  A sequence that does not fit its cache
+    is left as it is; the next ``cc.Synchronize()`` behind this stream reports
+    it."""
+    return (_binding or _native()).fill(cc.h.value, cc.params.device, k_cache, v_cache, lens, k, v, starts)
+
+
+def row4_bytes(head_dim):
+    """Bytes of one row of a 4-bit cache: the head's elements as 4-bit floating
+    point numbers (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives) in groups of
+    16, behind them a scale of 8 bits for each group (a sixth of its largest
+    magnitude, to three bits of mantissa), then zeros up to a multiple of four
+    bytes.  A 4-bit cache is a uint8 tensor [B, Hkv, capacity, row4_bytes(D)];
+    zeros are an empty one.  Magnitudes over 61440 become 61440, and a group
+    with an infinity or a NaN in it reads as NaN."""
+    return (_binding or _native()).row4_bytes(head_dim)
+
+
+def fill4(cc, k_cache, v_cache, lens, k, v, starts):
+    """``fill`` into 4-bit caches: rounds each element once, to the nearest
+    number of its group's scale."""
+    return (_binding or _native()).fill4(cc.h.value, cc.params.device, k_cache, v_cache, lens, k, v, starts)
+
+
+def commit4(cc, k_cache, v_cache, lens, k_new, v_new, path, count):
+    """``commit`` into 4-bit caches, rounded as by ``fill4``."""
+    return (_binding or _native()).commit4(cc.h.value, cc.params.device, k_cache, v_cache, lens, k_new, v_new, path,
+                                           count)
+
+
+def read4(cc, cache, lens, head_dim, dtype):
+    """The values of a 4-bit cache, [B, Hkv, capacity, head_dim] in ``dtype``
+    (bfloat16, float16 or float32; each holds them exactly), 0 behind lens."""
+    return (_binding or _native()).read4(cc.h.value, cc.params.device, cache, lens, head_dim, dtype)
+
+
+def attention4(cc, q, k_cache, v_cache, lens, k_new, v_new, parents, scale=None):
+    """``attention`` over 4-bit caches [B, Hkv, capacity, row4_bytes(D)], of
+    their exact values; the new rows are in q's type."""
+    return (_binding or _native()).attention4(cc.h.value, cc.params.device, q, k_cache, v_cache, lens, k_new, v_new,
+                                              parents, scale)
 
 
 class DraftModel:
