@@ -11,7 +11,7 @@
 #include <algorithm>
 #include <cmath>
 
-#include "draft.hpp"
+#include "draft_tc.cuh"
 
 namespace ckks {
 namespace draft {
@@ -250,6 +250,504 @@ void run_prompt(const PromptParams& p, cudaStream_t st) {
   }
 }
 
+// ---- 16-bit types: tensor cores -------------------------------------------------
+// A unit is 256 rows of one query head of one sequence: two groups of four
+// softmax warps have 128 rows each (over 128 elements there is one group, as
+// tensor memory holds one S and O then), a thread a row.  Keys come in tiles of
+// 128, each copied once for both groups: S_g = Q_g K^T into tensor memory, the
+// weights back into S's place as the 16-bit A operand of O_g += P_g V.  One warp
+// issues copies, one the products; while one group exponentiates, the products
+// of the other run.  The first group has one tile less than the second, and
+// only a group's last tile is cut by the causal mask.
+//
+// CTAs are one to an SM and take the units of the list in turns, one round
+// upwards and the next one downwards: a sequence's units lie in the list from
+// the longest on, so every CTA gets about the same.
+//
+// A row's reference point m follows the maximum only when that has grown by
+// more than 2^8; O is seldom rescaled.  A weight is rounded once, to the
+// operands' type (half a step, as the result is), and summed in 32 bits before
+// that.  Two numbers a weight, as over a cache, would be half as many products
+// again, which bound this kernel where heads are wide; one number leaves a
+// result 1.4 times as far from the exact one as its own rounding takes it.
+//
+// The exponential unit takes 8 cycles for a warp's 32: 2048 cycles for a pair of
+// tiles, whose products take 1024 at 64 elements and 2048 at 128.  So some of
+// the exponentials are computed with multiply-adds: 2^x = 2^n 2^r, n the nearest
+// integer, and 2^r the polynomial of degree 4 with the least largest relative
+// error on [-1/2, 1/2] (2.7e-6, fitted to 2^r).
+template <int PANELS>
+struct PromptShape {
+  static constexpr int kGroups = PANELS <= 2 ? 2 : 1, kThreads = 32 * (4 * kGroups + 2), kUnitRows = kM * kGroups;
+  static constexpr int kSlots = PANELS == 1 ? 10 : PANELS == 2 ? 5 : PANELS == 3 ? 3 : 2;
+  static constexpr uint32_t kTileBytes = PANELS * kPanel;
+  // Q of each group, the ring of K and V tiles, barriers, masks, one word
+  static constexpr uint32_t kRing = kGroups * kTileBytes, kExtra = kRing + kSlots * kTileBytes;
+  static constexpr int kBars = 2 * kSlots + 10;
+  static constexpr size_t kSmem = kExtra + kBars * 8 + 6 * 4 * 4 + 16;
+  // of eight pairs of exponentials, how many the multiply-adds take
+  static constexpr int kPoly = PANELS == 1 ? 3 : PANELS == 2 ? 1 : 0;
+};
+
+// a place in the list of units; walked upwards by a whole warp
+struct Unit {
+  int seq, len, row0, head;  // first row of the sequence, its length, the unit's first row of it, query head
+};
+template <int ROWS>
+struct Units {
+  Starts starts;
+  int b0 = 0, before = 0, first, len, units, sum, all;
+  __device__ __forceinline__ void load(const PromptParams& p) {
+    const int lane = threadIdx.x & 31;
+    const int2 at = starts.next(p, b0);
+    first = at.x, len = at.y;
+    sum = units = (len + ROWS - 1) / ROWS * p.q_heads;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, sum, o);
+      if (lane >= o) sum += y;
+    }
+    all = __shfl_sync(0xffffffffu, sum, 31);
+  }
+  __device__ __forceinline__ void begin(const PromptParams& p) {
+    starts.begin(p);
+    load(p);
+  }
+  // unit w, no earlier than the one before; false behind the last
+  __device__ __forceinline__ bool find(const PromptParams& p, int w, Unit& u) {
+    while (w - before >= all) {
+      if (b0 + 32 >= p.batch) return false;
+      before += all;
+      b0 += 32;
+      load(p);
+    }
+    const int k = __ffs(__ballot_sync(0xffffffffu, sum > w - before)) - 1;
+    const int n = __shfl_sync(0xffffffffu, units, k), off = w - before - (__shfl_sync(0xffffffffu, sum, k) - n);
+    u.seq = __shfl_sync(0xffffffffu, first, k);
+    u.len = __shfl_sync(0xffffffffu, len, k);
+    u.row0 = ((n - 1 - off) / p.q_heads) * ROWS;
+    u.head = off % p.q_heads;
+    return true;
+  }
+};
+
+// 2^x for x >= -126; what lies below comes out next to 0
+__device__ __forceinline__ float2 exp2_poly(float2 x) {
+  const float2 big = make_float2(12582912.0f, 12582912.0f);  // 1.5 2^23: the sum's low bits are the nearest integer
+  x.x = fmaxf(x.x, -126.0f), x.y = fmaxf(x.y, -126.0f);
+  const float2 t = add2(x, big), r = sub2(x, sub2(t, big));
+  auto two = [](float v) { return make_float2(v, v); };
+  float2 y = fma2(r, two(0.00957053154706955f), two(0.05591866374015808f));
+  y = fma2(y, r, two(0.24024735391139984f));
+  y = fma2(y, r, two(0.6931216716766357f));
+  y = fma2(y, r, two(0.9999992847442627f));
+  return make_float2(__uint_as_float(__float_as_uint(y.x) + (__float_as_uint(t.x) << 23)),
+                     __uint_as_float(__float_as_uint(y.y) + (__float_as_uint(t.y) << 23)));
+}
+
+// the largest of three; a NaN wins
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
+// takes the elements that are not finite out of a piece of a row; whether there were any
+template <typename T>
+__device__ __forceinline__ bool take_out(uint4* piece) {
+  constexpr uint32_t e = std::is_same_v<T, __nv_bfloat16> ? 0x7F80u : 0x7C00u;
+  const uint4 v = *piece;
+  if (!not_finite<T>(v)) return false;
+  uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    if ((w[k] & e) == e) w[k] &= 0xFFFF0000u;
+    if ((w[k] >> 16 & e) == e) w[k] &= 0xFFFFu;
+  }
+  *piece = make_uint4(w[0], w[1], w[2], w[3]);
+  return true;
+}
+
+// adds to a finished row what was taken out of the rows `which` (32 from `key0`
+// on) that it sees: an infinity or a NaN shows whatever its weight
+template <typename T>
+__device__ __noinline__ void add_taken_out(const PromptParams& p, const Unit& u, uint32_t which, int key0, int row,
+                                           T* out) {
+  for (; which; which &= which - 1) {
+    const int j = key0 + __ffs(which) - 1;
+    if (j > row) break;
+    const T* v = static_cast<const T*>(p.v.data) + (int64_t)(u.seq + j) * p.v.row + u.head / p.group * p.v.head;
+    for (int d = 0; d < p.head_dim; ++d) {
+      const float x = to_f32(v[d]);
+      if (!(fabsf(x) < INFINITY)) out[d] = from_f32<T>(to_f32(out[d]) + x);
+    }
+  }
+}
+
+struct PromptMaps {
+  CUtensorMap q, k, v;
+};
+
+template <typename T, int PANELS>
+__global__ void __launch_bounds__(PromptShape<PANELS>::kThreads, 1)
+    prompt_tc_kernel(const __grid_constant__ PromptParams p, const __grid_constant__ PromptMaps maps, bool negative,
+                     float c, unsigned int* __restrict__ faults) {
+  using S = PromptShape<PANELS>;
+  constexpr int DP = 64 * PANELS, NS = S::kSlots, GR = S::kGroups, ROWS = S::kUnitRows;
+  constexpr bool kBf = std::is_same_v<T, __nv_bfloat16>;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  uint64_t* const s_bar = reinterpret_cast<uint64_t*>(smem + S::kExtra);
+  // rows of a group's last tile from which elements were taken out, of two
+  // units; then the same of the first group's for the second, of two pairs
+  uint32_t(*const s_out)[4] = reinterpret_cast<uint32_t(*)[4]>(s_bar + S::kBars);
+  uint32_t* const s_tmem = reinterpret_cast<uint32_t*>(s_out + 6);
+  const uint32_t sq = smem_addr(smem), ring = sq + S::kRing, bars = smem_addr(s_bar);
+  auto full = [&](int s) { return bars + 8 * s; };
+  auto empty = [&](int s) { return bars + 8 * (NS + s); };
+  auto s_full = [&](int g) { return bars + 8 * (2 * NS + g); };
+  auto p_ready = [&](int g) { return bars + 8 * (2 * NS + 2 + g); };
+  auto q_full = [&](int g) { return bars + 8 * (2 * NS + 4 + g); };
+  auto q_empty = [&](int g) { return bars + 8 * (2 * NS + 6 + g); };
+  auto o_full = [&](int g) { return bars + 8 * (2 * NS + 8 + g); };
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (tid == 0) {
+    for (int s = 0; s < NS; ++s) {
+      mbar_init(full(s), 1);
+      mbar_init(empty(s), 1);
+    }
+    for (int g = 0; g < 2; ++g) {
+      mbar_init(s_full(g), 1);
+      mbar_init(p_ready(g), 4);
+      mbar_init(q_full(g), 1);
+      mbar_init(q_empty(g), 1);
+      mbar_init(o_full(g), 1);
+    }
+  }
+  if (warp == 4 * GR + 1) tmem_alloc(smem_addr(s_tmem), kTmemCols);
+  if (warp == 4 * GR && lane == 0) {
+    tile_prefetch(&maps.q);
+    tile_prefetch(&maps.k);
+    tile_prefetch(&maps.v);
+  }
+  tmem_fence_before();
+  __syncthreads();
+  tmem_fence_after();
+  const uint32_t tmem = *s_tmem;  // S of every group, then O of every group
+  Units<ROWS> list;
+  list.begin(p);
+  Unit u;
+  // round r's unit of this CTA
+  auto unit_of = [&](int r) {
+    return r * (int)gridDim.x + (r & 1 ? (int)gridDim.x - 1 - (int)blockIdx.x : (int)blockIdx.x);
+  };
+  // tiles of group g in this unit
+  auto tiles_of = [&](int g) { return u.row0 + kM * g < u.len ? u.row0 / kM + g + 1 : 0; };
+  bool fine = true;  // no wait gave up
+  if (warp == 4 * GR) {
+    // ---- copies
+    int slot = 0, lap = 0, nq[2] = {0, 0}, k = 0;
+    for (int r = 0; fine && list.find(p, unit_of(r), u); ++r) {
+      if (lane == 0) {
+        const int n = max(tiles_of(0), GR > 1 ? tiles_of(1) : 0), kv = u.head / p.group;
+        auto load = [&](const CUtensorMap* m, int tile) {
+          if (lap > 0 && !mbar_wait_short(empty(slot), (lap - 1) & 1)) return fine = false;
+          mbar_expect_tx(full(slot), S::kTileBytes);
+#pragma unroll
+          for (int x = 0; x < PANELS; ++x)
+            tile_load(ring + slot * S::kTileBytes + x * kPanel, m, 64 * x, u.seq + tile * kKeys, kv, 0, full(slot));
+          ++k;
+          if (++slot == NS) slot = 0, ++lap;
+          return true;
+        };
+        load(&maps.k, 0);
+#pragma unroll
+        for (int g = 0; g < GR; ++g) {
+          if (!fine || !tiles_of(g)) continue;
+          if (nq[g] > 0 && !(fine = mbar_wait_short(q_empty(g), (nq[g] - 1) & 1))) continue;
+          ++nq[g];
+          mbar_expect_tx(q_full(g), S::kTileBytes);
+#pragma unroll
+          for (int x = 0; x < PANELS; ++x)
+            tile_load(sq + g * S::kTileBytes + x * kPanel, &maps.q, 64 * x, u.seq + u.row0 + kM * g, u.head, 0,
+                      q_full(g));
+        }
+        for (int t = 0; t < n && fine; ++t)
+          if (load(&maps.v, t) && t + 1 < n) load(&maps.k, t + 1);
+      }
+      fine = __shfl_sync(0xffffffffu, fine, 0);
+    }
+    if (lane == 0) {
+      // copies still in flight land before the CTA ends
+      for (int j = k > NS ? k - NS : 0; j < k; ++j) fine = mbar_wait_short(full(j % NS), (j / NS) & 1) && fine;
+#pragma unroll
+      for (int g = 0; g < GR; ++g)
+        if (nq[g]) fine = mbar_wait_short(q_full(g), (nq[g] - 1) & 1) && fine;
+    }
+  } else if (warp == 4 * GR + 1) {
+    // ---- products, by the whole warp in step
+    constexpr uint32_t word_s = mma_word(kBf, kM, kKeys, false), word_o = mma_word(kBf, kM, DP, true);
+    const uint32_t t_base = __shfl_sync(0xffffffffu, tmem, 0);
+    int slot = 0;
+    uint32_t lap = 0, q_phase = 0, p_phase = 0;
+    for (int r = 0; fine && list.find(p, unit_of(r), u); ++r) {
+      int n[2] = {__shfl_sync(0xffffffffu, tiles_of(0), 0), GR > 1 ? __shfl_sync(0xffffffffu, tiles_of(1), 0) : 0};
+      const int most = max(n[0], n[1]);
+      auto next = [&] {
+        if (++slot == NS) slot = 0, lap ^= 1u;
+      };
+      auto scores = [&](int g, int t, int s) {
+        const uint32_t qb = sq + g * S::kTileBytes, kb = ring + s * S::kTileBytes;
+#pragma unroll
+        for (int i = 0; i < DP / 16; ++i) {
+          const uint32_t off = (i / 4) * kPanel + (i % 4) * 32;
+          mma_smem(t_base + 128 * g, smem_operand(qb + off, 16), smem_operand(kb + off, 16), word_s, i > 0);
+        }
+        mma_commit(s_full(g));
+        if (t + 1 == n[g]) mma_commit(q_empty(g));
+      };
+      if (!(fine = warp_wait(full(slot), lap))) break;
+#pragma unroll
+      for (int g = 0; g < GR; ++g) {
+        if (!n[g]) continue;
+        if (!(fine = warp_wait(q_full(g), q_phase >> g & 1))) break;
+        q_phase ^= 1u << g;
+        tmem_fence_after();
+        scores(g, 0, slot);
+      }
+      if (!fine) break;
+      mma_commit(empty(slot));
+      next();
+      for (int t = 0; t < most && fine; ++t) {
+        const int vs = slot;
+        const uint32_t vlap = lap;
+        next();
+        const int ks = slot;  // of the next tile's keys
+        const uint32_t klap = lap;
+        bool waited = false, waited_k = false;
+#pragma unroll
+        for (int g = 0; g < GR; ++g) {
+          if (t >= n[g]) continue;
+          if (!waited) {
+            if (!(fine = warp_wait(full(vs), vlap))) break;
+            waited = true;
+          }
+          if (!(fine = warp_wait(p_ready(g), p_phase >> g & 1))) break;
+          p_phase ^= 1u << g;
+          tmem_fence_after();
+          const uint32_t vb = ring + vs * S::kTileBytes;
+#pragma unroll
+          for (int i = 0; i < kKeys / 16; ++i)
+            mma_tmem(t_base + 128 * (GR + g), t_base + 128 * g + 8 * i, smem_operand(vb + 2048 * i, kPanel), word_o,
+                     i > 0 || t > 0);
+          if (t + 1 < n[g]) {
+            if (!waited_k) {
+              if (!(fine = warp_wait(full(ks), klap))) break;
+              waited_k = true;
+            }
+            scores(g, t + 1, ks);
+          } else {
+            mma_commit(o_full(g));
+          }
+        }
+        if (!fine) break;
+        mma_commit(empty(vs));
+        if (t + 1 < most) {
+          mma_commit(empty(ks));
+          next();
+        }
+      }
+    }
+  } else {
+    // ---- softmax: group g, tensor-memory lane L, that is row L of the group's
+    const int g = warp >> 2, quarter = warp & 3, L = quarter * 32 + lane;
+    const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+    const uint32_t t_s = tmem + 128 * g + lanes, t_o = tmem + 128 * (GR + g) + lanes;
+    int base = 0, nu = 0, pairs = 0;  // tiles of keys and values before this unit's; units of this group, of both
+    uint32_t phase = 0;
+    for (int r = 0; fine && list.find(p, unit_of(r), u); ++r) {
+      const int n = tiles_of(g), most = max(n, GR > 1 ? tiles_of(g ^ 1) : 0);
+      const bool both = GR > 1 && n && tiles_of(g ^ 1);
+      float m = -INFINITY, l = 0.0f;
+#pragma unroll 1
+      for (int t = 0; t < n; ++t) {
+        const bool last = t + 1 == n;
+        if (!(fine = warp_wait(s_full(g), phase))) break;
+        phase ^= 1u;
+        if (last) {
+          // The values of keys that only some rows of this tile see: what is
+          // not finite is taken out of the product.  (The copy that had the slot
+          // before was used ahead of this tile's scores, so the wait cannot take
+          // its arrival for this one's.)
+          const int kv = base + 2 * t + 1;
+          if (!(fine = warp_wait(full(kv % NS), (kv / NS) & 1))) break;
+          uint8_t* vs = smem + S::kRing + (kv % NS) * S::kTileBytes + L * 128;
+          bool out = false;
+#pragma unroll
+          for (int i = 0; i < DP / 8; ++i)
+            out |= take_out<T>(reinterpret_cast<uint4*>(vs + (i / 8) * kPanel + ((i % 8) << 4)));
+          const uint32_t some = __ballot_sync(0xffffffffu, out);
+          if (some) smem_fence_async();
+          if (lane == 0) {
+            s_out[2 * g + (nu & 1)][quarter] = some;
+            if (both && g == 0) s_out[4 + (pairs & 1)][quarter] = some;
+          }
+        }
+        tmem_fence_after();
+        uint32_t x[kKeys];
+        tmem_load<kKeys>(t_s, x);
+        tmem_wait_load();
+        if (negative) {  // scores of -q
+#pragma unroll
+          for (int i = 0; i < kKeys; ++i) x[i] ^= 0x80000000u;
+        }
+        if (last) {
+#pragma unroll
+          for (int i = 0; i < kKeys; ++i)
+            if (i > L) x[i] = __float_as_uint(-INFINITY);
+        }
+        float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int i = 0; i < kKeys; i += 2)
+          mx4[i / 2 & 3] = max3(mx4[i / 2 & 3], __uint_as_float(x[i]), __uint_as_float(x[i + 1]));
+        const float mx = max3(max3(mx4[0], mx4[1], mx4[2]), mx4[3], -INFINITY);
+        float top = mx == -INFINITY ? mx : fmaf(mx, c, -kBelow<T>);
+        float f = 1.0f;
+        if (!(top <= m + kSlack)) {  // grown, or no number
+          if (!(top < INFINITY)) top = __uint_as_float(0x7FC00000u);  // an infinite score leaves no number
+          f = m == -INFINITY && top == top ? 0.0f : ex2(m - top);
+          m = top;
+          l *= f;
+        }
+        if (t > 0 && __any_sync(0xffffffffu, f != 1.0f)) {
+          // the sums so far, on the new reference point
+#pragma unroll 1
+          for (int i = 0; i < DP; i += 16) {
+            uint32_t o[16];
+            tmem_load<16>(t_o + i, o);
+            tmem_wait_load();
+#pragma unroll
+            for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
+            tmem_store<16>(t_o + i, o);
+          }
+        }
+        const float ref = m == -INFINITY ? 0.0f : m;
+        // the weights take the place of their scores.  A masked score's is 0, and
+        // so are those of a row that has seen none above -inf
+        float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+        auto weights = [&](auto poly) {
+#pragma unroll
+          for (int i0 = 0; i0 < kKeys; i0 += 32) {
+            uint32_t w[16];
+#pragma unroll
+            for (int i = 0; i < 32; i += 2) {
+              const float2 s2 = fma2(make_float2(__uint_as_float(x[i0 + i]), __uint_as_float(x[i0 + i + 1])),
+                                     make_float2(c, c), make_float2(-ref, -ref));
+              float2 e;
+              if ((i / 2) % 8 < decltype(poly)::value)
+                e = exp2_poly(s2);
+              else
+                e = make_float2(ex2(s2.x), ex2(s2.y));
+              sum[i / 2 & 1] = add2(sum[i / 2 & 1], e);
+              w[i / 2] = pack2<T>(e.x, e.y);
+            }
+            tmem_store<16>(t_s + i0 / 2, w);
+          }
+        };
+        if (last || __any_sync(0xffffffffu, m == -INFINITY))
+          weights(std::integral_constant<int, 0>{});
+        else
+          weights(std::integral_constant<int, S::kPoly>{});
+        l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+        tmem_wait_store();
+        tmem_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(p_ready(g));
+      }
+      if (!fine) break;
+      base += 2 * most;
+      if (n) {
+        if (!(fine = warp_wait(o_full(g), nu & 1))) break;
+        tmem_fence_after();
+        const int row = u.row0 + kM * g + L;
+        const bool mine = row < u.len;
+        const float inv = l != 0.0f ? 1.0f / l : 0.0f;
+        T* const out = static_cast<T*>(p.out.data) + (int64_t)(u.seq + row) * p.out.row + u.head * p.out.head;
+#pragma unroll 1
+        for (int i = 0; i < DP; i += 32) {
+          uint32_t o[32];
+          tmem_load<32>(t_o + i, o);
+          tmem_wait_load();
+          if (mine) {
+#pragma unroll
+            for (int j = 0; j < 32; j += 8) {
+              uint32_t w[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                w[e] = pack2<T>(__uint_as_float(o[j + 2 * e]) * inv, __uint_as_float(o[j + 2 * e + 1]) * inv);
+              if (i + j < p.head_dim) *reinterpret_cast<uint4*>(out + i + j) = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+          }
+        }
+        if (mine) {
+          p.lse[(int64_t)(u.seq + row) * p.q_heads + u.head] = l != 0.0f ? kLn2 * (m + log2f(l)) : -INFINITY;
+          const uint32_t* own = s_out[2 * g + (nu & 1)];
+          const uint32_t* other = s_out[4 + (pairs & 1)];
+          uint32_t any = own[0] | own[1] | own[2] | own[3];
+          if (both && g == 1) any |= other[0] | other[1] | other[2] | other[3];
+          if (any) {
+            const int tile0 = (n - 1) * kKeys;
+            if (both && g == 1)
+              for (int q = 0; q < 4; ++q) add_taken_out<T>(p, u, other[q], tile0 - kKeys + 32 * q, row, out);
+            for (int q = 0; q < 4; ++q) add_taken_out<T>(p, u, own[q], tile0 + 32 * q, row, out);
+          }
+        }
+        __syncwarp();
+        ++nu;
+        pairs += both;
+        tmem_fence_before();
+      }
+    }
+    if (fine) clear_spare<T>(p, list.starts.first, list.starts.last, 128 * GR);
+  }
+  if (!fine && (warp < 4 * GR || lane == 0)) atomicAdd(faults, 1u);
+  tmem_fence_before();
+  __syncthreads();
+  if (warp == 4 * GR + 1) {
+    __syncwarp();
+    tmem_free(tmem, kTmemCols);
+  }
+}
+
+template <typename T, int PANELS>
+void launch_prompt_tc(const Context& c, const PromptParams& p, const PromptMaps& maps, cudaStream_t st) {
+  using S = PromptShape<PANELS>;
+  static_assert(S::kSmem <= 232448, "shared memory of one block");
+  auto* k = prompt_tc_kernel<T, PANELS>;
+  CKKS_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::kSmem));
+  // a scale of 0 becomes one that changes no weight: a masked score times 0 would be no number
+  const float factor = std::max(std::fabs(p.scale) * kLog2e, 1e-30f);
+  const long long units = (long long)std::max(1, p.batch + p.tokens / S::kUnitRows) * p.q_heads;
+  k<<<(unsigned)std::min<long long>(units, c.sms), S::kThreads, S::kSmem, st>>>(p, maps, p.scale < 0.0f, factor,
+                                                                               c.d_faults);
+  CKKS_CUDA(cudaGetLastError());
+}
+
+template <typename T>
+bool run_prompt_tc(const Context& c, int dtype, int kv_heads, const PromptParams& p, cudaStream_t st) {
+  PromptMaps m;
+  auto map = [&](CUtensorMap* t, const ckks_rows& r, int heads) {
+    return tile_map(t, r.data, dtype, p.head_dim, p.tokens, r.row, kM, heads, r.head, 1, 1, 0);
+  };
+  if (!map(&m.q, p.q, p.q_heads) || !map(&m.k, p.k, kv_heads) || !map(&m.v, p.v, kv_heads)) return false;
+  switch ((p.head_dim + 63) / 64) {
+    case 1: launch_prompt_tc<T, 1>(c, p, m, st); break;
+    case 2: launch_prompt_tc<T, 2>(c, p, m, st); break;
+    case 3: launch_prompt_tc<T, 3>(c, p, m, st); break;
+    default: launch_prompt_tc<T, 4>(c, p, m, st); break;
+  }
+  return true;
+}
+
 }  // namespace
 }  // namespace draft
 }  // namespace ckks
@@ -289,6 +787,12 @@ extern "C" int ckks_draft_prompt(ckks_ctx* ctx, const ckks_draft_prompt_args* ar
     OnDevice dev(c);
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     ProfScope ps(c, "draft_prompt", 2.0 * e * a.tokens * (a.q_heads + a.kv_heads) * a.head_dim, st);
+    // strides that no tensor map holds are left to the plain kernel
+    if (p.wide && a.dtype != CKKS_FP32) {
+      if (a.dtype == CKKS_BF16 ? run_prompt_tc<__nv_bfloat16>(c, a.dtype, a.kv_heads, p, st)
+                               : run_prompt_tc<__half>(c, a.dtype, a.kv_heads, p, st))
+        return;
+    }
     if (a.dtype == CKKS_BF16)
       run_prompt<__nv_bfloat16>(p, st);
     else if (a.dtype == CKKS_FP16)
