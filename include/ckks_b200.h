@@ -634,7 +634,9 @@ typedef struct {
 int ckks_draft_read4(ckks_ctx* ctx, const ckks_draft_read4_args* args, void* stream);
 
 /* ckks_draft_attention over 4-bit caches (dtype: of q, k_new, v_new and out).
- * Scores and sums are those of the caches' exact values. */
+ * Scores and sums are those of the caches' exact values; between the two
+ * products a softmax weight keeps 11 bits with 16-bit tensors (in steps of
+ * 2^-31 of the row's largest at the finest) and 24 with float32 ones. */
 int ckks_draft_attention4(ckks_ctx* ctx, const ckks_draft_attention_args* args, void* stream);
 long long ckks_draft_attention4_workspace(ckks_ctx* ctx, const ckks_draft_attention_args* args);
 

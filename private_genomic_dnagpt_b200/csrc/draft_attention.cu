@@ -1324,7 +1324,9 @@ size_t workspace_of(const Context& c, const ckks_draft_attention_args& a) {
 size_t workspace4_of(const Context& c, const ckks_draft_attention_args& a) {
   if (a.batch == 0) return 0;
   const int s = split_count(c, a);
-  return s == 1 ? 0 : sizeof(float) * (size_t)a.batch * a.q_heads * a.nodes * s * (a.head_dim + 2);
+  // the caches' strides decide which kernel runs
+  const size_t plain = s == 1 ? 0 : sizeof(float) * (size_t)a.batch * a.q_heads * a.nodes * s * (a.head_dim + 2);
+  return std::max(plain, attention4_tc_workspace(c, a));
 }
 
 AttnParams with(AttnParams p, const Division& d) {
@@ -1481,7 +1483,9 @@ int run(ckks_ctx* ctx, const ckks_draft_attention_args* args, void* stream) {
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     const double bytes = 2.0 * a.batch * a.kv_heads * a.capacity * (FOUR ? row4_bytes(a.head_dim) : e * a.head_dim);
     ProfScope ps(c, FOUR ? "draft_attention4" : "draft_attention", bytes, st);
-    if constexpr (!FOUR) {
+    if constexpr (FOUR) {
+      if (attention4_tc(c, a, st)) return;
+    } else {
       // strides that no tensor map holds are left to the plain kernel
       if (p.wide && takes_tc(c, a)) {
         if (a.dtype == CKKS_BF16 ? run_tc<__nv_bfloat16>(c, a, p, st) : run_tc<__half>(c, a, p, st)) return;

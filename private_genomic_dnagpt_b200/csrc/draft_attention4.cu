@@ -1,0 +1,764 @@
+// draft_attention4.cu -- attention of a tree of drafted nodes over a 4-bit
+// cache on the tensor cores (what ckks_draft_attention4 does with 16-bit rows
+// and contiguous caches; draft_attention.cu has the rest).
+//
+// For the rows r = (node, query head) of one key/value head over the cached
+// keys k < len, with the codes' values K and V (draft_fp4.cuh):
+//   S^T = K Q^T,  P^T = 2^(c_r S^T - m_r),  O^T += V^T P,  l_r = sum_k P_rk.
+// Few rows read many keys, so the keys are the 128 rows of the first product
+// and the elements of V those of the second: their cost grows with the rows
+// (4 cycles a row and 128 keys of 128), and not with 128 rows whatever there are.
+//
+// One CTA per SM.  A thread copies tiles of 128 keys as they are (9/16 of a
+// byte an element); four warps decode K, a thread a key, into tensor memory as the first
+// product's A operand, four decode V into shared memory as the second's; one
+// warp issues the products; one or two groups of four warps, a thread a key,
+// turn scores into weights.  Every step has two buffers, so that each works on
+// another tile.
+//
+// All operands are float16: it holds the caches' values exactly, and a
+// bfloat16 query, scaled by a power of two for each row, to 2^-24 of the
+// row's largest element, which is what a 32-bit sum of products keeps.  A weight
+// has float16's 11 bits.  A row's reference point m lies 2^7 below the maximum
+// when it is set, and is set anew where a score passes it by more than 2^8 more: weights
+// end at 2^15.  Sums are in 32 bits.
+//
+// The lengths are known on the device only, so the CTAs divide the list of all
+// units' tiles evenly, a unit being (sequence, head, up to 64 rows).  Each
+// leaves (m, l, O) of its part of a unit in the workspace, and a second kernel,
+// a warp a row, joins them with the new keys of the row's ancestors, which it
+// takes on the CUDA cores while the first kernel still runs.
+#include <algorithm>
+#include <cmath>
+
+#include "draft_fp4.cuh"
+#include "draft_tc.cuh"
+
+namespace ckks {
+namespace draft {
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+constexpr float kUnset = -3.0e38f;  // reference point of a row that has seen no key
+
+struct Params4 {
+  ckks_rows q, kc, vc, kn, vn, out;
+  const int32_t* lens;
+  const int32_t* parents;
+  float* lse;
+  float* part;  // [units + CTAs][N][DP + 4]
+  int batch, kv_heads, group, head_dim, nodes, capacity;
+  int tiles_r, unit_cost, ctas, row_bytes;
+  float scale;
+  bool bf16, wide;  // of the queries; new rows are whole, aligned 16-byte pieces
+};
+
+__device__ __forceinline__ int length_of(const Params4& p, int b) { return min(max(p.lens[b], 0), p.capacity); }
+// entries of a unit of sequence b in the list: its tiles, and what its start and end cost
+__device__ __forceinline__ int entries_of(const Params4& p, int b) {
+  const int t = (length_of(p, b) + kKeys - 1) / kKeys;
+  return t ? t + p.unit_cost : 0;
+}
+
+// A part of a unit: the tiles [tile, tile + n) of sequence b's unit `unit`
+struct Piece {
+  int b, unit, tile, n;
+};
+
+// The pieces of one CTA, in their order; by a whole warp
+struct Pieces4 {
+  int w, w1, b, unit, entry, entries, units;
+  __device__ __forceinline__ void begin(const Params4& p, int& all) {
+    units = p.kv_heads * p.tiles_r;
+    auto of = [&](int i) { return entries_of(p, i); };
+    int first;
+    all = list_sum(p.batch, of, first) * units;
+    const int ctas = min((int)gridDim.x, all), i = blockIdx.x;
+    w = w1 = 0;
+    if (i >= ctas) return;
+    w = list_start(all, i, ctas), w1 = list_start(all, i + 1, ctas);
+    const ListPlace at = list_find(p.batch, units, w, first, of);
+    b = at.b, unit = at.unit, entry = at.entry, entries = at.entries;
+  }
+  // false behind the last piece; a piece may have no tiles (n = 0)
+  __device__ __forceinline__ bool next(const Params4& p, Piece& x) {
+    if (w >= w1) return false;
+    const int here = min(entries - entry, w1 - w);
+    const int skip = max(0, min(p.unit_cost - entry, here));
+    x = {b, unit, max(0, entry - p.unit_cost), here - skip};
+    w += here;
+    entry = 0;
+    if (w < w1 && ++unit == units) {
+      unit = 0;
+      do entries = entries_of(p, ++b);
+      while (entries == 0);  // w1 lies behind no sequence without keys
+    }
+    return true;
+  }
+};
+
+// by panels of 64 elements of head_dim (1, 2 or 4) and rows of a unit
+template <int PANELS, int N>
+struct Shape4 {
+  static constexpr int DP = 64 * PANELS;
+  static constexpr int kBlocks = PANELS <= 2 ? 1 : 2;    // of 128 elements, in the second product
+  static constexpr int kGroups = N == 64 ? 2 : 1;        // of softmax warps
+  static constexpr int kCols = N / kGroups;              // rows that a softmax thread has
+  static constexpr int kWarps = 4 * kGroups + 10, kThreads = 32 * kWarps;
+  static constexpr int kRowMost = row4_bytes(DP);
+  static constexpr uint32_t kRaw = (kKeys * kRowMost + 16 + 127) / 128 * 128;  // one tile of K or V as it is
+  static constexpr int kSlots = PANELS == 1 ? 6 : PANELS == 2 ? 4 : 2;
+  static constexpr uint32_t kValues = kBlocks * 2 * kPanel;                    // one decoded tile of V
+  static constexpr int kValueBufs = PANELS <= 2 ? 2 : 1;
+  static constexpr uint32_t kQ = PANELS * N * 128;
+  static constexpr uint32_t kP = kPanel;                                       // 128 keys x up to 64 rows
+  static constexpr uint32_t kAtQ = kValueBufs * kValues, kAtP = kAtQ + (kQ + 1023) / 1024 * 1024, kAtRaw = kAtP + 2 * kP;
+  static constexpr uint32_t kAtRows = kAtRaw + 2 * kSlots * kRaw;              // float2 [2][N], float [5][N]
+  static constexpr uint32_t kAtBars = kAtRows + N * (2 * 8 + 5 * 4);
+  static constexpr int kBars = 2 * kSlots + 12;
+  static constexpr size_t kSmem = kAtBars + kBars * 8 + 16;
+  // tensor memory: K twice, S twice, O
+  static constexpr int kColS = DP, kColO = DP + 2 * N;
+  static_assert(kColO + kBlocks * N <= kTmemCols);
+};
+
+// the sum over a warp of N columns: lane x gets columns x, x + 32, ... (N 16: x % 16)
+template <int N>
+__device__ __forceinline__ float warp_columns(float* v) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int o = 16, n = N; o; o >>= 1) {
+    if (n > 1) {
+      // halves of the columns go to the lanes whose bit is clear and set
+      const bool up = lane & o;
+#pragma unroll
+      for (int i = 0; i < n / 2; ++i) {
+        const float give = up ? v[i] : v[i + n / 2], keep = up ? v[i + n / 2] : v[i];
+        v[i] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+      }
+      n /= 2;
+    } else {
+      v[0] += __shfl_xor_sync(0xffffffffu, v[0], o);
+    }
+  }
+  return v[0];
+}
+// the column that a lane has then
+template <int N>
+__device__ __forceinline__ int column_of(int lane) {
+  return N == 32 ? lane : lane >> 1;
+}
+
+// monotone integers of floats, for the largest of a warp
+__device__ __forceinline__ int ordered(float x) {
+  const int i = __float_as_int(x);
+  return i ^ (i >> 31 & 0x7FFFFFFF);
+}
+__device__ __forceinline__ float unordered(int i) { return __int_as_float(i ^ (i >> 31 & 0x7FFFFFFF)); }
+
+// a row's codes and scales from shared memory: word i of it
+struct RowWords {
+  const uint8_t* at;
+  __device__ __forceinline__ uint32_t word(int i) const { return *reinterpret_cast<const uint32_t*>(at + 4 * i); }
+};
+
+// one group of 16 elements as 8 pairs of float16
+__device__ __forceinline__ void decode_group(uint32_t a, uint32_t b, uint32_t scale, uint32_t* out) {
+  const __half2 s = __half2half2(scale4(scale));
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const __half2 h = decode4((i < 4 ? a >> (8 * i) : b >> (8 * (i - 4))) & 0xFFu, s);
+    out[i] = *reinterpret_cast<const uint32_t*>(&h);
+  }
+}
+
+template <int PANELS, int N>
+__global__ void __launch_bounds__(Shape4<PANELS, N>::kThreads, 1)
+    attend4_kernel(const __grid_constant__ Params4 p, unsigned int* __restrict__ faults) {
+  using S = Shape4<PANELS, N>;
+  constexpr int DP = S::DP, NS = S::kSlots, GR = S::kGroups, C = S::kCols, VB = S::kValueBufs;
+  constexpr int kWarpK = 4 * GR, kWarpV = kWarpK + 4, kWarpCopy = kWarpV + 4, kWarpMma = kWarpCopy + 1;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  float2* const s_row = reinterpret_cast<float2*>(smem + S::kAtRows);      // [2][N] factor and reference point
+  float* const s_max = reinterpret_cast<float*>(s_row + 2 * N);            // [4][N]
+  float* const s_fac = s_max + 4 * N;                                      // [N]
+  uint64_t* const s_bar = reinterpret_cast<uint64_t*>(smem + S::kAtBars);
+  uint32_t* const s_tmem = reinterpret_cast<uint32_t*>(s_bar + S::kBars);
+  const uint32_t base = smem_addr(smem), bars = smem_addr(s_bar);
+  auto raw_full = [&](int s) { return bars + 8 * s; };
+  auto raw_empty = [&](int s) { return bars + 8 * (NS + s); };
+  auto k_ready = [&](int i) { return bars + 8 * (2 * NS + i); };
+  auto s_full = [&](int i) { return bars + 8 * (2 * NS + 2 + i); };
+  auto v_ready = [&](int i) { return bars + 8 * (2 * NS + 4 + i); };
+  auto p_ready = [&](int i) { return bars + 8 * (2 * NS + 6 + i); };
+  auto pv_done = [&](int i) { return bars + 8 * (2 * NS + 8 + i); };
+  auto v_free = [&](int i) { return bars + 8 * (2 * NS + 8 + (VB == 2 ? i : 2)); };
+  const uint32_t q_ready = bars + 8 * (2 * NS + 11);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  asm volatile("griddepcontrol.launch_dependents;");
+  if (tid == 0) {
+    for (int s = 0; s < NS; ++s) {
+      mbar_init(raw_full(s), 1);
+      mbar_init(raw_empty(s), 8);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(k_ready(i), 4);
+      mbar_init(s_full(i), 1);
+      mbar_init(v_ready(i), 4);
+      mbar_init(p_ready(i), 4 * GR);
+      mbar_init(pv_done(i), 1);
+    }
+    mbar_init(bars + 8 * (2 * NS + 10), 1);
+    mbar_init(q_ready, 4 * GR);
+  }
+  if (warp == kWarpMma) tmem_alloc(smem_addr(s_tmem), kTmemCols);
+  // what a head has no elements for stays 0
+  for (int i = tid; i < (int)(S::kValueBufs * S::kValues / 16); i += S::kThreads)
+    reinterpret_cast<uint4*>(smem)[i] = make_uint4(0, 0, 0, 0);
+  smem_fence_async();
+  tmem_fence_before();
+  __syncthreads();
+  tmem_fence_after();
+  const uint32_t tmem = *s_tmem;
+  Pieces4 list;
+  int all;
+  list.begin(p, all);
+  Piece x = {0, 0, 0, 0};
+  bool fine = true;  // no wait gave up
+  const int G = groups4(p.head_dim), R = p.row_bytes;
+  auto source = [&](const ckks_rows& r, int tile) {
+    return static_cast<const uint8_t*>(r.data) + x.b * r.batch + x.unit / p.tiles_r * r.head + (int64_t)tile * (kKeys * R);
+  };
+  if (warp == kWarpCopy) {
+    // ---- copies.  A tile may start on any 4-byte boundary; the copy takes the
+    // aligned 16-byte pieces that hold its bytes (all of them in the tensor's own
+    // 16-byte pieces of memory).
+    int slot = 0, lap = 0, k = 0;
+    while (fine && list.next(p, x)) {
+      if (lane == 0) {
+        const int len = length_of(p, x.b);
+        for (int t = x.tile; t < x.tile + x.n && fine; ++t) {
+          if (lap > 0 && !(fine = mbar_wait_short(raw_empty(slot), (lap - 1) & 1))) break;
+          const uint32_t bytes = min(kKeys, len - t * kKeys) * R;
+          const uint8_t* from[2] = {source(p.kc, t), source(p.vc, t)};
+          uint32_t size[2];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const uint32_t off = (uint32_t)reinterpret_cast<uintptr_t>(from[i]) & 15u;
+            from[i] -= off;
+            size[i] = (off + bytes + 15u) & ~15u;
+          }
+          mbar_expect_tx(raw_full(slot), size[0] + size[1]);
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            bulk_load(base + S::kAtRaw + (2 * slot + i) * S::kRaw, from[i], size[i], raw_full(slot));
+          ++k;
+          if (++slot == NS) slot = 0, ++lap;
+        }
+      }
+      fine = __shfl_sync(0xffffffffu, fine, 0);
+    }
+    // copies still in flight land before the CTA ends
+    if (lane == 0)
+      for (int j = k > NS ? k - NS : 0; j < k; ++j) fine = mbar_wait_short(raw_full(j % NS), (j / NS) & 1) && fine;
+  } else if (warp >= kWarpK && warp < kWarpCopy) {
+    // ---- decoding, a thread a key: K into tensor memory, V into shared memory
+    const bool value = warp >= kWarpV;
+    const int key = (warp & 3) * 32 + lane;
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    int slot = 0, i = 0;
+    uint32_t lap = 0;
+    while (fine && list.next(p, x)) {
+      const int len = length_of(p, x.b);
+      for (int t = x.tile; t < x.tile + x.n; ++t, ++i) {
+        const uint32_t off = (uint32_t)reinterpret_cast<uintptr_t>(source(value ? p.vc : p.kc, t)) & 15u;
+        if (!(fine = warp_wait(raw_full(slot), lap))) break;
+        const RowWords row = {smem + S::kAtRaw + (2 * slot + (value ? 1 : 0)) * S::kRaw + off + key * R};
+        const bool there = t * kKeys + key < len;
+        const int buf = i & 1;
+        if (!value) {
+          // the product that read this buffer is done
+          if (i >= 2 && !(fine = warp_wait(s_full(buf), (i / 2 - 1) & 1))) break;
+          tmem_fence_after();
+#pragma unroll
+          for (int g = 0; g < 4 * PANELS; g += 2) {
+            uint32_t w[16];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              if (g + e < G)
+                decode_group(row.word(2 * (g + e)), row.word(2 * (g + e) + 1), row.at[8 * G + g + e], w + 8 * e);
+              else
+#pragma unroll
+                for (int j = 0; j < 8; ++j) w[8 * e + j] = 0u;
+            }
+            tmem_store<16>(tmem + lanes + buf * (DP / 2) + 8 * g, w);
+          }
+          tmem_wait_store();
+          tmem_fence_before();
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive(raw_empty(slot));
+            mbar_arrive(k_ready(buf));
+          }
+        } else {
+          const int vb = VB == 2 ? buf : 0;
+          if (i >= VB && !(fine = warp_wait(v_free(vb), (i / VB - 1) & 1))) break;
+          uint8_t* const to = smem + vb * S::kValues + key * 128;
+#pragma unroll
+          for (int g = 0; g < 4 * PANELS; ++g) {
+            if (g >= G) break;
+            uint32_t w[8];
+            decode_group(row.word(2 * g), row.word(2 * g + 1), row.at[8 * G + g], w);
+            if (!there) {  // a key that no row sees
+#pragma unroll
+              for (int j = 0; j < 8; ++j) w[j] = 0u;
+            }
+            uint8_t* const panel = to + (g / 4) * kPanel;
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+              *reinterpret_cast<uint4*>(panel + (((2 * (g % 4) + h) ^ (key & 7)) << 4)) =
+                  make_uint4(w[4 * h], w[4 * h + 1], w[4 * h + 2], w[4 * h + 3]);
+          }
+          smem_fence_async();
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive(raw_empty(slot));
+            mbar_arrive(v_ready(vb));
+          }
+        }
+        if (++slot == NS) slot = 0, lap ^= 1u;
+      }
+    }
+  } else if (warp == kWarpMma) {
+    // ---- products, by the whole warp in step
+    constexpr uint32_t word_s = mma_word(false, kM, N, false), word_o = mma_word(false, kM, N, true) | 1u << 15;
+    const uint32_t t_base = __shfl_sync(0xffffffffu, tmem, 0);
+    int i = 0;
+    uint32_t units = 0;
+    while (fine && list.next(p, x)) {
+      const int n = __shfl_sync(0xffffffffu, x.n, 0);
+      if (!n) continue;
+      auto scores = [&](int j) {
+        if (!warp_wait(k_ready(j & 1), (j / 2) & 1)) return fine = false;
+        tmem_fence_after();
+#pragma unroll
+        for (int s = 0; s < DP / 16; ++s)
+          mma_tmem(t_base + S::kColS + (j & 1) * N, t_base + (j & 1) * (DP / 2) + 8 * s,
+                   smem_operand(base + S::kAtQ + (s / 4) * (N * 128) + (s % 4) * 32, 16), word_s, s > 0);
+        mma_commit(s_full(j & 1));
+        return true;
+      };
+      if (!(fine = warp_wait(q_ready, units & 1))) break;
+      ++units;
+      if (!scores(i)) break;
+      for (int t = 0; t < n && fine; ++t, ++i) {
+        if (t + 1 < n && !scores(i + 1)) break;
+        const int vb = VB == 2 ? i & 1 : 0;
+        if (!(fine = warp_wait_both(v_ready(vb), (i / VB) & 1, p_ready(i & 1), (i / 2) & 1))) break;
+        tmem_fence_after();
+#pragma unroll
+        for (int m = 0; m < S::kBlocks; ++m)
+#pragma unroll
+          for (int s = 0; s < kKeys / 16; ++s)
+            mma_smem(t_base + S::kColO + m * N, smem_operand(base + vb * S::kValues + m * 2 * kPanel + 2048 * s, kPanel),
+                     smem_operand(base + S::kAtP + (i & 1) * S::kP + 2048 * s, kPanel), word_o, s > 0 || t > 0);
+        mma_commit(pv_done(i & 1));
+        if constexpr (VB == 1) mma_commit(v_free(0));
+      }
+    }
+  } else {
+    // ---- softmax: group g has rows C g .. C g + C - 1, a thread key L of a tile
+    const int g = warp >> 2, quarter = warp & 3, L = quarter * 32 + lane, r0 = C * g, id = 1 + g;
+    const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+    const int rows = p.nodes * p.group;
+    int i = 0, units = 0;
+    // queries of a piece, a warp a row: scaled by a power of two into float16
+    auto queries = [&](const Piece& y) {
+      const int h = y.unit / p.tiles_r, first = y.unit % p.tiles_r * N;
+      float2* const row_of = s_row + (units & 1) * N;
+#pragma unroll 2
+      for (int r = r0 + quarter; r < r0 + C; r += 4) {
+        const int row = first + r;
+        const bool real = row < rows;
+        const int64_t at = y.b * p.q.batch + (h * p.group + row % p.group) * p.q.head + (int64_t)(row / p.group) * p.q.row;
+        float v[2 * PANELS];
+        uint32_t top = 0;
+#pragma unroll
+        for (int j = 0; j < 2 * PANELS; ++j) {
+          const int d = 2 * lane + 64 * (j / 2) + (j & 1);
+          v[j] = 0.0f;
+          if (real && d < p.head_dim)
+            v[j] = p.bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(p.q.data)[at + d])
+                          : __half2float(static_cast<const __half*>(p.q.data)[at + d]);
+          const uint32_t u = __float_as_uint(v[j]) & 0x7FFFFFFFu;
+          top = max(top, u < 0x7F800000u ? u : 0u);
+        }
+        top = __reduce_max_sync(0xffffffffu, top);
+        // 2^-e times the row: its largest finite element becomes 1 to 2
+        const int e = !p.bf16 || top < 0x00800000u ? 0 : (int)(top >> 23) - 127;
+        // in two steps, as 2^-e need not be a float
+        const float s1 = __int_as_float((127 - e / 2) << 23), s2 = __int_as_float((127 - (e - e / 2)) << 23);
+#pragma unroll
+        for (int j = 0; j < PANELS; ++j) {
+          const __half2 w = __floats2half2_rn(v[2 * j] * s1 * s2, v[2 * j + 1] * s1 * s2);
+          const int piece = lane / 4;
+          *reinterpret_cast<__half2*>(smem + S::kAtQ + j * (N * 128) + r * 128 + ((piece ^ (r & 7)) << 4) +
+                                      (lane % 4) * 4) = w;
+        }
+        if (lane == 0) {
+          const float up1 = __int_as_float((127 + e / 2) << 23), up2 = __int_as_float((127 + (e - e / 2)) << 23);
+          row_of[r] = make_float2(p.scale * kLog2e * up1 * up2, kUnset);
+        }
+      }
+      smem_fence_async();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(q_ready);
+    };
+    bool have = list.next(p, x);
+    while (have && x.n == 0) have = list.next(p, x);
+    if (have) queries(x);
+    while (have) {
+      const int len = length_of(p, x.b), n = x.n;
+      float2* const row_of = s_row + (units & 1) * N + r0;
+      float l[C];
+#pragma unroll
+      for (int r = 0; r < C; ++r) l[r] = 0.0f;
+      // every warp's rows are there, whatever the waits before gave
+      if (!(fine = group_all(id, 128, fine))) break;
+#pragma unroll 1
+      for (int t = 0; t < n; ++t, ++i) {
+        const int buf = i & 1;
+        const bool there = (x.tile + t) * kKeys + L < len;
+        fine = fine && warp_wait(s_full(buf), (i / 2) & 1);
+        float y[C];
+        bool above = false;
+        if (fine) {
+          tmem_fence_after();
+          tmem_load<C>(tmem + lanes + S::kColS + buf * N + r0, reinterpret_cast<uint32_t*>(y));
+          tmem_wait_load();
+          float top = -INFINITY;
+#pragma unroll
+          for (int r = 0; r < C; ++r) {
+            const float2 f = row_of[r];
+            const float z = fmaf(y[r], f.x, -f.y);
+            top = fmaxf(top, z);
+          }
+          above = there && top > kSlack + kBelow<__half>;
+        }
+        // one warp's score above its row's reference point, or a wait that gave up, concerns all
+        if (!group_all(id, 128, fine && !above)) {
+          if (!(fine = group_all(id, 128, fine))) break;
+#pragma unroll
+          for (int r = 0; r < C; ++r) {
+            const int best = __reduce_max_sync(0xffffffffu, ordered(there ? y[r] * row_of[r].x : -INFINITY));
+            if (lane == 0) s_max[quarter * N + r0 + r] = unordered(best);
+          }
+          // sums so far are on the old points until the last product is done
+          if (t > 0) fine = warp_wait(pv_done(buf ^ 1), ((i - 1) / 2) & 1);
+          if (!(fine = group_all(id, 128, fine))) break;
+          if (L < C) {
+            float best = s_max[r0 + L];
+            bool nan = best != best;
+#pragma unroll
+            for (int q = 1; q < 4; ++q) {
+              const float o = s_max[q * N + r0 + L];
+              nan |= o != o;
+              best = fmaxf(best, o);
+            }
+            if (nan) best = __int_as_float(0x7FC00000);
+            const float2 f = row_of[L];
+            // (a point that is no number stays)
+            const bool set = f.y == f.y && !(best <= f.y + (kSlack + kBelow<__half>)) && best != -INFINITY;
+            const float to = set ? best - kBelow<__half> : f.y;
+            s_fac[r0 + L] = set ? ex2(f.y - to) : 1.0f;
+            row_of[L].y = to;
+          }
+          group_sync(id, 128);
+          float f[C];
+#pragma unroll
+          for (int r = 0; r < C; ++r) {
+            f[r] = s_fac[r0 + r];
+            l[r] *= f[r];
+          }
+          if (t > 0) {
+            tmem_fence_after();
+#pragma unroll
+            for (int m = 0; m < S::kBlocks; ++m) {
+              float o[C];
+              tmem_load<C>(tmem + lanes + S::kColO + m * N + r0, reinterpret_cast<uint32_t*>(o));
+              tmem_wait_load();
+#pragma unroll
+              for (int r = 0; r < C; ++r) o[r] *= f[r];
+              tmem_store<C>(tmem + lanes + S::kColO + m * N + r0, reinterpret_cast<const uint32_t*>(o));
+            }
+            tmem_wait_store();
+          }
+          group_sync(id, 128);  // s_max and s_fac are read
+        }
+        uint32_t w[C / 2];
+#pragma unroll
+        for (int r = 0; r < C; r += 2) {
+          const float4 f = *reinterpret_cast<const float4*>(row_of + r);
+          float2 e = make_float2(ex2(fmaf(y[r], f.x, -f.y)), ex2(fmaf(y[r + 1], f.z, -f.w)));
+          if (!there) e = make_float2(0.0f, 0.0f);
+          l[r] += e.x, l[r + 1] += e.y;
+          w[r / 2] = pack2<__half>(e.x, e.y);
+        }
+        // the product that read this buffer is done
+        if (i >= 2) fine = warp_wait(pv_done(buf), (i / 2 - 1) & 1);
+        if (fine) {
+          uint8_t* const to = smem + S::kAtP + buf * S::kP + L * 128;
+#pragma unroll
+          for (int j = 0; j < C / 8; ++j)
+            *reinterpret_cast<uint4*>(to + (((r0 / 8 + j) ^ (L & 7)) << 4)) =
+                make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+        }
+        smem_fence_async();
+        tmem_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(p_ready(buf));
+      }
+      if (!(fine = group_all(id, 128, fine))) break;
+      // the next piece's queries may come: every product over this one's is done
+      const Piece done = x;
+      const int last = i - 1;
+      do have = list.next(p, x);
+      while (have && x.n == 0);
+      ++units;
+      if (have) queries(x);
+      // this piece's sums: l over the keys of all warps, O as it is
+      const float mine = warp_columns<C>(l);
+      if (C == 32 || !(lane & 1)) s_max[quarter * N + r0 + column_of<C>(lane)] = mine;
+      fine = warp_wait(pv_done(last & 1), (last / 2) & 1);
+      if (!(fine = group_all(id, 128, fine))) break;
+      tmem_fence_after();
+      float* const keep = p.part + ((int64_t)done.b * list.units + done.unit + blockIdx.x) * (N * (DP + 4));
+#pragma unroll
+      for (int m = 0; m < S::kBlocks; ++m) {
+        float o[C];
+        tmem_load<C>(tmem + lanes + S::kColO + m * N + r0, reinterpret_cast<uint32_t*>(o));
+        tmem_wait_load();
+        if (128 * m + L < DP)
+#pragma unroll
+          for (int r = 0; r < C; ++r) keep[(r0 + r) * (DP + 4) + 128 * m + L] = o[r];
+      }
+      if (L < C)
+        *reinterpret_cast<float2*>(keep + (r0 + L) * (DP + 4) + DP) =
+            make_float2(row_of[L].y, (s_max[r0 + L] + s_max[N + r0 + L]) + (s_max[2 * N + r0 + L] + s_max[3 * N + r0 + L]));
+      tmem_fence_before();
+    }
+  }
+  if (!fine && (warp < kWarpK || lane == 0)) atomicAdd(faults, 1u);
+  tmem_fence_before();
+  __syncthreads();
+  if (warp == kWarpMma) {
+    __syncwarp();
+    tmem_free(tmem, kTmemCols);
+  }
+}
+
+// Joins the parts of a row over the cache and adds its new keys; a warp a row.
+// What does not wait for the first kernel comes first.
+template <typename T, int PANELS, int N>
+__global__ void __launch_bounds__(256) join4_kernel(const __grid_constant__ Params4 p) {
+  constexpr int DP = 64 * PANELS;
+  __shared__ uint64_t s_mask[8][kMaxNodes];
+  __shared__ int s_jump[8][kMaxNodes];
+  const int rows = p.nodes * p.group, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int per = (rows + 7) / 8, bh = blockIdx.x / per, row = blockIdx.x % per * 8 + warp;
+  const int b = bh / p.kv_heads, h = bh % p.kv_heads;
+  if (row >= rows) {
+    CKKS_PDL_ENTRY();
+    return;
+  }
+  tree_masks(p.parents + (size_t)b * p.nodes, p.nodes, s_mask[warp], s_jump[warp]);
+  const int node = row / p.group, qh = h * p.group + row % p.group;
+  const uint64_t mask = s_mask[warp][node];
+  T* const out = static_cast<T*>(p.out.data) + b * p.out.batch + qh * p.out.head + (int64_t)node * p.out.row;
+  float* const lse = p.lse + ((size_t)b * p.nodes + node) * p.kv_heads * p.group + qh;
+  // the new keys: lane x has elements x, x + 32, ...
+  float q[2 * PANELS], acc[2 * PANELS], m = -INFINITY, l = 0.0f;
+  const T* const q_row = static_cast<const T*>(p.q.data) + b * p.q.batch + qh * p.q.head + (int64_t)node * p.q.row;
+  const T* const kn = static_cast<const T*>(p.kn.data) + b * p.kn.batch + h * p.kn.head;
+  const T* const vn = static_cast<const T*>(p.vn.data) + b * p.vn.batch + h * p.vn.head;
+#pragma unroll
+  for (int j = 0; j < 2 * PANELS; ++j) {
+    const int d = lane + 32 * j;
+    q[j] = mask && d < p.head_dim ? to_f32(q_row[d]) : 0.0f;
+    acc[j] = 0.0f;
+  }
+  for (uint64_t left = mask; left;) {
+    // four keys at a time, so that their reads wait together
+    int key[4];
+    float s[4], v[4][2 * PANELS];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      key[i] = left ? __ffsll((long long)left) - 1 : -1;
+      left &= left - 1;
+      s[i] = 0.0f;
+#pragma unroll
+      for (int j = 0; j < 2 * PANELS; ++j) {
+        const int d = lane + 32 * j;
+        const bool is = key[i] >= 0 && d < p.head_dim;
+        s[i] = fmaf(q[j], is ? to_f32(kn[(int64_t)key[i] * p.kn.row + d]) : 0.0f, s[i]);
+        v[i][j] = is ? to_f32(vn[(int64_t)key[i] * p.vn.row + d]) : 0.0f;
+      }
+    }
+    float top = m;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+#pragma unroll
+      for (int o = 16; o; o >>= 1) s[i] += __shfl_xor_sync(0xffffffffu, s[i], o);
+      s[i] = key[i] >= 0 ? s[i] * (p.scale * kLog2e) : -INFINITY;
+      top = fmaxf(top, s[i]);
+    }
+    const float ref = top == -INFINITY ? 0.0f : top, f = exp2f(m - ref);
+    m = top;
+    l *= f;
+#pragma unroll
+    for (int j = 0; j < 2 * PANELS; ++j) acc[j] *= f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (key[i] < 0) continue;
+      const float w = exp2f(s[i] - ref);
+      l += w;
+#pragma unroll
+      for (int j = 0; j < 2 * PANELS; ++j) acc[j] = fmaf(w, v[i][j], acc[j]);
+    }
+  }
+  // this row's unit: its tiles [u0, u0 + tiles) of the list, and the CTAs that
+  // have the first and the last: CTA i begins at list_start(i), so entry w is
+  // CTA floor((ctas (w + 1) - 1) / entries)'s
+  const int units = p.kv_heads * p.tiles_r, unit = h * p.tiles_r + row / N;
+  int before = 0, all = 0;
+  for (int i = lane; i < p.batch; i += 32) {
+    const int t = entries_of(p, i);
+    all += t;
+    if (i < b) before += t;
+  }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) {
+    all += __shfl_xor_sync(0xffffffffu, all, o);
+    before += __shfl_xor_sync(0xffffffffu, before, o);
+  }
+  const int entries = entries_of(p, b);
+  CKKS_PDL_ENTRY();  // what is read above no kernel of this call writes
+  if (entries) {
+    const long long W = (long long)all * units, ctas = min((long long)p.ctas, W);
+    const long long u0 = (long long)before * units + (long long)unit * entries + p.unit_cost;
+    const int c0 = (int)((ctas * (u0 + 1) - 1) / W), c1 = (int)((ctas * (u0 + entries - p.unit_cost) - 1) / W);
+    const float* const part = p.part + ((int64_t)(b * units + unit) * N + row % N) * (DP + 4);
+    // the parts' sums are read eight at a time, so that a row seldom waits for memory twice
+    for (int c = c0; c <= c1; c += 8) {
+      float2 ml[8];
+      float y[8][2 * PANELS];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const bool is = c + i <= c1;
+        const float* const o = part + (int64_t)(c + i) * (N * (DP + 4));
+        ml[i] = is ? *reinterpret_cast<const float2*>(o + DP) : make_float2(-INFINITY, 0.0f);
+#pragma unroll
+        for (int j = 0; j < 2 * PANELS; ++j) y[i][j] = is ? o[lane + 32 * j] : 0.0f;
+      }
+      float top = m;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) top = fmaxf(top, ml[i].x);
+      const float ref = top == -INFINITY ? 0.0f : top, f = exp2f(m - ref);
+      m = top;
+      l *= f;
+#pragma unroll
+      for (int j = 0; j < 2 * PANELS; ++j) acc[j] *= f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float w = exp2f(ml[i].x - ref);
+        l = fmaf(ml[i].y, w, l);
+#pragma unroll
+        for (int j = 0; j < 2 * PANELS; ++j) acc[j] = fmaf(y[i][j], w, acc[j]);
+      }
+    }
+  }
+  const float inv = l != 0.0f ? 1.0f / l : 0.0f;
+#pragma unroll
+  for (int j = 0; j < 2 * PANELS; ++j)
+    if (lane + 32 * j < p.head_dim) out[lane + 32 * j] = from_f32<T>(mask ? acc[j] * inv : 0.0f);
+  if (lane == 0) *lse = mask && l != 0.0f ? kLn2 * (m + log2f(l)) : -INFINITY;
+}
+
+struct Plan4 {
+  int rows, tiles_r, ctas;  // rows of a unit, units of a (sequence, head)
+  long long units;
+  bool listed;  // the list has fewer than 2^31 entries
+};
+
+constexpr int kUnitCost = 3;
+
+Plan4 plan4(const Context& c, const ckks_draft_attention_args& a) {
+  const int rows = a.nodes * (a.q_heads / a.kv_heads);
+  Plan4 d;
+  d.rows = rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
+  d.tiles_r = (rows + d.rows - 1) / d.rows;
+  d.units = (long long)a.batch * a.kv_heads * d.tiles_r;
+  const long long tiles = (a.capacity + kKeys - 1) / kKeys;
+  d.listed = d.units * (tiles + kUnitCost) < (1ll << 31) - 1;
+  d.ctas = (int)std::max(1ll, std::min<long long>(c.sms, d.units * std::max(1ll, tiles / 2)));
+  return d;
+}
+
+template <int PANELS, int N>
+void launch4(const Context& c, const ckks_draft_attention_args& a, const Params4& p, cudaStream_t st) {
+  using S = Shape4<PANELS, N>;
+  static_assert(S::kSmem <= 232448, "shared memory of one block");
+  auto* k = attend4_kernel<PANELS, N>;
+  CKKS_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::kSmem));
+  k<<<p.ctas, S::kThreads, S::kSmem, st>>>(p, c.d_faults);
+  CKKS_CUDA(cudaGetLastError());
+  const dim3 grid((unsigned)(a.batch * a.kv_heads * ((a.nodes * p.group + 7) / 8)));
+  if (p.bf16)
+    launch_pdl(join4_kernel<__nv_bfloat16, PANELS, N>, grid, dim3(256), 0, st, p);
+  else
+    launch_pdl(join4_kernel<__half, PANELS, N>, grid, dim3(256), 0, st, p);
+}
+
+template <int PANELS>
+void launch4(const Context& c, const ckks_draft_attention_args& a, const Params4& p, int rows, cudaStream_t st) {
+  if (rows == 16)
+    launch4<PANELS, 16>(c, a, p, st);
+  else if (rows == 32)
+    launch4<PANELS, 32>(c, a, p, st);
+  else
+    launch4<PANELS, 64>(c, a, p, st);
+}
+
+int panels4(int head_dim) { return head_dim <= 64 ? 1 : head_dim <= 128 ? 2 : 4; }
+
+}  // namespace
+
+size_t attention4_tc_workspace(const Context& c, const ckks_draft_attention_args& a) {
+  const Plan4 d = plan4(c, a);
+  if (a.dtype == CKKS_FP32 || !d.listed) return 0;
+  return sizeof(float) * (size_t)(d.units + d.ctas) * d.rows * (64 * panels4(a.head_dim) + 4);
+}
+
+bool attention4_tc(const Context& c, const ckks_draft_attention_args& a, cudaStream_t st) {
+  const Plan4 d = plan4(c, a);
+  const int R = row4_bytes(a.head_dim);
+  if (a.dtype == CKKS_FP32 || !d.listed) return false;
+  // a head's rows one behind the other
+  if (a.capacity > 1 && (a.k_cache.row != R || a.v_cache.row != R)) return false;
+  Params4 p{};
+  p.q = a.q, p.kc = a.k_cache, p.vc = a.v_cache, p.kn = a.k_new, p.vn = a.v_new, p.out = a.out;
+  p.lens = a.lens, p.parents = a.parents, p.lse = a.lse, p.part = static_cast<float*>(a.workspace);
+  p.batch = a.batch, p.kv_heads = a.kv_heads, p.group = a.q_heads / a.kv_heads, p.head_dim = a.head_dim;
+  p.nodes = a.nodes, p.capacity = a.capacity, p.scale = (float)a.scale, p.bf16 = a.dtype == CKKS_BF16;
+  p.tiles_r = d.tiles_r, p.unit_cost = kUnitCost, p.ctas = d.ctas, p.row_bytes = R;
+  switch (panels4(a.head_dim)) {
+    case 1: launch4<1>(c, a, p, d.rows, st); break;
+    case 2: launch4<2>(c, a, p, d.rows, st); break;
+    default: launch4<4>(c, a, p, d.rows, st); break;
+  }
+  return true;
+}
+
+}  // namespace draft
+}  // namespace ckks

@@ -98,5 +98,10 @@ __device__ __forceinline__ void load_row4_4bit(float* dst, const uint8_t* row, i
   dst[0] = a.x, dst[1] = a.y, dst[2] = b.x, dst[3] = b.y;
 }
 
+// attention over a 4-bit cache on the tensor cores (draft_attention4.cu): false,
+// and nothing is launched, where the sizes or the caches' strides are not its
+size_t attention4_tc_workspace(const Context& c, const ckks_draft_attention_args& a);
+bool attention4_tc(const Context& c, const ckks_draft_attention_args& a, cudaStream_t st);
+
 }  // namespace draft
 }  // namespace ckks

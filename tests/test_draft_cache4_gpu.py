@@ -5,9 +5,11 @@ float64 definition of draft_reference.py on the values that they hold.
 Bounds as in tests/test_draft_gpu.py, and half of the smallest steps: one in
 nine values of a 4-bit cache is 0, so a row whose heaviest keys have the value 0
 has results far below its weights.  A float16 result below 2^-14 is off by up
-to 2^-25 whatever its size (half a step of 2^-24), and its softmax weights come
-in steps of 2^-31 of the largest, so each is off by up to 2^-32 of a weight of
-at most 1, times |v|; the other types' smallest steps are below 1e-30."""
+to 2^-25 whatever its size (half a step of 2^-24).  With 16-bit queries, of
+either type, the weights are float16 numbers: steps of 2^-24 where the largest
+is 2^7 or more, so each is off by up to 2^-25 / 2^7 = 2^-32 of the largest,
+times |v|, and their sum is at least the largest.  The other smallest steps are
+below 1e-30."""
 
 import numpy as np
 import pytest
@@ -160,9 +162,11 @@ def check_attention(x, out, lse, scale=None):
     got, glse = f64(out), f64(lse)
     noise = 2.0 ** -23 * ((D + 8) * big + keys + 8)
     room = (2 * HALF[x["q"].dtype] + noise)[..., None] * mag + 1e-30
-    if x["q"].dtype == torch.float16:
+    if x["q"].dtype != torch.float32:
         top = max(np.abs(v).max(initial=0.0), np.abs(f64(x["v_new"])).max())
-        room += 2.0 ** -25 + 2.0 ** -32 * top * keys[..., None]
+        room += 2.0 ** -32 * top * keys[..., None]
+    if x["q"].dtype == torch.float16:
+        room += 2.0 ** -25
     assert np.isfinite(want).all() and np.isfinite(got).all()
     worst = (np.abs(got - want) / room).max()
     assert worst <= 1.0, f"out: {worst:.3g} times the bound"
