@@ -157,22 +157,6 @@ __device__ __forceinline__ int ordered(float x) {
 }
 __device__ __forceinline__ float unordered(int i) { return __int_as_float(i ^ (i >> 31 & 0x7FFFFFFF)); }
 
-// a row's codes and scales from shared memory: word i of it
-struct RowWords {
-  const uint8_t* at;
-  __device__ __forceinline__ uint32_t word(int i) const { return *reinterpret_cast<const uint32_t*>(at + 4 * i); }
-};
-
-// one group of 16 elements as 8 pairs of float16
-__device__ __forceinline__ void decode_group(uint32_t a, uint32_t b, uint32_t scale, uint32_t* out) {
-  const __half2 s = __half2half2(scale4(scale));
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const __half2 h = decode4((i < 4 ? a >> (8 * i) : b >> (8 * (i - 4))) & 0xFFu, s);
-    out[i] = *reinterpret_cast<const uint32_t*>(&h);
-  }
-}
-
 template <int PANELS, int N>
 __global__ void __launch_bounds__(Shape4<PANELS, N>::kThreads, 1)
     attend4_kernel(const __grid_constant__ Params4 p, unsigned int* __restrict__ faults) {
@@ -213,9 +197,10 @@ __global__ void __launch_bounds__(Shape4<PANELS, N>::kThreads, 1)
     mbar_init(q_ready, 4 * GR);
   }
   if (warp == kWarpMma) tmem_alloc(smem_addr(s_tmem), kTmemCols);
-  // what a head has no elements for stays 0
-  for (int i = tid; i < (int)(S::kValueBufs * S::kValues / 16); i += S::kThreads)
-    reinterpret_cast<uint4*>(smem)[i] = make_uint4(0, 0, 0, 0);
+  // the panel that a head of up to 64 elements has none for stays 0
+  if constexpr (PANELS == 1)
+    for (int i = tid; i < (int)(S::kValueBufs * kPanel / 16); i += S::kThreads)
+      reinterpret_cast<uint4*>(smem + i / (kPanel / 16) * S::kValues + kPanel)[i % (kPanel / 16)] = make_uint4(0, 0, 0, 0);
   smem_fence_async();
   tmem_fence_before();
   __syncthreads();
@@ -274,7 +259,19 @@ __global__ void __launch_bounds__(Shape4<PANELS, N>::kThreads, 1)
       for (int t = x.tile; t < x.tile + x.n; ++t, ++i) {
         const uint32_t off = (uint32_t)reinterpret_cast<uintptr_t>(source(value ? p.vc : p.kc, t)) & 15u;
         if (!(fine = warp_wait(raw_full(slot), lap))) break;
-        const RowWords row = {smem + S::kAtRaw + (2 * slot + (value ? 1 : 0)) * S::kRaw + off + key * R};
+        const uint32_t* const row = reinterpret_cast<const uint32_t*>(smem + S::kAtRaw + (2 * slot + (value ? 1 : 0)) * S::kRaw +
+                                                                      off + key * R);
+        // the row's groups four at a time: 8 words of codes and one of scales
+        struct Quad {
+          uint32_t code[8], scale;
+        };
+        auto read = [&](int g) {
+          Quad y;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) y.code[j] = g + j / 2 < G ? row[2 * g + j] : 0u;
+          y.scale = g < G ? row[2 * G + g / 4] : 0u;
+          return y;
+        };
         const bool there = t * kKeys + key < len;
         const int buf = i & 1;
         if (!value) {
@@ -282,17 +279,12 @@ __global__ void __launch_bounds__(Shape4<PANELS, N>::kThreads, 1)
           if (i >= 2 && !(fine = warp_wait(s_full(buf), (i / 2 - 1) & 1))) break;
           tmem_fence_after();
 #pragma unroll
-          for (int g = 0; g < 4 * PANELS; g += 2) {
-            uint32_t w[16];
+          for (int g = 0; g < 4 * PANELS; g += 4) {
+            const Quad y = read(g);
+            uint32_t w[32];
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              if (g + e < G)
-                decode_group(row.word(2 * (g + e)), row.word(2 * (g + e) + 1), row.at[8 * G + g + e], w + 8 * e);
-              else
-#pragma unroll
-                for (int j = 0; j < 8; ++j) w[8 * e + j] = 0u;
-            }
-            tmem_store<16>(tmem + lanes + buf * (DP / 2) + 8 * g, w);
+            for (int j = 0; j < 8; ++j) decode4_word(y.code[j], scale4_pair(y.scale, j / 2), w + 4 * j);
+            tmem_store<32>(tmem + lanes + buf * (DP / 2) + 8 * g, w);
           }
           tmem_wait_store();
           tmem_fence_before();
@@ -306,19 +298,16 @@ __global__ void __launch_bounds__(Shape4<PANELS, N>::kThreads, 1)
           if (i >= VB && !(fine = warp_wait(v_free(vb), (i / VB - 1) & 1))) break;
           uint8_t* const to = smem + vb * S::kValues + key * 128;
 #pragma unroll
-          for (int g = 0; g < 4 * PANELS; ++g) {
-            if (g >= G) break;
-            uint32_t w[8];
-            decode_group(row.word(2 * g), row.word(2 * g + 1), row.at[8 * G + g], w);
-            if (!there) {  // a key that no row sees
-#pragma unroll
-              for (int j = 0; j < 8; ++j) w[j] = 0u;
-            }
+          for (int g = 0; g < 4 * PANELS; g += 4) {
+            Quad y = read(g);
+            if (!there) y.scale = 0u;  // a key that no row sees: zeros
             uint8_t* const panel = to + (g / 4) * kPanel;
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
-              *reinterpret_cast<uint4*>(panel + (((2 * (g % 4) + h) ^ (key & 7)) << 4)) =
-                  make_uint4(w[4 * h], w[4 * h + 1], w[4 * h + 2], w[4 * h + 3]);
+            for (int j = 0; j < 8; ++j) {
+              uint32_t w[4];
+              decode4_word(y.code[j], scale4_pair(y.scale, j / 2), w);
+              *reinterpret_cast<uint4*>(panel + ((j ^ (key & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+            }
           }
           smem_fence_async();
           __syncwarp();

@@ -90,6 +90,24 @@ __device__ __forceinline__ uint64_t encode4(const float* x, uint32_t& scale) {
 __device__ __forceinline__ __half2 decode4(uint32_t byte, __half2 scale) {
   return __hmul2(__half2(__nv_cvt_fp4x2_to_halfraw2((__nv_fp4x2_storage_t)byte, __NV_E2M1)), scale);
 }
+// the eight elements of a word
+__device__ __forceinline__ void decode4_word(uint32_t word, __half2 scale, uint32_t* out) {
+  uint32_t h[4];
+  asm("{\n .reg .b8 a, b, c, d;\n mov.b32 {a, b, c, d}, %4;\n cvt.rn.f16x2.e2m1x2 %0, a;\n"
+      " cvt.rn.f16x2.e2m1x2 %1, b;\n cvt.rn.f16x2.e2m1x2 %2, c;\n cvt.rn.f16x2.e2m1x2 %3, d;\n}"
+      : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3])
+      : "r"(word));
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const __half2 x = __hmul2(*reinterpret_cast<const __half2*>(&h[i]), scale);
+    out[i] = *reinterpret_cast<const uint32_t*>(&x);
+  }
+}
+// scale byte `i` of a word, in both halves
+__device__ __forceinline__ __half2 scale4_pair(uint32_t word, int i) {
+  const uint32_t b = (word >> (8 * i) & 0xFFu) * 0x00800080u;
+  return *reinterpret_cast<const __half2*>(&b);
+}
 
 // elements d .. d + 3 of a row (d a multiple of 4)
 __device__ __forceinline__ void load_row4_4bit(float* dst, const uint8_t* row, int d, int D) {

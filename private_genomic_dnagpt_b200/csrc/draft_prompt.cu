@@ -276,6 +276,8 @@ void run_prompt(const PromptParams& p, cudaStream_t st) {
 // the exponentials are computed with multiply-adds: 2^x = 2^n 2^r, n the nearest
 // integer, and 2^r the polynomial of degree 4 with the least largest relative
 // error on [-1/2, 1/2] (2.7e-6, fitted to 2^r).
+constexpr int kHalf = 64;  // keys of a half tile
+
 template <int PANELS>
 struct PromptShape {
   static constexpr int kGroups = PANELS <= 2 ? 2 : 1, kThreads = 32 * (4 * kGroups + 2), kUnitRows = kM * kGroups;
@@ -283,7 +285,7 @@ struct PromptShape {
   static constexpr uint32_t kTileBytes = PANELS * kPanel;
   // Q of each group, the ring of K and V tiles, barriers, masks, one word
   static constexpr uint32_t kRing = kGroups * kTileBytes, kExtra = kRing + kSlots * kTileBytes;
-  static constexpr int kBars = 2 * kSlots + 10;
+  static constexpr int kBars = 2 * kSlots + 16;
   static constexpr size_t kSmem = kExtra + kBars * 8 + 6 * 4 * 4 + 16;
   // of eight pairs of exponentials, how many the multiply-adds take
   static constexpr int kPoly = PANELS == 1 ? 3 : PANELS == 2 ? 1 : 0;
@@ -293,21 +295,19 @@ struct PromptShape {
 struct Unit {
   int seq, len, row0, head;  // first row of the sequence, its length, the unit's first row of it, query head
 };
+// Of 32 sequences after the others, the units come by their place in the
+// sequence, the last (and longest) ones first.
 template <int ROWS>
 struct Units {
   Starts starts;
-  int b0 = 0, before = 0, first, len, units, sum, all;
+  int b0 = 0, before = 0, first, len, rungs, all, level, above;  // rungs of ROWS rows; those above `level`, of all lanes
   __device__ __forceinline__ void load(const PromptParams& p) {
-    const int lane = threadIdx.x & 31;
     const int2 at = starts.next(p, b0);
     first = at.x, len = at.y;
-    sum = units = (len + ROWS - 1) / ROWS * p.q_heads;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int y = __shfl_up_sync(0xffffffffu, sum, o);
-      if (lane >= o) sum += y;
-    }
-    all = __shfl_sync(0xffffffffu, sum, 31);
+    rungs = (len + ROWS - 1) / ROWS;
+    all = __reduce_add_sync(0xffffffffu, rungs) * p.q_heads;
+    level = __reduce_max_sync(0xffffffffu, rungs) - 1;
+    above = 0;
   }
   __device__ __forceinline__ void begin(const PromptParams& p) {
     starts.begin(p);
@@ -321,12 +321,20 @@ struct Units {
       b0 += 32;
       load(p);
     }
-    const int k = __ffs(__ballot_sync(0xffffffffu, sum > w - before)) - 1;
-    const int n = __shfl_sync(0xffffffffu, units, k), off = w - before - (__shfl_sync(0xffffffffu, sum, k) - n);
+    const int rung = (w - before) / p.q_heads;
+    uint32_t with = __ballot_sync(0xffffffffu, rungs > level);
+    while (rung >= above + __popc(with)) {
+      above += __popc(with);
+      --level;
+      with = __ballot_sync(0xffffffffu, rungs > level);
+    }
+    const uint32_t lower = (1u << (threadIdx.x & 31)) - 1u;
+    const bool mine = rungs > level && __popc(with & lower) == rung - above;
+    const int k = __ffs(__ballot_sync(0xffffffffu, mine)) - 1;
     u.seq = __shfl_sync(0xffffffffu, first, k);
     u.len = __shfl_sync(0xffffffffu, len, k);
-    u.row0 = ((n - 1 - off) / p.q_heads) * ROWS;
-    u.head = off % p.q_heads;
+    u.row0 = level * ROWS;
+    u.head = (w - before) % p.q_heads;
     return true;
   }
 };
@@ -404,11 +412,12 @@ __global__ void __launch_bounds__(PromptShape<PANELS>::kThreads, 1)
   const uint32_t sq = smem_addr(smem), ring = sq + S::kRing, bars = smem_addr(s_bar);
   auto full = [&](int s) { return bars + 8 * s; };
   auto empty = [&](int s) { return bars + 8 * (NS + s); };
-  auto s_full = [&](int g) { return bars + 8 * (2 * NS + g); };
-  auto p_ready = [&](int g) { return bars + 8 * (2 * NS + 2 + g); };
-  auto q_full = [&](int g) { return bars + 8 * (2 * NS + 4 + g); };
-  auto q_empty = [&](int g) { return bars + 8 * (2 * NS + 6 + g); };
-  auto o_full = [&](int g) { return bars + 8 * (2 * NS + 8 + g); };
+  // of a group and a half tile
+  auto s_full = [&](int g, int half) { return bars + 8 * (2 * NS + 2 * g + half); };
+  auto p_ready = [&](int g, int half) { return bars + 8 * (2 * NS + 4 + 2 * g + half); };
+  auto pv_done = [&](int g, int half) { return bars + 8 * (2 * NS + 8 + 2 * g + half); };
+  auto q_full = [&](int g) { return bars + 8 * (2 * NS + 12 + g); };
+  auto q_empty = [&](int g) { return bars + 8 * (2 * NS + 14 + g); };
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
     for (int s = 0; s < NS; ++s) {
@@ -416,11 +425,13 @@ __global__ void __launch_bounds__(PromptShape<PANELS>::kThreads, 1)
       mbar_init(empty(s), 1);
     }
     for (int g = 0; g < 2; ++g) {
-      mbar_init(s_full(g), 1);
-      mbar_init(p_ready(g), 4);
+      for (int h = 0; h < 2; ++h) {
+        mbar_init(s_full(g, h), 1);
+        mbar_init(p_ready(g, h), 4);
+        mbar_init(pv_done(g, h), 1);
+      }
       mbar_init(q_full(g), 1);
       mbar_init(q_empty(g), 1);
-      mbar_init(o_full(g), 1);
     }
   }
   if (warp == 4 * GR + 1) tmem_alloc(smem_addr(s_tmem), kTmemCols);
@@ -485,7 +496,7 @@ __global__ void __launch_bounds__(PromptShape<PANELS>::kThreads, 1)
     }
   } else if (warp == 4 * GR + 1) {
     // ---- products, by the whole warp in step
-    constexpr uint32_t word_s = mma_word(kBf, kM, kKeys, false), word_o = mma_word(kBf, kM, DP, true);
+    constexpr uint32_t word_s = mma_word(kBf, kM, kHalf, false), word_o = mma_word(kBf, kM, DP, true);
     const uint32_t t_base = __shfl_sync(0xffffffffu, tmem, 0);
     int slot = 0;
     uint32_t lap = 0, q_phase = 0, p_phase = 0;
@@ -495,15 +506,16 @@ __global__ void __launch_bounds__(PromptShape<PANELS>::kThreads, 1)
       auto next = [&] {
         if (++slot == NS) slot = 0, lap ^= 1u;
       };
-      auto scores = [&](int g, int t, int s) {
-        const uint32_t qb = sq + g * S::kTileBytes, kb = ring + s * S::kTileBytes;
+      // half `h` of tile t, in slot s
+      auto scores = [&](int g, int t, int h, int s) {
+        const uint32_t qb = sq + g * S::kTileBytes, kb = ring + s * S::kTileBytes + h * (kPanel / 2);
 #pragma unroll
         for (int i = 0; i < DP / 16; ++i) {
           const uint32_t off = (i / 4) * kPanel + (i % 4) * 32;
-          mma_smem(t_base + 128 * g, smem_operand(qb + off, 16), smem_operand(kb + off, 16), word_s, i > 0);
+          mma_smem(t_base + 128 * g + kHalf * h, smem_operand(qb + off, 16), smem_operand(kb + off, 16), word_s, i > 0);
         }
-        mma_commit(s_full(g));
-        if (t + 1 == n[g]) mma_commit(q_empty(g));
+        mma_commit(s_full(g, h));
+        if (h == 1 && t + 1 == n[g]) mma_commit(q_empty(g));
       };
       if (!(fine = warp_wait(full(slot), lap))) break;
 #pragma unroll
@@ -512,7 +524,8 @@ __global__ void __launch_bounds__(PromptShape<PANELS>::kThreads, 1)
         if (!(fine = warp_wait(q_full(g), q_phase >> g & 1))) break;
         q_phase ^= 1u << g;
         tmem_fence_after();
-        scores(g, 0, slot);
+        scores(g, 0, 0, slot);
+        scores(g, 0, 1, slot);
       }
       if (!fine) break;
       mma_commit(empty(slot));
@@ -523,30 +536,31 @@ __global__ void __launch_bounds__(PromptShape<PANELS>::kThreads, 1)
         next();
         const int ks = slot;  // of the next tile's keys
         const uint32_t klap = lap;
-        bool waited = false, waited_k = false;
+        if (!(fine = warp_wait(full(vs), vlap))) break;
+        bool waited = false;
 #pragma unroll
-        for (int g = 0; g < GR; ++g) {
-          if (t >= n[g]) continue;
-          if (!waited) {
-            if (!(fine = warp_wait(full(vs), vlap))) break;
-            waited = true;
-          }
-          if (!(fine = warp_wait(p_ready(g), p_phase >> g & 1))) break;
-          p_phase ^= 1u << g;
-          tmem_fence_after();
-          const uint32_t vb = ring + vs * S::kTileBytes;
+        for (int h = 0; h < 2; ++h) {
 #pragma unroll
-          for (int i = 0; i < kKeys / 16; ++i)
-            mma_tmem(t_base + 128 * (GR + g), t_base + 128 * g + 8 * i, smem_operand(vb + 2048 * i, kPanel), word_o,
-                     i > 0 || t > 0);
-          if (t + 1 < n[g]) {
-            if (!waited_k) {
-              if (!(fine = warp_wait(full(ks), klap))) break;
-              waited_k = true;
+          for (int g = 0; g < GR; ++g) {
+            if (t >= n[g] || !fine) continue;
+            if (!(fine = warp_wait(p_ready(g, h), p_phase >> g & 1))) continue;
+            if (h == 1) p_phase ^= 1u << g;
+            tmem_fence_after();
+            const uint32_t vb = ring + vs * S::kTileBytes + h * (kPanel / 2);
+#pragma unroll
+            for (int i = 0; i < kHalf / 16; ++i)
+              mma_tmem(t_base + 128 * (GR + g), t_base + 128 * g + kHalf * h + 8 * i, smem_operand(vb + 2048 * i, kPanel),
+                       word_o, i > 0 || h > 0 || t > 0);
+            mma_commit(pv_done(g, h));
+            // the next scores take the place of these weights
+            if (t + 1 < n[g]) {
+              if (!waited) {
+                if (!(fine = warp_wait(full(ks), klap))) continue;
+                waited = true;
+                tmem_fence_after();
+              }
+              scores(g, t + 1, h, ks);
             }
-            scores(g, t + 1, ks);
-          } else {
-            mma_commit(o_full(g));
           }
         }
         if (!fine) break;
@@ -563,17 +577,17 @@ __global__ void __launch_bounds__(PromptShape<PANELS>::kThreads, 1)
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
     const uint32_t t_s = tmem + 128 * g + lanes, t_o = tmem + 128 * (GR + g) + lanes;
     int base = 0, nu = 0, pairs = 0;  // tiles of keys and values before this unit's; units of this group, of both
-    uint32_t phase = 0;
+    uint32_t phase = 0;               // of this group's tile
     for (int r = 0; fine && list.find(p, unit_of(r), u); ++r) {
       const int n = tiles_of(g), most = max(n, GR > 1 ? tiles_of(g ^ 1) : 0);
       const bool both = GR > 1 && n && tiles_of(g ^ 1);
       float m = -INFINITY, l = 0.0f;
 #pragma unroll 1
-      for (int t = 0; t < n; ++t) {
+      for (int step = 0; step < 2 * n; ++step) {
+        const int h = step & 1, t = step >> 1;
         const bool last = t + 1 == n;
-        if (!(fine = warp_wait(s_full(g), phase))) break;
-        phase ^= 1u;
-        if (last) {
+        if (!(fine = warp_wait(s_full(g, h), phase))) break;
+        if (last && h == 0) {
           // The values of keys that only some rows of this tile see: what is
           // not finite is taken out of the product.  (The copy that had the slot
           // before was used ahead of this tile's scores, so the wait cannot take
@@ -593,21 +607,22 @@ __global__ void __launch_bounds__(PromptShape<PANELS>::kThreads, 1)
           }
         }
         tmem_fence_after();
-        uint32_t x[kKeys];
-        tmem_load<kKeys>(t_s, x);
+        uint32_t x[kHalf];
+        tmem_load<kHalf>(t_s + kHalf * h, x);
         tmem_wait_load();
         if (negative) {  // scores of -q
 #pragma unroll
-          for (int i = 0; i < kKeys; ++i) x[i] ^= 0x80000000u;
+          for (int i = 0; i < kHalf; ++i) x[i] ^= 0x80000000u;
         }
         if (last) {
+          const int seen = L - kHalf * h;
 #pragma unroll
-          for (int i = 0; i < kKeys; ++i)
-            if (i > L) x[i] = __float_as_uint(-INFINITY);
+          for (int i = 0; i < kHalf; ++i)
+            if (i > seen) x[i] = __float_as_uint(-INFINITY);
         }
         float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int i = 0; i < kKeys; i += 2)
+        for (int i = 0; i < kHalf; i += 2)
           mx4[i / 2 & 3] = max3(mx4[i / 2 & 3], __uint_as_float(x[i]), __uint_as_float(x[i + 1]));
         const float mx = max3(max3(mx4[0], mx4[1], mx4[2]), mx4[3], -INFINITY);
         float top = mx == -INFINITY ? mx : fmaf(mx, c, -kBelow<T>);
@@ -618,8 +633,10 @@ __global__ void __launch_bounds__(PromptShape<PANELS>::kThreads, 1)
           m = top;
           l *= f;
         }
-        if (t > 0 && __any_sync(0xffffffffu, f != 1.0f)) {
-          // the sums so far, on the new reference point
+        if (step > 0 && __any_sync(0xffffffffu, f != 1.0f)) {
+          // the sums so far, on the new reference point, once the product before is done
+          if (!(fine = warp_wait(pv_done(g, h ^ 1), h ? phase : phase ^ 1u))) break;
+          tmem_fence_after();
 #pragma unroll 1
           for (int i = 0; i < DP; i += 16) {
             uint32_t o[16];
@@ -636,7 +653,7 @@ __global__ void __launch_bounds__(PromptShape<PANELS>::kThreads, 1)
         float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
         auto weights = [&](auto poly) {
 #pragma unroll
-          for (int i0 = 0; i0 < kKeys; i0 += 32) {
+          for (int i0 = 0; i0 < kHalf; i0 += 32) {
             uint32_t w[16];
 #pragma unroll
             for (int i = 0; i < 32; i += 2) {
@@ -650,7 +667,7 @@ __global__ void __launch_bounds__(PromptShape<PANELS>::kThreads, 1)
               sum[i / 2 & 1] = add2(sum[i / 2 & 1], e);
               w[i / 2] = pack2<T>(e.x, e.y);
             }
-            tmem_store<16>(t_s + i0 / 2, w);
+            tmem_store<16>(t_s + kHalf * h + i0 / 2, w);
           }
         };
         if (last || __any_sync(0xffffffffu, m == -INFINITY))
@@ -661,12 +678,13 @@ __global__ void __launch_bounds__(PromptShape<PANELS>::kThreads, 1)
         tmem_wait_store();
         tmem_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(p_ready(g));
+        if (lane == 0) mbar_arrive(p_ready(g, h));
+        if (h) phase ^= 1u;
       }
       if (!fine) break;
       base += 2 * most;
       if (n) {
-        if (!(fine = warp_wait(o_full(g), nu & 1))) break;
+        if (!(fine = warp_wait(pv_done(g, 1), phase ^ 1u))) break;
         tmem_fence_after();
         const int row = u.row0 + kM * g + L;
         const bool mine = row < u.len;
