@@ -280,12 +280,12 @@ constexpr int kHalf = 64;  // keys of a half tile
 
 template <int PANELS>
 struct PromptShape {
-  static constexpr int kGroups = PANELS <= 2 ? 2 : 1, kThreads = 32 * (4 * kGroups + 2), kUnitRows = kM * kGroups;
+  static constexpr int kGroups = PANELS <= 2 ? 2 : 1, kThreads = 32 * (5 * kGroups + 1), kUnitRows = kM * kGroups;
   static constexpr int kSlots = PANELS == 1 ? 10 : PANELS == 2 ? 5 : PANELS == 3 ? 3 : 2;
   static constexpr uint32_t kTileBytes = PANELS * kPanel;
   // Q of each group, the ring of K and V tiles, barriers, masks, one word
   static constexpr uint32_t kRing = kGroups * kTileBytes, kExtra = kRing + kSlots * kTileBytes;
-  static constexpr int kBars = 2 * kSlots + 16;
+  static constexpr int kBars = 2 * kSlots + 20;
   static constexpr size_t kSmem = kExtra + kBars * 8 + 6 * 4 * 4 + 16;
   // of eight pairs of exponentials, how many the multiply-adds take
   static constexpr int kPoly = PANELS == 1 ? 3 : PANELS == 2 ? 1 : 0;
@@ -418,12 +418,17 @@ __global__ void __launch_bounds__(PromptShape<PANELS>::kThreads, 1)
   auto pv_done = [&](int g, int half) { return bars + 8 * (2 * NS + 8 + 2 * g + half); };
   auto q_full = [&](int g) { return bars + 8 * (2 * NS + 12 + g); };
   auto q_empty = [&](int g) { return bars + 8 * (2 * NS + 14 + g); };
+  // The first group's last values are clean, in one of four units of two groups.
+  // (While the second group's products wait for one, the fourth after it does
+  // not get that far: its keys would lie 15 slots behind the one that they hold.)
+  auto clean = [&](int pair) { return bars + 8 * (2 * NS + 16 + (pair & 3)); };
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
     for (int s = 0; s < NS; ++s) {
       mbar_init(full(s), 1);
-      mbar_init(empty(s), 1);
+      mbar_init(empty(s), GR);
     }
+    for (int i = 0; i < 4; ++i) mbar_init(clean(i), 4);
     for (int g = 0; g < 2; ++g) {
       for (int h = 0; h < 2; ++h) {
         mbar_init(s_full(g, h), 1);
@@ -494,82 +499,90 @@ __global__ void __launch_bounds__(PromptShape<PANELS>::kThreads, 1)
       for (int g = 0; g < GR; ++g)
         if (nq[g]) fine = mbar_wait_short(q_full(g), (nq[g] - 1) & 1) && fine;
     }
-  } else if (warp == 4 * GR + 1) {
-    // ---- products, by the whole warp in step
+  } else if (warp > 4 * GR) {
+    // ---- products of group g, by the whole warp in step
+    const int g = warp - (4 * GR + 1);
     constexpr uint32_t word_s = mma_word(kBf, kM, kHalf, false), word_o = mma_word(kBf, kM, DP, true);
-    const uint32_t t_base = __shfl_sync(0xffffffffu, tmem, 0);
-    int slot = 0;
+    const uint32_t t_base = __shfl_sync(0xffffffffu, tmem, 0), t_s = t_base + 128 * g, t_o = t_base + 128 * (GR + g);
+    int slot = 0, pairs = 0;
     uint32_t lap = 0, q_phase = 0, p_phase = 0;
     for (int r = 0; fine && list.find(p, unit_of(r), u); ++r) {
-      int n[2] = {__shfl_sync(0xffffffffu, tiles_of(0), 0), GR > 1 ? __shfl_sync(0xffffffffu, tiles_of(1), 0) : 0};
-      const int most = max(n[0], n[1]);
+      const int n = __shfl_sync(0xffffffffu, tiles_of(g), 0);
+      const int other = GR > 1 ? __shfl_sync(0xffffffffu, tiles_of(g ^ 1), 0) : 0, most = max(n, other);
       auto next = [&] {
         if (++slot == NS) slot = 0, lap ^= 1u;
       };
+      // a tile of the other group alone: this one is done with it as soon as it is there
+      auto pass = [&](int s, uint32_t l) {
+        if (!warp_wait(full(s), l)) return false;
+        if (lane == 0) mbar_arrive(empty(s));
+        return true;
+      };
       // half `h` of tile t, in slot s
-      auto scores = [&](int g, int t, int h, int s) {
+      auto scores = [&](int t, int h, int s) {
         const uint32_t qb = sq + g * S::kTileBytes, kb = ring + s * S::kTileBytes + h * (kPanel / 2);
 #pragma unroll
         for (int i = 0; i < DP / 16; ++i) {
           const uint32_t off = (i / 4) * kPanel + (i % 4) * 32;
-          mma_smem(t_base + 128 * g + kHalf * h, smem_operand(qb + off, 16), smem_operand(kb + off, 16), word_s, i > 0);
+          mma_smem(t_s + kHalf * h, smem_operand(qb + off, 16), smem_operand(kb + off, 16), word_s, i > 0);
         }
         mma_commit(s_full(g, h));
-        if (h == 1 && t + 1 == n[g]) mma_commit(q_empty(g));
+        if (h == 1 && t + 1 == n) mma_commit(q_empty(g));
       };
-      if (!(fine = warp_wait(full(slot), lap))) break;
+      auto sums = [&](int t, int h, int s) {
+        const uint32_t vb = ring + s * S::kTileBytes + h * (kPanel / 2);
 #pragma unroll
-      for (int g = 0; g < GR; ++g) {
-        if (!n[g]) continue;
-        if (!(fine = warp_wait(q_full(g), q_phase >> g & 1))) break;
-        q_phase ^= 1u << g;
+        for (int i = 0; i < kHalf / 16; ++i)
+          mma_tmem(t_o, t_s + kHalf * h + 8 * i, smem_operand(vb + 2048 * i, kPanel), word_o, i > 0 || h > 0 || t > 0);
+        mma_commit(pv_done(g, h));
+      };
+      if (n) {
+        if (!(fine = warp_wait_both(full(slot), lap, q_full(g), q_phase))) break;
+        q_phase ^= 1u;
         tmem_fence_after();
-        scores(g, 0, 0, slot);
-        scores(g, 0, 1, slot);
+        scores(0, 0, slot);
+        scores(0, 1, slot);
+        mma_commit(empty(slot));
+      } else if (!(fine = pass(slot, lap))) {
+        break;
       }
-      if (!fine) break;
-      mma_commit(empty(slot));
       next();
-      for (int t = 0; t < most && fine; ++t) {
+      for (int t = 0; t < most; ++t) {
         const int vs = slot;
         const uint32_t vlap = lap;
         next();
         const int ks = slot;  // of the next tile's keys
         const uint32_t klap = lap;
-        if (!(fine = warp_wait(full(vs), vlap))) break;
-        bool waited = false;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-#pragma unroll
-          for (int g = 0; g < GR; ++g) {
-            if (t >= n[g] || !fine) continue;
-            if (!(fine = warp_wait(p_ready(g, h), p_phase >> g & 1))) continue;
-            if (h == 1) p_phase ^= 1u << g;
-            tmem_fence_after();
-            const uint32_t vb = ring + vs * S::kTileBytes + h * (kPanel / 2);
-#pragma unroll
-            for (int i = 0; i < kHalf / 16; ++i)
-              mma_tmem(t_base + 128 * (GR + g), t_base + 128 * g + kHalf * h + 8 * i, smem_operand(vb + 2048 * i, kPanel),
-                       word_o, i > 0 || h > 0 || t > 0);
-            mma_commit(pv_done(g, h));
-            // the next scores take the place of these weights
-            if (t + 1 < n[g]) {
-              if (!waited) {
-                if (!(fine = warp_wait(full(ks), klap))) continue;
-                waited = true;
-                tmem_fence_after();
-              }
-              scores(g, t + 1, h, ks);
-            }
-          }
+        if (t + 1 < most) next();
+        if (t >= n) {
+          if (!(fine = pass(vs, vlap) && (t + 1 == most || pass(ks, klap)))) break;
+          continue;
         }
-        if (!fine) break;
-        mma_commit(empty(vs));
-        if (t + 1 < most) {
+        if (GR > 1 && g == 1 && t + 2 == n && !(fine = warp_wait_done(clean(pairs), pairs >> 2 & 1))) break;
+        if (t + 1 < n) {
+          if (!(fine = warp_wait_all(full(vs), vlap, p_ready(g, 0), p_phase, full(ks), klap))) break;
+          tmem_fence_after();
+          sums(t, 0, vs);
+          scores(t + 1, 0, ks);  // in the place of these weights
+          if (!(fine = warp_wait_done(p_ready(g, 1), p_phase))) break;
+          tmem_fence_after();
+          sums(t, 1, vs);
+          mma_commit(empty(vs));
+          scores(t + 1, 1, ks);
           mma_commit(empty(ks));
-          next();
+        } else {
+          if (!(fine = warp_wait_both(full(vs), vlap, p_ready(g, 0), p_phase))) break;
+          tmem_fence_after();
+          sums(t, 0, vs);
+          if (!(fine = warp_wait_done(p_ready(g, 1), p_phase))) break;
+          tmem_fence_after();
+          sums(t, 1, vs);
+          mma_commit(empty(vs));
+          if (t + 1 < most && !(fine = pass(ks, klap))) break;
         }
+        p_phase ^= 1u;
       }
+      pairs += GR > 1 && n && other;
     }
   } else {
     // ---- softmax: group g, tensor-memory lane L, that is row L of the group's
@@ -601,9 +614,13 @@ __global__ void __launch_bounds__(PromptShape<PANELS>::kThreads, 1)
             out |= take_out<T>(reinterpret_cast<uint4*>(vs + (i / 8) * kPanel + ((i % 8) << 4)));
           const uint32_t some = __ballot_sync(0xffffffffu, out);
           if (some) smem_fence_async();
+          __syncwarp();
           if (lane == 0) {
             s_out[2 * g + (nu & 1)][quarter] = some;
-            if (both && g == 0) s_out[4 + (pairs & 1)][quarter] = some;
+            if (both && g == 0) {
+              s_out[4 + (pairs & 1)][quarter] = some;
+              mbar_arrive(clean(pairs));
+            }
           }
         }
         tmem_fence_after();

@@ -72,6 +72,10 @@ __device__ __forceinline__ void group_sync(int id, int threads) {
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity) {
   return (bool)__all_sync(0xffffffffu, mbar_wait_short(bar, parity));
 }
+// the same where the phase is mostly complete already: one look without a loop
+__device__ __forceinline__ bool warp_wait_done(uint32_t bar, uint32_t parity) {
+  return __all_sync(0xffffffffu, mbar_test(bar, parity)) || warp_wait(bar, parity);
+}
 // two such waits; done both, they cost one look (a look takes about 200 cycles of
 // the warp that issues the products: trees of 21 over 4001 keys 29.2 -> 27.6 us)
 __device__ __forceinline__ bool warp_wait_both(uint32_t a, uint32_t pa, uint32_t b, uint32_t pb) {
@@ -83,6 +87,18 @@ __device__ __forceinline__ bool warp_wait_both(uint32_t a, uint32_t pa, uint32_t
       : "r"(a), "r"(pa), "r"(b), "r"(pb)
       : "memory");
   return __all_sync(0xffffffffu, done) || (warp_wait(a, pa) && warp_wait(b, pb));
+}
+// three
+__device__ __forceinline__ bool warp_wait_all(uint32_t a, uint32_t pa, uint32_t b, uint32_t pb, uint32_t c, uint32_t pc) {
+  uint32_t done;
+  asm volatile(
+      "{\n .reg .pred p, q, r;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+      " mbarrier.try_wait.parity.shared::cta.b64 q, [%3], %4;\n mbarrier.try_wait.parity.shared::cta.b64 r, [%5], %6;\n"
+      " and.pred p, p, q;\n and.pred p, p, r;\n selp.u32 %0, 1, 0, p;\n}\n"
+      : "=r"(done)
+      : "r"(a), "r"(pa), "r"(b), "r"(pb), "r"(c), "r"(pc)
+      : "memory");
+  return __all_sync(0xffffffffu, done) || (warp_wait(a, pa) && warp_wait(b, pb) && warp_wait(c, pc));
 }
 __device__ __forceinline__ bool group_all(int id, int threads, bool ok) {
   uint32_t all;
