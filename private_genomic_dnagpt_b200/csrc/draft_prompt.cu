@@ -288,7 +288,7 @@ struct PromptShape {
   static constexpr int kBars = 2 * kSlots + 20;
   static constexpr size_t kSmem = kExtra + kBars * 8 + 6 * 4 * 4 + 16;
   // of eight pairs of exponentials, how many the multiply-adds take
-  static constexpr int kPoly = PANELS == 1 ? 3 : PANELS == 2 ? 1 : 0;
+  static constexpr int kPoly = PANELS <= 2 ? 2 : 0;
 };
 
 // a place in the list of units; walked upwards by a whole warp
@@ -637,61 +637,72 @@ __global__ void __launch_bounds__(PromptShape<PANELS>::kThreads, 1)
           for (int i = 0; i < kHalf; ++i)
             if (i > seen) x[i] = __float_as_uint(-INFINITY);
         }
-        float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        float mx4[4] = {__uint_as_float(x[0]), __uint_as_float(x[1]), __uint_as_float(x[2]), __uint_as_float(x[3])};
 #pragma unroll
-        for (int i = 0; i < kHalf; i += 2)
+        for (int i = 4; i < kHalf; i += 2)
           mx4[i / 2 & 3] = max3(mx4[i / 2 & 3], __uint_as_float(x[i]), __uint_as_float(x[i + 1]));
         const float mx = max3(max3(mx4[0], mx4[1], mx4[2]), mx4[3], -INFINITY);
         float top = mx == -INFINITY ? mx : fmaf(mx, c, -kBelow<T>);
-        float f = 1.0f;
-        if (!(top <= m + kSlack)) {  // grown, or no number
-          if (!(top < INFINITY)) top = __uint_as_float(0x7FC00000u);  // an infinite score leaves no number
-          f = m == -INFINITY && top == top ? 0.0f : ex2(m - top);
-          m = top;
-          l *= f;
-        }
-        if (step > 0 && __any_sync(0xffffffffu, f != 1.0f)) {
-          // the sums so far, on the new reference point, once the product before is done
-          if (!(fine = warp_wait(pv_done(g, h ^ 1), h ? phase : phase ^ 1u))) break;
-          tmem_fence_after();
+        bool bare = false;  // a row that has seen no score above -inf
+        if (__any_sync(0xffffffffu, !(top <= m + kSlack) || m == -INFINITY)) {  // grown, no number, or bare
+          float f = 1.0f;
+          if (!(top <= m + kSlack)) {
+            if (!(top < INFINITY)) top = __uint_as_float(0x7FC00000u);  // an infinite score leaves no number
+            f = m == -INFINITY && top == top ? 0.0f : ex2(m - top);
+            m = top;
+            l *= f;
+          }
+          bare = __any_sync(0xffffffffu, m == -INFINITY);
+          if (step > 0 && __any_sync(0xffffffffu, f != 1.0f)) {
+            // the sums so far, on the new reference point, once the product before is done
+            if (!(fine = warp_wait(pv_done(g, h ^ 1), h ? phase : phase ^ 1u))) break;
+            tmem_fence_after();
 #pragma unroll 1
-          for (int i = 0; i < DP; i += 16) {
-            uint32_t o[16];
-            tmem_load<16>(t_o + i, o);
-            tmem_wait_load();
+            for (int i = 0; i < DP; i += 16) {
+              uint32_t o[16];
+              tmem_load<16>(t_o + i, o);
+              tmem_wait_load();
 #pragma unroll
-            for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
-            tmem_store<16>(t_o + i, o);
+              for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
+              tmem_store<16>(t_o + i, o);
+            }
           }
         }
         const float ref = m == -INFINITY ? 0.0f : m;
         // the weights take the place of their scores.  A masked score's is 0, and
         // so are those of a row that has seen none above -inf
-        float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+        float2 sum[4];
         auto weights = [&](auto poly) {
 #pragma unroll
           for (int i0 = 0; i0 < kHalf; i0 += 32) {
+            // all exponentials of a piece before the first is used
+            float2 e[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+              e[i] = fma2(make_float2(__uint_as_float(x[i0 + 2 * i]), __uint_as_float(x[i0 + 2 * i + 1])),
+                          make_float2(c, c), make_float2(-ref, -ref));
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              if (i % 8 < decltype(poly)::value)
+                e[i] = exp2_poly(e[i]);
+              else
+                e[i] = make_float2(ex2(e[i].x), ex2(e[i].y));
+            }
             uint32_t w[16];
 #pragma unroll
-            for (int i = 0; i < 32; i += 2) {
-              const float2 s2 = fma2(make_float2(__uint_as_float(x[i0 + i]), __uint_as_float(x[i0 + i + 1])),
-                                     make_float2(c, c), make_float2(-ref, -ref));
-              float2 e;
-              if ((i / 2) % 8 < decltype(poly)::value)
-                e = exp2_poly(s2);
-              else
-                e = make_float2(ex2(s2.x), ex2(s2.y));
-              sum[i / 2 & 1] = add2(sum[i / 2 & 1], e);
-              w[i / 2] = pack2<T>(e.x, e.y);
+            for (int i = 0; i < 16; ++i) {
+              sum[i & 3] = i0 == 0 && i < 4 ? e[i] : add2(sum[i & 3], e[i]);
+              w[i] = pack2<T>(e[i].x, e[i].y);
             }
             tmem_store<16>(t_s + kHalf * h + i0 / 2, w);
           }
         };
-        if (last || __any_sync(0xffffffffu, m == -INFINITY))
+        if (last || bare)
           weights(std::integral_constant<int, 0>{});
         else
           weights(std::integral_constant<int, S::kPoly>{});
-        l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+        const float2 all = add2(add2(sum[0], sum[1]), add2(sum[2], sum[3]));
+        l += all.x + all.y;
         tmem_wait_store();
         tmem_fence_before();
         __syncwarp();
