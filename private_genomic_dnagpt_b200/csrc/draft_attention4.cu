@@ -103,9 +103,8 @@ template <int PANELS, int N>
 struct Shape4 {
   static constexpr int DP = 64 * PANELS;
   static constexpr int kBlocks = PANELS <= 2 ? 1 : 2;    // of 128 elements, in the second product
-  static constexpr int kGroups = N == 64 ? 2 : 1;        // of softmax warps
-  static constexpr int kCols = N / kGroups;              // rows that a softmax thread has
-  static constexpr int kWarps = 4 * kGroups + 10, kThreads = 32 * kWarps;
+  static constexpr int kCols = 16, kGroups = N / kCols;  // rows that a softmax thread has; groups of four softmax warps
+  static constexpr int kWarps = 4 * kGroups + 11, kThreads = 32 * kWarps;
   static constexpr int kRowMost = row4_bytes(DP);
   static constexpr uint32_t kRaw = (kKeys * kRowMost + 16 + 127) / 128 * 128;  // one tile of K or V as it is
   static constexpr int kSlots = PANELS == 1 ? 6 : PANELS == 2 ? 4 : 2;
@@ -123,31 +122,21 @@ struct Shape4 {
   static_assert(kColO + kBlocks * N <= kTmemCols);
 };
 
-// the sum over a warp of N columns: lane x gets columns x, x + 32, ... (N 16: x % 16)
-template <int N>
+// the sum over a warp of 16 columns: lane x gets column x / 2
 __device__ __forceinline__ float warp_columns(float* v) {
   const int lane = threadIdx.x & 31;
 #pragma unroll
-  for (int o = 16, n = N; o; o >>= 1) {
-    if (n > 1) {
-      // halves of the columns go to the lanes whose bit is clear and set
-      const bool up = lane & o;
+  for (int o = 16, n = 16; o > 1; o >>= 1) {
+    // halves of the columns go to the lanes whose bit is clear and set
+    const bool up = lane & o;
+    n /= 2;
 #pragma unroll
-      for (int i = 0; i < n / 2; ++i) {
-        const float give = up ? v[i] : v[i + n / 2], keep = up ? v[i + n / 2] : v[i];
-        v[i] = keep + __shfl_xor_sync(0xffffffffu, give, o);
-      }
-      n /= 2;
-    } else {
-      v[0] += __shfl_xor_sync(0xffffffffu, v[0], o);
+    for (int i = 0; i < n; ++i) {
+      const float give = up ? v[i] : v[i + n], keep = up ? v[i + n] : v[i];
+      v[i] = keep + __shfl_xor_sync(0xffffffffu, give, o);
     }
   }
-  return v[0];
-}
-// the column that a lane has then
-template <int N>
-__device__ __forceinline__ int column_of(int lane) {
-  return N == 32 ? lane : lane >> 1;
+  return v[0] + __shfl_xor_sync(0xffffffffu, v[0], 1);
 }
 
 // monotone integers of floats, for the largest of a warp
@@ -162,7 +151,7 @@ __global__ void __launch_bounds__(Shape4<PANELS, N>::kThreads, 1)
     attend4_kernel(const __grid_constant__ Params4 p, unsigned int* __restrict__ faults) {
   using S = Shape4<PANELS, N>;
   constexpr int DP = S::DP, NS = S::kSlots, GR = S::kGroups, C = S::kCols, VB = S::kValueBufs;
-  constexpr int kWarpK = 4 * GR, kWarpV = kWarpK + 4, kWarpCopy = kWarpV + 4, kWarpMma = kWarpCopy + 1;
+  constexpr int kWarpK = 4 * GR, kWarpV = kWarpK + 4, kWarpCopy = kWarpV + 4, kWarpQk = kWarpCopy + 1, kWarpPv = kWarpQk + 1;
   extern __shared__ __align__(1024) uint8_t smem[];
   float2* const s_row = reinterpret_cast<float2*>(smem + S::kAtRows);      // [2][N] factor and reference point
   float* const s_max = reinterpret_cast<float*>(s_row + 2 * N);            // [4][N]
@@ -196,7 +185,7 @@ __global__ void __launch_bounds__(Shape4<PANELS, N>::kThreads, 1)
     mbar_init(bars + 8 * (2 * NS + 10), 1);
     mbar_init(q_ready, 4 * GR);
   }
-  if (warp == kWarpMma) tmem_alloc(smem_addr(s_tmem), kTmemCols);
+  if (warp == kWarpQk) tmem_alloc(smem_addr(s_tmem), kTmemCols);
   // the panel that a head of up to 64 elements has none for stays 0
   if constexpr (PANELS == 1)
     for (int i = tid; i < (int)(S::kValueBufs * kPanel / 16); i += S::kThreads)
@@ -258,7 +247,7 @@ __global__ void __launch_bounds__(Shape4<PANELS, N>::kThreads, 1)
       const int len = length_of(p, x.b);
       for (int t = x.tile; t < x.tile + x.n; ++t, ++i) {
         const uint32_t off = (uint32_t)reinterpret_cast<uintptr_t>(source(value ? p.vc : p.kc, t)) & 15u;
-        if (!(fine = warp_wait(raw_full(slot), lap))) break;
+        if (!(fine = warp_wait_done(raw_full(slot), lap))) break;
         const uint32_t* const row = reinterpret_cast<const uint32_t*>(smem + S::kAtRaw + (2 * slot + (value ? 1 : 0)) * S::kRaw +
                                                                       off + key * R);
         // the row's groups four at a time: 8 words of codes and one of scales
@@ -276,7 +265,7 @@ __global__ void __launch_bounds__(Shape4<PANELS, N>::kThreads, 1)
         const int buf = i & 1;
         if (!value) {
           // the product that read this buffer is done
-          if (i >= 2 && !(fine = warp_wait(s_full(buf), (i / 2 - 1) & 1))) break;
+          if (i >= 2 && !(fine = warp_wait_done(s_full(buf), (i / 2 - 1) & 1))) break;
           tmem_fence_after();
 #pragma unroll
           for (int g = 0; g < 4 * PANELS; g += 4) {
@@ -295,7 +284,7 @@ __global__ void __launch_bounds__(Shape4<PANELS, N>::kThreads, 1)
           }
         } else {
           const int vb = VB == 2 ? buf : 0;
-          if (i >= VB && !(fine = warp_wait(v_free(vb), (i / VB - 1) & 1))) break;
+          if (i >= VB && !(fine = warp_wait_done(v_free(vb), (i / VB - 1) & 1))) break;
           uint8_t* const to = smem + vb * S::kValues + key * 128;
 #pragma unroll
           for (int g = 0; g < 4 * PANELS; g += 4) {
@@ -319,40 +308,49 @@ __global__ void __launch_bounds__(Shape4<PANELS, N>::kThreads, 1)
         if (++slot == NS) slot = 0, lap ^= 1u;
       }
     }
-  } else if (warp == kWarpMma) {
-    // ---- products, by the whole warp in step
-    constexpr uint32_t word_s = mma_word(false, kM, N, false), word_o = mma_word(false, kM, N, true) | 1u << 15;
+  } else if (warp == kWarpQk) {
+    // ---- the scores' products, by the whole warp in step
+    constexpr uint32_t word = mma_word(false, kM, N, false);
     const uint32_t t_base = __shfl_sync(0xffffffffu, tmem, 0);
     int i = 0;
     uint32_t units = 0;
     while (fine && list.next(p, x)) {
       const int n = __shfl_sync(0xffffffffu, x.n, 0);
       if (!n) continue;
-      auto scores = [&](int j) {
-        if (!warp_wait(k_ready(j & 1), (j / 2) & 1)) return fine = false;
+      if (!(fine = warp_wait(q_ready, units & 1))) break;
+      ++units;
+      for (int t = 0; t < n; ++t, ++i) {
+        const int buf = i & 1;
+        // (the scores that this buffer had are read)
+        if (!(fine = i < 2 ? warp_wait(k_ready(buf), 0)
+                           : warp_wait_both(k_ready(buf), (i / 2) & 1, p_ready(buf), (i / 2 - 1) & 1)))
+          break;
         tmem_fence_after();
 #pragma unroll
         for (int s = 0; s < DP / 16; ++s)
-          mma_tmem(t_base + S::kColS + (j & 1) * N, t_base + (j & 1) * (DP / 2) + 8 * s,
-                   smem_operand(base + S::kAtQ + (s / 4) * (N * 128) + (s % 4) * 32, 16), word_s, s > 0);
-        mma_commit(s_full(j & 1));
-        return true;
-      };
-      if (!(fine = warp_wait(q_ready, units & 1))) break;
-      ++units;
-      if (!scores(i)) break;
-      for (int t = 0; t < n && fine; ++t, ++i) {
-        if (t + 1 < n && !scores(i + 1)) break;
-        const int vb = VB == 2 ? i & 1 : 0;
-        if (!(fine = warp_wait_both(v_ready(vb), (i / VB) & 1, p_ready(i & 1), (i / 2) & 1))) break;
+          mma_tmem(t_base + S::kColS + buf * N, t_base + buf * (DP / 2) + 8 * s,
+                   smem_operand(base + S::kAtQ + (s / 4) * (N * 128) + (s % 4) * 32, 16), word, s > 0);
+        mma_commit(s_full(buf));
+      }
+    }
+  } else if (warp == kWarpPv) {
+    // ---- the sums' products, by the whole warp in step
+    constexpr uint32_t word = mma_word(false, kM, N, true) | 1u << 15;  // A is as the values lie
+    const uint32_t t_base = __shfl_sync(0xffffffffu, tmem, 0);
+    int i = 0;
+    while (fine && list.next(p, x)) {
+      const int n = __shfl_sync(0xffffffffu, x.n, 0);
+      for (int t = 0; t < n; ++t, ++i) {
+        const int buf = i & 1, vb = VB == 2 ? buf : 0;
+        if (!(fine = warp_wait_both(v_ready(vb), (i / VB) & 1, p_ready(buf), (i / 2) & 1))) break;
         tmem_fence_after();
 #pragma unroll
         for (int m = 0; m < S::kBlocks; ++m)
 #pragma unroll
           for (int s = 0; s < kKeys / 16; ++s)
             mma_smem(t_base + S::kColO + m * N, smem_operand(base + vb * S::kValues + m * 2 * kPanel + 2048 * s, kPanel),
-                     smem_operand(base + S::kAtP + (i & 1) * S::kP + 2048 * s, kPanel), word_o, s > 0 || t > 0);
-        mma_commit(pv_done(i & 1));
+                     smem_operand(base + S::kAtP + buf * S::kP + 2048 * s, kPanel), word, s > 0 || t > 0);
+        mma_commit(pv_done(buf));
         if constexpr (VB == 1) mma_commit(v_free(0));
       }
     }
@@ -417,30 +415,43 @@ __global__ void __launch_bounds__(Shape4<PANELS, N>::kThreads, 1)
       if (!(fine = group_all(id, 128, fine))) break;
 #pragma unroll 1
       for (int t = 0; t < n; ++t, ++i) {
-        const int buf = i & 1;
-        const bool there = (x.tile + t) * kKeys + L < len;
-        fine = fine && warp_wait(s_full(buf), (i / 2) & 1);
-        float y[C];
+        const int buf = i & 1, seen = len - (x.tile + t) * kKeys;
+        const bool there = L < seen;
+        const uint32_t t_s = tmem + lanes + S::kColS + buf * N + r0;
+        float z[C];
+        // scores against their rows' reference points
+        auto scores = [&] {
+          tmem_load<C>(t_s, reinterpret_cast<uint32_t*>(z));
+          tmem_wait_load();
+#pragma unroll
+          for (int r = 0; r < C; r += 2) {
+            const float4 f = *reinterpret_cast<const float4*>(row_of + r);
+            z[r] = fmaf(z[r], f.x, -f.y);
+            z[r + 1] = fmaf(z[r + 1], f.z, -f.w);
+          }
+          if (seen < kKeys) {
+#pragma unroll
+            for (int r = 0; r < C; ++r) z[r] = there ? z[r] : -INFINITY;
+          }
+        };
+        fine = fine && warp_wait_done(s_full(buf), (i / 2) & 1);
         bool above = false;
         if (fine) {
           tmem_fence_after();
-          tmem_load<C>(tmem + lanes + S::kColS + buf * N + r0, reinterpret_cast<uint32_t*>(y));
-          tmem_wait_load();
-          float top = -INFINITY;
+          scores();
+          float top[2] = {z[0], z[1]};
 #pragma unroll
-          for (int r = 0; r < C; ++r) {
-            const float2 f = row_of[r];
-            const float z = fmaf(y[r], f.x, -f.y);
-            top = fmaxf(top, z);
-          }
-          above = there && top > kSlack + kBelow<__half>;
+          for (int r = 2; r < C; ++r) top[r & 1] = fmaxf(top[r & 1], z[r]);
+          above = fmaxf(top[0], top[1]) > kSlack + kBelow<__half>;
         }
         // one warp's score above its row's reference point, or a wait that gave up, concerns all
         if (!group_all(id, 128, fine && !above)) {
           if (!(fine = group_all(id, 128, fine))) break;
+          tmem_load<C>(t_s, reinterpret_cast<uint32_t*>(z));
+          tmem_wait_load();
 #pragma unroll
           for (int r = 0; r < C; ++r) {
-            const int best = __reduce_max_sync(0xffffffffu, ordered(there ? y[r] * row_of[r].x : -INFINITY));
+            const int best = __reduce_max_sync(0xffffffffu, ordered(there ? z[r] * row_of[r].x : -INFINITY));
             if (lane == 0) s_max[quarter * N + r0 + r] = unordered(best);
           }
           // sums so far are on the old points until the last product is done
@@ -464,38 +475,31 @@ __global__ void __launch_bounds__(Shape4<PANELS, N>::kThreads, 1)
             row_of[L].y = to;
           }
           group_sync(id, 128);
-          float f[C];
+          if (t > 0) tmem_fence_after();
 #pragma unroll
-          for (int r = 0; r < C; ++r) {
-            f[r] = s_fac[r0 + r];
-            l[r] *= f[r];
+          for (int m = 0; m < (t > 0 ? S::kBlocks : 0); ++m) {
+            float o[C];
+            tmem_load<C>(tmem + lanes + S::kColO + m * N + r0, reinterpret_cast<uint32_t*>(o));
+            tmem_wait_load();
+#pragma unroll
+            for (int r = 0; r < C; ++r) o[r] *= s_fac[r0 + r];
+            tmem_store<C>(tmem + lanes + S::kColO + m * N + r0, reinterpret_cast<const uint32_t*>(o));
           }
-          if (t > 0) {
-            tmem_fence_after();
+          tmem_wait_store();
 #pragma unroll
-            for (int m = 0; m < S::kBlocks; ++m) {
-              float o[C];
-              tmem_load<C>(tmem + lanes + S::kColO + m * N + r0, reinterpret_cast<uint32_t*>(o));
-              tmem_wait_load();
-#pragma unroll
-              for (int r = 0; r < C; ++r) o[r] *= f[r];
-              tmem_store<C>(tmem + lanes + S::kColO + m * N + r0, reinterpret_cast<const uint32_t*>(o));
-            }
-            tmem_wait_store();
-          }
+          for (int r = 0; r < C; ++r) l[r] *= s_fac[r0 + r];
+          scores();
           group_sync(id, 128);  // s_max and s_fac are read
         }
         uint32_t w[C / 2];
 #pragma unroll
         for (int r = 0; r < C; r += 2) {
-          const float4 f = *reinterpret_cast<const float4*>(row_of + r);
-          float2 e = make_float2(ex2(fmaf(y[r], f.x, -f.y)), ex2(fmaf(y[r + 1], f.z, -f.w)));
-          if (!there) e = make_float2(0.0f, 0.0f);
+          const float2 e = make_float2(ex2(z[r]), ex2(z[r + 1]));
           l[r] += e.x, l[r + 1] += e.y;
           w[r / 2] = pack2<__half>(e.x, e.y);
         }
         // the product that read this buffer is done
-        if (i >= 2) fine = warp_wait(pv_done(buf), (i / 2 - 1) & 1);
+        if (i >= 2) fine = warp_wait_done(pv_done(buf), (i / 2 - 1) & 1);
         if (fine) {
           uint8_t* const to = smem + S::kAtP + buf * S::kP + L * 128;
 #pragma unroll
@@ -517,8 +521,8 @@ __global__ void __launch_bounds__(Shape4<PANELS, N>::kThreads, 1)
       ++units;
       if (have) queries(x);
       // this piece's sums: l over the keys of all warps, O as it is
-      const float mine = warp_columns<C>(l);
-      if (C == 32 || !(lane & 1)) s_max[quarter * N + r0 + column_of<C>(lane)] = mine;
+      const float mine = warp_columns(l);
+      if (!(lane & 1)) s_max[quarter * N + r0 + (lane >> 1)] = mine;
       fine = warp_wait(pv_done(last & 1), (last / 2) & 1);
       if (!(fine = group_all(id, 128, fine))) break;
       tmem_fence_after();
@@ -541,7 +545,7 @@ __global__ void __launch_bounds__(Shape4<PANELS, N>::kThreads, 1)
   if (!fine && (warp < kWarpK || lane == 0)) atomicAdd(faults, 1u);
   tmem_fence_before();
   __syncthreads();
-  if (warp == kWarpMma) {
+  if (warp == kWarpQk) {
     __syncwarp();
     tmem_free(tmem, kTmemCols);
   }
