@@ -180,18 +180,25 @@ class DraftModel:
     context's GPU over a key/value cache of ``capacity`` rows per block.
 
     ``forward`` evaluates a tree of drafted nodes behind the cached tokens,
-    ``accept`` appends the nodes that the target confirmed, ``prefill`` takes
-    a prompt.  With ``budget``, a tree that would not fit behind the longest
+    ``accept`` appends the nodes that the target confirmed, ``prompt`` takes
+    the packed prompts of all sequences, ``prefill`` prompts of one length in
+    trees.  With ``budget``, a tree that would not fit behind the longest
     sequence's rows has every sequence cut to its ``recent`` latest and its
     heaviest keys first.  Where it might not fit, ``forward`` reads the lengths
-    back (it waits for the GPU then)."""
+    back (it waits for the GPU then).  With ``cache_bits=4`` the cache is kept
+    in 4 bits (``row4_bytes``), without a budget: the weights that eviction
+    goes by are not gathered over such a cache."""
 
     def __init__(self, cc, block_weights: list, capacity: int, batch: int = 1, heads: int = 12, dtype=None,
-                 budget: int | None = None, recent: int = 0):
+                 budget: int | None = None, recent: int = 0, cache_bits: int | None = None):
         import torch
+        if cache_bits not in (None, 4):
+            raise ValueError(f"cache_bits: expected 4, or None for rows of the model's type, got {cache_bits}")
+        if cache_bits == 4 and budget is not None:
+            raise ValueError("budget: a 4-bit cache is not cut")
         device = torch.device("cuda", cc.params.device)
         self.cc, self.heads, self.batch, self.capacity = cc, heads, batch, capacity
-        self.budget, self.recent = budget, recent
+        self.budget, self.recent, self._four = budget, recent, cache_bits == 4
         self.dtype = torch.bfloat16 if dtype is None else dtype
         if budget is not None and budget + MAX_NODES > capacity:
             raise ValueError(f"budget: {budget} rows and a tree of {MAX_NODES} nodes do not fit a capacity of {capacity}")
@@ -201,8 +208,10 @@ class DraftModel:
         self.width = self.weights[0]["ln1"].shape[0]
 
         def caches():
-            rows = (batch, heads, capacity, self.width // heads)
-            return [(torch.zeros(rows, dtype=self.dtype, device=device), torch.zeros(rows, dtype=self.dtype, device=device),
+            size = self.width // heads
+            rows, kind = (batch, heads, capacity, row4_bytes(size) if self._four else size), \
+                torch.uint8 if self._four else self.dtype
+            return [(torch.zeros(rows, dtype=kind, device=device), torch.zeros(rows, dtype=kind, device=device),
                      torch.zeros(rows[:3], device=device)) for _ in block_weights]
 
         self.caches, self._spare = caches(), caches() if budget is not None else None
@@ -218,31 +227,67 @@ class DraftModel:
         b, n, width = x.shape
         if self._most + n > self.capacity:
             self._make_room(n)
-        x, steps = x.to(torch.float32), []
+        x, steps, attend = x.to(torch.float32), [], attention4 if self._four else attention
         for w, (k_cache, v_cache, _) in zip(self.weights, self.caches):
-            h = torch.layer_norm(x, (width,), w["ln1"], None, 1e-5).to(self.dtype)
-            q, k, v = (h @ w["attn_qkv"].T).view(b, n, 3, self.heads, width // self.heads).unbind(2)
-            out, lse = attention(self.cc, q, k_cache, v_cache, self.lens, k, v, parents)
-            x = x + (out.reshape(b, n, width) @ w["attn_proj"].T).float()
-            h = torch.layer_norm(x, (width,), w["ln2"], None, 1e-5).to(self.dtype)
-            h = torch.nn.functional.gelu(h @ w["mlp_fc"].T, approximate="tanh")
-            x = x + (h @ w["mlp_proj"].T).float()
+            q, k, v = self._qkv(x, w).view(b, n, 3, self.heads, width // self.heads).unbind(2)
+            out, lse = attend(self.cc, q, k_cache, v_cache, self.lens, k, v, parents)
+            x = self._rest(x, out.reshape(b, n, width), w)
             steps.append((q, lse, k, v))
         self._steps = steps
         return x
+
+    def _qkv(self, x, w):
+        import torch
+        return torch.layer_norm(x, (self.width,), w["ln1"], None, 1e-5).to(self.dtype) @ w["attn_qkv"].T
+
+    def _rest(self, x, out, w):
+        """A block behind its attention."""
+        import torch
+        x = x + (out @ w["attn_proj"].T).float()
+        h = torch.layer_norm(x, (self.width,), w["ln2"], None, 1e-5).to(self.dtype)
+        h = torch.nn.functional.gelu(h @ w["mlp_fc"].T, approximate="tanh")
+        return x + (h @ w["mlp_proj"].T).float()
 
     def accept(self, path, count):
         """Appends the nodes path[:, :count] of the last ``forward`` to every
         block's cache, and their attention weights to its keys'."""
         if self._steps is None:
             raise RuntimeError("accept follows a forward")
-        lens = self.lens
+        lens, append = self.lens, commit4 if self._four else commit
         for (q, lse, k, v), (k_cache, v_cache, acc) in zip(self._steps, self.caches):
-            self.lens = commit(self.cc, k_cache, v_cache, lens, k, v, path, count)
+            self.lens = append(self.cc, k_cache, v_cache, lens, k, v, path, count)
             if self.budget is not None:
                 accumulate(self.cc, q, lse, k_cache, lens, path, count, acc)
         self._most = min(self.capacity, self._most + path.shape[1])
         self._steps = None
+
+    def prompt(self, x, starts):
+        """The sequences' prompts, packed: embeddings x [T, D], starts
+        [batch + 1] int32 as for ``drafting.prompt``.  Returns the hidden states
+        [T, D] (float32).  The caches must be empty, and hold the longest prompt
+        (``starts`` is read back where the rows might be more than the
+        capacity).  A model with a budget takes its prompt through ``prefill``,
+        which gathers the weights that eviction goes by."""
+        import torch
+        if self.budget is not None:
+            raise ValueError("prompt: a model with a budget gathers its prompt's weights through prefill")
+        if self._most:
+            raise ValueError("prompt: the cache holds rows already")
+        t, width = x.shape
+        most = t
+        if t > self.capacity:
+            s = starts.clamp(0, t).cummax(0).values
+            most = int((s[1:] - s[:-1]).max())
+            if most > self.capacity:
+                raise ValueError(f"a prompt of {most} tokens exceeds the capacity of {self.capacity}")
+        x, lens, append = x.to(torch.float32), self.lens, fill4 if self._four else fill
+        for w, (k_cache, v_cache, _) in zip(self.weights, self.caches):
+            q, k, v = self._qkv(x, w).view(t, 3, self.heads, width // self.heads).unbind(1)
+            out, _ = prompt(self.cc, q, k, v, starts)
+            self.lens = append(self.cc, k_cache, v_cache, lens, k, v, starts)
+            x = self._rest(x, out.reshape(t, width), w)
+        self._most, self._steps = most, None
+        return x
 
     def prefill(self, x):
         """A prompt's embeddings [batch, m, D], in chains of 64 nodes; returns
