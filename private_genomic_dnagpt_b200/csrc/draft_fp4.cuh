@@ -41,49 +41,50 @@ __device__ __forceinline__ __half scale4(uint32_t byte) { return __ushort_as_hal
 // (to even in the middle).  The quotient rounded to 24 bits first gives the
 // same result as the exact one: it can only reach a middle m of five bits from
 // 6 m itself, because the float next to 6 m is off by more than half a step of m.
+// (Rounded as in encode4; below 2^-18, where that need not hold, all become 0.)
 __device__ __forceinline__ uint32_t scale4_of(float top) {
-  const float a = __fdiv_rn(top, 6.0f);
+  constexpr float sixth = 1.0f / 6.0f;
+  const float q = __fmul_rn(top, sixth), a = __fmaf_rn(__fmaf_rn(-q, 6.0f, top), sixth, q);
   const uint32_t u = __float_as_uint(a);
-  if (a < 6.103515625e-5f) return (uint32_t)__float2int_rn(a * 131072.0f);  // 2^-14 and below: multiples of 2^-17
-  const uint32_t b = ((u + 0x7FFFFu + (u >> 20 & 1u)) >> 20) - (112u << 3);
-  return b < kScaleTop ? b : kScaleTop;
+  const uint32_t b = min(((u + 0x7FFFFu + (u >> 20 & 1u)) >> 20) - (112u << 3), kScaleTop);
+  return a < 6.103515625e-5f ? (uint32_t)__float2int_rn(a * 131072.0f) : b;  // below 2^-14: multiples of 2^-17
 }
 
-// One group: the 16 codes and the scale.  x / s is rounded to 24 bits, which
-// moves no quotient onto or over the border between two codes (a border times
-// s has at most seven bits, and the float next to it is off by more than half
-// a step of the border).  The quotient is q + r e with q = x r, e = x - q s and
-// r = 1 / s rounded: with r rounded correctly this is x / s rounded correctly
-// (Markstein, "Computation of elementary functions on the IBM RISC System/6000
-// processor", 1990).
-__device__ __forceinline__ uint64_t encode4(const float* x, uint32_t& scale) {
-  uint32_t top = 0;
-#pragma unroll
-  for (int i = 0; i < kGroup4; ++i) top = max(top, __float_as_uint(x[i]) & 0x7FFFFFFFu);
-  if (top >= 0x7F800000u) {
-    scale = kScaleNone;
-    return 0;
-  }
+// One group: the 16 codes, and the scale from the largest magnitude (as bits).
+// x / s is rounded to 24 bits, which moves no quotient onto or over
+// the border between two codes (a border times s has at most seven bits, and
+// the float next to it is off by more than half a step of the border).  The
+// quotient is q + r e with q = x r, e = x - q s and r = 1 / s rounded: with r
+// rounded correctly this is x / s rounded correctly (Markstein, "Computation
+// of elementary functions on the IBM RISC System/6000 processor", 1990).
+// r is one Newton step from an approximation to 2^-23, off by 2^-46 before it is
+// rounded: s is a power of two times 8/8, 9/8, ..., 15/8, and the binary
+// expansions of 8/9, 8/10, ..., 8/15 have periods of 2 to 12 digits, none of
+// which continues a middle between two floats for 22 digits.
+__device__ __forceinline__ uint2 encode4(const float* x, uint32_t top, uint32_t& scale) {
+  const bool none = top >= 0x7F800000u;
   scale = scale4_of(__uint_as_float(top));
-  if (scale == 0) {
-    uint64_t w = 0;  // zeros keep their signs
+  // what is too small for any scale rounds to zeros, which keep their signs
+  const float s = scale ? __half2float(scale4(scale)) : 1.0f;
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(s));
+  r = __fmaf_rn(r, __fmaf_rn(-s, r, 1.0f), r);
+  uint32_t w[2];
 #pragma unroll
-    for (int i = 0; i < kGroup4; ++i) w |= (uint64_t)(__float_as_uint(x[i]) >> 31) << (4 * i + 3);
-    return w;
-  }
-  const float s = __half2float(scale4(scale)), r = __frcp_rn(s);
-  uint32_t w[2] = {0, 0};
+  for (int h = 0; h < 2; ++h) {
+    float t[8];
 #pragma unroll
-  for (int i = 0; i < kGroup4; i += 2) {
-    float t[2];
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const float q = __fmul_rn(x[i + k], r);
-      t[k] = copysignf(__fmaf_rn(__fmaf_rn(-q, s, x[i + k]), r, q), x[i + k]);  // -0 stays
+    for (int i = 0; i < 8; ++i) {
+      const float v = x[8 * h + i], q = __fmul_rn(v, r);
+      t[i] = copysignf(__fmaf_rn(__fmaf_rn(-q, s, v), r, q), v);  // -0 stays
     }
-    w[i / 8] |= (uint32_t)__nv_cvt_float2_to_fp4x2(make_float2(t[0], t[1]), __NV_E2M1, cudaRoundNearest) << (4 * (i % 8));
+    asm("{\n .reg .b8 a, b, c, d;\n cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n cvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n"
+        " cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n cvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n mov.b32 %0, {a, b, c, d};\n}"
+        : "=r"(w[h])
+        : "f"(t[0]), "f"(t[1]), "f"(t[2]), "f"(t[3]), "f"(t[4]), "f"(t[5]), "f"(t[6]), "f"(t[7]));
   }
-  return (uint64_t)w[1] << 32 | w[0];
+  if (none) scale = kScaleNone;
+  return none ? make_uint2(0u, 0u) : make_uint2(w[0], w[1]);
 }
 
 // two elements from a byte, times the scale (in both halves), exactly
