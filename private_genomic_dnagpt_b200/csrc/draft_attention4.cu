@@ -247,7 +247,12 @@ __global__ void __launch_bounds__(Shape4<PANELS, N>::kThreads, 1)
       const int len = length_of(p, x.b);
       for (int t = x.tile; t < x.tile + x.n; ++t, ++i) {
         const uint32_t off = (uint32_t)reinterpret_cast<uintptr_t>(source(value ? p.vc : p.kc, t)) & 15u;
-        if (!(fine = warp_wait_done(raw_full(slot), lap))) break;
+        // (what this tile takes the place of is used)
+        const int back = value ? VB : 2;
+        const uint32_t used = value ? v_free(VB == 2 ? i & 1 : 0) : s_full(i & 1);
+        if (!(fine = i < back ? warp_wait_done(raw_full(slot), lap)
+                              : warp_wait_both(raw_full(slot), lap, used, (i / back - 1) & 1)))
+          break;
         const uint32_t* const row = reinterpret_cast<const uint32_t*>(smem + S::kAtRaw + (2 * slot + (value ? 1 : 0)) * S::kRaw +
                                                                       off + key * R);
         // the row's groups four at a time: 8 words of codes and one of scales
@@ -264,8 +269,6 @@ __global__ void __launch_bounds__(Shape4<PANELS, N>::kThreads, 1)
         const bool there = t * kKeys + key < len;
         const int buf = i & 1;
         if (!value) {
-          // the product that read this buffer is done
-          if (i >= 2 && !(fine = warp_wait_done(s_full(buf), (i / 2 - 1) & 1))) break;
           tmem_fence_after();
 #pragma unroll
           for (int g = 0; g < 4 * PANELS; g += 4) {
@@ -284,7 +287,6 @@ __global__ void __launch_bounds__(Shape4<PANELS, N>::kThreads, 1)
           }
         } else {
           const int vb = VB == 2 ? buf : 0;
-          if (i >= VB && !(fine = warp_wait_done(v_free(vb), (i / VB - 1) & 1))) break;
           uint8_t* const to = smem + vb * S::kValues + key * 128;
 #pragma unroll
           for (int g = 0; g < 4 * PANELS; g += 4) {

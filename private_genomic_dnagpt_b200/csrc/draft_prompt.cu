@@ -54,243 +54,6 @@ struct Starts {
   }
 };
 
-// rows of no sequence: out 0, lse -inf; by the first `threads` of all CTAs
-template <typename T>
-__device__ __forceinline__ void clear_spare(const PromptParams& p, int first, int last, int threads) {
-  const int spare = p.tokens - (last - first);
-  for (int i = blockIdx.x; i < spare; i += gridDim.x) {
-    const int t = i < first ? i : last + (i - first);
-    for (int x = threadIdx.x; x < p.q_heads * p.head_dim; x += threads)
-      static_cast<T*>(p.out.data)[(int64_t)t * p.out.row + x / p.head_dim * p.out.head + x % p.head_dim] = from_f32<T>(0.0f);
-    for (int h = threadIdx.x; h < p.q_heads; h += threads) p.lse[(int64_t)t * p.q_heads + h] = -INFINITY;
-  }
-}
-
-// ---- every type, size and stride: CUDA cores ------------------------------------
-// A CTA of 16 x 16 threads takes 64 rows of one query head, the longest first,
-// over tiles of 64 keys staged in shared memory as floats.  Scores: a thread
-// has 4 rows x 4 keys; values: 4 rows x 4 elements of every 64.  A row's 16
-// threads are half a warp, so its maximum and sum are shuffles.
-constexpr int kRows = 64, kThreads = 256;
-
-template <typename T, int DC>
-__global__ void __launch_bounds__(kThreads) prompt_kernel(PromptParams p) {
-  extern __shared__ __align__(16) float sm[];
-  const int D = p.head_dim, D4 = (D + 3) & ~3, KS = D4 + 4, PS = kRows + 4;
-  float* sq = sm;                  // [kRows][D4]
-  float* sk = sq + kRows * D4;     // [kRows][KS]
-  float* sv = sk + kRows * KS;     // [kRows][D4]
-  float* sp = sv + kRows * D4;     // [kRows][PS]
-  __shared__ int s_place[5];       // first row of the sequence, its length, first row of the tile, start(0), start(batch)
-  const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
-  const int h = blockIdx.x % p.q_heads;
-  if (tid < 32) {
-    Starts s;
-    s.begin(p);
-    int unit = blockIdx.x / p.q_heads;
-    if (tid == 0) s_place[2] = -1;
-    __syncwarp();
-    for (int b0 = 0; b0 < p.batch; b0 += 32) {
-      const int2 at = s.next(p, b0);
-      const int tiles = (at.y + kRows - 1) / kRows;
-      int sum = tiles;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int y = __shfl_up_sync(0xffffffffu, sum, o);
-        if ((tid & 31) >= o) sum += y;
-      }
-      if (unit >= sum - tiles && unit < sum) {
-        s_place[0] = at.x;
-        s_place[1] = at.y;
-        s_place[2] = (sum - 1 - unit) * kRows;
-      }
-      unit -= __shfl_sync(0xffffffffu, sum, 31);
-    }
-    if (tid == 0) s_place[3] = s.first, s_place[4] = s.last;
-  }
-  __syncthreads();
-  clear_spare<T>(p, s_place[3], s_place[4], kThreads);
-  const int seq = s_place[0], len = s_place[1], row0 = s_place[2];
-  if (row0 < 0) return;
-  const T* q = static_cast<const T*>(p.q.data) + (int64_t)(seq + row0) * p.q.row + h * p.q.head;
-  const T* k = static_cast<const T*>(p.k.data) + (int64_t)seq * p.k.row + h / p.group * p.k.head;
-  const T* v = static_cast<const T*>(p.v.data) + (int64_t)seq * p.v.row + h / p.group * p.v.head;
-  const int rows = min(kRows, len - row0);
-  for (int i = tid; i < kRows * (D4 / 4); i += kThreads) {
-    const int r = i / (D4 / 4), d = i % (D4 / 4) * 4;
-    float x[4] = {0.f, 0.f, 0.f, 0.f};
-    if (r < rows) load_row4(x, q + (int64_t)r * p.q.row, d, D, p.wide);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) sq[r * D4 + d + e] = x[e] * (p.scale * kLog2e);
-  }
-  float m[4], l[4], acc[DC][4][4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    m[i] = -INFINITY, l[i] = 0.0f;
-#pragma unroll
-    for (int c = 0; c < DC; ++c)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) acc[c][i][e] = 0.0f;
-  }
-  for (int t0 = 0; t0 < row0 + rows; t0 += kRows) {
-    const int nk = min(kRows, len - t0);
-    const bool last = t0 == row0;  // the tile that the causal mask cuts
-    __syncthreads();
-    for (int i = tid; i < kRows * (D4 / 4); i += kThreads) {
-      const int r = i / (D4 / 4), d = i % (D4 / 4) * 4;
-      float x[4] = {0.f, 0.f, 0.f, 0.f}, y[4] = {0.f, 0.f, 0.f, 0.f};
-      if (r < nk) {
-        load_row4(x, k + (int64_t)(t0 + r) * p.k.row, d, D, p.wide);
-        load_row4(y, v + (int64_t)(t0 + r) * p.v.row, d, D, p.wide);
-      }
-      *reinterpret_cast<float4*>(sk + r * KS + d) = make_float4(x[0], x[1], x[2], x[3]);
-      *reinterpret_cast<float4*>(sv + r * D4 + d) = make_float4(y[0], y[1], y[2], y[3]);
-    }
-    __syncthreads();
-    float s[4][4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) s[i][j] = 0.0f;
-    for (int d = 0; d < D4; d += 4) {
-      float4 a[4], c[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) a[i] = *reinterpret_cast<const float4*>(sq + (4 * ty + i) * D4 + d);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) c[j] = *reinterpret_cast<const float4*>(sk + (tx + 16 * j) * KS + d);
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          s[i][j] = fmaf(a[i].x, c[j].x, fmaf(a[i].y, c[j].y, fmaf(a[i].z, c[j].z, fmaf(a[i].w, c[j].w, s[i][j]))));
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (last)
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (tx + 16 * j > 4 * ty + i) s[i][j] = -INFINITY;
-      float mx = fmaxf(fmaxf(s[i][0], s[i][1]), fmaxf(s[i][2], s[i][3]));
-#pragma unroll
-      for (int o = 8; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-      const float top = fmaxf(m[i], mx), base = top == -INFINITY ? 0.0f : top, f = exp2f(m[i] - base);
-      m[i] = top;
-      float sum = 0.0f;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float e = exp2f(s[i][j] - base);
-        sum += e;
-        sp[(4 * ty + i) * PS + tx + 16 * j] = e;
-      }
-#pragma unroll
-      for (int o = 8; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      l[i] = fmaf(l[i], f, sum);
-#pragma unroll
-      for (int c = 0; c < DC; ++c)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) acc[c][i][e] *= f;
-    }
-    __syncwarp();  // a row's weights are of one half warp
-    const int to = last ? rows : kRows;
-    for (int j = 0; j < to; ++j) {
-      float w[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) w[i] = sp[(4 * ty + i) * PS + j];
-#pragma unroll
-      for (int c = 0; c < DC; ++c) {
-        const int d = 64 * c + 4 * tx;
-        if (d >= D4) continue;
-        const float4 y = *reinterpret_cast<const float4*>(sv + j * D4 + d);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          // a value reaches the rows that see it only, whatever it holds
-          if (last && j > 4 * ty + i) continue;
-          acc[c][i][0] = fmaf(w[i], y.x, acc[c][i][0]);
-          acc[c][i][1] = fmaf(w[i], y.y, acc[c][i][1]);
-          acc[c][i][2] = fmaf(w[i], y.z, acc[c][i][2]);
-          acc[c][i][3] = fmaf(w[i], y.w, acc[c][i][3]);
-        }
-      }
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int r = 4 * ty + i;
-    if (r >= rows) continue;
-    const float inv = l[i] != 0.0f ? 1.0f / l[i] : 0.0f;  // 0: no score is above -inf
-    T* o = static_cast<T*>(p.out.data) + (int64_t)(seq + row0 + r) * p.out.row + h * p.out.head;
-#pragma unroll
-    for (int c = 0; c < DC; ++c)
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (64 * c + 4 * tx + e < D) o[64 * c + 4 * tx + e] = from_f32<T>(acc[c][i][e] * inv);
-    if (tx == 0) p.lse[(int64_t)(seq + row0 + r) * p.q_heads + h] = l[i] != 0.0f ? kLn2 * (m[i] + log2f(l[i])) : -INFINITY;
-  }
-}
-
-constexpr size_t prompt_smem(int D4) { return sizeof(float) * kRows * (3 * D4 + 4 + kRows + 4); }
-
-template <typename T, int DC>
-void launch_prompt(const PromptParams& p, cudaStream_t st) {
-  auto* k = prompt_kernel<T, DC>;
-  static_assert(prompt_smem(64 * DC) <= 232448 - 64, "shared memory of one block");
-  CKKS_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)prompt_smem(64 * DC)));
-  const unsigned grid = (unsigned)(std::max(1, p.batch + p.tokens / kRows) * p.q_heads);
-  k<<<grid, kThreads, prompt_smem((p.head_dim + 3) & ~3), st>>>(p);
-  CKKS_CUDA(cudaGetLastError());
-}
-
-template <typename T>
-void run_prompt(const PromptParams& p, cudaStream_t st) {
-  switch ((p.head_dim + 63) / 64) {
-    case 1: launch_prompt<T, 1>(p, st); break;
-    case 2: launch_prompt<T, 2>(p, st); break;
-    case 3: launch_prompt<T, 3>(p, st); break;
-    default: launch_prompt<T, 4>(p, st); break;
-  }
-}
-
-// ---- 16-bit types: tensor cores -------------------------------------------------
-// A unit is 256 rows of one query head of one sequence: two groups of four
-// softmax warps have 128 rows each (over 128 elements there is one group, as
-// tensor memory holds one S and O then), a thread a row.  Keys come in tiles of
-// 128, each copied once for both groups: S_g = Q_g K^T into tensor memory, the
-// weights back into S's place as the 16-bit A operand of O_g += P_g V.  One warp
-// issues copies, one the products; while one group exponentiates, the products
-// of the other run.  The first group has one tile less than the second, and
-// only a group's last tile is cut by the causal mask.
-//
-// CTAs are one to an SM and take the units of the list in turns, one round
-// upwards and the next one downwards: a sequence's units lie in the list from
-// the longest on, so every CTA gets about the same.
-//
-// A row's reference point m follows the maximum only when that has grown by
-// more than 2^8; O is seldom rescaled.  A weight is rounded once, to the
-// operands' type (half a step, as the result is), and summed in 32 bits before
-// that.  Two numbers a weight, as over a cache, would be half as many products
-// again, which bound this kernel where heads are wide; one number leaves a
-// result 1.4 times as far from the exact one as its own rounding takes it.
-//
-// The exponential unit takes 8 cycles for a warp's 32: 2048 cycles for a pair of
-// tiles, whose products take 1024 at 64 elements and 2048 at 128.  So some of
-// the exponentials are computed with multiply-adds: 2^x = 2^n 2^r, n the nearest
-// integer, and 2^r the polynomial of degree 4 with the least largest relative
-// error on [-1/2, 1/2] (2.7e-6, fitted to 2^r).
-constexpr int kHalf = 64;  // keys of a half tile
-
-template <int PANELS>
-struct PromptShape {
-  static constexpr int kGroups = PANELS <= 2 ? 2 : 1, kThreads = 32 * (5 * kGroups + 1), kUnitRows = kM * kGroups;
-  static constexpr int kSlots = PANELS == 1 ? 10 : PANELS == 2 ? 5 : PANELS == 3 ? 3 : 2;
-  static constexpr uint32_t kTileBytes = PANELS * kPanel;
-  // Q of each group, the ring of K and V tiles, barriers, masks, one word
-  static constexpr uint32_t kRing = kGroups * kTileBytes, kExtra = kRing + kSlots * kTileBytes;
-  static constexpr int kBars = 2 * kSlots + 20;
-  static constexpr size_t kSmem = kExtra + kBars * 8 + 6 * 4 * 4 + 16;
-  // of eight pairs of exponentials, how many the multiply-adds take
-  static constexpr int kPoly = PANELS <= 2 ? 2 : 0;
-};
-
 // a place in the list of units; walked upwards by a whole warp
 struct Unit {
   int seq, len, row0, head;  // first row of the sequence, its length, the unit's first row of it, query head
@@ -337,6 +100,250 @@ struct Units {
     u.head = (w - before) % p.q_heads;
     return true;
   }
+};
+
+// rows of no sequence: out 0, lse -inf; by the first `threads` of all CTAs
+template <typename T>
+__device__ __forceinline__ void clear_spare(const PromptParams& p, int first, int last, int threads) {
+  const int spare = p.tokens - (last - first);
+  for (int i = blockIdx.x; i < spare; i += gridDim.x) {
+    const int t = i < first ? i : last + (i - first);
+    for (int x = threadIdx.x; x < p.q_heads * p.head_dim; x += threads)
+      static_cast<T*>(p.out.data)[(int64_t)t * p.out.row + x / p.head_dim * p.out.head + x % p.head_dim] = from_f32<T>(0.0f);
+    for (int h = threadIdx.x; h < p.q_heads; h += threads) p.lse[(int64_t)t * p.q_heads + h] = -INFINITY;
+  }
+}
+
+// ---- every type, size and stride: CUDA cores ------------------------------------
+// A CTA of 16 x 16 threads takes 16 RT rows of one query head, the longest
+// first, over tiles of 64 keys staged in shared memory as floats.  Scores: a
+// thread has RT rows x 4 keys; values: RT rows x 4 elements of every 64.  A row's
+// 16 threads are half a warp, so its maximum and sum are shuffles.  Reads from
+// shared memory bound it (8 of 16 bytes for 64 multiply-adds, 12 for 128 with RT
+// 8): 29 TFLOP/s for one prompt of 4096 and 16 heads of 64 in float32.
+constexpr int kKeyTile = 64, kThreads = 256;
+
+template <typename T, int DC, int RT>
+__global__ void __launch_bounds__(kThreads) prompt_kernel(PromptParams p) {
+  constexpr int ROWS = 16 * RT, PS = kKeyTile + 4;
+  extern __shared__ __align__(16) float sm[];
+  const int D = p.head_dim, D4 = (D + 3) & ~3, KS = D4 + 4;
+  float* sq = sm;                     // [ROWS][D4]
+  float* sk = sq + ROWS * D4;         // [kKeyTile][KS]
+  float* sv = sk + kKeyTile * KS;     // [kKeyTile][D4]
+  float* sp = sv + kKeyTile * D4;     // [ROWS][PS]
+  const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
+  Units<ROWS> list;
+  list.begin(p);
+  Unit u;
+  const bool some = list.find(p, blockIdx.x, u);
+  while (list.b0 + 32 < p.batch) list.b0 += 32, list.load(p);  // the rest of the starts
+  clear_spare<T>(p, list.starts.first, list.starts.last, kThreads);
+  if (!some) return;
+  const int seq = u.seq, len = u.len, row0 = u.row0, h = u.head;
+  const T* q = static_cast<const T*>(p.q.data) + (int64_t)(seq + row0) * p.q.row + h * p.q.head;
+  const T* k = static_cast<const T*>(p.k.data) + (int64_t)seq * p.k.row + h / p.group * p.k.head;
+  const T* v = static_cast<const T*>(p.v.data) + (int64_t)seq * p.v.row + h / p.group * p.v.head;
+  const int rows = min(ROWS, len - row0);
+  for (int i = tid; i < ROWS * (D4 / 4); i += kThreads) {
+    const int r = i / (D4 / 4), d = i % (D4 / 4) * 4;
+    float x[4] = {0.f, 0.f, 0.f, 0.f};
+    if (r < rows) load_row4(x, q + (int64_t)r * p.q.row, d, D, p.wide);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) sq[r * D4 + d + e] = x[e] * (p.scale * kLog2e);
+  }
+  float m[RT], l[RT], acc[DC][RT][4];
+#pragma unroll
+  for (int i = 0; i < RT; ++i) {
+    m[i] = -INFINITY, l[i] = 0.0f;
+#pragma unroll
+    for (int c = 0; c < DC; ++c)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[c][i][e] = 0.0f;
+  }
+  for (int t0 = 0; t0 < row0 + rows; t0 += kKeyTile) {
+    const int nk = min(kKeyTile, len - t0);
+    const bool cut = t0 + kKeyTile - 1 > row0;  // by the causal mask
+    __syncthreads();
+    for (int i = tid; i < kKeyTile * (D4 / 4); i += kThreads) {
+      const int r = i / (D4 / 4), d = i % (D4 / 4) * 4;
+      float x[4] = {0.f, 0.f, 0.f, 0.f}, y[4] = {0.f, 0.f, 0.f, 0.f};
+      if (r < nk) {
+        load_row4(x, k + (int64_t)(t0 + r) * p.k.row, d, D, p.wide);
+        load_row4(y, v + (int64_t)(t0 + r) * p.v.row, d, D, p.wide);
+      }
+      *reinterpret_cast<float4*>(sk + r * KS + d) = make_float4(x[0], x[1], x[2], x[3]);
+      *reinterpret_cast<float4*>(sv + r * D4 + d) = make_float4(y[0], y[1], y[2], y[3]);
+    }
+    __syncthreads();
+    float s[RT][4];
+#pragma unroll
+    for (int i = 0; i < RT; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) s[i][j] = 0.0f;
+#pragma unroll 2
+    for (int d = 0; d < D4; d += 4) {
+      float4 c[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) c[j] = *reinterpret_cast<const float4*>(sk + (tx + 16 * j) * KS + d);
+#pragma unroll
+      for (int i = 0; i < RT; ++i) {
+        const float4 a = *reinterpret_cast<const float4*>(sq + (RT * ty + i) * D4 + d);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          s[i][j] = fmaf(a.x, c[j].x, fmaf(a.y, c[j].y, fmaf(a.z, c[j].z, fmaf(a.w, c[j].w, s[i][j]))));
+      }
+    }
+    // the last key of this tile that row i sees
+    const int seen = row0 + RT * ty - t0;
+#pragma unroll
+    for (int i = 0; i < RT; ++i) {
+      if (cut)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (tx + 16 * j > seen + i) s[i][j] = -INFINITY;
+      float mx = fmaxf(fmaxf(s[i][0], s[i][1]), fmaxf(s[i][2], s[i][3]));
+#pragma unroll
+      for (int o = 8; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+      const float top = fmaxf(m[i], mx), base = top == -INFINITY ? 0.0f : top, f = exp2f(m[i] - base);
+      m[i] = top;
+      float sum = 0.0f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float e = exp2f(s[i][j] - base);
+        sum += e;
+        sp[(RT * ty + i) * PS + tx + 16 * j] = e;
+      }
+#pragma unroll
+      for (int o = 8; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      l[i] = fmaf(l[i], f, sum);
+#pragma unroll
+      for (int c = 0; c < DC; ++c)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[c][i][e] *= f;
+    }
+    __syncwarp();  // a row's weights are of one half warp
+    // four keys at a time; a value reaches the rows that see it only, whatever it holds
+    auto values = [&](auto masked) {
+#pragma unroll 1
+      for (int j0 = 0; j0 < kKeyTile; j0 += 4) {
+        float4 w[RT];
+#pragma unroll
+        for (int i = 0; i < RT; ++i) w[i] = *reinterpret_cast<const float4*>(sp + (RT * ty + i) * PS + j0);
+#pragma unroll
+        for (int c = 0; c < DC; ++c) {
+          const int d = 64 * c + 4 * tx;
+          if (d >= D4) continue;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float4 y = *reinterpret_cast<const float4*>(sv + (j0 + j) * D4 + d);
+#pragma unroll
+            for (int i = 0; i < RT; ++i) {
+              if (decltype(masked)::value && j0 + j > seen + i) continue;
+              const float x = j == 0 ? w[i].x : j == 1 ? w[i].y : j == 2 ? w[i].z : w[i].w;
+              acc[c][i][0] = fmaf(x, y.x, acc[c][i][0]);
+              acc[c][i][1] = fmaf(x, y.y, acc[c][i][1]);
+              acc[c][i][2] = fmaf(x, y.z, acc[c][i][2]);
+              acc[c][i][3] = fmaf(x, y.w, acc[c][i][3]);
+            }
+          }
+        }
+      }
+    };
+    if (cut)
+      values(std::true_type{});
+    else
+      values(std::false_type{});
+  }
+#pragma unroll
+  for (int i = 0; i < RT; ++i) {
+    const int r = RT * ty + i;
+    if (r >= rows) continue;
+    const float inv = l[i] != 0.0f ? 1.0f / l[i] : 0.0f;  // 0: no score is above -inf
+    T* o = static_cast<T*>(p.out.data) + (int64_t)(seq + row0 + r) * p.out.row + h * p.out.head;
+#pragma unroll
+    for (int c = 0; c < DC; ++c)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (64 * c + 4 * tx + e < D) o[64 * c + 4 * tx + e] = from_f32<T>(acc[c][i][e] * inv);
+    if (tx == 0)
+      p.lse[(int64_t)(seq + row0 + r) * p.q_heads + h] = l[i] != 0.0f ? kLn2 * (m[i] + log2f(l[i])) : -INFINITY;
+  }
+}
+
+constexpr size_t prompt_smem(int rows, int D4) {
+  return sizeof(float) * (rows * (D4 + kKeyTile + 4) + kKeyTile * (2 * D4 + 4));
+}
+
+template <typename T, int DC, int RT>
+void launch_prompt(const PromptParams& p, cudaStream_t st) {
+  constexpr int ROWS = 16 * RT;
+  auto* k = prompt_kernel<T, DC, RT>;
+  static_assert(prompt_smem(ROWS, 64 * DC) <= 232448, "shared memory of one block");
+  CKKS_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)prompt_smem(ROWS, 64 * DC)));
+  const unsigned grid = (unsigned)(std::max(1, p.batch + p.tokens / ROWS) * p.q_heads);
+  k<<<grid, kThreads, prompt_smem(ROWS, (p.head_dim + 3) & ~3), st>>>(p);
+  CKKS_CUDA(cudaGetLastError());
+}
+
+template <typename T>
+void run_prompt(const Context& c, const PromptParams& p, cudaStream_t st) {
+  switch ((p.head_dim + 63) / 64) {
+    case 1: launch_prompt<T, 1, 4>(p, st); break;
+    case 2:
+      // 128 rows, for fewer reads a multiply-add, where that leaves three units for each
+      // SM: four prompts of 2048, 8 heads of 128, 1218 us (1431 with 64 rows); two of
+      // 1500, 12 heads of 100, 545 (501).  Heads of 64 gain nothing: one of 4096, 16
+      // heads, 1281 (1193).
+      if ((long long)p.tokens / 128 * p.q_heads >= 3ll * c.sms)
+        launch_prompt<T, 2, 8>(p, st);
+      else
+        launch_prompt<T, 2, 4>(p, st);
+      break;
+    case 3: launch_prompt<T, 3, 4>(p, st); break;
+    default: launch_prompt<T, 4, 4>(p, st); break;
+  }
+}
+
+// ---- 16-bit types: tensor cores -------------------------------------------------
+// A unit is 256 rows of one query head of one sequence: two groups of four
+// softmax warps have 128 rows each (over 128 elements there is one group, as
+// tensor memory holds one S and O then), a thread a row.  Keys come in tiles of
+// 128, each copied once for both groups: S_g = Q_g K^T into tensor memory, the
+// weights back into S's place as the 16-bit A operand of O_g += P_g V.  One warp
+// issues copies, one the products; while one group exponentiates, the products
+// of the other run.  The first group has one tile less than the second, and
+// only a group's last tile is cut by the causal mask.
+//
+// CTAs are one to an SM and take the units of the list in turns, one round
+// upwards and the next one downwards: a sequence's units lie in the list from
+// the longest on, so every CTA gets about the same.
+//
+// A row's reference point m follows the maximum only when that has grown by
+// more than 2^8; O is seldom rescaled.  A weight is rounded once, to the
+// operands' type (half a step, as the result is), and summed in 32 bits before
+// that.  Two numbers a weight, as over a cache, would be half as many products
+// again, which bound this kernel where heads are wide; one number leaves a
+// result 1.4 times as far from the exact one as its own rounding takes it.
+//
+// The exponential unit takes 8 cycles for a warp's 32: 2048 cycles for a pair of
+// tiles, whose products take 1024 at 64 elements and 2048 at 128.  So some of
+// the exponentials are computed with multiply-adds: 2^x = 2^n 2^r, n the nearest
+// integer, and 2^r the polynomial of degree 4 with the least largest relative
+// error on [-1/2, 1/2] (2.7e-6, fitted to 2^r).
+constexpr int kHalf = 64;  // keys of a half tile
+
+template <int PANELS>
+struct PromptShape {
+  static constexpr int kGroups = PANELS <= 2 ? 2 : 1, kThreads = 32 * (5 * kGroups + 1), kUnitRows = kM * kGroups;
+  static constexpr int kSlots = PANELS == 1 ? 10 : PANELS == 2 ? 5 : PANELS == 3 ? 3 : 2;
+  static constexpr uint32_t kTileBytes = PANELS * kPanel;
+  // Q of each group, the ring of K and V tiles, barriers, masks, one word
+  static constexpr uint32_t kRing = kGroups * kTileBytes, kExtra = kRing + kSlots * kTileBytes;
+  static constexpr int kBars = 2 * kSlots + 20;
+  static constexpr size_t kSmem = kExtra + kBars * 8 + 6 * 4 * 4 + 16;
+  // of eight pairs of exponentials, how many the multiply-adds take
+  static constexpr int kPoly = PANELS <= 2 ? 2 : 0;
 };
 
 // 2^x for x >= -126; what lies below comes out next to 0
@@ -812,7 +819,7 @@ extern "C" int ckks_draft_prompt(ckks_ctx* ctx, const ckks_draft_prompt_args* ar
     need(a.kv_heads >= 1 && a.q_heads >= 1 && a.q_heads % a.kv_heads == 0,
          "query heads are not a multiple of the key/value heads");
     need(a.head_dim >= 1 && a.head_dim <= kMaxHeadDim, "head_dim outside 1..256");
-    need(((long long)a.batch + a.tokens / kRows) * a.q_heads < (1ll << 31) - 1, "sizes too large");
+    need(((long long)a.batch + a.tokens / 64) * a.q_heads < (1ll << 31) - 1, "sizes too large");
     need(std::isfinite((float)a.scale * kLog2e), "scale is not finite");
     if (a.tokens == 0) return;
     const int e = element_bytes(a.dtype);
@@ -840,10 +847,10 @@ extern "C" int ckks_draft_prompt(ckks_ctx* ctx, const ckks_draft_prompt_args* ar
         return;
     }
     if (a.dtype == CKKS_BF16)
-      run_prompt<__nv_bfloat16>(p, st);
+      run_prompt<__nv_bfloat16>(c, p, st);
     else if (a.dtype == CKKS_FP16)
-      run_prompt<__half>(p, st);
+      run_prompt<__half>(c, p, st);
     else
-      run_prompt<float>(p, st);
+      run_prompt<float>(c, p, st);
   });
 }
