@@ -10,11 +10,11 @@
 // (4 cycles a row and 128 keys of 128), and not with 128 rows whatever there are.
 //
 // One CTA per SM.  A thread copies tiles of 128 keys as they are (9/16 of a
-// byte an element); four warps decode K, a thread a key, into tensor memory as the first
-// product's A operand, four decode V into shared memory as the second's; one
-// warp issues the products; one or two groups of four warps, a thread a key,
-// turn scores into weights.  Every step has two buffers, so that each works on
-// another tile.
+// byte an element); four warps decode K, a thread a key, into tensor memory as
+// the first product's A operand, four decode V into shared memory as the
+// second's; a warp for each product issues it; a group of four warps for every
+// 16 rows, a thread a key, turns scores into weights.  Every step has two
+// buffers, so that each works on another tile.
 //
 // All operands are float16: it holds the caches' values exactly, and a
 // bfloat16 query, scaled by a power of two for each row, to 2^-24 of the
@@ -26,8 +26,20 @@
 // The lengths are known on the device only, so the CTAs divide the list of all
 // units' tiles evenly, a unit being (sequence, head, up to 64 rows).  Each
 // leaves (m, l, O) of its part of a unit in the workspace, and a second kernel,
-// a warp a row, joins them with the new keys of the row's ancestors, which it
+// a warp or eight a row, joins them with the new keys of the row's ancestors, which it
 // takes on the CUDA cores while the first kernel still runs.
+//
+// Measured: one node over four sequences of 65536 to 40960 keys, 32/8 heads of 128,
+// 88 us (245 MB, 2.8 TB/s, 43 % of the copy rate; 1326 on the CUDA cores); trees of 21
+// over 4001 keys, eight ragged sequences of 12 heads of 64, 28 us; trees of 16 over
+// 32768 and 24576 keys, 64 rows on each of 8 heads, 55 us.  A tile takes about 1670
+// cycles with 16 rows of 128, start and end included, where its bytes take 710:
+// decoding V (1100 of a warp's cycles), the softmax warps (1000) and
+// the two products (560, and their looks at barriers) are all near that, issue
+// slots are half used and so is shared memory.  Two sets of softmax warps
+// that take the tiles in turns, twice as many warps for V, K's warps decoding
+// some of V, and 8-byte reads of the rows all left it where it is or slower
+// (88 to 101 us); with 64 rows the softmax warps' chain bounds it (2700 cycles).
 #include <algorithm>
 #include <cmath>
 
@@ -49,9 +61,9 @@ struct Params4 {
   float* lse;
   float* part;  // [units + CTAs][N][DP + 4]
   int batch, kv_heads, group, head_dim, nodes, capacity;
-  int tiles_r, unit_cost, ctas, row_bytes;
+  int rows, tiles_r, unit_cost, ctas, row_bytes;  // rows of a unit, units of a (sequence, head), ...
   float scale;
-  bool bf16, wide;  // of the queries; new rows are whole, aligned 16-byte pieces
+  bool bf16;  // of the queries and the new rows
 };
 
 __device__ __forceinline__ int length_of(const Params4& p, int b) { return min(max(p.lens[b], 0), p.capacity); }
@@ -553,15 +565,17 @@ __global__ void __launch_bounds__(Shape4<PANELS, N>::kThreads, 1)
   }
 }
 
-// Joins the parts of a row over the cache and adds its new keys; a warp a row.
-// What does not wait for the first kernel comes first.
-template <typename T, int PANELS, int N>
+// Joins the parts of a row over the cache and adds its new keys; W warps a row,
+// which take the parts in turns.  What does not wait for the first kernel comes
+// first.
+template <typename T, int PANELS, int W>
 __global__ void __launch_bounds__(256) join4_kernel(const __grid_constant__ Params4 p) {
   constexpr int DP = 64 * PANELS;
   __shared__ uint64_t s_mask[8][kMaxNodes];
   __shared__ int s_jump[8][kMaxNodes];
-  const int rows = p.nodes * p.group, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int per = (rows + 7) / 8, bh = blockIdx.x / per, row = blockIdx.x % per * 8 + warp;
+  __shared__ float s_sum[W > 1 ? 8 : 1][W > 1 ? DP + 2 : 1];
+  const int rows = p.nodes * p.group, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, N = p.rows;
+  const int per = (rows * W + 7) / 8, bh = blockIdx.x / per, row = (blockIdx.x % per * 8 + warp) / W, turn = warp % W;
   const int b = bh / p.kv_heads, h = bh % p.kv_heads;
   if (row >= rows) {
     CKKS_PDL_ENTRY();
@@ -583,7 +597,7 @@ __global__ void __launch_bounds__(256) join4_kernel(const __grid_constant__ Para
     q[j] = mask && d < p.head_dim ? to_f32(q_row[d]) : 0.0f;
     acc[j] = 0.0f;
   }
-  for (uint64_t left = mask; left;) {
+  for (uint64_t left = turn == 0 ? mask : 0ull; left;) {
     // four keys at a time, so that their reads wait together
     int key[4];
     float s[4], v[4][2 * PANELS];
@@ -640,37 +654,57 @@ __global__ void __launch_bounds__(256) join4_kernel(const __grid_constant__ Para
   const int entries = entries_of(p, b);
   CKKS_PDL_ENTRY();  // what is read above no kernel of this call writes
   if (entries) {
-    const long long W = (long long)all * units, ctas = min((long long)p.ctas, W);
+    const long long list = (long long)all * units, ctas = min((long long)p.ctas, list);
     const long long u0 = (long long)before * units + (long long)unit * entries + p.unit_cost;
-    const int c0 = (int)((ctas * (u0 + 1) - 1) / W), c1 = (int)((ctas * (u0 + entries - p.unit_cost) - 1) / W);
+    const int c0 = (int)((ctas * (u0 + 1) - 1) / list), c1 = (int)((ctas * (u0 + entries - p.unit_cost) - 1) / list);
     const float* const part = p.part + ((int64_t)(b * units + unit) * N + row % N) * (DP + 4);
-    // the parts' sums are read eight at a time, so that a row seldom waits for memory twice
-    for (int c = c0; c <= c1; c += 8) {
-      float2 ml[8];
-      float y[8][2 * PANELS];
+    // Parts read at once, so that a row seldom waits for memory twice: with 8 warps 20,
+    // which is a turn of every SM's part (one node of 4/1 heads over 65536 keys 13.6 us, 15.7
+    // with 8, 16.7 with 4), as far as the registers go; with one 12 (trees of 16 over
+    // 32768 and 24576 keys 52.8, with 8 54.7).
+    constexpr int kAtOnce = W > 1 && PANELS < 4 ? 20 : 12;
+    for (int c = c0 + turn; c <= c1; c += kAtOnce * W) {
+      float2 ml[kAtOnce];
+      float y[kAtOnce][2 * PANELS];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const bool is = c + i <= c1;
-        const float* const o = part + (int64_t)(c + i) * (N * (DP + 4));
+      for (int i = 0; i < kAtOnce; ++i) {
+        const bool is = c + W * i <= c1;
+        const float* const o = part + (int64_t)(c + W * i) * (N * (DP + 4));
         ml[i] = is ? *reinterpret_cast<const float2*>(o + DP) : make_float2(-INFINITY, 0.0f);
 #pragma unroll
         for (int j = 0; j < 2 * PANELS; ++j) y[i][j] = is ? o[lane + 32 * j] : 0.0f;
       }
       float top = m;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) top = fmaxf(top, ml[i].x);
+      for (int i = 0; i < kAtOnce; ++i) top = fmaxf(top, ml[i].x);
       const float ref = top == -INFINITY ? 0.0f : top, f = exp2f(m - ref);
       m = top;
       l *= f;
 #pragma unroll
       for (int j = 0; j < 2 * PANELS; ++j) acc[j] *= f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
+      for (int i = 0; i < kAtOnce; ++i) {
         const float w = exp2f(ml[i].x - ref);
         l = fmaf(ml[i].y, w, l);
 #pragma unroll
         for (int j = 0; j < 2 * PANELS; ++j) acc[j] = fmaf(y[i][j], w, acc[j]);
       }
+    }
+  }
+  if constexpr (W > 1) {
+    static_assert(W == 8, "a CTA has one row");
+#pragma unroll
+    for (int j = 0; j < 2 * PANELS; ++j) s_sum[warp][lane + 32 * j] = acc[j];
+    if (lane == 0) s_sum[warp][DP] = m, s_sum[warp][DP + 1] = l;
+    __syncthreads();
+    if (warp) return;
+    for (int i = 1; i < W; ++i) {
+      const float o = s_sum[i][DP], top = fmaxf(m, o), ref = top == -INFINITY ? 0.0f : top;
+      const float f = exp2f(m - ref), w = exp2f(o - ref);
+      m = top;
+      l = fmaf(s_sum[i][DP + 1], w, l * f);
+#pragma unroll
+      for (int j = 0; j < 2 * PANELS; ++j) acc[j] = fmaf(s_sum[i][lane + 32 * j], w, acc[j] * f);
     }
   }
   const float inv = l != 0.0f ? 1.0f / l : 0.0f;
@@ -686,18 +720,42 @@ struct Plan4 {
   bool listed;  // the list has fewer than 2^31 entries
 };
 
+// What a unit's start costs in the list, in tiles: its query rows are scaled and
+// laid out and its sums left.  With 1, 3 and 6: trees of 21 over 4001 keys, eight ragged
+// sequences of 12 heads of 64, 40.5, 27.7 and 27.4 us; one node of 16/4 heads over
+// 16 sequences of up to 3000 keys 25.2, 19.4 and 19.2; one node over 65536 to 40960 keys,
+// four sequences of 32/8 heads of 128, 86.6, 85.2 and 85.8.
 constexpr int kUnitCost = 3;
 
 Plan4 plan4(const Context& c, const ckks_draft_attention_args& a) {
   const int rows = a.nodes * (a.q_heads / a.kv_heads);
   Plan4 d;
+  // The fewest of 16, 32 and 64 rows that hold a (sequence, head)'s, and 64 at a time beyond:
+  // one node over 65536 to 40960 keys (4 rows) takes 85 us with 16 rows, 99 with 32 and 143
+  // with 64; trees of 21 (21 rows) 27.7 with 32 and 35.4 with 64.
   d.rows = rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
   d.tiles_r = (rows + d.rows - 1) / d.rows;
   d.units = (long long)a.batch * a.kv_heads * d.tiles_r;
   const long long tiles = (a.capacity + kKeys - 1) / kKeys;
   d.listed = d.units * (tiles + kUnitCost) < (1ll << 31) - 1;
+  // Two tiles of the longest sequence a CTA, if there are SMs for it: chains of 5 over 1000 keys
+  // of 12 heads take 10.6 us, 12.4 with four and 10.0 with one; 8 nodes of 8/2 heads over
+  // 20000 keys 18.0, 15.0 and 18.0.
   d.ctas = (int)std::max(1ll, std::min<long long>(c.sms, d.units * std::max(1ll, tiles / 2)));
   return d;
+}
+
+template <typename T, int PANELS>
+void launch_join4(const ckks_draft_attention_args& a, const Params4& p, cudaStream_t st) {
+  const long long heads = (long long)a.batch * a.kv_heads, rows = (long long)a.nodes * p.group;
+  // Many parts a unit go to eight warps a row, few to one: 8 nodes of 8/2 heads over
+  // 20000 keys, 74 parts, take 18 us with eight and 29 with one, 16 nodes of 12 heads
+  // over 8000 keys, 12.3 parts, 16 and 18; trees of 16 over 32768 and 24576 keys,
+  // 9 parts and 512 rows, 62 and 55.
+  if (p.ctas > 12 * heads * p.tiles_r)
+    launch_pdl(join4_kernel<T, PANELS, 8>, dim3((unsigned)(heads * rows)), dim3(256), 0, st, p);
+  else
+    launch_pdl(join4_kernel<T, PANELS, 1>, dim3((unsigned)(heads * ((rows + 7) / 8))), dim3(256), 0, st, p);
 }
 
 template <int PANELS, int N>
@@ -708,11 +766,10 @@ void launch4(const Context& c, const ckks_draft_attention_args& a, const Params4
   CKKS_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::kSmem));
   k<<<p.ctas, S::kThreads, S::kSmem, st>>>(p, c.d_faults);
   CKKS_CUDA(cudaGetLastError());
-  const dim3 grid((unsigned)(a.batch * a.kv_heads * ((a.nodes * p.group + 7) / 8)));
   if (p.bf16)
-    launch_pdl(join4_kernel<__nv_bfloat16, PANELS, N>, grid, dim3(256), 0, st, p);
+    launch_join4<__nv_bfloat16, PANELS>(a, p, st);
   else
-    launch_pdl(join4_kernel<__half, PANELS, N>, grid, dim3(256), 0, st, p);
+    launch_join4<__half, PANELS>(a, p, st);
 }
 
 template <int PANELS>
@@ -746,7 +803,7 @@ bool attention4_tc(const Context& c, const ckks_draft_attention_args& a, cudaStr
   p.lens = a.lens, p.parents = a.parents, p.lse = a.lse, p.part = static_cast<float*>(a.workspace);
   p.batch = a.batch, p.kv_heads = a.kv_heads, p.group = a.q_heads / a.kv_heads, p.head_dim = a.head_dim;
   p.nodes = a.nodes, p.capacity = a.capacity, p.scale = (float)a.scale, p.bf16 = a.dtype == CKKS_BF16;
-  p.tiles_r = d.tiles_r, p.unit_cost = kUnitCost, p.ctas = d.ctas, p.row_bytes = R;
+  p.rows = d.rows, p.tiles_r = d.tiles_r, p.unit_cost = kUnitCost, p.ctas = d.ctas, p.row_bytes = R;
   switch (panels4(a.head_dim)) {
     case 1: launch4<1>(c, a, p, d.rows, st); break;
     case 2: launch4<2>(c, a, p, d.rows, st); break;

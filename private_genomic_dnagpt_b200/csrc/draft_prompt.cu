@@ -308,29 +308,45 @@ void run_prompt(const Context& c, const PromptParams& p, cudaStream_t st) {
 // ---- 16-bit types: tensor cores -------------------------------------------------
 // A unit is 256 rows of one query head of one sequence: two groups of four
 // softmax warps have 128 rows each (over 128 elements there is one group, as
-// tensor memory holds one S and O then), a thread a row.  Keys come in tiles of
-// 128, each copied once for both groups: S_g = Q_g K^T into tensor memory, the
-// weights back into S's place as the 16-bit A operand of O_g += P_g V.  One warp
-// issues copies, one the products; while one group exponentiates, the products
-// of the other run.  The first group has one tile less than the second, and
-// only a group's last tile is cut by the causal mask.
+// tensor memory holds one O then), a thread a row.  Keys come in tiles of 128,
+// each copied once for both groups, and are worked on by halves: a group has two
+// places of 64 scores in tensor memory, S = Q K^T into one while its warps turn
+// the other into weights, which take their scores' place as the 16-bit A operand
+// of O += P V.  One warp issues copies, one for each group its products.  The
+// first group has one tile less than the second, and only a group's last tile
+// is cut by the causal mask.  (One place of 128 scores a group waited for its
+// products in turn with them, and one warp for both groups' products took 200
+// cycles at each barrier: 623 us for the first case below, where this takes 502.)
 //
 // CTAs are one to an SM and take the units of the list in turns, one round
-// upwards and the next one downwards: a sequence's units lie in the list from
-// the longest on, so every CTA gets about the same.
+// upwards and the next one downwards.  The longest units of 32 sequences come
+// first, so every CTA gets about the same (prompts up to 2001: 52 tiles at most
+// where 49 is the mean, 73 with one sequence behind the other).
 //
 // A row's reference point m follows the maximum only when that has grown by
 // more than 2^8; O is seldom rescaled.  A weight is rounded once, to the
 // operands' type (half a step, as the result is), and summed in 32 bits before
 // that.  Two numbers a weight, as over a cache, would be half as many products
-// again, which bound this kernel where heads are wide; one number leaves a
-// result 1.4 times as far from the exact one as its own rounding takes it.
+// again; one number leaves a bfloat16 result 1.3 times as far from the exact one
+// as its own rounding takes it (2.1e-3 of it against 1.6e-3).
 //
 // The exponential unit takes 8 cycles for a warp's 32: 2048 cycles for a pair of
-// tiles, whose products take 1024 at 64 elements and 2048 at 128.  So some of
-// the exponentials are computed with multiply-adds: 2^x = 2^n 2^r, n the nearest
-// integer, and 2^r the polynomial of degree 4 with the least largest relative
-// error on [-1/2, 1/2] (2.7e-6, fitted to 2^r).
+// tiles, whose products take 1024 at 64 elements and 2048 at 128.  So two in
+// eight of the exponentials are computed with multiply-adds: 2^x = 2^n 2^r, n
+// the nearest integer, and 2^r the polynomial of degree 4 with the least largest
+// relative error on [-1/2, 1/2] (2.7e-6, fitted to 2^r).  None, one, two, three, four
+// in eight: 553, 546, 542, 566, 580 us for the first case, 525, 495, 484, 501, 530 for
+// heads of 64.
+//
+// Measured: 8192 tokens, 32/8 heads of 128, bfloat16, 502 us (1.10 PFLOP/s, 65 % of
+// a library product; 581 us and 0.95 under sustained load and the power limit);
+// twelve prompts up to 2001, 12 heads of 64, float16, 107 us.  Half a tile takes a
+// softmax warp some 1600 cycles: 240 at the barrier of its scores, 300 for their
+// maximum, 1000 for the weights (two warps share an exponential unit), and no
+// stage of this chain is much shorter than the others: without exponentials,
+// maxima, most products or most copies heads of 64 still take 85 % of the time.
+// 103 tokens of 12 heads take 9 us: set-up, copies, two products and the write,
+// one behind the other.
 constexpr int kHalf = 64;  // keys of a half tile
 
 template <int PANELS>

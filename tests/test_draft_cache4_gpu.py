@@ -368,3 +368,81 @@ def test_one_row_of_each_size(cc):
     k = torch.zeros(3, 2, 64, device="cuda")
     assert cc.draft_fill4(none, none.clone(), i32([0, 0]), k[:0], k[:0], i32([0, 0, 0])).tolist() == [0, 0]
     cc.Synchronize()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("n,D", [(1, 64), (9, 128), (40, 256)])
+def test_attention4_of_queries_of_any_size(cc, dtype, n, D):
+    """Queries times 2^60 or 2^-60, with the scale that takes it back, give the
+    same bits; rows of a tree may differ in size."""
+    x = base.inputs(dtype, 2, n, 4, 2, D, 500, [500, 129], [tree(n, 2)] * 2, seed=30)
+    y, z = quantised(x)
+    want = cc.draft_attention4(**y)
+    for power in (2.0 ** 60, 2.0 ** -60):
+        got = cc.draft_attention4(**(y | {"q": y["q"] * power}), scale=D ** -0.5 / power)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    sizes = torch.tensor([10.0 ** (i % 5 - 3) for i in range(n)], device="cuda")[:, None, None]
+    q = (y["q"].float() * sizes).to(dtype)
+    check_attention(z | {"q": q}, *cc.draft_attention4(**(y | {"q": q})))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_attention4_from_two_threads(cc, dtype):
+    """Calls of other sizes at the same time from two host threads."""
+    import threading
+    xs = [quantised(base.inputs(dtype, 1, n, 4, 4, D, 700, [650], [tree(n, 2)], seed=31))[0] for n, D in ((1, 64), (20, 128))]
+    want = [cc.draft_attention4(**x) for x in xs]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def calls(x, w):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(50):
+                got = cc.draft_attention4(**x)
+                torch.cuda.current_stream().synchronize()
+                if not (torch.equal(got[0], w[0]) and torch.equal(got[1], w[1])):
+                    wrong.append(1)
+
+    threads = [threading.Thread(target=calls, args=a) for a in zip(xs, want)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+    cc.Synchronize()
+
+
+def test_captured_run_of_prompt_fill_and_trees(cc):
+    """A whole run captured into one graph and replayed over other inputs:
+    prompt, its rows into 4 bits, a tree over them, its commit, a second tree."""
+    g = torch.Generator(device="cuda").manual_seed(32)
+    normal = lambda *s: torch.randn(*s, generator=g, device="cuda").to(torch.bfloat16)  # noqa: E731
+    H, D, T, n = 4, 64, 300, 6
+    q, k, v = normal(T, H, D), normal(T, H, D), normal(T, H, D)
+    qt, kt, vt = normal(2, n, H, D), normal(2, n, H, D), normal(2, n, H, D)
+    starts, parents, path, count = i32([0, 120, 300]), i32([tree(n, 2)] * 2), i32([[0, 2, -1, -1, -1, -1]] * 2), i32([2, 1])
+
+    def run():
+        caches = [torch.zeros(2, H, 256, drafting.row4_bytes(D), dtype=torch.uint8, device="cuda") for _ in range(2)]
+        out, lse = cc.draft_prompt(q, k, v, starts)
+        lens = cc.draft_fill4(*caches, i32([0, 0]) if not torch.cuda.is_current_stream_capturing() else zero, k, v, starts)
+        tree_out, _ = cc.draft_attention4(qt, *caches, lens, kt, vt, parents)
+        lens = cc.draft_commit4(*caches, lens, kt, vt, path, count)
+        again, _ = cc.draft_attention4(qt, *caches, lens, kt, vt, parents)
+        return out, lse, tree_out, again, lens, cc.draft_read4(caches[0], lens, D, torch.bfloat16)
+
+    zero = i32([0, 0])
+    run()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = run()
+    for t in (q, k, v, qt, kt, vt):
+        t.copy_(normal(*t.shape))
+    starts.copy_(i32([0, 200, 290]))
+    graph.replay()
+    torch.cuda.synchronize()
+    for a, b in zip(got, run()):
+        assert torch.equal(a, b)
+    assert got[4].tolist() == [202, 91]
+    cc.Synchronize()
