@@ -10,6 +10,7 @@
 // written: they stay on the chip, and arithmetic bounds all but short prompts.
 #include <algorithm>
 #include <cmath>
+#include <limits>
 
 #include "draft_tc.cuh"
 
@@ -793,8 +794,9 @@ void launch_prompt_tc(const Context& c, const PromptParams& p, const PromptMaps&
   static_assert(S::kSmem <= 232448, "shared memory of one block");
   auto* k = prompt_tc_kernel<T, PANELS>;
   CKKS_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::kSmem));
-  // a scale of 0 becomes one that changes no weight: a masked score times 0 would be no number
-  const float factor = std::max(std::fabs(p.scale) * kLog2e, 1e-30f);
+  // a scale of 0 becomes the least there is: a masked score times 0 would be no
+  // number, and no finite score times 2^-149 reaches 2^-21
+  const float factor = std::max(std::fabs(p.scale) * kLog2e, std::numeric_limits<float>::denorm_min());
   const long long units = (long long)std::max(1, p.batch + p.tokens / S::kUnitRows) * p.q_heads;
   k<<<(unsigned)std::min<long long>(units, c.sms), S::kThreads, S::kSmem, st>>>(p, maps, p.scale < 0.0f, factor,
                                                                                c.d_faults);

@@ -145,8 +145,9 @@ def row4_bytes(head_dim):
     magnitude, to three bits of mantissa), then zeros up to a multiple of four
     bytes.  A 4-bit cache is a uint8 tensor [B, Hkv, capacity, row4_bytes(D)]
     whose rows start on 4-byte boundaries (``attention4`` is fastest where a
-    head's rows lie one behind the other); zeros are an empty one.  Magnitudes over 61440 become 61440, and a group
-    with an infinity or a NaN in it reads as NaN."""
+    head's rows lie one behind the other); zeros are an empty one.  Magnitudes
+    over 61440 become 61440, and a group with an infinity or a NaN in it reads
+    as NaN."""
     return (_binding or _native()).row4_bytes(head_dim)
 
 

@@ -109,6 +109,17 @@ def test_sharp_rows_and_scales(cc, dtype, D):
         check(x, *cc.draft_prompt(**x, scale=scale), scale=scale)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("scale", [0.0, 2.0 ** -112])
+def test_scales_that_undo_large_scores(cc, dtype, scale):
+    """Scores around 2^115: with a scale of 0 every key weighs the same."""
+    starts = packed([200, 70])
+    x = inputs(dtype, starts[-1], 4, 2, 64, starts, seed=3)
+    x["q"] = x["q"] * 2.0 ** 56
+    x["k"] = x["k"] * 2.0 ** 56
+    check(x, *cc.draft_prompt(**x, scale=scale), scale=scale)
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("rising", [True, False])
 def test_rows_of_rising_scores(cc, dtype, rising):
