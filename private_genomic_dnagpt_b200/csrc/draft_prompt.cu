@@ -119,13 +119,16 @@ __device__ __forceinline__ void clear_spare(const PromptParams& p, int first, in
 // A CTA of 16 x 16 threads takes 16 RT rows of one query head, the longest
 // first, over tiles of 64 keys staged in shared memory as floats.  Scores: a
 // thread has RT rows x 4 keys; values: RT rows x 4 elements of every 64.  A row's
-// 16 threads are half a warp, so its maximum and sum are shuffles.  Reads from
-// shared memory bound it (8 of 16 bytes for 64 multiply-adds, 12 for 128 with RT
-// 8): 29 TFLOP/s for one prompt of 4096 and 16 heads of 64 in float32.
+// 16 threads are half a warp, so its maximum and sum are shuffles.  Issue slots
+// and reads from shared memory bound it (8 of 16 bytes for 64 multiply-adds, 12
+// for 128 with RT 8): 31 TFLOP/s for one prompt of 4096 and 16 heads of 64 in
+// float32, 34 for four of 2048 and 8 of 128.  Two CTAs an SM are worth more than
+// the few registers that then go to memory (up to 1030 four prompts of 12 heads of 64:
+// 186 us, with one CTA 225); multiply-adds in pairs took 243.
 constexpr int kKeyTile = 64, kThreads = 256;
 
 template <typename T, int DC, int RT>
-__global__ void __launch_bounds__(kThreads) prompt_kernel(PromptParams p) {
+__global__ void __launch_bounds__(kThreads, DC <= 2 && RT == 4 ? 2 : 1) prompt_kernel(PromptParams p) {
   constexpr int ROWS = 16 * RT, PS = kKeyTile + 4;
   extern __shared__ __align__(16) float sm[];
   const int D = p.head_dim, D4 = (D + 3) & ~3, KS = D4 + 4;
@@ -166,15 +169,27 @@ __global__ void __launch_bounds__(kThreads) prompt_kernel(PromptParams p) {
     const int nk = min(kKeyTile, len - t0);
     const bool cut = t0 + kKeyTile - 1 > row0;  // by the causal mask
     __syncthreads();
-    for (int i = tid; i < kKeyTile * (D4 / 4); i += kThreads) {
-      const int r = i / (D4 / 4), d = i % (D4 / 4) * 4;
-      float x[4] = {0.f, 0.f, 0.f, 0.f}, y[4] = {0.f, 0.f, 0.f, 0.f};
-      if (r < nk) {
-        load_row4(x, k + (int64_t)(t0 + r) * p.k.row, d, D, p.wide);
-        load_row4(y, v + (int64_t)(t0 + r) * p.v.row, d, D, p.wide);
+#pragma unroll
+    for (int c = 0; c < DC; ++c) {
+      const int d = 64 * c + 4 * tx;
+      if (d >= D4) continue;
+      float x[4][4], y[4][4];  // all reads before the first write
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int r = ty + 16 * j;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[j][e] = y[j][e] = 0.0f;
+        if (r < nk) {
+          load_row4(x[j], k + (int64_t)(t0 + r) * p.k.row, d, D, p.wide);
+          load_row4(y[j], v + (int64_t)(t0 + r) * p.v.row, d, D, p.wide);
+        }
       }
-      *reinterpret_cast<float4*>(sk + r * KS + d) = make_float4(x[0], x[1], x[2], x[3]);
-      *reinterpret_cast<float4*>(sv + r * D4 + d) = make_float4(y[0], y[1], y[2], y[3]);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int r = ty + 16 * j;
+        *reinterpret_cast<float4*>(sk + r * KS + d) = make_float4(x[j][0], x[j][1], x[j][2], x[j][3]);
+        *reinterpret_cast<float4*>(sv + r * D4 + d) = make_float4(y[j][0], y[j][1], y[j][2], y[j][3]);
+      }
     }
     __syncthreads();
     float s[RT][4];
@@ -197,6 +212,8 @@ __global__ void __launch_bounds__(kThreads) prompt_kernel(PromptParams p) {
     }
     // the last key of this tile that row i sees
     const int seen = row0 + RT * ty - t0;
+    float f[RT];  // what the sums so far are scaled by
+    bool moved = false;
 #pragma unroll
     for (int i = 0; i < RT; ++i) {
       if (cut)
@@ -206,22 +223,28 @@ __global__ void __launch_bounds__(kThreads) prompt_kernel(PromptParams p) {
       float mx = fmaxf(fmaxf(s[i][0], s[i][1]), fmaxf(s[i][2], s[i][3]));
 #pragma unroll
       for (int o = 8; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-      const float top = fmaxf(m[i], mx), base = top == -INFINITY ? 0.0f : top, f = exp2f(m[i] - base);
+      const float top = fmaxf(m[i], mx), base = top == -INFINITY ? 0.0f : top;
+      f[i] = ex2(m[i] - base);
+      moved |= f[i] != 1.0f;
       m[i] = top;
       float sum = 0.0f;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const float e = exp2f(s[i][j] - base);
+        const float e = ex2(s[i][j] - base);
         sum += e;
         sp[(RT * ty + i) * PS + tx + 16 * j] = e;
       }
 #pragma unroll
       for (int o = 8; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      l[i] = fmaf(l[i], f, sum);
+      l[i] = fmaf(l[i], f[i], sum);
+    }
+    if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
-      for (int c = 0; c < DC; ++c)
+      for (int i = 0; i < RT; ++i)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) acc[c][i][e] *= f;
+        for (int c = 0; c < DC; ++c)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[c][i][e] *= f[i];
     }
     __syncwarp();  // a row's weights are of one half warp
     // four keys at a time; a value reaches the rows that see it only, whatever it holds
@@ -292,11 +315,12 @@ void run_prompt(const Context& c, const PromptParams& p, cudaStream_t st) {
   switch ((p.head_dim + 63) / 64) {
     case 1: launch_prompt<T, 1, 4>(p, st); break;
     case 2:
-      // 128 rows, for fewer reads a multiply-add, where that leaves three units for each
-      // SM: four prompts of 2048, 8 heads of 128, 1218 us (1431 with 64 rows); two of
-      // 1500, 12 heads of 100, 545 (501).  Heads of 64 gain nothing: one of 4096, 16
-      // heads, 1281 (1193).
-      if ((long long)p.tokens / 128 * p.q_heads >= 3ll * c.sms)
+      // 128 rows, for fewer reads a multiply-add, where that leaves three units for two
+      // SMs: one prompt of 8192, 4 heads of 128, 2096 us (2424 with 64 rows); two of
+      // 1500, 12 heads of 100, 455 (489); but one of 3000, 8 heads of 128, 774 (709).
+      // Heads of 64 gain little and lose on shorter prompts: one of 4096, 16 heads, 1080
+      // (1116), up to 1030 four of 12, 273 (186).
+      if ((long long)p.tokens / 128 * p.q_heads >= 3ll * c.sms / 2)
         launch_prompt<T, 2, 8>(p, st);
       else
         launch_prompt<T, 2, 4>(p, st);
