@@ -250,7 +250,7 @@ __global__ void __launch_bounds__(kThreads, DC <= 2 && RT == 4 ? 2 : 1) prompt_k
     // four keys at a time; a value reaches the rows that see it only, whatever it holds
     auto values = [&](auto masked) {
 #pragma unroll 1
-      for (int j0 = 0; j0 < kKeyTile; j0 += 4) {
+      for (int j0 = 0; j0 < (decltype(masked)::value ? min(kKeyTile, seen + RT) : kKeyTile); j0 += 4) {
         float4 w[RT];
 #pragma unroll
         for (int i = 0; i < RT; ++i) w[i] = *reinterpret_cast<const float4*>(sp + (RT * ty + i) * PS + j0);
