@@ -122,21 +122,26 @@ __device__ __forceinline__ void clear_spare(const PromptParams& p, int first, in
 // 16 threads are half a warp, so its maximum and sum are shuffles.  Issue slots
 // and reads from shared memory bound it (8 of 16 bytes for 64 multiply-adds, 12
 // for 128 with RT 8): 31 TFLOP/s for one prompt of 4096 and 16 heads of 64 in
-// float32, 34 for four of 2048 and 8 of 128.  Two CTAs an SM are worth more than
+// float32, 35 for four of 2048 and 8 of 128.  Two CTAs an SM are worth more than
 // the few registers that then go to memory (up to 1030 four prompts of 12 heads of 64:
-// 186 us, with one CTA 225); multiply-adds in pairs took 243.
+// 183 us, with one CTA 225); multiply-adds in pairs took 243.
 constexpr int kKeyTile = 64, kThreads = 256;
 
 template <typename T, int DC, int RT>
 __global__ void __launch_bounds__(kThreads, DC <= 2 && RT == 4 ? 2 : 1) prompt_kernel(PromptParams p) {
   constexpr int ROWS = 16 * RT, PS = kKeyTile + 4;
   extern __shared__ __align__(16) float sm[];
-  const int D = p.head_dim, D4 = (D + 3) & ~3, KS = D4 + 4;
-  float* sq = sm;                     // [ROWS][D4]
-  float* sk = sq + ROWS * D4;         // [kKeyTile][KS]
+  const int D = p.head_dim, D4 = (D + 3) & ~3, KS = D4 + 4, QS = DC == 1 ? D4 : KS;
+  float* sq = sm;                     // [ROWS][QS]
+  float* sk = sq + ROWS * QS;         // [kKeyTile][KS]
   float* sv = sk + kKeyTile * KS;     // [kKeyTile][D4]
   float* sp = sv + kKeyTile * D4;     // [ROWS][PS]
   const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
+  // A thread has rows 4 ty to 4 ty + 3 of every 64: with rows of K's pitch the two that
+  // a warp reads at once lie 16 banks apart (one prompt of 8192, 4 heads of 128, 2051 us,
+  // 2086 without either; heads of 64 are faster without the pitch, 183 us for 189 in the
+  // case below, as reads are not what they wait for)
+  auto after = [](int i) { return i % 4 + i / 4 * 64; };
   Units<ROWS> list;
   list.begin(p);
   Unit u;
@@ -154,7 +159,7 @@ __global__ void __launch_bounds__(kThreads, DC <= 2 && RT == 4 ? 2 : 1) prompt_k
     float x[4] = {0.f, 0.f, 0.f, 0.f};
     if (r < rows) load_row4(x, q + (int64_t)r * p.q.row, d, D, p.wide);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) sq[r * D4 + d + e] = x[e] * (p.scale * kLog2e);
+    for (int e = 0; e < 4; ++e) sq[r * QS + d + e] = x[e] * (p.scale * kLog2e);
   }
   float m[RT], l[RT], acc[DC][RT][4];
 #pragma unroll
@@ -204,14 +209,14 @@ __global__ void __launch_bounds__(kThreads, DC <= 2 && RT == 4 ? 2 : 1) prompt_k
       for (int j = 0; j < 4; ++j) c[j] = *reinterpret_cast<const float4*>(sk + (tx + 16 * j) * KS + d);
 #pragma unroll
       for (int i = 0; i < RT; ++i) {
-        const float4 a = *reinterpret_cast<const float4*>(sq + (RT * ty + i) * D4 + d);
+        const float4 a = *reinterpret_cast<const float4*>(sq + (4 * ty + after(i)) * QS + d);
 #pragma unroll
         for (int j = 0; j < 4; ++j)
           s[i][j] = fmaf(a.x, c[j].x, fmaf(a.y, c[j].y, fmaf(a.z, c[j].z, fmaf(a.w, c[j].w, s[i][j]))));
       }
     }
-    // the last key of this tile that row i sees
-    const int seen = row0 + RT * ty - t0;
+    // the last key of this tile that the thread's first row sees
+    const int seen = row0 + 4 * ty - t0;
     float f[RT];  // what the sums so far are scaled by
     bool moved = false;
 #pragma unroll
@@ -219,7 +224,7 @@ __global__ void __launch_bounds__(kThreads, DC <= 2 && RT == 4 ? 2 : 1) prompt_k
       if (cut)
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          if (tx + 16 * j > seen + i) s[i][j] = -INFINITY;
+          if (tx + 16 * j > seen + after(i)) s[i][j] = -INFINITY;
       float mx = fmaxf(fmaxf(s[i][0], s[i][1]), fmaxf(s[i][2], s[i][3]));
 #pragma unroll
       for (int o = 8; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
@@ -232,7 +237,7 @@ __global__ void __launch_bounds__(kThreads, DC <= 2 && RT == 4 ? 2 : 1) prompt_k
       for (int j = 0; j < 4; ++j) {
         const float e = ex2(s[i][j] - base);
         sum += e;
-        sp[(RT * ty + i) * PS + tx + 16 * j] = e;
+        sp[(4 * ty + after(i)) * PS + tx + 16 * j] = e;
       }
 #pragma unroll
       for (int o = 8; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
@@ -250,10 +255,10 @@ __global__ void __launch_bounds__(kThreads, DC <= 2 && RT == 4 ? 2 : 1) prompt_k
     // four keys at a time; a value reaches the rows that see it only, whatever it holds
     auto values = [&](auto masked) {
 #pragma unroll 1
-      for (int j0 = 0; j0 < (decltype(masked)::value ? min(kKeyTile, seen + RT) : kKeyTile); j0 += 4) {
+      for (int j0 = 0; j0 < (decltype(masked)::value ? min(kKeyTile, seen + after(RT - 1) + 1) : kKeyTile); j0 += 4) {
         float4 w[RT];
 #pragma unroll
-        for (int i = 0; i < RT; ++i) w[i] = *reinterpret_cast<const float4*>(sp + (RT * ty + i) * PS + j0);
+        for (int i = 0; i < RT; ++i) w[i] = *reinterpret_cast<const float4*>(sp + (4 * ty + after(i)) * PS + j0);
 #pragma unroll
         for (int c = 0; c < DC; ++c) {
           const int d = 64 * c + 4 * tx;
@@ -263,7 +268,7 @@ __global__ void __launch_bounds__(kThreads, DC <= 2 && RT == 4 ? 2 : 1) prompt_k
             const float4 y = *reinterpret_cast<const float4*>(sv + (j0 + j) * D4 + d);
 #pragma unroll
             for (int i = 0; i < RT; ++i) {
-              if (decltype(masked)::value && j0 + j > seen + i) continue;
+              if (decltype(masked)::value && j0 + j > seen + after(i)) continue;
               const float x = j == 0 ? w[i].x : j == 1 ? w[i].y : j == 2 ? w[i].z : w[i].w;
               acc[c][i][0] = fmaf(x, y.x, acc[c][i][0]);
               acc[c][i][1] = fmaf(x, y.y, acc[c][i][1]);
@@ -281,7 +286,7 @@ __global__ void __launch_bounds__(kThreads, DC <= 2 && RT == 4 ? 2 : 1) prompt_k
   }
 #pragma unroll
   for (int i = 0; i < RT; ++i) {
-    const int r = RT * ty + i;
+    const int r = 4 * ty + after(i);
     if (r >= rows) continue;
     const float inv = l[i] != 0.0f ? 1.0f / l[i] : 0.0f;  // 0: no score is above -inf
     T* o = static_cast<T*>(p.out.data) + (int64_t)(seq + row0 + r) * p.out.row + h * p.out.head;
@@ -296,7 +301,7 @@ __global__ void __launch_bounds__(kThreads, DC <= 2 && RT == 4 ? 2 : 1) prompt_k
 }
 
 constexpr size_t prompt_smem(int rows, int D4) {
-  return sizeof(float) * (rows * (D4 + kKeyTile + 4) + kKeyTile * (2 * D4 + 4));
+  return sizeof(float) * (rows * (D4 + kKeyTile + 8) + kKeyTile * (2 * D4 + 4));
 }
 
 template <typename T, int DC, int RT>
