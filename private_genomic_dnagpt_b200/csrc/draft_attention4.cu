@@ -16,9 +16,11 @@
 // 16 rows, a thread a key, turns scores into weights.  Every step has two
 // buffers, so that each works on another tile.
 //
-// All operands are float16: it holds the caches' values exactly, and a
-// bfloat16 query, scaled by a power of two for each row, to 2^-24 of the
-// row's largest element, which is what a 32-bit sum of products keeps.  A weight
+// The first product's operands have the queries' type, the second's are
+// float16: either type holds the caches' values exactly, so every product of
+// a query's element and a key's is exact, however far apart the elements of a
+// row lie (a group of small keys may meet the large ones: rounding a bfloat16
+// row to float16 would lose its small elements).  A weight
 // has float16's 11 bits.  A row's reference point m lies 2^7 below the maximum
 // when it is set, and is set anew where a score passes it by more than 2^8 more: weights
 // end at 2^15.  Sums are in 32 bits.
@@ -30,16 +32,16 @@
 // takes on the CUDA cores while the first kernel still runs.
 //
 // Measured: one node over four sequences of 65536 to 40960 keys, 32/8 heads of 128,
-// 88 us (245 MB, 2.8 TB/s, 43 % of the copy rate; 1326 on the CUDA cores); trees of 21
-// over 4001 keys, eight ragged sequences of 12 heads of 64, 28 us; trees of 16 over
-// 32768 and 24576 keys, 64 rows on each of 8 heads, 55 us.  A tile takes about 1670
-// cycles with 16 rows of 128, start and end included, where its bytes take 710:
-// decoding V (1100 of a warp's cycles), the softmax warps (1000) and
-// the two products (560, and their looks at barriers) are all near that, issue
-// slots are half used and so is shared memory.  Two sets of softmax warps
-// that take the tiles in turns, twice as many warps for V, K's warps decoding
-// some of V, and 8-byte reads of the rows all left it where it is or slower
-// (88 to 101 us); with 64 rows the softmax warps' chain bounds it (2700 cycles).
+// bfloat16, 93 us (245 MB, 2.6 TB/s, 40 % of the copy rate; in a replayed graph 91, with
+// float16 queries 84; 1326 on the CUDA cores); trees of 21 over 4001 keys, eight ragged
+// sequences of 12 heads of 64, 29 us; trees of 16 over 32768 and 24576 keys, 64 rows on each
+// of 8 heads, 53 us.  A tile takes about 1670 cycles with 16 rows of 128 and float16 queries,
+// start and end included, where its bytes take 710: decoding V (1100 of a warp's cycles), the
+// softmax warps (1000) and the two products (560, and their looks at barriers) are all near
+// that, issue slots are half used and so is shared memory.  K in bfloat16 goes through floats
+// and takes 8 % more.  Two sets of softmax warps that take the tiles in turns, twice as many
+// warps for V, K's warps decoding some of V, and 8-byte reads of the rows all left 85 us
+// where they were or at 88 to 101; with 64 rows the softmax warps' chain bounds it (2700 cycles).
 #include <algorithm>
 #include <cmath>
 
@@ -63,7 +65,6 @@ struct Params4 {
   int batch, kv_heads, group, head_dim, nodes, capacity;
   int rows, tiles_r, unit_cost, ctas, row_bytes;  // rows of a unit, units of a (sequence, head), ...
   float scale;
-  bool bf16;  // of the queries and the new rows
 };
 
 __device__ __forceinline__ int length_of(const Params4& p, int b) { return min(max(p.lens[b], 0), p.capacity); }
@@ -158,11 +159,13 @@ __device__ __forceinline__ int ordered(float x) {
 }
 __device__ __forceinline__ float unordered(int i) { return __int_as_float(i ^ (i >> 31 & 0x7FFFFFFF)); }
 
-template <int PANELS, int N>
+// T: of the queries
+template <typename T, int PANELS, int N>
 __global__ void __launch_bounds__(Shape4<PANELS, N>::kThreads, 1)
     attend4_kernel(const __grid_constant__ Params4 p, unsigned int* __restrict__ faults) {
   using S = Shape4<PANELS, N>;
   constexpr int DP = S::DP, NS = S::kSlots, GR = S::kGroups, C = S::kCols, VB = S::kValueBufs;
+  constexpr bool kBf = std::is_same_v<T, __nv_bfloat16>;
   constexpr int kWarpK = 4 * GR, kWarpV = kWarpK + 4, kWarpCopy = kWarpV + 4, kWarpQk = kWarpCopy + 1, kWarpPv = kWarpQk + 1;
   extern __shared__ __align__(1024) uint8_t smem[];
   float2* const s_row = reinterpret_cast<float2*>(smem + S::kAtRows);      // [2][N] factor and reference point
@@ -282,13 +285,19 @@ __global__ void __launch_bounds__(Shape4<PANELS, N>::kThreads, 1)
         const int buf = i & 1;
         if (!value) {
           tmem_fence_after();
+          // 16 columns a store, and the next words read ahead of it (one node over 65536
+          // bfloat16 keys 91 us, with 32 columns 94)
+          Quad y = read(0);
 #pragma unroll
           for (int g = 0; g < 4 * PANELS; g += 4) {
-            const Quad y = read(g);
-            uint32_t w[32];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) decode4_word(y.code[j], scale4_pair(y.scale, j / 2), w + 4 * j);
-            tmem_store<32>(tmem + lanes + buf * (DP / 2) + 8 * g, w);
+            for (int i0 = 0; i0 < 8; i0 += 4) {
+              uint32_t w[16];
+#pragma unroll
+              for (int j = 0; j < 4; ++j) decode4_word<T>(y.code[i0 + j], scale4_pair(y.scale, (i0 + j) / 2), w + 4 * j);
+              if (i0 && g + 4 < 4 * PANELS) y = read(g + 4);
+              tmem_store<16>(tmem + lanes + buf * (DP / 2) + 8 * g + 4 * i0, w);
+            }
           }
           tmem_wait_store();
           tmem_fence_before();
@@ -308,7 +317,7 @@ __global__ void __launch_bounds__(Shape4<PANELS, N>::kThreads, 1)
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
               uint32_t w[4];
-              decode4_word(y.code[j], scale4_pair(y.scale, j / 2), w);
+              decode4_word<__half>(y.code[j], scale4_pair(y.scale, j / 2), w);
               *reinterpret_cast<uint4*>(panel + ((j ^ (key & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
             }
           }
@@ -324,7 +333,7 @@ __global__ void __launch_bounds__(Shape4<PANELS, N>::kThreads, 1)
     }
   } else if (warp == kWarpQk) {
     // ---- the scores' products, by the whole warp in step
-    constexpr uint32_t word = mma_word(false, kM, N, false);
+    constexpr uint32_t word = mma_word(kBf, kM, N, false);
     const uint32_t t_base = __shfl_sync(0xffffffffu, tmem, 0);
     int i = 0;
     uint32_t units = 0;
@@ -374,7 +383,9 @@ __global__ void __launch_bounds__(Shape4<PANELS, N>::kThreads, 1)
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
     const int rows = p.nodes * p.group;
     int i = 0, units = 0;
-    // queries of a piece, a warp a row: scaled by a power of two into float16
+    // Queries of a piece, a warp a row.  A bfloat16 row whose largest element is
+    // above 2^101 or below 2^-60 is scaled to there, so that the sums stay within a
+    // float's range; what that costs lies 2^226 below the largest.
     auto queries = [&](const Piece& y) {
       const int h = y.unit / p.tiles_r, first = y.unit % p.tiles_r * N;
       float2* const row_of = s_row + (units & 1) * N;
@@ -382,35 +393,28 @@ __global__ void __launch_bounds__(Shape4<PANELS, N>::kThreads, 1)
       for (int r = r0 + quarter; r < r0 + C; r += 4) {
         const int row = first + r;
         const bool real = row < rows;
-        const int64_t at = y.b * p.q.batch + (h * p.group + row % p.group) * p.q.head + (int64_t)(row / p.group) * p.q.row;
+        const T* const q = static_cast<const T*>(p.q.data) + y.b * p.q.batch + (h * p.group + row % p.group) * p.q.head +
+                           (int64_t)(row / p.group) * p.q.row;
         float v[2 * PANELS];
         uint32_t top = 0;
 #pragma unroll
         for (int j = 0; j < 2 * PANELS; ++j) {
           const int d = 2 * lane + 64 * (j / 2) + (j & 1);
-          v[j] = 0.0f;
-          if (real && d < p.head_dim)
-            v[j] = p.bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(p.q.data)[at + d])
-                          : __half2float(static_cast<const __half*>(p.q.data)[at + d]);
+          v[j] = real && d < p.head_dim ? to_f32(q[d]) : 0.0f;
           const uint32_t u = __float_as_uint(v[j]) & 0x7FFFFFFFu;
           top = max(top, u < 0x7F800000u ? u : 0u);
         }
-        top = __reduce_max_sync(0xffffffffu, top);
-        // 2^-e times the row: its largest finite element becomes 1 to 2
-        const int e = !p.bf16 || top < 0x00800000u ? 0 : (int)(top >> 23) - 127;
-        // in two steps, as 2^-e need not be a float
-        const float s1 = __int_as_float((127 - e / 2) << 23), s2 = __int_as_float((127 - (e - e / 2)) << 23);
+        int e = 0;  // the row is scaled by 2^-e
+        if constexpr (kBf) {
+          const int high = (int)(__reduce_max_sync(0xffffffffu, top) >> 23) - 127;
+          e = high > 100 ? high - 100 : high < -60 ? high + 60 : 0;
+        }
+        const float down = __int_as_float((127 - e) << 23);
 #pragma unroll
-        for (int j = 0; j < PANELS; ++j) {
-          const __half2 w = __floats2half2_rn(v[2 * j] * s1 * s2, v[2 * j + 1] * s1 * s2);
-          const int piece = lane / 4;
-          *reinterpret_cast<__half2*>(smem + S::kAtQ + j * (N * 128) + r * 128 + ((piece ^ (r & 7)) << 4) +
-                                      (lane % 4) * 4) = w;
-        }
-        if (lane == 0) {
-          const float up1 = __int_as_float((127 + e / 2) << 23), up2 = __int_as_float((127 + (e - e / 2)) << 23);
-          row_of[r] = make_float2(p.scale * kLog2e * up1 * up2, kUnset);
-        }
+        for (int j = 0; j < PANELS; ++j)
+          *reinterpret_cast<uint32_t*>(smem + S::kAtQ + j * (N * 128) + r * 128 + (((lane / 4) ^ (r & 7)) << 4) +
+                                       (lane % 4) * 4) = pack2<T>(v[2 * j] * down, v[2 * j + 1] * down);
+        if (lane == 0) row_of[r] = make_float2(p.scale * kLog2e * __int_as_float((127 + e) << 23), kUnset);
       }
       smem_fence_async();
       __syncwarp();
@@ -722,17 +726,17 @@ struct Plan4 {
 
 // What a unit's start costs in the list, in tiles: its query rows are scaled and
 // laid out and its sums left.  With 1, 3 and 6: trees of 21 over 4001 keys, eight ragged
-// sequences of 12 heads of 64, 40.5, 27.7 and 27.4 us; one node of 16/4 heads over
-// 16 sequences of up to 3000 keys 25.2, 19.4 and 19.2; one node over 65536 to 40960 keys,
-// four sequences of 32/8 heads of 128, 86.6, 85.2 and 85.8.
+// sequences of 12 heads of 64, 35.7, 27.2 and 26.9 us; one node of 16/4 heads over
+// 16 sequences of 1500 to 3000 keys 20.8, 20.0 and 20.9; one node over 65536 to 40960 keys,
+// four sequences of 32/8 heads of 128, 92.3, 90.9 and 91.6.
 constexpr int kUnitCost = 3;
 
 Plan4 plan4(const Context& c, const ckks_draft_attention_args& a) {
   const int rows = a.nodes * (a.q_heads / a.kv_heads);
   Plan4 d;
   // The fewest of 16, 32 and 64 rows that hold a (sequence, head)'s, and 64 at a time beyond:
-  // one node over 65536 to 40960 keys (4 rows) takes 85 us with 16 rows, 99 with 32 and 143
-  // with 64; trees of 21 (21 rows) 27.7 with 32 and 35.4 with 64.
+  // one node over 65536 to 40960 keys (4 rows) takes 91 us with 16 rows, 101 with 32 and 138
+  // with 64; trees of 21 (21 rows) 27.2 with 32 and 35.9 with 64.
   d.rows = rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
   d.tiles_r = (rows + d.rows - 1) / d.rows;
   d.units = (long long)a.batch * a.kv_heads * d.tiles_r;
@@ -758,28 +762,34 @@ void launch_join4(const ckks_draft_attention_args& a, const Params4& p, cudaStre
     launch_pdl(join4_kernel<T, PANELS, 1>, dim3((unsigned)(heads * ((rows + 7) / 8))), dim3(256), 0, st, p);
 }
 
-template <int PANELS, int N>
+template <typename T, int PANELS, int N>
 void launch4(const Context& c, const ckks_draft_attention_args& a, const Params4& p, cudaStream_t st) {
   using S = Shape4<PANELS, N>;
   static_assert(S::kSmem <= 232448, "shared memory of one block");
-  auto* k = attend4_kernel<PANELS, N>;
+  auto* k = attend4_kernel<T, PANELS, N>;
   CKKS_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::kSmem));
   k<<<p.ctas, S::kThreads, S::kSmem, st>>>(p, c.d_faults);
   CKKS_CUDA(cudaGetLastError());
-  if (p.bf16)
-    launch_join4<__nv_bfloat16, PANELS>(a, p, st);
-  else
-    launch_join4<__half, PANELS>(a, p, st);
+  launch_join4<T, PANELS>(a, p, st);
 }
 
-template <int PANELS>
-void launch4(const Context& c, const ckks_draft_attention_args& a, const Params4& p, int rows, cudaStream_t st) {
-  if (rows == 16)
-    launch4<PANELS, 16>(c, a, p, st);
-  else if (rows == 32)
-    launch4<PANELS, 32>(c, a, p, st);
+template <typename T, int PANELS>
+void launch4(const Context& c, const ckks_draft_attention_args& a, const Params4& p, cudaStream_t st) {
+  if (p.rows == 16)
+    launch4<T, PANELS, 16>(c, a, p, st);
+  else if (p.rows == 32)
+    launch4<T, PANELS, 32>(c, a, p, st);
   else
-    launch4<PANELS, 64>(c, a, p, st);
+    launch4<T, PANELS, 64>(c, a, p, st);
+}
+
+template <typename T>
+void launch4(const Context& c, const ckks_draft_attention_args& a, const Params4& p, int panels, cudaStream_t st) {
+  switch (panels) {
+    case 1: launch4<T, 1>(c, a, p, st); break;
+    case 2: launch4<T, 2>(c, a, p, st); break;
+    default: launch4<T, 4>(c, a, p, st); break;
+  }
 }
 
 int panels4(int head_dim) { return head_dim <= 64 ? 1 : head_dim <= 128 ? 2 : 4; }
@@ -802,13 +812,12 @@ bool attention4_tc(const Context& c, const ckks_draft_attention_args& a, cudaStr
   p.q = a.q, p.kc = a.k_cache, p.vc = a.v_cache, p.kn = a.k_new, p.vn = a.v_new, p.out = a.out;
   p.lens = a.lens, p.parents = a.parents, p.lse = a.lse, p.part = static_cast<float*>(a.workspace);
   p.batch = a.batch, p.kv_heads = a.kv_heads, p.group = a.q_heads / a.kv_heads, p.head_dim = a.head_dim;
-  p.nodes = a.nodes, p.capacity = a.capacity, p.scale = (float)a.scale, p.bf16 = a.dtype == CKKS_BF16;
+  p.nodes = a.nodes, p.capacity = a.capacity, p.scale = (float)a.scale;
   p.rows = d.rows, p.tiles_r = d.tiles_r, p.unit_cost = kUnitCost, p.ctas = d.ctas, p.row_bytes = R;
-  switch (panels4(a.head_dim)) {
-    case 1: launch4<1>(c, a, p, d.rows, st); break;
-    case 2: launch4<2>(c, a, p, d.rows, st); break;
-    default: launch4<4>(c, a, p, d.rows, st); break;
-  }
+  if (a.dtype == CKKS_BF16)
+    launch4<__nv_bfloat16>(c, a, p, panels4(a.head_dim), st);
+  else
+    launch4<__half>(c, a, p, panels4(a.head_dim), st);
   return true;
 }
 

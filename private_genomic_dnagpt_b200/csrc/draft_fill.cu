@@ -245,8 +245,8 @@ __global__ void __launch_bounds__(256) read4_kernel(ReadParams p) {
           const uint32_t* c = reinterpret_cast<const uint32_t*>(row) + 2 * g;
           const uint32_t a = __ldg(c), b = __ldg(c + 1);
           const __half2 s = scale4_pair(__ldg(row + 8 * G + g), 0);
-          decode4_word(a, s, y);
-          decode4_word(b, s, y + 4);
+          decode4_word<__half>(a, s, y);
+          decode4_word<__half>(b, s, y + 4);
         }
         if constexpr (WIDE && std::is_same_v<T, __half>) {
           *reinterpret_cast<uint4*>(dst) = make_uint4(y[0], y[1], y[2], y[3]);

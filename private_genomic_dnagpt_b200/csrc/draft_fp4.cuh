@@ -91,7 +91,8 @@ __device__ __forceinline__ uint2 encode4(const float* x, uint32_t top, uint32_t&
 __device__ __forceinline__ __half2 decode4(uint32_t byte, __half2 scale) {
   return __hmul2(__half2(__nv_cvt_fp4x2_to_halfraw2((__nv_fp4x2_storage_t)byte, __NV_E2M1)), scale);
 }
-// the eight elements of a word
+// the eight elements of a word, as pairs of T (bfloat16 or float16; exact in either)
+template <typename T>
 __device__ __forceinline__ void decode4_word(uint32_t word, __half2 scale, uint32_t* out) {
   uint32_t h[4];
   asm("{\n .reg .b8 a, b, c, d;\n mov.b32 {a, b, c, d}, %4;\n cvt.rn.f16x2.e2m1x2 %0, a;\n"
@@ -100,8 +101,18 @@ __device__ __forceinline__ void decode4_word(uint32_t word, __half2 scale, uint3
       : "r"(word));
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const __half2 x = __hmul2(*reinterpret_cast<const __half2*>(&h[i]), scale);
-    out[i] = *reinterpret_cast<const uint32_t*>(&x);
+    if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+      float lo, hi;  // the products as floats at once
+      asm("{\n .reg .b16 a, b, s, t;\n mov.b32 {a, b}, %2;\n mov.b32 {s, t}, %3;\n fma.rn.f32.f16 %0, a, s, %4;\n"
+          " fma.rn.f32.f16 %1, b, t, %4;\n}"
+          : "=f"(lo), "=f"(hi)
+          : "r"(h[i]), "r"(*reinterpret_cast<const uint32_t*>(&scale)), "f"(0.0f));
+      const __nv_bfloat162 x = __floats2bfloat162_rn(lo, hi);
+      out[i] = *reinterpret_cast<const uint32_t*>(&x);
+    } else {
+      const __half2 x = __hmul2(*reinterpret_cast<const __half2*>(&h[i]), scale);
+      out[i] = *reinterpret_cast<const uint32_t*>(&x);
+    }
   }
 }
 // scale byte `i` of a word, in both halves

@@ -446,3 +446,42 @@ def test_captured_run_of_prompt_fill_and_trees(cc):
         assert torch.equal(a, b)
     assert got[4].tolist() == [202, 91]
     cc.Synchronize()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,D", [(1, 64), (9, 128), (40, 256)])
+@pytest.mark.parametrize("power", [8, 13, 20, 24, 40, 120])
+def test_attention4_of_rows_with_elements_far_apart(cc, dtype, n, D, power):
+    """The keys are 0 where a query's elements are 2^power times its others,
+    so that the scores consist of the others; then keys and queries scaled
+    oppositely by 2^13, so that both parts weigh the same.  Every product of a
+    cached value and an element has its place in a 32-bit sum, so the bounds are
+    those of every other row."""
+    if dtype == torch.float16 and power > 8:
+        power = 13  # of 16
+    x = base.inputs(dtype, 2, n, 4, 2, D, 500, [500, 129], [tree(n, 2)] * 2, seed=50)
+    big = dict(x) | {name: x[name].clone() for name in ("q", "k_cache", "k_new")}
+    big["q"][..., :16] *= 2.0 ** power
+    for name in ("k_cache", "k_new"):
+        big[name][..., :16] = 0.0
+    y, z = quantised(big)
+    check_attention(z, *cc.draft_attention4(**y))
+    for sign in (13, -13):
+        both = dict(x)
+        for name, e in (("q", sign), ("k_cache", -sign), ("k_new", -sign)):
+            t = x[name].float()
+            t[..., :16] *= 2.0 ** e
+            t[..., 16:] *= 2.0 ** (0 if dtype == torch.float16 else -e)
+            both[name] = t.to(dtype)
+        y, z = quantised(both)
+        check_attention(z, *cc.draft_attention4(**y))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("power", [-110, 110])
+def test_attention4_at_the_ends_of_the_range(cc, dtype, power):
+    x = base.inputs(dtype, 2, 9, 4, 2, 64, 500, [500, 129], [tree(9, 2)] * 2, seed=51)
+    y, z = quantised(x)
+    q = y["q"] * 2.0 ** power
+    scale = 0.125 * 2.0 ** -power
+    check_attention(z | {"q": q}, *cc.draft_attention4(**(y | {"q": q}), scale=scale), scale=scale)
