@@ -363,8 +363,8 @@ void run_prompt(const Context& c, const PromptParams& p, cudaStream_t st) {
 // The exponential unit takes 8 cycles for a warp's 32: 2048 cycles for a pair of
 // tiles, whose products take 1024 at 64 elements and 2048 at 128.  So two in
 // eight of the exponentials are computed with multiply-adds: 2^x = 2^n 2^r, n
-// the nearest integer, and 2^r the polynomial of degree 4 with the least largest
-// relative error on [-1/2, 1/2] (2.7e-6, fitted to 2^r).  None, one, two, three, four
+// the nearest integer, and 2^r the polynomial 1 + ... of degree 4 with the least
+// largest relative error on [-1/2, 1/2] (2.9e-6, fitted to 2^r).  None, one, two, three, four
 // in eight: 553, 546, 542, 566, 580 us for the first case, 525, 495, 484, 501, 530 for
 // heads of 64.
 //
@@ -392,16 +392,18 @@ struct PromptShape {
   static constexpr int kPoly = PANELS <= 2 ? 2 : 0;
 };
 
-// 2^x for x >= -126; what lies below comes out next to 0
+// 2^x for x >= -126; off by 2^-127 at most below, and 0 from -127 on (r is 0 there,
+// and the bits of 1 less 127 exponents are those of 0): a key whose weight is nothing
+// leaves nothing, however large its value
 __device__ __forceinline__ float2 exp2_poly(float2 x) {
   const float2 big = make_float2(12582912.0f, 12582912.0f);  // 1.5 2^23: the sum's low bits are the nearest integer
-  x.x = fmaxf(x.x, -126.0f), x.y = fmaxf(x.y, -126.0f);
+  x.x = fmaxf(x.x, -127.0f), x.y = fmaxf(x.y, -127.0f);
   const float2 t = add2(x, big), r = sub2(x, sub2(t, big));
   auto two = [](float v) { return make_float2(v, v); };
-  float2 y = fma2(r, two(0.00957053154706955f), two(0.05591866374015808f));
-  y = fma2(y, r, two(0.24024735391139984f));
-  y = fma2(y, r, two(0.6931216716766357f));
-  y = fma2(y, r, two(0.9999992847442627f));
+  float2 y = fma2(r, two(0.009582852944731712f), two(0.055906426161527634f));
+  y = fma2(y, r, two(0.24024099111557007f));
+  y = fma2(y, r, two(0.6931241750717163f));
+  y = fma2(y, r, two(1.0f));
   return make_float2(__uint_as_float(__float_as_uint(y.x) + (__float_as_uint(t.x) << 23)),
                      __uint_as_float(__float_as_uint(y.y) + (__float_as_uint(t.y) << 23)));
 }

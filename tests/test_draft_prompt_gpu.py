@@ -371,3 +371,23 @@ def test_prompt_c_entry_point(cc):
         assert call(**more) == 1, more
     assert call(tokens=0) == 0
     cc.Synchronize()
+
+
+@pytest.mark.parametrize("D", [64, 128, 40])
+def test_a_weight_of_nothing_is_nothing(cc, D):
+    """Keys whose scores lie 1000 below the others' have the weight 0 in 32 bits,
+    so that the largest values of bfloat16 do not show through them."""
+    starts = packed([500, 300])
+    x = inputs(torch.bfloat16, starts[-1], 2, 1, D, starts, seed=20)
+    for name in ("q", "k"):
+        x[name][..., 0] = 0.0
+    x["q"][..., 0] = D ** 0.5
+    for first in (0, 500):
+        x["k"][first + 1:first + 70, :, 0] = -1000.0
+        x["v"][first + 1:first + 70] = 3e38
+    check(x, *cc.draft_prompt(**x))
+    x["k"][first + 1:first + 70, :, 0] = -3e38  # scores of -inf
+    y = dict(x) | {"v": x["v"].clone()}
+    y["v"][first + 1:first + 70] = 0.0
+    got, want = cc.draft_prompt(**x), cc.draft_prompt(**y)
+    assert torch.equal(got[0][500:], want[0][500:]) and torch.equal(got[1][500:], want[1][500:])
