@@ -391,3 +391,102 @@ def test_a_weight_of_nothing_is_nothing(cc, D):
     y["v"][first + 1:first + 70] = 0.0
     got, want = cc.draft_prompt(**x), cc.draft_prompt(**y)
     assert torch.equal(got[0][500:], want[0][500:]) and torch.equal(got[1][500:], want[1][500:])
+
+
+def sms():
+    return torch.cuda.get_device_properties(0).multi_processor_count
+
+
+def check_exactly(x, out, lse, scale):
+    """``check`` with the definition in float64 on the GPU, as the sizes ask
+    for; elements that see a value that is no number are none."""
+    q, k, v = (x[n].double() for n in ("q", "k", "v"))
+    T, Hq, D = q.shape
+    G = Hq // k.shape[1]
+    k, v = k.repeat_interleave(G, 1), v.repeat_interleave(G, 1)
+    bad = ~torch.isfinite(v)
+    v = torch.where(bad, 0.0, v)
+    s = ref.starts_of(x["starts"].cpu().numpy(), T)
+    seen = torch.zeros(T, dtype=torch.bool, device="cuda")
+    for a, e in zip(s, s[1:]):
+        if a == e:
+            continue
+        seen[a:e] = True
+        n = e - a
+        above = torch.ones(n, n, dtype=torch.bool, device="cuda").triu(1)
+        for h in range(0, Hq, 8):
+            qq, kk, vv = (t[a:e, h:h + 8].transpose(0, 1) for t in (q, k, v))
+            score = (qq @ kk.transpose(1, 2) * scale).masked_fill(above, -float("inf"))
+            want_lse = torch.logsumexp(score, 2)
+            p = torch.exp(score - want_lse[..., None])
+            big = (qq.abs() @ kk.abs().transpose(1, 2)).masked_fill(above, 0.0).amax(2) * abs(scale)
+            noise = 2.0 ** -23 * ((D + 8) * big + torch.arange(1, n + 1, device="cuda") + 8)
+            room = (2 * HALF[x["q"].dtype] + noise)[..., None] * (p @ vv.abs()) + 1e-30
+            got = out[a:e, h:h + 8].transpose(0, 1).double()
+            none = bad[a:e, h:h + 8].transpose(0, 1).cumsum(1) > 0
+            assert not torch.isfinite(got[none]).any()
+            off = torch.where(none, 0.0, (got - p @ vv).abs() / room)  # (a NaN fails too)
+            assert (off <= 1.0).all(), f"rows {a} to {e}, heads from {h}: {off.max():.3g} times the bound"
+            off = (lse[a:e, h:h + 8].T.double() - want_lse).abs()
+            assert (off <= 0.5 * noise + 2.0 ** -22 * (1 + want_lse.abs())).all()
+    assert not out[~seen].any() and (lse[~seen] == -float("inf")).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("D", [64, 128, 192, 256])
+@pytest.mark.parametrize("spoiled", [False, True])
+def test_several_units_a_cta(cc, dtype, D, spoiled):
+    """Three units and more of unequal lengths for every CTA of the tensor-core
+    kernel, with both row groups and one; then with values that are no numbers next
+    to the causal border in some of the units."""
+    lengths, rows = [1, 120, 129, 257, 0, 700, 1500], 256 if D <= 128 else 128
+    units = sum(-(-n // rows) for n in lengths)
+    Hk = 4
+    Hq = Hk * -(-3 * sms() // (units * Hk))
+    assert units * Hq >= 3 * sms()
+    starts = packed(lengths, 2)
+    x = inputs(dtype, starts[-1] + 3, Hq, Hk, D, starts, seed=21)
+    if spoiled:
+        for seq, at, head, d in ((2, 100, 0, 3), (2, 128, 3, 5), (3, 127, 1, 1), (3, 200, 1, D - 1), (3, 256, 0, 9),
+                                 (5, 130, 2, 0), (5, 255, 1, 7), (5, 256, 3, 11), (5, 699, 0, 2), (6, 600, 3, 4),
+                                 (6, 1279, 1, 6), (6, 1280, 2, 8), (6, 1407, 0, 13), (6, 1499, 1, 15)):
+            x["v"][starts[seq] + at, head, d] = float("nan") if at % 2 else float("inf")
+    out, lse = cc.draft_prompt(**x)
+    check_exactly(x, out, lse, D ** -0.5)
+    again = cc.draft_prompt(**x)
+    fine = torch.isfinite(out)
+    assert torch.equal(fine, torch.isfinite(again[0])) and torch.equal(out[fine], again[0][fine]) and torch.equal(lse, again[1])
+    cc.Synchronize()
+
+
+@pytest.mark.parametrize("dtype,D", [(torch.float32, 128), (torch.float32, 100), (torch.float32, 65), (torch.bfloat16, 100),
+                                     (torch.float16, 128)])
+@pytest.mark.parametrize("scale", [None, -0.05])
+def test_tall_tiles_on_the_cuda_cores(cc, dtype, D, scale):
+    """Heads of 65 to 128 in as many rows and heads as the kernel takes 128 rows
+    at a time for; in 16 bits off every wide boundary."""
+    lengths = [1, 63, 64, 65, 127, 128, 129, 500]
+    starts = packed(lengths, 1)
+    T = starts[-1] + 2
+    Hk = 8
+    Hq = Hk * -(-(3 * sms() // 2) // (T // 128 * Hk))
+    assert T // 128 * Hq >= 3 * sms() // 2
+    x = inputs(dtype, T, Hq, Hk, D, starts, seed=22)
+    if dtype != torch.float32:
+        flat = torch.zeros(x["k"].numel() + 1, dtype=dtype, device="cuda")
+        flat[1:] = x["k"].reshape(-1)
+        x["k"] = flat[1:].view(x["k"].shape)
+    out, lse = cc.draft_prompt(**x, scale=scale)
+    check_exactly(x, out, lse, D ** -0.5 if scale is None else scale)
+    # what only the last rows of two sequences see, and rows of no sequence
+    y = {k: v.clone() if dtype == torch.float32 else v for k, v in x.items()}
+    for at in (starts[5] + 120, starts[8] - 3):
+        for name in ("k", "v"):
+            y[name][at] = float("nan")
+    y["q"][0] = y["k"][0] = y["v"][0] = y["v"][T - 1] = float("nan")
+    got, glse = cc.draft_prompt(**y, scale=scale)
+    bad = torch.zeros(T, dtype=torch.bool, device="cuda")
+    bad[starts[5] + 120:starts[6]] = bad[starts[8] - 3:starts[8]] = True
+    assert torch.isnan(got[bad]).all() and torch.isnan(glse[bad]).all()
+    assert torch.equal(got[~bad], out[~bad]) and torch.equal(glse[~bad], lse[~bad])
+    cc.Synchronize()
