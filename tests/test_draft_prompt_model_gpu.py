@@ -125,3 +125,31 @@ def test_prompt_and_prefill_agree(cc, dtype, most):
     chain = i32([[-1, 0, 1, 2, 3]])
     assert plain_block.rel_inf(f64(b.forward(nodes, chain)), f64(a.forward(nodes, chain))) < most
     cc.Synchronize()
+
+
+@pytest.mark.parametrize("dtype,most", [(torch.bfloat16, 0.05), (torch.float16, 0.01)])
+def test_four_bits_in_the_16_bit_types(cc, dtype, most):
+    """The default type: prompt, trees and commits over a 4-bit cache against the
+    same model over a plain cache that is given the values of the other's."""
+    ws = [weights(76), weights(77)]
+    x = torch.from_numpy(np.float32(plain_block.synthetic_input(78, 300, d=D))).cuda()
+    starts, n = [0, 150, 151, 260], 7
+    a = DraftModel(cc, ws, capacity=200, batch=3, heads=HEADS, dtype=dtype, cache_bits=4)
+    b = DraftModel(cc, ws, capacity=200, batch=3, heads=HEADS, dtype=dtype)
+    got, want = a.prompt(x[:260], i32(starts)), b.prompt(x[:260], i32(starts))
+    assert torch.equal(got, want)  # attention within the prompts reads no cache
+
+    def give():
+        for (k4, v4, _), (k, v, _) in zip(a.caches, b.caches):
+            k.copy_(cc.draft_read4(k4, a.lens, D // HEADS, dtype))
+            v.copy_(cc.draft_read4(v4, a.lens, D // HEADS, dtype))
+
+    for step in range(2):
+        give()
+        nodes = x[260 + n * step:260 + n * (step + 1)].repeat(3, 1, 1)
+        got, want = (m.forward(nodes, i32([tree(n, 2)] * 3)) for m in (a, b))
+        assert plain_block.rel_inf(f64(want), f64(got)) < most
+        for m in (a, b):
+            m.accept(i32([[0, 2, 5, -1, -1, -1, -1]] * 3), i32([3, 0, 1]))
+        assert a.lens.tolist() == b.lens.tolist() == [150 + 3 * (step + 1), 1, 109 + step + 1]
+    cc.Synchronize()
