@@ -268,12 +268,13 @@ class DraftModel:
         [batch + 1] int32 as for ``drafting.prompt``.  Returns the hidden states
         [T, D] (float32).  The caches must be empty, and hold the longest prompt
         (``starts`` is read back where the rows might be more than the
-        capacity).  A model with a budget takes its prompt through ``prefill``,
+        capacity, the lengths where the caches were in use: ``lens.zero_()``
+        empties them for the next prompts).  A model with a budget takes its prompt through ``prefill``,
         which gathers the weights that eviction goes by."""
         import torch
         if self.budget is not None:
             raise ValueError("prompt: a model with a budget gathers its prompt's weights through prefill")
-        if self._most:
+        if self._most and self.lens.any():  # `_most` may count rows that were never accepted, or are gone
             raise ValueError("prompt: the cache holds rows already")
         t, width = x.shape
         most = t

@@ -91,3 +91,23 @@ def test_prefill_into_four_bits(more):
     m = model(100, cache_bits=4)
     m.prefill(torch.zeros(1, 70, 8))
     assert m.lens.tolist() == [70] and more == ["attention4", "commit4"] * 2
+
+
+@pytest.mark.parametrize("four", [False, True])
+def test_prompts_after_the_caches_were_emptied(more, four):
+    """Rows that were offered and not accepted, and lengths set back to 0, leave
+    room for the next prompts; a single row does not."""
+    m = model(20, batch=2, cache_bits=4 if four else None)
+    step(m, 3, [0, 0])
+    m.prompt(torch.zeros(9, 8), i32([0, 6, 9]))
+    assert m.lens.tolist() == [6, 3]
+    step(m, 5, [2, 1])
+    with pytest.raises(ValueError, match="holds rows already"):
+        m.prompt(torch.zeros(9, 8), i32([0, 6, 9]))
+    m.lens.zero_()
+    m.prompt(torch.zeros(7, 8), i32([0, 0, 7]))
+    assert m.lens.tolist() == [0, 7]
+    with pytest.raises(ValueError, match="holds rows already"):
+        m.prompt(torch.zeros(3, 8), i32([0, 3, 3]))
+    step(m, 13, [13, 13])
+    assert m.lens.tolist() == [13, 20]

@@ -153,3 +153,24 @@ def test_four_bits_in_the_16_bit_types(cc, dtype, most):
             m.accept(i32([[0, 2, 5, -1, -1, -1, -1]] * 3), i32([3, 0, 1]))
         assert a.lens.tolist() == b.lens.tolist() == [150 + 3 * (step + 1), 1, 109 + step + 1]
     cc.Synchronize()
+
+
+@pytest.mark.parametrize("four", [False, True])
+def test_a_model_serves_batch_after_batch(cc, four):
+    """Emptied caches give the results of new ones."""
+    ws = [weights(79), weights(80)]
+    x = torch.from_numpy(np.float32(plain_block.synthetic_input(81, 200, d=D))).cuda()
+    used = DraftModel(cc, ws, capacity=128, batch=2, heads=HEADS, cache_bits=4 if four else None)
+    chain = i32([[-1, 0, 1]] * 2)
+    for lengths in ([90, 20], [3, 120], [0, 70]):
+        new = DraftModel(cc, ws, capacity=128, batch=2, heads=HEADS, cache_bits=4 if four else None)
+        starts, nodes = i32([0, lengths[0], sum(lengths)]), x[150:153].repeat(2, 1, 1)
+        used.lens.zero_()
+        got, want = (m.prompt(x[:sum(lengths)], starts) for m in (used, new))
+        assert torch.equal(got, want)
+        got, want = (m.forward(nodes, chain) for m in (used, new))
+        assert torch.equal(got, want)
+        for m in (used, new):
+            m.accept(chain + 1, i32([3, 1]))
+        assert used.lens.tolist() == new.lens.tolist() == [lengths[0] + 3, lengths[1] + 1]
+    cc.Synchronize()
