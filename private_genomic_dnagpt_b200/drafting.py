@@ -213,8 +213,9 @@ class DraftModel:
             size = self.width // heads
             rows, kind = (batch, heads, capacity, row4_bytes(size) if self._four else size), \
                 torch.uint8 if self._four else self.dtype
+            # (keys, values, the keys' weights: none over 4-bit rows, which are not cut)
             return [(torch.zeros(rows, dtype=kind, device=device), torch.zeros(rows, dtype=kind, device=device),
-                     torch.zeros(rows[:3], device=device)) for _ in block_weights]
+                     None if self._four else torch.zeros(rows[:3], device=device)) for _ in block_weights]
 
         self.caches, self._spare = caches(), caches() if budget is not None else None
         self.lens = torch.zeros(batch, dtype=torch.int32, device=device)

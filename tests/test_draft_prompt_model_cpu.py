@@ -111,3 +111,10 @@ def test_prompts_after_the_caches_were_emptied(more, four):
         m.prompt(torch.zeros(3, 8), i32([0, 3, 3]))
     step(m, 13, [13, 13])
     assert m.lens.tolist() == [13, 20]
+
+
+def test_a_4_bit_model_keeps_its_rows_only(more):
+    """9/16 of a byte an element, and nothing beside the rows."""
+    for (k, v, acc), rest in zip(model(50, batch=2, cache_bits=4).caches, model(50, batch=2).caches):
+        assert k.shape == v.shape == (2, 2, 50, 12) and acc is None
+        assert rest[0].shape == (2, 2, 50, 4) and rest[2].shape == (2, 2, 50)
