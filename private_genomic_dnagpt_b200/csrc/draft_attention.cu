@@ -1464,7 +1464,8 @@ int run(ckks_ctx* ctx, const ckks_draft_attention_args* args, void* stream) {
     check_ptr(a.parents, "parents");
     check_ptr(a.lse, "lse");
     const size_t ws = FOUR ? workspace4_of(c, a) : workspace_of(c, a);
-    need(a.workspace_bytes >= ws && (ws == 0 || a.workspace), "workspace smaller than ckks_draft_attention_workspace");
+    need(a.workspace_bytes >= ws && (ws == 0 || a.workspace),
+         FOUR ? "workspace smaller than ckks_draft_attention4_workspace" : "workspace smaller than ckks_draft_attention_workspace");
     need(reinterpret_cast<uintptr_t>(a.workspace) % 16 == 0, "workspace not aligned to 16 bytes");
     AttnParams p{};
     p.q = a.q, p.kc = a.k_cache, p.vc = a.v_cache, p.kn = a.k_new, p.vn = a.v_new, p.out = a.out;

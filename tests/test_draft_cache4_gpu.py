@@ -11,6 +11,8 @@ is 2^7 or more, so each is off by up to 2^-25 / 2^7 = 2^-32 of the largest,
 times |v|, and their sum is at least the largest.  The other smallest steps are
 below 1e-30."""
 
+import ctypes
+
 import numpy as np
 import pytest
 
@@ -485,3 +487,24 @@ def test_attention4_at_the_ends_of_the_range(cc, dtype, power):
     q = y["q"] * 2.0 ** power
     scale = 0.125 * 2.0 ** -power
     check_attention(z | {"q": q}, *cc.draft_attention4(**(y | {"q": q}), scale=scale), scale=scale)
+
+
+def test_refused_attention4_structs(cc):
+    """What torch tensors never hold, at the C entry point."""
+    lib, buf = eng.lib(), torch.zeros(1 << 16, device="cuda")
+    at = buf.data_ptr()
+
+    def attention4(**change):
+        f = dict(dtype=0, batch=1, q_heads=2, kv_heads=1, head_dim=16, nodes=2, capacity=4, reserved=0, scale=1.0,
+                 lens=at, parents=at, lse=at, workspace=at, workspace_bytes=1 << 14)
+        f |= {n: base.Rows(at, 64, 64, 16) for n in ("q", "k_new", "v_new", "out")}
+        f |= {n: base.Rows(at, 48, 48, 12) for n in ("k_cache", "v_cache")}
+        return lib.ckks_draft_attention4(cc.h, ctypes.byref(base.AttentionArgs(**(f | change))), None)
+
+    assert attention4(batch=0) == 0
+    for change in (dict(dtype=3), dict(nodes=0), dict(nodes=65), dict(capacity=1 << 30), dict(reserved=1),
+                   dict(k_cache=base.Rows(at + 2, 48, 48, 12)), dict(v_cache=base.Rows(at, 48, 48, 14)),
+                   dict(v_cache=base.Rows(0, 48, 48, 12)), dict(scale=float("nan")), dict(workspace=at + 4)):
+        assert attention4(**change) == 1, change
+    assert attention4(capacity=4000, workspace_bytes=16) == 1 and "ckks_draft_attention4_workspace" in lib.ckks_last_error().decode()
+    cc.Synchronize()
