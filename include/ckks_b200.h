@@ -624,7 +624,8 @@ int ckks_draft_commit4(ckks_ctx* ctx, const ckks_draft_commit_args* args, void* 
 
 typedef struct {
   int32_t dtype; /* of out: CKKS_BF16, CKKS_FP16 or CKKS_FP32 */
-  int32_t batch, kv_heads, head_dim, capacity, reserved;
+  int32_t batch, kv_heads, head_dim, capacity;
+  int32_t reserved;    /* 0 */
   ckks_rows cache;     /* 4-bit rows */
   ckks_rows out;       /* [batch][kv_heads][capacity][head_dim], not overlapping the cache */
   const int32_t* lens; /* [batch]; taken as 0..capacity */

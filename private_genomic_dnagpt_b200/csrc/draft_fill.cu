@@ -441,6 +441,7 @@ extern "C" int ckks_draft_read4(ckks_ctx* ctx, const ckks_draft_read4_args* args
     need(args != nullptr, "null argument");
     const ckks_draft_read4_args& a = *args;
     check_sizes(a.dtype, a.batch, a.kv_heads, a.head_dim, a.capacity);
+    need(a.reserved == 0, "reserved field is not 0");
     if (a.batch == 0 || a.capacity == 0) return;
     const int e = element_bytes(a.dtype), R = row4_bytes(a.head_dim);
     check_rows(a.cache, 1, "cache");

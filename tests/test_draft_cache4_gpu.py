@@ -508,3 +508,28 @@ def test_refused_attention4_structs(cc):
         assert attention4(**change) == 1, change
     assert attention4(capacity=4000, workspace_bytes=16) == 1 and "ckks_draft_attention4_workspace" in lib.ckks_last_error().decode()
     cc.Synchronize()
+
+
+class Read4Args(ctypes.Structure):
+    """ckks_draft_read4_args of include/ckks_b200.h."""
+    _fields_ = ([(n, ctypes.c_int32) for n in ("dtype", "batch", "kv_heads", "head_dim", "capacity", "reserved")] +
+                [(n, base.Rows) for n in ("cache", "out")] + [("lens", ctypes.c_void_p)])
+
+
+def test_refused_read4_structs(cc):
+    """What torch tensors never hold, at the C entry point."""
+    lib, buf = eng.lib(), torch.zeros(1 << 16, device="cuda")
+    at = buf.data_ptr()
+
+    def read4(**change):
+        f = dict(dtype=0, batch=1, kv_heads=1, head_dim=16, capacity=4, cache=base.Rows(at, 48, 48, 12),
+                 out=base.Rows(at + 1024, 64, 64, 16), lens=at + 4096)
+        return lib.ckks_draft_read4(cc.h, ctypes.byref(Read4Args(**(f | change))), None)
+
+    assert read4() == 0 and read4(batch=0) == 0 and read4(capacity=0) == 0
+    for change in (dict(dtype=3), dict(batch=-1), dict(kv_heads=0), dict(head_dim=257), dict(capacity=-1), dict(lens=0),
+                   dict(cache=base.Rows(at + 2, 48, 48, 12)), dict(cache=base.Rows(at, 48, 48, 13)),
+                   dict(out=base.Rows(at + 40, 64, 64, 16)), dict(out=base.Rows(0, 64, 64, 16))):
+        assert read4(**change) == 1, change
+    assert read4(reserved=1) == 1 and "reserved" in lib.ckks_last_error().decode()
+    cc.Synchronize()
