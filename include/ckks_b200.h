@@ -586,7 +586,10 @@ typedef struct {
  * see does not reach it, whatever it holds; an infinite or NaN value that a
  * row sees makes that element of the row infinite or NaN.  Products and sums
  * are in 32 bits; between the two products a softmax weight keeps 8 bits with
- * bfloat16 tensors, 11 with float16 and 24 with float32 ones.  No workspace. */
+ * bfloat16 tensors, 11 with float16 (in steps of 2^-31 of the row's largest at
+ * the finest) and 24 with float32 ones (ckks_draft_attention keeps 16 and 22 in
+ * the 16-bit types).  A sum is divided at its end: bfloat16 and float32 values
+ * beyond 2^119 over the number of keys may take it out of range.  No workspace. */
 int ckks_draft_prompt(ckks_ctx* ctx, const ckks_draft_prompt_args* args, void* stream);
 
 /* A 4-bit cache holds rows of ckks_draft_row4_bytes(head_dim) bytes on 4-byte

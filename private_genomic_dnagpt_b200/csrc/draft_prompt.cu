@@ -124,7 +124,10 @@ __device__ __forceinline__ void clear_spare(const PromptParams& p, int first, in
 // for 128 with RT 8): 31 TFLOP/s for one prompt of 4096 and 16 heads of 64 in
 // float32, 35 for four of 2048 and 8 of 128.  Two CTAs an SM are worth more than
 // the few registers that then go to memory (up to 1030 four prompts of 12 heads of 64:
-// 183 us, with one CTA 225); multiply-adds in pairs took 243.
+// 183 us, with one CTA 225); multiply-adds in pairs took 243.  Heads of 125 to 128 ask for
+// 118 KB of shared memory with 64 rows, so one CTA runs there on the registers of two.
+// (These and the rules' figures below are of calls back to back; replayed in a graph the
+// four prompts take 195 us.)
 constexpr int kKeyTile = 64, kThreads = 256;
 
 template <typename T, int DC, int RT>
@@ -369,7 +372,7 @@ void run_prompt(const Context& c, const PromptParams& p, cudaStream_t st) {
 // heads of 64.
 //
 // Measured: 8192 tokens, 32/8 heads of 128, bfloat16, 502 us (1.10 PFLOP/s, 65 % of
-// a library product; 581 us and 0.95 under sustained load and the power limit);
+// a library product) in bursts; 586 us and 0.94 in calls back to back, under the power limit;
 // twelve prompts up to 2001, 12 heads of 64, float16, 107 us.  Half a tile takes a
 // softmax warp some 1600 cycles: 240 at the barrier of its scores, 300 for their
 // maximum, 1000 for the weights (two warps share an exponential unit), and no

@@ -125,7 +125,10 @@ def prompt(cc, q, k, v, starts, scale=None):
     less than those before it).  bfloat16, float16 or float32, Hq a multiple of
     Hkv, D <= 256, any strides with a contiguous last dimension.  scale defaults
     to 1 / sqrt(D).  Returns out [T, Hq, D] in q's type and lse [T, Hq] float32,
-    the log of each row's sum; a row of no sequence is 0, its lse -inf."""
+    the log of each row's sum; a row of no sequence is 0, its lse -inf.  A
+    softmax weight is rounded to the tensors' type before it meets the values.
+    16-bit tensors whose rows are whole, aligned 16-byte pieces run on the tensor
+    cores, others many times slower."""
     return (_binding or _native()).prompt(cc.h.value, cc.params.device, q, k, v, starts, scale)
 
 
@@ -144,8 +147,10 @@ def row4_bytes(head_dim):
     16, behind them a scale of 8 bits for each group (a sixth of its largest
     magnitude, to three bits of mantissa), then zeros up to a multiple of four
     bytes.  A 4-bit cache is a uint8 tensor [B, Hkv, capacity, row4_bytes(D)]
-    whose rows start on 4-byte boundaries (``attention4`` is fastest where a
-    head's rows lie one behind the other); zeros are an empty one.  Magnitudes
+    whose rows start on 4-byte boundaries; zeros are an empty one.
+    ``attention4`` wants a head's rows one behind the other and 16-bit queries:
+    over long caches in other orders, or in float32, it takes 15 times as
+    long.  Magnitudes
     over 61440 become 61440, and a group with an infinity or a NaN in it reads
     as NaN."""
     return (_binding or _native()).row4_bytes(head_dim)
