@@ -533,3 +533,53 @@ def test_refused_read4_structs(cc):
         assert read4(**change) == 1, change
     assert read4(reserved=1) == 1 and "reserved" in lib.ckks_last_error().decode()
     cc.Synchronize()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("n,G", [(1, 4), (7, 3), (13, 4), (40, 2)])
+def test_attention4_several_units_a_cta(cc, dtype, D, n, G):
+    """Three units and more of unequal lengths for every CTA, of up to 16, 32 and
+    64 rows and of two units a head; against the definition in float64 on the
+    GPU, as the sizes ask for."""
+    Hk, some = 6, [300, 0, 1, 129, 128, 0, 640, 127, 257]
+    B = -(-3 * torch.cuda.get_device_properties(0).multi_processor_count // Hk)
+    lens = [some[b % len(some)] for b in range(B)]
+    parents = tree(n, 2, 1 if n > 1 else 0)
+    x = base.inputs(dtype, B, n, G * Hk, Hk, D, 640, lens, [parents] * B, seed=52)
+    R = drafting.row4_bytes(D)
+    caches = [torch.zeros(B, Hk, 640, R, dtype=torch.uint8, device="cuda") for _ in range(2)]
+    for b in range(B):  # every row of the caches, those behind the lengths too
+        cc.draft_fill4(*(c[b:b + 1] for c in caches), i32([0]), x["k_cache"][b].transpose(0, 1), x["v_cache"][b].transpose(0, 1),
+                       i32([0, 640]))
+    y = x | {"k_cache": caches[0], "v_cache": caches[1]}
+    out, lse = cc.draft_attention4(**y)
+    k, v = (cc.draft_read4(c, i32(lens), D, torch.float32).double() for c in caches)
+    see = torch.zeros(n, n, dtype=torch.bool, device="cuda")
+    for i, p in enumerate(parents):
+        if p >= -1:
+            see[i] = see[p] if p >= 0 else False
+            see[i, i] = True
+    real = see.any(1)
+    for b, m in enumerate(lens):
+        kk = torch.cat([k[b, :, :m], x["k_new"][b].double().transpose(0, 1)], 1).repeat_interleave(G, 0)
+        vv = torch.cat([v[b, :, :m], x["v_new"][b].double().transpose(0, 1)], 1).repeat_interleave(G, 0)
+        q = x["q"][b].double().transpose(0, 1)
+        hidden = torch.cat([(~real)[:, None].expand(n, m), ~see], 1)
+        score = (q @ kk.transpose(1, 2) * D ** -0.5).masked_fill(hidden, -float("inf"))[:, real]
+        want_lse = torch.logsumexp(score, 2)
+        p = torch.exp(score - want_lse[..., None])
+        big = (q.abs() @ kk.abs().transpose(1, 2)).masked_fill(hidden, 0.0)[:, real].amax(2) * D ** -0.5
+        keys = (~hidden).sum(1)[real]
+        noise = 2.0 ** -23 * ((D + 8) * big + keys + 8)
+        room = (2 * HALF[dtype] + noise)[..., None] * (p @ vv.abs()) + 2.0 ** -32 * vv.abs().max() * keys[:, None] + 1e-30
+        if dtype == torch.float16:
+            room = room + 2.0 ** -25
+        off = (out[b].double().transpose(0, 1)[:, real] - p @ vv).abs() / room
+        assert (off <= 1.0).all(), f"sequence {b}: {off.max():.3g} times the bound"
+        off = (lse[b].double().T[:, real] - want_lse).abs()
+        assert (off <= 0.5 * noise + 2.0 ** -22 * (1 + want_lse.abs())).all()
+    assert not out[:, ~real].any() and (lse[:, ~real] == -float("inf")).all()
+    again = cc.draft_attention4(**y)
+    assert torch.equal(out, again[0]) and torch.equal(lse, again[1])
+    cc.Synchronize()

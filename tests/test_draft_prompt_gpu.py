@@ -490,3 +490,37 @@ def test_tall_tiles_on_the_cuda_cores(cc, dtype, D, scale):
     assert torch.isnan(got[bad]).all() and torch.isnan(glse[bad]).all()
     assert torch.equal(got[~bad], out[~bad]) and torch.equal(glse[~bad], lse[~bad])
     cc.Synchronize()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_prompts_and_fills_from_two_threads(cc, dtype):
+    """Calls of other sizes at the same time from two host threads."""
+    import threading
+    runs, wrong = [], []
+    for lengths, H, D in (([700, 129], 4, 64), ([90, 300], 2, 200)):
+        starts = packed(lengths)
+        x = inputs(dtype, starts[-1], H, H, D, starts, seed=23)
+        zero, st = i32([0, 0]), x["starts"]
+
+        def call(x=x, H=H, D=D, zero=zero, st=st):
+            caches = [torch.zeros(2, H, 700, D, dtype=dtype, device="cuda") for _ in range(2)]
+            return (*cc.draft_prompt(**x), cc.draft_fill(*caches, zero, x["k"], x["v"], st), *caches)
+
+        runs.append((call, call()))
+    torch.cuda.synchronize()
+
+    def calls(call, want):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(50):
+                got = call()
+                torch.cuda.current_stream().synchronize()
+                if not all(torch.equal(a, b) for a, b in zip(got, want)):
+                    wrong.append(1)
+
+    threads = [threading.Thread(target=calls, args=r) for r in runs]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+    cc.Synchronize()
